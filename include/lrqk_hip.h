@@ -36,6 +36,12 @@ extern "C" {
 #define LRQK_MAX_TOPK 8192
 #define LRQK_MAX_DECODE_ITERS 16
 
+#define LRQK_ROPE_PLAIN 0
+#define LRQK_ROPE_LINEAR 1
+#define LRQK_ROPE_NTK 2
+#define LRQK_ROPE_LLAMA3 3
+#define LRQK_ROPE_YARN 4
+
 typedef struct lrqk_ctx lrqk_ctx;
 
 int lrqk_version(void);
@@ -246,6 +252,70 @@ int lrqk_attention(lrqk_ctx* ctx, const void* q, const void* k_act, const void* 
  * runtime load the kernels): make it outside a graph capture. */
 int lrqk_attention_static(const void* q, const void* k_act, const void* v_act, int n_slots, int n_valid,
                           void* out, int bh, int d, int dtype, void* stream);
+
+/* No counterpart in the reference (its model patch takes the embedding from the model).  Rotary positions.
+ * lrqk_rotary_frequencies (host only) fills freq[rotary_dim / 2] with the angles per position of a head's pairs,
+ * theta^(-2 i / rotary_dim), scaled for contexts longer than the trained one:
+ *   LRQK_ROPE_LINEAR  divided by `factor`
+ *   LRQK_ROPE_NTK     of theta * factor^(rotary_dim / (rotary_dim - 2))
+ *   LRQK_ROPE_LLAMA3  by their turns over original_context: divided by `factor` below p0 (low_freq_factor), kept above p1
+ *                     (high_freq_factor), in between the mean weighted by where they lie
+ *   LRQK_ROPE_YARN    by their pair: kept before the one that makes p0 (beta_fast) turns over original_context, divided by
+ *                     `factor` behind the one that makes p1 (beta_slow), a ramp in between; *result_factor = 0.1 ln(factor) + 1
+ * (LRQK_ROPE_PLAIN: as they are.)  *result_factor, 1 but for the last, goes into lrqk_rotary's `factor`.
+ *
+ * lrqk_rotary turns q [b][hq][s][d] and k [b][hk][s][d] (hk = 0: none) to their positions: every pair (x, y) of the first
+ * rotary_dim elements of a head -- elements i and i + rotary_dim / 2, or 2 i and 2 i + 1 if interleaved -- becomes
+ * factor (x cos a - y sin a, y cos a + x sin a), a = position * freq[i] (formed and reduced in fp64; freq on the device);
+ * the others are copied.  transpose: by -a, the gradient of the turn.  strides (host): elements between sequences, heads
+ * and tokens of q, q_out, k, k_out, three each; rows are contiguous.  An output may be its input (with its strides).
+ * positions: int32 [b][s], sequences pos_stride apart (0: one for all), or NULL: first, first + 1, ... */
+int lrqk_rotary_frequencies(int rotary_dim, double theta, int scaling, double factor, double p0, double p1,
+                            double original_context, double* freq, double* result_factor);
+int lrqk_rotary(const void* q, const void* k, void* q_out, void* k_out, const int64_t* strides, const int32_t* positions,
+                int64_t pos_stride, int32_t first, const double* freq, double factor, int b, int hq, int hk, int64_t s, int d,
+                int rotary_dim, int interleaved, int transpose, int dtype, void* stream);
+
+/* No counterpart in the reference (it attends with one query at a time, py:2326-2327).  Attention of t drafted tokens a
+ * sequence: query head h attends to the cached tokens of cache head h / (hq / hc) -- rows [0, lengths[sequence]) of
+ * k_cache, v_cache, at most n; all n where lengths (int32, device) is NULL -- and to the drafted tokens j, k_new, v_new
+ * [b][hn][t][d] of head h / (hq / hn), with mask[i][j] != 0 (u8 [t][t], sequences mask_batch_stride apart, 0: one mask
+ * for all).  hc = hn: a dense cache; hc = hq: the active set (k_act, v_act), whose tokens every query head picks itself.
+ * q, out: [b][hq][t][d]; lse (or NULL): fp32 [b][hq][t], log of the sum of exp(scale q.k).  A query that sees nothing
+ * gives zeros and -inf.  What a masked drafted token or a row behind the length holds, infinities and NaN included, does
+ * not matter.  Strides in elements, the same for k_cache and v_cache, multiples of 16 bytes.  Head widths up to 256
+ * elements, t up to 1024.
+ * These calls take no ctx: their scratch is the caller's (lrqk_*_workspace bytes of device memory, 16-byte aligned,
+ * contents of no meaning before and after), so that calls on several streams and captured graphs need not share any. */
+int64_t lrqk_tree_attention_workspace(int b, int hq, int hc, int t, int64_t n, int d, int dtype);
+int lrqk_tree_attention(const void* q, const void* k_cache, const void* v_cache, int64_t kv_batch_stride, int64_t kv_head_stride,
+                        int64_t kv_row_stride, int64_t n, const int32_t* lengths, const void* k_new, const void* v_new,
+                        const uint8_t* mask, int64_t mask_batch_stride, void* out, float* lse, int b, int hq, int hc, int hn,
+                        int t, int d, float scale, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
+/* No counterpart in the reference.  The attention that every cached token got from the last t tokens of its sequence:
+ * out[b][hc][j] = weights[b][hc][j] (0 if NULL; may be out) + the sum over the hq / hc query heads of the cache head and
+ * over the queries i with j <= length - t + i of exp(scale q_i.k_j - lse_i), j < n; tokens behind the length get nothing.
+ * q: [b][hq][t][d], k: rows of d elements by strides as above.  lse: fp32 [b][hq][t] as lrqk_tree_attention leaves it
+ * (a query of -inf adds nothing), or NULL: of the keys that the query sees here.  weights, out: fp32 [b][hc][n].
+ * Deterministic: no atomics.  Workspace as above (with lse none is needed). */
+int64_t lrqk_attention_weights_workspace(int b, int hq, int hc, int t, int64_t n, int d, int have_lse, int dtype);
+int lrqk_attention_weights(const void* q, const void* k, int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,
+                           int64_t n, const int32_t* lengths, const float* lse, const float* weights, float* out, int b, int hq,
+                           int hc, int t, int d, float scale, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
+/* No counterpart in the reference.  Eviction from a cache by those weights: of the first lengths[sequence] tokens (cap if
+ * NULL) of every head, min(length, budget) stay -- those whose ids are within `recent` of the head's largest one (of the
+ * lowest slots, if ids that repeat make them more than the budget), then those of the largest weights (NaN in front; equal
+ * ones: of the lowest slots).  A token that stays and is in the first
+ * min(length, budget) slots keeps its slot; the others that stay move, in order, into the slots that became free, in
+ * order.  weights fp32, ids int32 [b][heads][cap], k, v [b][heads][cap][d].  In place where weights_out, ids_out, k_out,
+ * v_out are NULL; otherwise those ([b][heads][cap_out], rows of d) take the tokens that stay and the inputs keep theirs.
+ * Slots behind the tokens that stay are left as they were.  new_lengths int32 [b] (may be lengths). */
+int64_t lrqk_evict_workspace(int b, int heads, int cap, int budget);
+int lrqk_evict(float* weights, int32_t* ids, void* k, void* v, const int32_t* lengths, int cap, float* weights_out,
+               int32_t* ids_out, void* k_out, void* v_out, int cap_out, int32_t* new_lengths, int b, int heads, int d, int budget,
+               int recent, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
 
 /* py:803-839 cast_lrqk_decode -> py:529-628 _lrqk_decode_inv_w1 + py:651-665 -- the per-step
  * factor update.  b_q,b_k: [bh][r][d] storage dtype, updated in place.  The active A_K rows

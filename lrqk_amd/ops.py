@@ -508,6 +508,270 @@ def decode_step(ws: Workspace, b_q, b_k, a_k, active_idx, k_act, v_act, kv_store
         k_hat.data_ptr(), _ptr(attn_out), _ptr(evict), _ptr(miss_count), _dt(b_q), _stream(b_q)))
 
 
+# --------------------------------------------------------------------------- drafted tokens and budgets
+# These calls take no workspace object: their scratch comes from torch for the call's stream, so that several streams and
+# captured graphs need not share any.
+
+def _launch(t: torch.Tensor, fn, *args) -> int:
+    """The library call on t's device and its current stream."""
+    if torch.cuda.current_device() == t.get_device():
+        return check(fn(*args, _stream(t)))
+    with torch.cuda.device(t.device):
+        return check(fn(*args, _stream(t)))
+
+
+def _on_one_gpu(first: torch.Tensor, *ts):
+    _need_cuda(first, *ts)
+    for t in ts:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+
+
+def _expect(name: str, t: torch.Tensor, shape, dtype, contiguous: bool = True):
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype}: {tuple(shape)} {dtype} is wanted")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _row_strides(name: str, t: torch.Tensor):
+    """Strides of a cache [b,H,n,d] whose rows are contiguous."""
+    s = t.stride()
+    if t.shape[3] > 1 and s[3] != 1:
+        raise ValueError(f"the rows of {name} must be contiguous")
+    return s[0], s[1], s[2]
+
+
+def _lengths(lengths: Optional[torch.Tensor], b: int):
+    if lengths is not None:
+        _expect("lengths", lengths, (b,), torch.int32)
+
+
+class RotaryPlan:
+    """The angles per position of rotary embeddings over the first ``rotary_dim`` elements of a head, on ``device``.
+
+    ``scaling``: None, or a dict for contexts longer than the trained one, with ``type`` and ``factor``:
+      linear   angles divided by the factor
+      ntk      theta stretched by factor ** (rotary_dim / (rotary_dim - 2))
+      llama3   by their turns over ``original_context``: divided below ``low_freq_factor``, kept above ``high_freq_factor``
+      yarn     kept for the pairs that turn more than ``beta_fast`` times over ``original_context``, divided for those that
+               turn less than ``beta_slow`` times, a ramp in between; the results are multiplied by ``attention_factor``
+               (0.1 ln(factor) + 1 if it is not given)
+    ``interleaved``: pairs are elements 2 i and 2 i + 1, else i and i + rotary_dim / 2.  ``inv_freq``: fp64 on the device."""
+
+    _KEYS = {"linear": (), "ntk": (), "llama3": ("low_freq_factor", "high_freq_factor", "original_context"),
+             "yarn": ("beta_fast", "beta_slow", "original_context")}
+
+    def __init__(self, rotary_dim: int, theta: float = 10000.0, interleaved: bool = False, scaling: Optional[dict] = None,
+                 device="cuda:0"):
+        kind, s = "plain", dict(scaling or {})
+        if scaling is not None:
+            kind = s.pop("type", None)
+            if kind not in self._KEYS:
+                raise ValueError(f"unknown scaling {kind!r}: one of {sorted(self._KEYS)}")
+        attention_factor = s.pop("attention_factor", None) if kind == "yarn" else None
+        if kind == "yarn":
+            s = {"beta_fast": 32.0, "beta_slow": 1.0, **s}
+        wanted = ("factor",) + self._KEYS[kind] if kind != "plain" else ()
+        if set(s) != set(wanted):
+            raise ValueError(f"scaling {kind!r} takes {sorted(wanted)}, got {sorted(s)}")
+        p0, p1 = (float(s[k]) for k in self._KEYS[kind][:2]) if len(wanted) > 1 else (0.0, 0.0)
+        freq = torch.empty(max(rotary_dim // 2, 1), dtype=torch.float64)
+        result = ctypes.c_double()
+        check(_lib.load().lrqk_rotary_frequencies(rotary_dim, float(theta), _lib.ROPE[kind], float(s.get("factor", 1.0)), p0, p1,
+                                                  float(s.get("original_context", 0.0)), freq.data_ptr(), ctypes.byref(result)))
+        self.rotary_dim = rotary_dim
+        self.interleaved = bool(interleaved)
+        self.factor = result.value if attention_factor is None else float(attention_factor)
+        self.inv_freq = freq.to(device)
+
+
+def _same_view(x: torch.Tensor, y: torch.Tensor) -> bool:
+    return x.data_ptr() == y.data_ptr() and x.shape == y.shape and x.stride() == y.stride()
+
+
+def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether one of the two ends before the other begins."""
+    def end(t):
+        return t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    return x.numel() == 0 or y.numel() == 0 or end(x) <= y.data_ptr() or end(y) <= x.data_ptr()
+
+
+def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positions, transpose: bool = False, out=None):
+    """q [b,Hq,s,d] and k [b,Hk,s,d] (or None) turned to ``positions``: int32 [s] or [b,s] on the GPU, or the first one of
+    s that follow each other.  Any strides, rows contiguous.  ``out``: (q', k') to write to, each of them any view that is
+    its input or apart from both inputs; else new contiguous tensors.  ``transpose`` turns back: the gradient of the turn.
+    Returns (q', k'), or q' without a k."""
+    pos = positions if isinstance(positions, torch.Tensor) else None
+    _on_one_gpu(q, k, pos, plan.inv_freq)
+    b, hq, s, d = q.shape
+    hk = 0 if k is None else k.shape[1]
+    xs = (q,) if k is None else (q, k)
+    if k is not None and (tuple(k.shape) != (b, hk, s, d) or k.dtype != q.dtype):
+        raise ValueError(f"k is {tuple(k.shape)} {k.dtype} beside q {tuple(q.shape)} {q.dtype}")
+    if plan.rotary_dim > d:
+        raise ValueError(f"a plan of {plan.rotary_dim} elements for heads of {d}")
+    dt = _dt(q)
+    pos_stride, first = 0, 0
+    if pos is None:
+        first = int(positions)
+        if not -2 ** 31 <= first <= first + max(s - 1, 0) < 2 ** 31:
+            raise ValueError(f"positions {first} .. beyond 32 bits")
+    else:
+        _expect("positions", pos, (b, s) if pos.dim() == 2 else (s,), torch.int32, contiguous=False)
+        if s > 1 and pos.stride(-1) != 1:
+            raise ValueError("positions of a sequence must be contiguous")
+        pos_stride = pos.stride(0) if pos.dim() == 2 else 0
+    if out is None:
+        ys = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
+    else:
+        ys = tuple(out)[:len(xs)] if isinstance(out, (tuple, list)) else (out,)
+        if len(ys) != len(xs) or any(y is None for y in ys):
+            raise ValueError("out holds one tensor for q, and one for k if there is a k")
+        _on_one_gpu(q, *ys)
+        for x, y in zip(xs, ys):
+            _expect("out", y, x.shape, x.dtype, contiguous=False)
+            if any(n > 1 and st == 0 for n, st in zip(y.shape, y.stride())):
+                raise ValueError("out has several elements in one place")
+            if not _same_view(x, y) and not all(_apart(y, z) for z in xs):
+                raise ValueError("out overlaps an input and is not the view that is turned")
+    strides = []
+    for x, y in zip(xs, ys):
+        strides += [*_row_strides("q, k", x), *_row_strides("out", y)]
+    if b * s > 0:
+        _launch(q, _lib.load().lrqk_rotary, q.data_ptr(), _ptr(k), ys[0].data_ptr(), ys[1].data_ptr() if hk else None,
+                (ctypes.c_int64 * len(strides))(*strides), _ptr(pos), pos_stride, first, plan.inv_freq.data_ptr(), plan.factor,
+                b, hq, hk, s, d, plan.rotary_dim, int(plan.interleaved), int(transpose), dt)
+    return ys if k is not None else ys[0]
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
+                   mask: torch.Tensor, lengths: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                   return_lse: bool = False):
+    """Attention of t drafted tokens over the cached ones and over each other.
+
+    q [b,Hq,t,d]; k_cache, v_cache [b,Hc,n,d], of which sequence i has ``lengths[i]`` tokens (int32 [b] on the GPU; all n if
+    None), any strides that both share, rows contiguous; k_new, v_new [b,Hn,t,d] of the drafted tokens; mask bool or uint8
+    [t,t] or [b,t,t]: drafted token i sees j.  Hc = Hn for a dense cache, Hc = Hq for an active set (``engine.Kgpu``).
+    ``scale`` (1 / sqrt(d) if None) is positive.  -> [b,Hq,t,d], zeros for a token that sees nothing; with ``return_lse``
+    also fp32 [b,Hq,t], the logarithm of the sum of the exponentials (-inf for such a token)."""
+    _on_one_gpu(q, k_cache, v_cache, k_new, v_new, mask, lengths)
+    b, hq, t, d = q.shape
+    hc, n, hn = k_cache.shape[1], k_cache.shape[2], k_new.shape[1]
+    dt = _dt(q)
+    _expect("k_cache", k_cache, (b, hc, n, d), q.dtype, contiguous=False)
+    _expect("v_cache", v_cache, (b, hc, n, d), q.dtype, contiguous=False)
+    _expect("k_new", k_new, (b, hn, t, d), q.dtype, contiguous=False)
+    _expect("v_new", v_new, (b, hn, t, d), q.dtype, contiguous=False)
+    if hc == 0 or hn == 0 or hq % hc or hc % hn:
+        raise ValueError(f"{hq} query heads, {hc} heads of the cache, {hn} of the drafted tokens: each a multiple of the next")
+    if tuple(mask.shape) not in ((t, t), (b, t, t)) or mask.dtype not in (torch.bool, torch.uint8):
+        raise ValueError(f"mask is {tuple(mask.shape)} {mask.dtype}: bool or uint8 [t,t] or [b,t,t] is wanted")
+    _lengths(lengths, b)
+    st = _row_strides("k_cache", k_cache)
+    if _row_strides("v_cache", v_cache) != st and n > 0:
+        raise ValueError("k_cache and v_cache must have the same strides")
+    out = torch.empty((b, hq, t, d), dtype=q.dtype, device=q.device)
+    lse = torch.empty((b, hq, t), dtype=torch.float32, device=q.device) if return_lse else None
+    if b * hq * t:
+        lib = _lib.load()
+        q, k_new, v_new, mask = q.contiguous(), k_new.contiguous(), v_new.contiguous(), mask.contiguous()
+        need = check(lib.lrqk_tree_attention_workspace(b, hq, hc, t, n, d, dt))
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _launch(q, lib.lrqk_tree_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *st, n, _ptr(lengths),
+                k_new.data_ptr(), v_new.data_ptr(), mask.data_ptr(), t * t if mask.dim() == 3 else 0, out.data_ptr(), _ptr(lse), b,
+                hq, hc, hn, t, d, d ** -0.5 if scale is None else float(scale), ws.data_ptr(), need, dt)
+    return (out, lse) if return_lse else out
+
+
+def attention_weights(q: torch.Tensor, k: torch.Tensor, lengths: Optional[torch.Tensor] = None,
+                      lse: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                      weights: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """What attention every cached token got from the last t tokens of its sequence, added to ``weights``.
+
+    q [b,Hq,t,d] of those tokens; k [b,Hc,n,d], of which sequence i has ``lengths[i]`` tokens (n if None), any strides, rows
+    contiguous; a token sees those up to itself.  lse fp32 [b,Hq,t]: the logarithms of its sums that the attention left
+    (``tree_attention(return_lse=True)``; a query of -inf adds nothing); without it they are formed here.  -> fp32 [b,Hc,n]:
+    ``weights`` (0 if None) plus the sums over the query heads of each head and over the tokens, in ``out`` if that is given,
+    else in place if there are weights."""
+    _on_one_gpu(q, k, lengths, lse, weights, out)
+    b, hq, t, d = q.shape
+    hc, n = k.shape[1], k.shape[2]
+    dt = _dt(q)
+    _expect("k", k, (b, hc, n, d), q.dtype, contiguous=False)
+    if hc == 0 or hq % hc:
+        raise ValueError(f"{hq} query heads over {hc} heads of the cache")
+    _lengths(lengths, b)
+    if lse is not None:
+        _expect("lse", lse, (b, hq, t), torch.float32)
+    if weights is not None:
+        _expect("weights", weights, (b, hc, n), torch.float32)
+    if out is None:
+        out = weights if weights is not None else torch.empty((b, hc, n), dtype=torch.float32, device=q.device)
+    else:
+        _expect("out", out, (b, hc, n), torch.float32)
+        if weights is not None and not _same_view(out, weights) and not _apart(out, weights):
+            raise ValueError("out overlaps weights")
+    if out.numel() == 0:
+        return out
+    if t == 0:
+        return out.copy_(weights) if weights is not None else out.zero_()
+    lib = _lib.load()
+    q = q.contiguous()
+    need = check(lib.lrqk_attention_weights_workspace(b, hq, hc, t, n, d, int(lse is not None), dt))
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _launch(q, lib.lrqk_attention_weights, q.data_ptr(), k.data_ptr(), *_row_strides("k", k), n, _ptr(lengths), _ptr(lse),
+            _ptr(weights), out.data_ptr(), b, hq, hc, t, d, d ** -0.5 if scale is None else float(scale), _ptr(ws), need, dt)
+    return out
+
+
+def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tensor],
+          budget: int, recent: int, out=None) -> torch.Tensor:
+    """Brings a cache down to ``budget`` tokens a head by what attention they got.
+
+    weights fp32 and ids int32 [b,H,n] (the position of every slot's token), k, v [b,H,n,d], of which sequence i has
+    ``lengths[i]`` tokens (int32 [b]; n if None).  The tokens whose ids are within ``recent`` of their head's largest one
+    stay, and of the others those with the largest weights (equal ones: of the lowest slots).  A token that stays keeps its
+    slot if that is one of the first ``budget``; the others move, in order, into the slots that became free.  In place, or
+    into ``out`` = (weights, ids, k, v), buffers of at least min(budget, n) slots that are apart from the inputs; slots behind
+    the tokens that stay are left as they were.  -> the new lengths, int32 [b]."""
+    _on_one_gpu(weights, ids, k, v, lengths, *(out or ()))
+    b, h, n, d = k.shape
+    dt = _dt(k)
+    _expect("weights", weights, (b, h, n), torch.float32)
+    _expect("ids", ids, (b, h, n), torch.int32)
+    _expect("k", k, (b, h, n, d), k.dtype)
+    _expect("v", v, (b, h, n, d), k.dtype)
+    _lengths(lengths, b)
+    budget, recent, cap_out = int(budget), int(recent), n
+    if budget < 1 or not 0 <= recent <= budget:
+        raise ValueError(f"budget={budget}, recent={recent}: 0 <= recent <= budget and at least one token are wanted")
+    ptrs = (None,) * 4
+    if out is not None:
+        if len(out) != 4 or out[2].dim() != 4:
+            raise ValueError("out holds weights, ids, k and v")
+        cap_out = out[2].shape[2]
+        for name, y, shape, dtype in zip(("weights", "ids", "k", "v"), out, ((b, h, cap_out),) * 2 + ((b, h, cap_out, d),) * 2,
+                                         (torch.float32, torch.int32, k.dtype, k.dtype)):
+            _expect("out " + name, y, shape, dtype)
+        if cap_out < min(budget, n):
+            raise ValueError(f"out has {cap_out} slots for min(budget={budget}, {n}) tokens")
+        if not all(_apart(x, y) for x in (weights, ids, k, v) for y in out):
+            raise ValueError("out overlaps an input: leave it out to evict in place")
+        ptrs = tuple(y.data_ptr() for y in out)
+    new = torch.empty((b,), dtype=torch.int32, device=k.device)
+    if b * h * n == 0:
+        return new.zero_()
+    lib = _lib.load()
+    budget = min(budget, 2 ** 30)
+    recent = min(recent, budget)
+    need = check(lib.lrqk_evict_workspace(b, h, n, budget))
+    ws = torch.empty(need, dtype=torch.uint8, device=k.device)
+    _launch(k, lib.lrqk_evict, weights.data_ptr(), ids.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths), n, *ptrs, cap_out,
+            new.data_ptr(), b, h, d, budget, recent, ws.data_ptr(), need, dt)
+    return new
+
+
 def probe_bandwidth(nbytes: int, reps: int = 10, device="cuda:0"):
     """(read GB/s, copy GB/s of bytes read + bytes written) of plain streaming kernels over ``nbytes``."""
     src = torch.empty(nbytes, dtype=torch.uint8, device=device).fill_(1)

@@ -1,0 +1,602 @@
+"""The operators around a drafted, budgeted cache against plain implementations in 64 bits: rotary positions, attention of a
+tree of drafted tokens, the attention that cached tokens got, and eviction by it.
+
+Tolerances count roundings: an output's own (half a step: 2^-8 of a bf16 value, 2^-24 of an fp32 one) and those of the
+arithmetic, in units of U = 2^-23 (an fp32 addition on the matrix cores need not round to nearest, so a whole step each)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+U = 2.0 ** -23
+BF, FP = torch.bfloat16, torch.float32
+HALF = {BF: 2.0 ** -8, FP: 2.0 ** -24}
+NAN, INF = float("nan"), float("inf")
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    from lrqk_amd import ops as o
+    return o
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _randn(g, *shape, dtype=FP, scale=1.0):
+    return (torch.randn(shape, generator=g) * scale).to(dtype).to(DEV)
+
+
+def _within(got, exact, tol, what=""):
+    """got against exact (fp64) elementwise; where exact is not finite the same value is wanted."""
+    got = got.double()
+    fine = torch.isfinite(exact)
+    assert torch.equal(torch.isnan(got), torch.isnan(exact)), what
+    assert torch.equal(got[~fine & ~torch.isnan(exact)], exact[~fine & ~torch.isnan(exact)]), what
+    off = ((got - exact).abs() / tol.clamp(min=1e-300))[fine]
+    off = torch.where((got - exact).abs()[fine] == 0, torch.zeros_like(off), off)
+    assert off.numel() == 0 or float(off.max()) <= 1.0, (what, float(off.max()))
+
+
+# ------------------------------------------------------------------------------------------------------------- rotary
+
+SCALINGS = [None, {"type": "linear", "factor": 4.0}, {"type": "ntk", "factor": 2.5},
+            {"type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0, "original_context": 8192},
+            {"type": "yarn", "factor": 4.0, "original_context": 4096}]
+
+
+def _pairs(dim, interleaved):
+    i = torch.arange(dim // 2, device=DEV)
+    return (2 * i, 2 * i + 1) if interleaved else (i, i + dim // 2)
+
+
+def _rotary64(plan, x, pos, transpose=False):
+    """(turned, bound of the fp32 arithmetic's error)"""
+    y = x.double().clone(memory_format=torch.contiguous_format)
+    a = pos.double()[..., None] * plan.inv_freq
+    a = a[:, None] if pos.dim() == 2 else a
+    c, s = torch.cos(a) * plan.factor, torch.sin(a) * plan.factor * (-1 if transpose else 1)
+    i, j = _pairs(plan.rotary_dim, plan.interleaved)
+    u, v = y[..., i], y[..., j]
+    y[..., i], y[..., j] = u * c - v * s, v * c + u * s
+    # the reduced angle (up to pi) rounded to 2^-24, sine and cosine to 2 of their units, factor, product and sum
+    tol = torch.zeros_like(y)
+    tol[..., i] = tol[..., j] = 8 * 2.0 ** -24 * plan.factor * (u.abs() + v.abs())
+    return y, tol
+
+
+def _check_rotary(plan, x, y, pos, transpose=False, what=""):
+    exact, tol = _rotary64(plan, x, pos, transpose)
+    _within(y, exact, tol + HALF[x.dtype] * exact.abs(), what)
+    assert torch.equal(y[..., plan.rotary_dim:], x[..., plan.rotary_dim:])
+
+
+@pytest.mark.parametrize("scaling", SCALINGS, ids=lambda s: s["type"] if s else "plain")
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_rotary_turns_as_in_64_bits(ops, dtype, interleaved, scaling):
+    print("rotary", dtype, interleaved, scaling, flush=True)
+    g = _gen(1)
+    plan = ops.RotaryPlan(128, 5e5, interleaved, scaling, DEV)
+    q, k = (_randn(g, 2, 37, h, 128, dtype=dtype).transpose(1, 2) for h in (8, 2))
+    pos = torch.randint(0, 131072, (2, 37), generator=g, dtype=torch.int32).to(DEV)
+    a, b = ops.rotary(plan, q, k, pos)
+    assert a.is_contiguous() and b.is_contiguous()
+    _check_rotary(plan, q, a, pos)
+    _check_rotary(plan, k, b, pos)
+    a, b = ops.rotary(plan, q, k, pos, transpose=True)
+    _check_rotary(plan, q, a, pos, True)
+    _check_rotary(plan, k, b, pos, True)
+
+
+@pytest.mark.parametrize("d,rd", [(2, 2), (8, 4), (64, 64), (64, 32), (80, 80), (96, 64), (100, 36), (128, 96), (256, 256), (320, 256)])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_rotary_head_widths(ops, dtype, d, rd):
+    print("rotary width", dtype, d, rd, flush=True)
+    g = _gen(d + rd)
+    for interleaved in (False, True):
+        plan = ops.RotaryPlan(rd, 1e4, interleaved, None, DEV)
+        for b, h, s in ((1, 1, 1), (3, 5, 17), (1, 40, 33)):
+            q = _randn(g, b, h, s, d, dtype=dtype)
+            pos = torch.arange(1000, 1000 + s, dtype=torch.int32, device=DEV)
+            y = ops.rotary(plan, q, None, pos)
+            _check_rotary(plan, q, y, pos, what=(b, h, s, interleaved))
+            assert torch.equal(y, ops.rotary(plan, q, None, 1000))
+
+
+def test_rotary_places_and_strides(ops):
+    """In place, into a view of a cache, from a fused projection, rows that are not 16-byte aligned, positions shared and
+    far, and nothing at all."""
+    print("rotary places", flush=True)
+    g = _gen(3)
+    plan = ops.RotaryPlan(64, 1e4, False, None, DEV)
+    for dtype in (BF, FP):
+        qkv = _randn(g, 2, 9, 6 + 2 + 2, 64, dtype=dtype)
+        q, k = qkv[:, :, :6].transpose(1, 2), qkv[:, :, 6:8].transpose(1, 2)
+        pos = torch.tensor([0, 1, 2, 7, -5, 2 ** 31 - 1, 4, -2 ** 31, 100], dtype=torch.int32, device=DEV)
+        wide = _randn(g, 2, 2, 20, 64, dtype=dtype)
+        kept = wide.clone()
+        a, b = ops.rotary(plan, q, k, pos)
+        _check_rotary(plan, q, a, pos)
+        c, into = ops.rotary(plan, q, k, pos, out=(torch.empty_like(a), wide[:, :, 5:14]))
+        assert torch.equal(c, a) and torch.equal(into, b)
+        assert torch.equal(wide[:, :, 5:14], b)
+        wide[:, :, 5:14] = kept[:, :, 5:14]
+        assert torch.equal(wide, kept)          # nothing beside the view was written
+        before = qkv.clone()
+        ops.rotary(plan, q, k, pos, out=(q, k))  # in place
+        assert torch.equal(q, a) and torch.equal(k, b) and torch.equal(qkv[:, :, 8:], before[:, :, 8:])
+        # rows that begin two or four bytes into a piece
+        odd = _randn(g, 2 * 3 * 5 * 65 + 1, dtype=dtype)[1:].view(2, 3, 5, 65)[..., :64]
+        y = ops.rotary(plan, odd, None, torch.arange(5, dtype=torch.int32, device=DEV))
+        _check_rotary(plan, odd, y, torch.arange(5, dtype=torch.int32, device=DEV))
+        same = pos[None].expand(2, 9)            # one row for all sequences
+        assert torch.equal(ops.rotary(plan, q, None, same), ops.rotary(plan, q, None, pos))
+        assert ops.rotary(plan, q[:, :, :0], None, 5).shape == (2, 6, 0, 64)
+    # a turn and its transpose give back f^2 x
+    plan = ops.RotaryPlan(64, 1e4, True, {"type": "yarn", "factor": 8.0, "original_context": 100, "attention_factor": 0.5}, DEV)
+    x = _randn(g, 1, 3, 50, 64)
+    back = ops.rotary(plan, ops.rotary(plan, x, None, 77), None, 77, transpose=True)
+    # (each turn within 8 units of |u| + |v| <= 2 max|x|)
+    assert float((back.double() - 0.25 * x.double()).abs().max()) <= 2 * 0.25 * 16 * 2.0 ** -24 * 2 * float(x.abs().max())
+
+
+def test_rotary_transpose_is_the_gradient(ops):
+    """<turn(x), w> = <x, turn^T(w)>, against the formula and against differences of it (the turn is linear, so a
+    difference over any step is the derivative)."""
+    print("rotary gradient", flush=True)
+    g = _gen(4)
+    for interleaved in (False, True):
+        plan = ops.RotaryPlan(32, 1e4, interleaved, {"type": "yarn", "factor": 4.0, "original_context": 64}, DEV)
+        x, w = _randn(g, 1, 2, 7, 48), _randn(g, 1, 2, 7, 48)
+        grad = ops.rotary(plan, w, None, 90, transpose=True)
+        y = x.double().requires_grad_()
+        a = (90 + torch.arange(7, device=DEV)).double()[:, None] * plan.inv_freq
+        i, j = _pairs(32, interleaved)
+        u, v = y[..., i], y[..., j]
+        c, s = torch.cos(a) * plan.factor, torch.sin(a) * plan.factor
+        value = ((u * c - v * s) * w.double()[..., i]).sum() + ((v * c + u * s) * w.double()[..., j]).sum() + (y * w.double())[..., 32:].sum()
+        value.backward()
+        bound = 8 * 2.0 ** -24 * plan.factor * 2 * float(w.abs().max()) + 2.0 ** -24 * float(y.grad.abs().max())
+        assert float((grad.double() - y.grad).abs().max()) <= bound
+        step = torch.zeros_like(x)
+        step[0, 1, 3, 5] = 1.0
+        moved = ((ops.rotary(plan, x + step, None, 90).double() - ops.rotary(plan, x, None, 90).double()) * w.double()).sum()
+        # x + step and both turns are rounded: three times 8 units of two elements around 4, times w
+        assert abs(float(moved - grad.double()[0, 1, 3, 5])) <= 3 * 8 * 2.0 ** -24 * 2 * 10 * plan.factor * float(w.abs().max())
+
+
+def test_rotary_refusals(ops):
+    plan = ops.RotaryPlan(64, 1e4, False, None, DEV)
+    q, k = torch.zeros(2, 4, 3, 64, device=DEV), torch.zeros(2, 2, 3, 64, device=DEV)
+    pos = torch.zeros(3, dtype=torch.int32, device=DEV)
+    for bad in (lambda: ops.rotary(plan, q.half(), None, pos), lambda: ops.rotary(plan, q.cpu(), None, pos),
+                lambda: ops.rotary(plan, q, k.bfloat16(), pos), lambda: ops.rotary(plan, q, k[:, :, :2], pos),
+                lambda: ops.rotary(plan, q[..., :32], None, pos), lambda: ops.rotary(plan, q, k, pos.long()),
+                lambda: ops.rotary(plan, q, k, pos[:2]), lambda: ops.rotary(plan, q, k, 2 ** 31 - 2),
+                lambda: ops.rotary(plan, q.transpose(2, 3).contiguous().transpose(2, 3), None, pos),
+                lambda: ops.rotary(plan, q, k, pos, out=(q,)), lambda: ops.rotary(plan, q, k, pos, out=(q, k.bfloat16())),
+                lambda: ops.rotary(plan, q[:, 1:], None, pos, out=q[:, :3]),
+                lambda: ops.rotary(plan, q, None, pos, out=torch.zeros(1, 1, 1, 64, device=DEV).expand(2, 4, 3, 64)),
+                lambda: ops.rotary(plan, q, k, torch.zeros(6, dtype=torch.int32, device=DEV)[::2])):
+        with pytest.raises(ValueError):
+            bad()
+
+
+# --------------------------------------------------------------------------------------------------- tree attention
+
+def _tree64(q, kc, vc, kn, vn, mask, lengths, scale):
+    """(out, lse, tolerance of out, of lse) in fp64.  Where a masked token or one behind the length holds something that is
+    not finite, it is not met."""
+    b, hq, t, d = q.shape
+    hc, hn = kc.shape[1], kn.shape[1]
+    out = torch.zeros((b, hq, t, d), dtype=torch.float64, device=q.device)
+    lse = torch.full((b, hq, t), -INF, dtype=torch.float64, device=q.device)
+    tol, tol_l = torch.zeros_like(out), torch.zeros_like(lse)
+    mask = mask.bool().expand(b, t, t)
+    for i in range(b):
+        m = kc.shape[2] if lengths is None else min(max(int(lengths[i]), 0), kc.shape[2])
+        sees = torch.cat((torch.ones((t, m), dtype=torch.bool, device=q.device), mask[i]), 1)
+        for h in range(hq):
+            k = torch.cat((kc[i, h * hc // hq, :m], kn[i, h * hn // hq])).double()
+            v = torch.cat((vc[i, h * hc // hq, :m], vn[i, h * hn // hq])).double()
+            x = q[i, h].double()
+            s = torch.where(sees, x @ k.T * scale, -INF)
+            s = torch.where(sees, s, -INF)
+            # products of d elements summed in fp32, the exponent rounded, the exponential 2 units
+            ds = U * ((d + 4) * scale * torch.where(sees, x.abs() @ k.abs().nan_to_num(0, 0, 0).T, 0).amax(-1) + 4)
+            top = s.amax(-1, keepdim=True)
+            top = torch.where(top == -INF, 0.0, top)
+            p = torch.exp(s - top)
+            l = p.sum(-1, keepdim=True)
+            some = l[:, 0] != 0
+            w = torch.where(l > 0, p / l, torch.where(l == 0, 0.0, NAN))
+            odd = ~torch.isfinite(v)
+            o = w @ torch.where(odd, 0.0, v)
+            for j in torch.nonzero(odd.any(-1))[:, 0].tolist():   # (0 times infinity is not met where it is not seen)
+                o = o + torch.where(sees[:, j:j + 1] & odd[j], v[j], 0.0)
+            out[i, h] = o
+            lse[i, h] = torch.where(some, (top + torch.log(l))[:, 0], -INF)
+            # numerator and denominator: the exponents, the sums (m + t addends, joined over waves and splits), and the
+            # 16 bits of a bf16 probability
+            each = 2 * ds + U * (m + t + 64) * 2 + (2.0 ** -16 if q.dtype == BF else 0.0)
+            mag = w.nan_to_num(0) @ torch.where(odd, 0.0, v.abs())
+            tol[i, h] = each[:, None] * mag + HALF[q.dtype] * o.nan_to_num(0, 0, 0).abs()
+            tol_l[i, h] = ds + U * (m + t + 64) + 4 * U * lse[i, h].nan_to_num(0, 0, 0).abs()
+    return out, lse, tol, tol_l
+
+
+def _tree_inputs(seed, dtype, b, hq, hc, hn, t, n, d, density=0.5):
+    g = _gen(seed)
+    q = _randn(g, b, hq, t, d, dtype=dtype, scale=2.5)
+    kc, vc = (_randn(g, b, hc, n, d, dtype=dtype) for _ in range(2))
+    kn, vn = (_randn(g, b, hn, t, d, dtype=dtype) for _ in range(2))
+    mask = (torch.rand((b, t, t), generator=g) < density).to(DEV)
+    return q, kc, vc, kn, vn, mask
+
+
+def _check_tree(ops, q, kc, vc, kn, vn, mask, lengths=None, scale=None, what=""):
+    out, lse = ops.tree_attention(q, kc, vc, kn, vn, mask, lengths, scale, return_lse=True)
+    e, el, tol, tol_l = _tree64(q, kc, vc, kn, vn, mask, lengths, q.shape[-1] ** -0.5 if scale is None else scale)
+    _within(out, e, tol, what)
+    _within(lse, el, tol_l, what)
+    return out, lse
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("t,hq,hc,hn", [(1, 1, 1, 1), (1, 32, 8, 8), (3, 8, 8, 2), (7, 28, 4, 4), (16, 8, 2, 1), (33, 6, 2, 2), (64, 8, 2, 2),
+                                        (100, 7, 1, 1)])
+def test_tree_attention_rows(ops, dtype, t, hq, hc, hn):
+    """One query to hundreds a head, dense caches and one per query head; lengths that end in every part of a tile."""
+    print("tree rows", dtype, t, hq, hc, hn, flush=True)
+    for n in (1, 31, 32, 33, 100, 700):
+        q, kc, vc, kn, vn, mask = _tree_inputs(n + t, dtype, 2, hq, hc, hn, t, n, 128)
+        lengths = torch.tensor([n, n // 2], dtype=torch.int32, device=DEV)
+        _check_tree(ops, q, kc, vc, kn, vn, mask, lengths, what=n)
+
+
+@pytest.mark.parametrize("d", [4, 8, 16, 24, 32, 40, 64, 80, 96, 128, 136, 200, 256])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_tree_attention_head_widths(ops, dtype, d):
+    print("tree width", dtype, d, flush=True)
+    from lrqk_amd import _lib
+    for t, n in ((1, 65), (5, 300), (40, 77)):
+        args = _tree_inputs(d + t, dtype, 1, 4, 2, 2, t, n, d)
+        if d * dtype.itemsize % 16:
+            with pytest.raises(_lib.LrqkError):
+                ops.tree_attention(*args)
+            continue
+        _check_tree(ops, *args, what=(t, n))
+
+
+def test_tree_attention_long_cache_and_splits(ops):
+    print("tree long", flush=True)
+    for dtype, b, hq, hc, t, n in ((BF, 1, 8, 2, 1, 20000), (BF, 3, 4, 1, 25, 9001), (FP, 1, 8, 2, 9, 5003), (BF, 2, 16, 16, 4, 2112)):
+        q, kc, vc, kn, vn, mask = _tree_inputs(t, dtype, b, hq, hc, 1, t, n, 128)
+        lengths = torch.tensor([n, 1, n - 33][:b], dtype=torch.int32, device=DEV)
+        a = _check_tree(ops, q, kc, vc, kn, vn, mask, lengths, what=(n, t))
+        z = ops.tree_attention(q, kc, vc, kn, vn, mask, lengths, return_lse=True)
+        assert torch.equal(a[0], z[0]) and torch.equal(a[1], z[1])   # the same bits every time
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_tree_attention_masks(ops, dtype):
+    """Masks of a tree, of nothing, shared by all sequences, of bytes; empty caches; rows that see nothing at all."""
+    print("tree masks", dtype, flush=True)
+    q, kc, vc, kn, vn, _ = _tree_inputs(5, dtype, 3, 4, 2, 2, 13, 50, 64)
+    tree = torch.tril(torch.ones((13, 13), dtype=torch.bool, device=DEV))
+    none = torch.zeros((13, 13), dtype=torch.bool, device=DEV)
+    for lengths in (None, torch.tensor([50, 0, 7], dtype=torch.int32, device=DEV), torch.tensor([0, 0, 0], dtype=torch.int32, device=DEV),
+                    torch.tensor([-3, 1000, 50], dtype=torch.int32, device=DEV)):   # (lengths are cut to the cache)
+        for mask in (tree, none, torch.eye(13, dtype=torch.bool, device=DEV), torch.stack((tree, none, ~tree)),
+                     tree.to(torch.uint8) * 255, tree.T):
+            _check_tree(ops, q, kc, vc, kn, vn, mask, lengths)
+    out, lse = ops.tree_attention(q, kc, vc, kn, vn, none, torch.zeros(3, dtype=torch.int32, device=DEV), return_lse=True)
+    assert not out.any() and bool((lse == -INF).all())
+    _check_tree(ops, q, kc[:, :, :0], vc[:, :, :0], kn, vn, tree)      # no cache at all
+    assert ops.tree_attention(q, kc, vc, kn, vn, tree, scale=0.3).shape == q.shape
+    _check_tree(ops, q, kc, vc, kn, vn, tree, scale=0.3)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_tree_attention_does_not_meet_what_is_masked(ops, dtype):
+    """Infinities and NaN in drafted tokens that a query does not see, and behind the lengths; where it sees them they are
+    in its result."""
+    print("tree poison", dtype, flush=True)
+    for t, hq, hc, d in ((9, 4, 2, 128), (40, 4, 1, 64), (9, 4, 4, 32), (9, 2, 1, 256)):
+        q, kc, vc, kn, vn, _ = _tree_inputs(t, dtype, 2, hq, hc, 1, t, 70, d)
+        lengths = torch.tensor([70, 37], dtype=torch.int32, device=DEV)
+        kc[1, :, 37:], vc[1, :, 37:] = NAN, INF
+        mask = torch.tril(torch.ones((t, t), dtype=torch.bool, device=DEV)).repeat(2, 1, 1)
+        mask[:, :, 3] = False
+        kn[:, :, 3], vn[:, :, 3] = NAN, NAN
+        kn[1, :, 5], mask[1, :, 5] = INF, False
+        out, _ = _check_tree(ops, q, kc, vc, kn, vn, mask, lengths)
+        assert bool(torch.isfinite(out).all())
+        # V of token 6 is seen by the tokens from 6 on
+        vn[0, :, 6, 0], vn[0, :, 6, 1], vn[0, :, 6, 2], vn[0, :, 7, 2], vn[1, :, 6, d - 1] = INF, -INF, INF, -INF, NAN
+        out, _ = _check_tree(ops, q, kc, vc, kn, vn, mask, lengths)
+        assert bool(torch.isfinite(out[:, :, :6]).all()) and bool((out[0, :, 6:, 0] == INF).all())
+        assert bool((out[0, :, 6:, 1] == -INF).all()) and bool(torch.isnan(out[0, :, 7:, 2]).all())
+        assert bool(torch.isnan(out[1, :, 6:, d - 1]).all())
+
+
+def test_tree_attention_places_and_strides(ops):
+    """A cache that is a part of a wider one, the [K|V] store's rows, heads behind each other's rows, a transposed query,
+    and sums that pass 32 bits of elements."""
+    print("tree strides", flush=True)
+    g = _gen(8)
+    q, kc, vc, kn, vn, mask = _tree_inputs(8, BF, 2, 8, 2, 2, 6, 90, 128)
+    ref = ops.tree_attention(q, kc, vc, kn, vn, mask)
+    wide_k, wide_v = (torch.full((2, 2, 200, 128), NAN, dtype=BF, device=DEV) for _ in range(2))
+    wide_k[:, :, 40:130], wide_v[:, :, 40:130] = kc, vc
+    assert torch.equal(ops.tree_attention(q, wide_k[:, :, 40:130], wide_v[:, :, 40:130], kn, vn, mask), ref)
+    store = torch.cat((kc, vc), -1)
+    assert torch.equal(ops.tree_attention(q, store[..., :128], store[..., 128:], kn, vn, mask), ref)
+    by_token = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, kc, vc, kn, vn)]
+    assert torch.equal(ops.tree_attention(*by_token, mask), ref)
+    assert torch.equal(ops.tree_attention(q, kc[:1].expand(2, -1, -1, -1), vc[:1].expand(2, -1, -1, -1), kn, vn, mask)[0], ref[0])
+    # head 1 of a cache begins beyond 2^31 elements, 2^32 bytes
+    big = torch.empty((1, 2, 2 ** 31 // 128 + 8, 128), dtype=BF, device=DEV)
+    big[:, :, -90:] = kc[:1]
+    tail = big[:, :, -90:]
+    out = ops.tree_attention(q[:1], tail, tail, kn[:1], vn[:1], mask[:1])
+    assert torch.equal(out, ops.tree_attention(q[:1], kc[:1], kc[:1], kn[:1], vn[:1], mask[:1]))
+    del big, tail
+    assert ops.tree_attention(q[:, :, :0], kc, vc, kn[:, :, :0], vn[:, :, :0], mask[:, :0, :0]).shape == (2, 8, 0, 128)
+    _randn(g, 1)
+
+
+def test_tree_attention_refusals(ops):
+    from lrqk_amd import _lib
+    q, kc, vc, kn, vn, mask = _tree_inputs(1, BF, 1, 4, 2, 2, 3, 40, 64)
+    for bad in (lambda: ops.tree_attention(q.half(), kc, vc, kn, vn, mask), lambda: ops.tree_attention(q, kc.float(), vc, kn, vn, mask),
+                lambda: ops.tree_attention(q.cpu(), kc, vc, kn, vn, mask), lambda: ops.tree_attention(q, kc, vc, kn, vn, mask.cpu()),
+                lambda: ops.tree_attention(q, kc, vc, kn, vn, mask.float()), lambda: ops.tree_attention(q, kc, vc, kn, vn, mask[:, :2]),
+                lambda: ops.tree_attention(q[:, :3], kc, vc, kn, vn, mask), lambda: ops.tree_attention(q, kc, vc[:, :, :39], kn, vn, mask),
+                lambda: ops.tree_attention(q, kc, vc, kn, vn, mask, scale=0.0), lambda: ops.tree_attention(q, kc, vc, kn, vn, mask, scale=-1.0),
+                lambda: ops.tree_attention(q, kc, vc, kn, vn, mask, scale=NAN), lambda: ops.tree_attention(q, kc, vc, kn[..., :32], vn, mask),
+                lambda: ops.tree_attention(q, kc, vc, kn, vn, mask, torch.zeros(1, device=DEV)),
+                lambda: ops.tree_attention(q, kc, vc, kn, vn, mask, torch.zeros(2, dtype=torch.int32, device=DEV)),
+                lambda: ops.tree_attention(q, kc, vc.transpose(1, 2).contiguous().transpose(1, 2), kn, vn, mask),
+                lambda: ops.tree_attention(q, kc.transpose(2, 3).contiguous().transpose(2, 3), vc, kn, vn, mask),
+                lambda: ops.tree_attention(q, torch.zeros(2 * 40 * 64 + 1, dtype=BF, device=DEV)[1:].view(1, 2, 40, 64), vc, kn, vn, mask)):
+        with pytest.raises(ValueError):
+            bad()
+    z = torch.zeros((1, 1, 1025, 64), dtype=BF, device=DEV)
+    with pytest.raises(_lib.LrqkError):
+        ops.tree_attention(z, z, z, z, z, torch.zeros((1025, 1025), dtype=torch.bool, device=DEV))
+    z = torch.zeros((1, 1, 2, 264), dtype=BF, device=DEV)
+    with pytest.raises(_lib.LrqkError):
+        ops.tree_attention(z, z, z, z, z, torch.zeros((2, 2), dtype=torch.bool, device=DEV))
+
+
+# ------------------------------------------------------------------------------------------------ attention weights
+
+def _weights64(q, k, lengths, lse, scale, weights):
+    """(sums, tolerance) in fp64"""
+    b, hq, t, d = q.shape
+    hc, n = k.shape[1], k.shape[2]
+    out = torch.zeros((b, hc, n), dtype=torch.float64, device=q.device) if weights is None else weights.double()
+    tol = 2.0 ** -24 * out.abs()
+    for i in range(b):
+        m = n if lengths is None else min(max(int(lengths[i]), 0), n)
+        sees = torch.arange(m, device=q.device) <= m - t + torch.arange(t, device=q.device)[:, None]
+        for h in range(hq):
+            x, y = q[i, h].double(), k[i, h * hc // hq, :m].double()
+            s = torch.where(sees, x @ y.T * scale, -INF)
+            ds = U * ((d + 4) * scale * (torch.where(sees, x.abs() @ y.abs().T, 0).amax(-1) if m else 0.0) + 4)
+            own = torch.logsumexp(s, -1) if m else torch.full((t,), -INF, device=q.device, dtype=torch.float64)
+            at = own if lse is None else lse[i, h].double()
+            p = torch.where(sees & (at != -INF)[:, None], torch.exp(s - torch.where(at == -INF, 0.0, at)[:, None]), 0.0)
+            out[i, h * hc // hq, :m] += p.sum(0)
+            # the exponent (scores, and their lse of as many addends where it is formed here), rounded at its magnitude, and the sum
+            big = torch.where(at == -INF, 0.0, at).abs()
+            each = ds + (ds + U * (m + 64) if lse is None else 0.0) + 4 * U * (1 + big)
+            tol[i, h * hc // hq, :m] += (p * each[:, None]).sum(0) + U * (64 + t // 64) * p.sum(0)
+    return out, tol + 2.0 ** -24 * out.abs()
+
+
+def _check_weights(ops, q, k, lengths=None, lse=None, scale=None, weights=None, what=""):
+    w0 = None if weights is None else weights.clone()
+    got = ops.attention_weights(q, k, lengths, lse, scale, weights, out=None if weights is None else torch.empty_like(weights))
+    exact, tol = _weights64(q, k, lengths, lse, q.shape[-1] ** -0.5 if scale is None else scale, w0)
+    _within(got, exact, tol, what)
+    if weights is not None:
+        assert torch.equal(weights, w0)
+        same = ops.attention_weights(q, k, lengths, lse, scale, w0)
+        assert same is w0 and torch.equal(w0, got)     # in place, and the same bits
+    return got
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("t,n", [(1, 1), (1, 70), (2, 2), (15, 40), (16, 64), (17, 17), (33, 500), (100, 100), (257, 257), (300, 900)])
+def test_attention_weights_sizes(ops, dtype, t, n):
+    """Whole prompts and last tokens, with the logarithms of the sums given and formed."""
+    print("weights", dtype, t, n, flush=True)
+    g = _gen(t + n)
+    for hq, hc in ((4, 4), (8, 2), (7, 1)):
+        q, k = _randn(g, 2, hq, t, 128, dtype=dtype, scale=2.0), _randn(g, 2, hc, n, 128, dtype=dtype)
+        total = _check_weights(ops, q, k)
+        # a query's attention adds up to one
+        assert float((total.double().sum((1, 2)) - hq * t).abs().max()) <= hq * t * 1e-3
+        lengths = torch.tensor([n, max(1, n // 2)], dtype=torch.int32, device=DEV)   # (shorter than t: its first queries see nothing)
+        _check_weights(ops, q, k, lengths)
+        lse = _randn(g, 2, hq, t) + 6.0
+        lse[0, 0, 0] = -INF
+        w = torch.rand((2, hc, n), generator=g).to(DEV)
+        _check_weights(ops, q, k, lengths, lse, weights=w)
+        _check_weights(ops, q, k, None, None, 0.2, w)
+
+
+@pytest.mark.parametrize("d", [8, 16, 32, 48, 64, 96, 128, 200, 256])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_attention_weights_head_widths(ops, dtype, d):
+    print("weights width", dtype, d, flush=True)
+    g = _gen(d)
+    for t, n in ((3, 90), (70, 70)):
+        _check_weights(ops, _randn(g, 1, 4, t, d, dtype=dtype), _randn(g, 1, 2, n, d, dtype=dtype), what=(t, n))
+
+
+def test_attention_weights_long_and_strided(ops):
+    print("weights long", flush=True)
+    g = _gen(9)
+    for dtype, t, n in ((BF, 5, 20001), (BF, 1500, 1500), (FP, 40, 4100), (BF, 1, 9000)):
+        _check_weights(ops, _randn(g, 1, 4, t, 128, dtype=dtype, scale=2.0), _randn(g, 1, 2, n, 128, dtype=dtype), what=(t, n))
+    q, store = _randn(g, 2, 4, 6, 64, dtype=BF), _randn(g, 2, 2, 100, 128, dtype=BF)
+    store[:, :, 80:] = NAN     # behind the lengths
+    lengths = torch.tensor([80, 0], dtype=torch.int32, device=DEV)
+    got = ops.attention_weights(q, store[..., :64], lengths)
+    assert torch.equal(got, ops.attention_weights(q, store[..., :64].contiguous(), lengths))
+    assert not got[1].any() and not got[0, :, 80:].any() and bool(torch.isfinite(got).all())
+    # a key that later queries alone see does not spoil the earlier ones' sums
+    q, k = _randn(g, 1, 2, 40, 64), _randn(g, 1, 1, 40, 64)
+    k[:, :, 39] = NAN
+    lse = torch.full((1, 2, 40), 5.0, device=DEV)
+    got = ops.attention_weights(q, k, lse=lse)
+    assert bool(torch.isfinite(got[..., :39]).all()) and bool(torch.isnan(got[..., 39]).all())
+
+
+def test_attention_weights_take_the_attention_lse(ops):
+    """What tree_attention leaves makes the same sums as they are formed here."""
+    print("weights lse", flush=True)
+    q, kc, vc, kn, vn, _ = _tree_inputs(3, BF, 2, 8, 2, 2, 6, 400, 128)
+    tree = torch.tril(torch.ones((6, 6), dtype=torch.bool, device=DEV))
+    lse = ops.tree_attention(q, kc, vc, kn, vn, tree, return_lse=True)[1]
+    k = torch.cat((kc, kn), 2)
+    _check_weights(ops, q, k, None, lse)
+    a, b = ops.attention_weights(q, k), ops.attention_weights(q, k, lse=lse)
+    _, tol = _weights64(q, k, None, None, 128 ** -0.5, None)
+    _within(a, b.double(), 2 * tol)
+
+
+def test_attention_weights_refusals(ops):
+    from lrqk_amd import _lib
+    q, k = torch.zeros(1, 4, 3, 64, device=DEV), torch.zeros(1, 2, 9, 64, device=DEV)
+    w = torch.zeros(1, 2, 9, device=DEV)
+    for bad in (lambda: ops.attention_weights(q.half(), k.half()), lambda: ops.attention_weights(q, k.bfloat16()),
+                lambda: ops.attention_weights(q[:, :3], k), lambda: ops.attention_weights(q, k.cpu()),
+                lambda: ops.attention_weights(q, k, lse=torch.zeros(1, 4, 2, device=DEV)), lambda: ops.attention_weights(q, k, scale=0.0),
+                lambda: ops.attention_weights(q, k, weights=w[..., :8]), lambda: ops.attention_weights(q, k, weights=w.double()),
+                lambda: ops.attention_weights(q, k, out=torch.zeros(1, 2, 18, device=DEV)[..., ::2]),
+                lambda: ops.attention_weights(q, k, weights=torch.zeros(19, device=DEV)[:18].view(1, 2, 9),
+                                              out=torch.zeros(19, device=DEV)[1:].view(1, 2, 9)[..., :8])):
+        with pytest.raises(ValueError):
+            bad()
+    base = torch.zeros(19, device=DEV)
+    with pytest.raises(ValueError):
+        ops.attention_weights(q, k, weights=base[:18].view(1, 2, 9), out=base[1:].view(1, 2, 9))
+    with pytest.raises(_lib.LrqkError):
+        ops.attention_weights(q[..., :3].contiguous(), k[..., :3].contiguous())
+
+
+# ----------------------------------------------------------------------------------------------------------- eviction
+
+def _evict64(weights, ids, lengths, budget, recent):
+    """(lengths, per head the slots whose tokens the first slots get) on the CPU"""
+    b, h, n = weights.shape
+    src, new = {}, []
+    for i in range(b):
+        m = n if lengths is None else min(max(int(lengths[i]), 0), n)
+        keep = min(m, budget)
+        new.append(keep)
+        for j in range(h):
+            w, c = weights[i, j, :m].double().tolist(), ids[i, j, :m].tolist()
+            last = max(c, default=0)
+            new_one = [c[s] > last - recent for s in range(m)]   # (ids that repeat may make them more than the budget: lowest slots)
+            rank = [(0, 0, 0.0, s) if new_one[s] else (1, 0, 0.0, s) if w[s] != w[s] else (2, -w[s], 0.0, s) for s in range(m)]
+            stay = {r[3] for r in sorted(rank)[:keep]}
+            late = iter(sorted(s for s in stay if s >= keep))
+            src[i, j] = [s if s in stay else next(late) for s in range(keep)]
+    return new, src
+
+
+def _check_evict(ops, weights, ids, k, v, lengths, budget, recent, what=""):
+    held = (weights, ids, k, v)
+    new, src = _evict64(weights.cpu(), ids.cpu(), None if lengths is None else lengths.cpu(), budget, recent)
+    want = [x.clone() for x in held]
+    room = min(budget, k.shape[2]) + 3
+    out = [torch.full((*x.shape[:2], room, *x.shape[3:]), 7, dtype=x.dtype, device=DEV) for x in held]
+    want_out = [x.clone() for x in out]
+    for (i, j), s in src.items():
+        s = torch.tensor(s, dtype=torch.int64, device=DEV)
+        for x, y, z in zip(held, want, want_out):
+            y[i, j, :len(s)] = x[i, j][s]
+            z[i, j, :len(s)] = x[i, j][s]
+
+    def same(xs, ys):
+        return all(torch.equal(x.view(torch.int32) if x.dtype == FP else x.view(torch.int16) if x.dtype == BF else x,
+                               y.view(torch.int32) if y.dtype == FP else y.view(torch.int16) if y.dtype == BF else y) for x, y in zip(xs, ys))
+    before = [x.clone() for x in held]
+    got = ops.evict(*held, lengths, budget, recent, out=tuple(out))
+    assert got.dtype == torch.int32 and got.tolist() == new, what
+    assert same(out, want_out), what
+    assert same(held, before), what
+    got = ops.evict(*held, lengths, budget, recent)
+    assert got.tolist() == new and same(held, want), what
+
+
+def _cache(g, b, h, n, d, dtype):
+    return (torch.rand((b, h, n), generator=g).to(DEV), torch.arange(n, dtype=torch.int32).repeat(b, h, 1).to(DEV),
+            _randn(g, b, h, n, d, dtype=dtype), _randn(g, b, h, n, d, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("n,budget,recent", [(1, 1, 0), (1, 1, 1), (2, 1, 1), (5, 8, 2), (64, 64, 8), (65, 64, 8), (100, 10, 10), (300, 1, 0),
+                                             (1000, 999, 0), (1025, 512, 32), (5000, 4096, 64), (9000, 100, 16), (70000, 3000, 7)])
+def test_evict_sizes(ops, dtype, n, budget, recent):
+    print("evict", dtype, n, budget, recent, flush=True)
+    g = _gen(n)
+    for d in (16, 128):
+        _check_evict(ops, *_cache(g, 2, 2, n, d, dtype), torch.tensor([n, max(0, n - n // 3)], dtype=torch.int32, device=DEV), budget, recent)
+    _check_evict(ops, *_cache(g, 1, 3, n, 24, dtype), None, budget, recent)
+
+
+def test_evict_ties_and_odd_values(ops):
+    """Equal weights everywhere, weights of a few values, NaN, infinities, zeros of both signs, negative ones; ids in any
+    order, ids that repeat, all of them new."""
+    print("evict ties", flush=True)
+    g = _gen(2)
+    n = 6000
+    w, ids, k, v = _cache(g, 1, 4, n, 8, BF)
+    lengths = torch.tensor([n - 5], dtype=torch.int32, device=DEV)
+    _check_evict(ops, torch.zeros_like(w), ids, k, v, lengths, 777, 0)
+    _check_evict(ops, torch.ones_like(w), ids, k, v, lengths, 777, 50)
+    _check_evict(ops, (w * 4).floor(), ids, k, v, lengths, 3000, 5)
+    odd = torch.randn((1, 4, n), generator=g).to(DEV)
+    odd[..., ::7], odd[..., 1::7], odd[..., 2::7] = 0.0, -0.0, NAN
+    odd[..., 3::70], odd[..., 4::70] = INF, -INF
+    odd[0, 0, 5::7] = torch.tensor(-NAN)
+    for budget in (100, 860, 2000, 5000):
+        _check_evict(ops, odd.clone(), ids.clone(), k.clone(), v.clone(), lengths, budget, 40, what=budget)
+    mixed = ids.gather(2, torch.rand((1, 4, n), generator=g).argsort(-1).to(DEV)) * 5 - 9000
+    _check_evict(ops, w.clone(), mixed, k.clone(), v.clone(), lengths, 1000, 400)
+    _check_evict(ops, w.clone(), torch.zeros_like(ids), k.clone(), v.clone(), lengths, 1000, 1)
+    _check_evict(ops, w.clone(), torch.full_like(ids, -2 ** 31), k.clone(), v.clone(), lengths, 1000, 1)
+    _check_evict(ops, w.clone(), torch.full_like(ids, 2 ** 31 - 1), k.clone(), v.clone(), lengths, 1000, 0)
+    for odd_length in (0, -4, n + 10, 777, 778):
+        _check_evict(ops, w.clone(), ids.clone(), k.clone(), v.clone(), torch.tensor([odd_length], dtype=torch.int32, device=DEV), 777, 7)
+    _check_evict(ops, w, ids, k, v, lengths, 2 ** 31 - 1, 2 ** 31 - 1)
+
+
+def test_evict_refusals(ops):
+    from lrqk_amd import _lib
+    w, ids, k, v = _cache(_gen(0), 1, 2, 20, 64, BF)
+    n = torch.tensor([20], dtype=torch.int32, device=DEV)
+    out = (torch.zeros(1, 2, 9, device=DEV), torch.zeros(1, 2, 9, dtype=torch.int32, device=DEV), k[:, :, :9].clone(), v[:, :, :9].clone())
+    for bad in (lambda: ops.evict(w, ids, k, v, n, 0, 0), lambda: ops.evict(w, ids, k, v, n, 5, 6), lambda: ops.evict(w, ids, k, v, n, 5, -1),
+                lambda: ops.evict(w.double(), ids, k, v, n, 5, 1), lambda: ops.evict(w, ids.long(), k, v, n, 5, 1),
+                lambda: ops.evict(w, ids, k, v.float(), n, 5, 1), lambda: ops.evict(w, ids, k[:, :, ::2], v[:, :, ::2], n, 5, 1),
+                lambda: ops.evict(w, ids, k.cpu(), v, n, 5, 1), lambda: ops.evict(w, ids, k, v, n.float(), 5, 1),
+                lambda: ops.evict(w, ids, k, v, n, 10, 1, out=out), lambda: ops.evict(w, ids, k, v, n, 9, 1, out=(w, ids, k, v)),
+                lambda: ops.evict(w, ids, k, v, n, 9, 1, out=out[:3]), lambda: ops.evict(w, ids, k.half(), v.half(), n, 5, 1)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(_lib.LrqkError):
+        ops.evict(w, ids, k[..., :5].contiguous(), v[..., :5].contiguous(), n, 5, 1)
