@@ -20,7 +20,8 @@
 namespace lrqk {
 
 constexpr int kAwWaves = 4, kAwThreads = kAwWaves * kWave;
-constexpr float kAwNone = -3.0e38f;
+constexpr float kAwNone = -3.0e38f;    // maximum of no scores
+constexpr float kAwSlack = 8.0f;        // a maximum may be exceeded by 2^8 before a sum is rescaled to the new one
 
 struct WeightArgs {
   const void *q, *k;
@@ -28,11 +29,12 @@ struct WeightArgs {
   const float* lse;        // natural logarithms of the caller's, or those of base 2 of the first pass
   float lse_scale;         // what makes them base 2
   float* lse2;             // first pass: [b][hq][t]
-  float* part;             // first pass: [b][hq][t][parts][2]
+  float* part;             // first pass: [b][hq][t][parts][2]; second pass: [chunks][b][hc][n]
   const float* weights;    // or null
   float* out;
   int64_t kv_b, kv_h, kv_r;
-  int n, hq, hc, t, d, parts, groups, blocks;
+  int n, hq, hc, t, d, parts, groups, chunks;
+  uint32_t heads;           // of the cache, of all sequences
   float scale_log2e;
 };
 
@@ -43,8 +45,10 @@ template <typename T, int DP, int MT>
 __global__ __launch_bounds__(kAwThreads) void weights_rows_kernel(WeightArgs a) {
   constexpr int STEPS = DP * (int)sizeof(T) / 64, NU = 2, KT = 16 * NU;
   const int lane = lane_id(), col = lane & 15, quad = lane >> 4;
-  const int item = (int)blockIdx.x * kAwWaves + __builtin_amdgcn_readfirstlane(wave_id());
-  const int head = (int)blockIdx.y, b = head / a.hc, hc = head % a.hc;
+  // (the heads of a place follow each other: with 8 of them, or a divisor, a head's workgroups are on one XCD, whose L2 holds
+  // its keys)
+  const int item = (int)(blockIdx.x / a.heads) * kAwWaves + __builtin_amdgcn_readfirstlane(wave_id());
+  const int head = (int)(blockIdx.x % a.heads), b = head / a.hc, hc = head % a.hc;
   if (item >= a.groups * a.parts) return;
   const int part = item % a.parts, group = a.groups - 1 - item / a.parts;   // (the longest walks first)
   const int gc = a.hq / a.hc, M = gc * a.t, row0 = group * 16 * MT;
@@ -70,33 +74,55 @@ __global__ __launch_bounds__(kAwThreads) void weights_rows_kernel(WeightArgs a) 
   least = (int)(wave_reduce_u32((uint32_t)least ^ 0x80000000u, [](uint32_t x, uint32_t y) { return min(x, y); }) ^ 0x80000000u);
   const int tiles = (most + KT - 1) / KT, per = (tiles + a.parts - 1) / a.parts;
   const int end = min(tiles, (part + 1) * per);
+  ar_u4 kf[NU][STEPS];
+  auto load = [&](int tile) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) ar_row(k + (int64_t)min(tile * KT + 16 * u + col, most - 1) * a.kv_r, quad, pieces, kf[u]);
+  };
+  if (part * per < end) load(part * per);
   for (int tile = part * per; tile < end; ++tile) {
     const int first = tile * KT;
-    ar_u4 kf[NU][STEPS];
-#pragma unroll
-    for (int u = 0; u < NU; ++u) ar_row(k + (int64_t)min(first + 16 * u + col, most - 1) * a.kv_r, quad, pieces, kf[u]);
     const bool whole = first + KT - 1 <= least;
+    float x[MT][4 * NU];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      float x[4 * NU];
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         ar_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < STEPS; ++c) s = ar_step<T>(kf[u][c], qf[m][c], s);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[4 * u + r] = whole | (first + 16 * u + 4 * quad + r <= last[m]) ? s[r] : -INFINITY;
+        for (int r = 0; r < 4; ++r) x[m][4 * u + r] = s[r];
       }
-      float now = x[0];
+    load(min(tile + 1, end - 1));   // (while the exponentials of this one are formed)
+    if (!whole) {
 #pragma unroll
-      for (int e = 1; e < 4 * NU; ++e) now = fmaxf(now, x[e]);
-      now = fmaxf(top[m], now * a.scale_log2e);
-      float add = 0.0f;
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int e = 0; e < 4 * NU; ++e) add += ar_exp2(fmaf(x[e], a.scale_log2e, -now));
-      sum[m] = fmaf(sum[m], ar_exp2(top[m] - now), add);
-      top[m] = now;
+        for (int e = 0; e < 4 * NU; ++e) x[m][e] = first + 16 * (e >> 2) + 4 * quad + (e & 3) <= last[m] ? x[m][e] : -INFINITY;
     }
+    float high[MT];
+    bool more = false;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      high[m] = x[m][0];
+#pragma unroll
+      for (int e = 1; e < 4 * NU; ++e) high[m] = fmaxf(high[m], x[m][e]);
+      high[m] *= a.scale_log2e;
+      more = more | (high[m] > top[m] + kAwSlack);
+    }
+    if (__ballot(more)) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const float now = fmaxf(top[m], high[m]);
+        sum[m] *= ar_exp2(top[m] - now);
+        top[m] = now;
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int e = 0; e < 4 * NU; ++e) sum[m] += ar_exp2(fmaf(x[m][e], a.scale_log2e, -top[m]));
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -128,24 +154,28 @@ __global__ __launch_bounds__(kAwThreads) void weights_merge_kernel(WeightArgs a,
   if (lane_id() == 0) a.lse2[row] = sum == 0.0f ? -INFINITY : top + log2f(sum);
 }
 
-// 16 NT keys a wave.  SHARE: the four waves of a workgroup have the same keys and take the queries in turn (many
-// queries), else they have keys of their own and all queries.
-template <typename T, int DP, int NT, bool SHARE>
+// 16 NT keys a wave; the waves of a workgroup walk over the same queries, a chunk of them, so that the L1 has what the
+// others read.
+template <typename T, int DP, int NT>
 __global__ __launch_bounds__(kAwThreads) void weights_columns_kernel(WeightArgs a) {
   constexpr int STEPS = DP * (int)sizeof(T) / 64, KEYS = 16 * NT;
-  __shared__ float joint[SHARE ? kAwWaves : 1][KEYS];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), col = lane & 15, quad = lane >> 4;
-  const int head = (int)blockIdx.y, b = head / a.hc, hc = head % a.hc;
-  const int first = ((int)blockIdx.x * (SHARE ? 1 : kAwWaves) + (SHARE ? 0 : wave)) * KEYS;
+  const int head = (int)(blockIdx.x % a.heads), b = head / a.hc, hc = head % a.hc, place = (int)(blockIdx.x / a.heads);
+  const int chunk = place % a.chunks, first = (place / a.chunks * kAwWaves + wave) * KEYS;   // (the most queries first)
+  if (first >= a.n) return;
   const int gc = a.hq / a.hc, M = gc * a.t;
   const int len = weights_len(a, b), behind = len - a.t;
   const T* q = (const T*)a.q + ((int64_t)b * a.hq + (int64_t)hc * gc) * a.t * a.d;
   const T* k = (const T*)a.k + b * a.kv_b + hc * a.kv_h;
   const float* lse = a.lse + (int64_t)head * M;
   const int pieces = a.d * (int)sizeof(T) / 16;
-  float sum[NT], part[NT];
+  const int64_t row = (int64_t)head * a.n + first;
+  float had[NT], sum[NT], part[NT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) sum[j] = part[j] = 0.0f;
+  for (int j = 0; j < NT; ++j) {
+    sum[j] = part[j] = 0.0f;
+    had[j] = a.weights && a.chunks == 1 ? a.weights[row + min(16 * j + col, a.n - 1 - first)] : 0.0f;
+  }
   if (first < len) {
     ar_u4 kf[NT][STEPS];
 #pragma unroll
@@ -155,31 +185,51 @@ __global__ __launch_bounds__(kAwThreads) void weights_columns_kernel(WeightArgs 
     const int t0 = packed ? 0 : max(0, first - behind) / 16;
     const int per = packed ? 1 : (a.t + 15) / 16 - t0;
     const int items = packed ? (M + 15) / 16 : gc * per;
-    int held = 0;
-    for (int item = SHARE ? wave : 0; item < items; item += SHARE ? kAwWaves : 1) {
-      const int g = packed ? 0 : item / per, tt = packed ? item : t0 + item % per;
-      const int base = g * a.t + 16 * tt, stop = packed ? M : (g + 1) * a.t;   // rows of the tile: base .. min(base + 16, stop)
-      ar_u4 qf[STEPS];
+    const int begin = (int)((int64_t)items * chunk / a.chunks), end = (int)((int64_t)items * (chunk + 1) / a.chunks);
+    ar_u4 qf[STEPS];
+    float l2[4];
+    auto load = [&](int g, int tt) {   // rows of the tile: base .. min(base + 16, stop) - 1
+      const int base = g * a.t + 16 * tt, stop = packed ? M : (g + 1) * a.t;
       ar_row(q + (int64_t)min(base + col, stop - 1) * a.d, quad, pieces, qf);
-      float l2[4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        l2[r] = lse[min(base + 4 * quad + r, stop - 1)] * a.lse_scale;
-        l2[r] = l2[r] == -INFINITY ? INFINITY : l2[r];   // (a query that saw nothing gives nothing)
-      }
-      const bool whole = base + 16 <= stop && first + KEYS - 1 <= behind + (packed ? 0 : 16 * tt);
+      for (int r = 0; r < 4; ++r) l2[r] = lse[min(base + 4 * quad + r, stop - 1)];
+    };
+    int g = packed ? 0 : begin / per, tt = packed ? begin : t0 + begin % per, held = 0;
+    if (begin < end) load(g, tt);
+    for (int item = begin; item < end; ++item) {
+      const int base = g * a.t + 16 * tt, stop = packed ? M : (g + 1) * a.t, at = packed ? 0 : 16 * tt;
+      ar_f4 s[NT];
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        ar_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+        s[j] = ar_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < STEPS; ++c) s = ar_step<T>(qf[c], kf[j][c], s);
+        for (int c = 0; c < STEPS; ++c) s[j] = ar_step<T>(qf[c], kf[j][c], s[j]);
+      }
+      float l[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        l[r] = l2[r] * a.lse_scale;
+        l[r] = l[r] == -INFINITY ? INFINITY : l[r];   // (a query that saw nothing gives nothing)
+      }
+      if (item + 1 < end) {   // (the next queries, while the exponentials of these are formed)
+        if (!packed && tt + 1 == t0 + per) {
+          ++g;
+          tt = t0;
+        } else {
+          ++tt;
+        }
+        load(g, tt);
+      }
+      const bool whole = base + 16 <= stop && first + KEYS - 1 <= behind + at;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
         float p[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[r] = ar_exp2(fmaf(s[r], a.scale_log2e, -l2[r]));
+        for (int r = 0; r < 4; ++r) p[r] = ar_exp2(fmaf(s[j][r], a.scale_log2e, -l[r]));
         if (!whole) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int row = base + 4 * quad + r, last = behind + (packed ? row % a.t : 16 * tt + 4 * quad + r);
+            const int row = base + 4 * quad + r, last = behind + (packed ? row % a.t : at + 4 * quad + r);
             const bool sees = (row < stop) & (first + 16 * j + col <= last);
             p[r] = sees ? p[r] : 0.0f;
           }
@@ -196,39 +246,40 @@ __global__ __launch_bounds__(kAwThreads) void weights_columns_kernel(WeightArgs 
       }
     }
   }
+  float* out = a.chunks == 1 ? a.out + row : a.part + (int64_t)chunk * a.heads * a.n + row;
 #pragma unroll
-  for (int j = 0; j < NT; ++j) sum[j] = ar_quad_sum(sum[j] + part[j]);
-  const int64_t row = (int64_t)head * a.n;
-  if constexpr (SHARE) {
-    if (quad == 0) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) joint[wave][16 * j + col] = sum[j];
-    }
-    __syncthreads();
-    const int key = threadIdx.x;
-    if (key < KEYS && first + key < a.n) {
-      float v = (joint[0][key] + joint[1][key]) + (joint[2][key] + joint[3][key]);
-      if (a.weights) v += a.weights[row + first + key];
-      a.out[row + first + key] = v;
-    }
-  } else if (quad == 0) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int key = first + 16 * j + col;
-      if (key < a.n) a.out[row + key] = a.weights ? a.weights[row + key] + sum[j] : sum[j];
-    }
+  for (int j = 0; j < NT; ++j) {
+    sum[j] = ar_quad_sum(sum[j] + part[j]);
+    if (quad == 0 && first + 16 * j + col < a.n) out[16 * j + col] = had[j] + sum[j];
   }
 }
 
+// out = weights + the chunks' sums, in their order.
+__global__ __launch_bounds__(kAwThreads) void weights_sum_kernel(WeightArgs a, int64_t count) {
+  const int64_t i = (int64_t)blockIdx.x * kAwThreads + threadIdx.x;
+  if (i >= count) return;
+  float v = 0.0f;
+#pragma unroll 8
+  for (int c = 0; c < a.chunks; ++c) v += a.part[c * count + i];
+  a.out[i] = a.weights ? a.weights[i] + v : v;
+}
+
 struct WeightPlan {
-  int dp, mt, groups, parts;
+  int dp, mt, groups, parts, nt, chunks;
   int64_t lse2, part;   // floats
 };
 static WeightPlan weights_plan(int b, int hq, int hc, int t, int64_t n, int d, int dtype, bool have_lse) {
   WeightPlan p{};
   p.dp = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256;
-  if (have_lse) return p;
   const int64_t M = (int64_t)(hq / hc) * t, heads = (int64_t)b * hc;
+  const int row = p.dp * (int)elem_size(dtype);
+  p.nt = row <= 256 ? 4 : row <= 512 ? 2 : 1;
+  // two thousand workgroups of keys and chunks of queries (half of a prompt's have little to do), sixteen tiles of queries
+  // for each
+  const int64_t blocks = (n + 16 * p.nt * kAwWaves - 1) / (16 * p.nt * kAwWaves), items = (M + 15) / 16;
+  p.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(2048 / (blocks * heads), items / 16));
+  if (p.chunks > 1) p.part = heads * n * p.chunks;
+  if (have_lse) return p;
   p.mt = M <= 16 || (p.dp == 256 && dtype == LRQK_F32) ? 1 : M <= 32 || p.dp == 256 || (p.dp == 128 && dtype == LRQK_F32) ? 2 : 4;
   p.groups = (int)((M + 16 * p.mt - 1) / (16 * p.mt));
   // two waves per SIMD, each with eight tiles of 32 keys at least
@@ -236,13 +287,13 @@ static WeightPlan weights_plan(int b, int hq, int hc, int t, int64_t n, int d, i
   parts = std::min<int64_t>(parts, (n + 255) / 256);
   p.parts = (int)std::max<int64_t>(1, parts);
   p.lse2 = heads * M;
-  p.part = p.parts > 1 ? heads * M * p.parts * 2 : 0;
+  if (p.parts > 1) p.part = std::max(p.part, heads * M * p.parts * 2);   // (the passes follow each other)
   return p;
 }
 
 template <typename T, int DP>
 static int weights_rows_launch(const WeightArgs& a, const WeightPlan& p, int heads, hipStream_t st) {
-  const dim3 grid((unsigned)(((int64_t)p.groups * p.parts + kAwWaves - 1) / kAwWaves), (unsigned)heads);
+  const dim3 grid((unsigned)(((int64_t)p.groups * p.parts + kAwWaves - 1) / kAwWaves * heads));
   constexpr int MOST = DP * (int)sizeof(T) <= 256 ? 4 : DP * (int)sizeof(T) <= 512 ? 2 : 1;
   if constexpr (MOST >= 4)
     if (p.mt == 4) hipLaunchKernelGGL((weights_rows_kernel<T, DP, 4>), grid, dim3(kAwThreads), 0, st, a);
@@ -265,15 +316,13 @@ static int weights_launch(WeightArgs a, const WeightPlan& p, int heads, hipStrea
     a.lse = a.lse2;
     a.lse_scale = 1.0f;
   }
-  constexpr int NT = DP * (int)sizeof(T) <= 256 ? 4 : DP * (int)sizeof(T) <= 512 ? 2 : 1, KEYS = 16 * NT;
-  const int items = a.t < 16 ? (a.hq / a.hc * a.t + 15) / 16 : a.hq / a.hc * ((a.t + 15) / 16);
-  if (items >= 2 * kAwWaves) {
-    hipLaunchKernelGGL((weights_columns_kernel<T, DP, NT, true>), dim3((unsigned)((a.n + KEYS - 1) / KEYS), (unsigned)heads),
-                       dim3(kAwThreads), 0, st, a);
-  } else {
-    hipLaunchKernelGGL((weights_columns_kernel<T, DP, NT, false>),
-                       dim3((unsigned)((a.n + KEYS * kAwWaves - 1) / (KEYS * kAwWaves)), (unsigned)heads), dim3(kAwThreads), 0, st, a);
-  }
+  constexpr int NT = DP * (int)sizeof(T) <= 256 ? 4 : DP * (int)sizeof(T) <= 512 ? 2 : 1, KEYS = 16 * NT * kAwWaves;
+  hipLaunchKernelGGL((weights_columns_kernel<T, DP, NT>), dim3((unsigned)((int64_t)(a.n + KEYS - 1) / KEYS * p.chunks * heads)),
+                     dim3(kAwThreads), 0, st, a);
+  LRQK_HIP_CHECK(hipGetLastError());
+  if (p.chunks == 1) return LRQK_OK;
+  const int64_t count = (int64_t)heads * a.n;
+  hipLaunchKernelGGL(weights_sum_kernel, dim3((unsigned)((count + kAwThreads - 1) / kAwThreads)), dim3(kAwThreads), 0, st, a, count);
   LRQK_HIP_CHECK(hipGetLastError());
   return LRQK_OK;
 }
@@ -314,7 +363,7 @@ extern "C" int lrqk_attention_weights(const void* q, const void* k, int64_t k_ba
                                       void* stream) {
   int rc = weights_check(b, hq, hc, t, n, d, dtype);
   if (rc) return rc;
-  LRQK_REQUIRE(q && k && out && (lse || workspace), LRQK_EINVAL, "null pointer");
+  LRQK_REQUIRE(q && k && out, LRQK_EINVAL, "null pointer");
   LRQK_REQUIRE(scale > 0.0f && scale < INFINITY, LRQK_EINVAL, "scale=%g has to be positive and finite", (double)scale);
   const int vec = 16 / (int)elem_size(dtype);
   LRQK_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)k % 16 == 0 && (uintptr_t)workspace % 16 == 0 && k_batch_stride % vec == 0 &&
@@ -322,10 +371,14 @@ extern "C" int lrqk_attention_weights(const void* q, const void* k, int64_t k_ba
                LRQK_EINVAL, "pointers and rows must be 16-byte aligned");
   const WeightPlan p = weights_plan(b, hq, hc, t, n, d, dtype, lse != nullptr);
   const int64_t need = (p.lse2 + p.part) * (int64_t)sizeof(float);
-  LRQK_REQUIRE(workspace_bytes >= need, LRQK_EINVAL, "workspace of %lld bytes: %lld are needed", (long long)workspace_bytes,
+  LRQK_REQUIRE(workspace_bytes >= need && (workspace || need == 0), LRQK_EINVAL, "workspace of %lld bytes: %lld are needed", (long long)workspace_bytes,
                (long long)need);
+  // (a launch's workgroups are counted in 31 bits; no memory holds what would need more)
+  const int64_t places = std::max((int64_t)p.groups * std::max(p.parts, 1), (n + 63) / 64 * p.chunks);
+  LRQK_REQUIRE(places * b * hc <= INT32_MAX, LRQK_ELIMIT, "%lld keys of %d heads and %d queries are more than a launch has places for",
+               (long long)n, b * hc, t);
   WeightArgs a{q, k, lengths, lse, kLog2e, (float*)workspace, (float*)workspace + p.lse2, weights, out, k_batch_stride, k_head_stride,
-               k_row_stride, (int)n, hq, hc, t, d, p.parts, p.groups, 0, scale * kLog2e};
+               k_row_stride, (int)n, hq, hc, t, d, p.parts, p.groups, p.chunks, (uint32_t)(b * hc), scale * kLog2e};
   hipStream_t st = (hipStream_t)stream;
   if (dtype == LRQK_F32) return weights_launch_dp<float>(a, p, b * hc, st);
   return weights_launch_dp<bf16_t>(a, p, b * hc, st);
