@@ -287,7 +287,7 @@ int lrqk_rotary(const void* q, const void* k, void* q_out, void* k_out, const in
  * elements, t up to 1024.
  * These calls take no ctx: their scratch is the caller's (lrqk_*_workspace bytes of device memory, 16-byte aligned,
  * contents of no meaning before and after), so that calls on several streams and captured graphs need not share any. */
-int64_t lrqk_tree_attention_workspace(int b, int hq, int hc, int t, int64_t n, int d, int dtype);
+int64_t lrqk_tree_attention_workspace(int b, int hq, int hc, int t, int64_t n, int d, int have_lengths, int dtype);
 int lrqk_tree_attention(const void* q, const void* k_cache, const void* v_cache, int64_t kv_batch_stride, int64_t kv_head_stride,
                         int64_t kv_row_stride, int64_t n, const int32_t* lengths, const void* k_new, const void* v_new,
                         const uint8_t* mask, int64_t mask_batch_stride, void* out, float* lse, int b, int hq, int hc, int hn,

@@ -78,7 +78,7 @@ def _sig(lib):
         "lrqk_rotary_frequencies": ([i32, c.c_double, i32, c.c_double, c.c_double, c.c_double, c.c_double, vp,
                                      c.POINTER(c.c_double)], i32),
         "lrqk_rotary": ([vp, vp, vp, vp, vp, vp, i64, i32, vp, c.c_double, i32, i32, i32, i64, i32, i32, i32, i32, i32, vp], i32),
-        "lrqk_tree_attention_workspace": ([i32, i32, i32, i32, i64, i32, i32], i64),
+        "lrqk_tree_attention_workspace": ([i32, i32, i32, i32, i64, i32, i32, i32], i64),
         "lrqk_tree_attention": ([vp, vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, f32, vp,
                                  i64, i32, vp], i32),
         "lrqk_attention_weights_workspace": ([i32, i32, i32, i32, i64, i32, i32, i32], i64),

@@ -50,6 +50,22 @@ __device__ __forceinline__ void ar_row(const void* row, int quad, int pieces, ar
   }
 }
 
+// Rows on their way from memory to those operands.  Read as operands they would be 64 accesses of 16 bytes per load (the
+// cache joins what adjacent lanes read, and those have different rows: a whole prompt's weights were bound by that, at a
+// third of the speed), so a wave reads whole rows, passes them through LDS and takes the operands from there.  Pieces
+// change places within their row so that the 16 rows of an operand come from 16 different banks.
+template <int CH>   // 16-byte pieces of a row: a power of two from 4 to 64
+__device__ __forceinline__ int ar_place(int row, int piece) {
+  constexpr int SH = CH >= 16 ? 0 : CH == 8 ? 1 : 2, MASK = CH >= 16 ? 15 : CH - 1;
+  return row * CH + (piece ^ ((row >> SH) & MASK));
+}
+
+__device__ __forceinline__ void ar_wave_sync() {  // orders one wave's LDS writes and reads
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Over the four quads of a wave (lanes l, l + 16, l + 32, l + 48), result in all of them.
 __device__ __forceinline__ float ar_quad_max(float v) {
   auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -13,13 +13,14 @@
 // Bf16 V is transposed between those lanes' registers; bf16 probabilities are the sum of two bf16 numbers (16 bits), so
 // that the one rounding to bf16 is the output's.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_rows.hpp"
 
 namespace lrqk {
 
 constexpr int kTrWaves = 4, kTrThreads = kTrWaves * kWave;
-constexpr int kTrCombThreads = 1024;
+constexpr int kTrCombThreads = 512;
 constexpr int kTrMaxSplits = 256;
 constexpr float kTrNone = -3.0e38f;   // running maximum of a query that has seen no key yet
 constexpr float kTrSlack = 8.0f;      // a maximum may be exceeded by 2^8 before the sums are rescaled to the new one
@@ -30,37 +31,45 @@ struct TreeArgs {
   const int32_t* lengths;   // or null: n each
   void* out;
   float* lse;               // or null
-  float *part, *part_ml;
-  int32_t* odd;             // per workgroup: whether its drafted rows of V hold infinities or NaN
+  float *part, *part_ml;    // of 16 queries of a split: VW float4 a lane, and (maximum, sum) of each query
+  int32_t* odd;             // per workgroup of a split: whether its drafted rows of V hold infinities or NaN
   int64_t kv_b, kv_h, kv_r; // elements between sequences, heads and rows of the cache
   int64_t mask_b;
-  int n, hq, hc, hn, t, d, S, row_blocks, units;
+  // splits: of all sequences together, for a cache head; least: tiles of a split, at least; rows: of a row block
+  int b, n, hq, hc, hn, t, d, splits, least, row_blocks, rows, row_tiles, units;
   float scale_log2e;
 };
 
-// One row's part of V for a lane: elements VW i .. of row `row`.
+template <typename V>
+__device__ __forceinline__ V tree_at(const void* base, uint32_t bytes) {   // (an address of the wave's and 32 bits of the lane's)
+  return *reinterpret_cast<const V*>((const char*)base + bytes);
+}
+
+// One row's part of V for a lane: elements VW i .. (of a head's d; what is beyond them is something that is not used).
 template <typename T, int VW>
 struct TreeV {
   static constexpr int DW = VW * (int)sizeof(T) / 4;
   uint32_t w[DW];
-  __device__ __forceinline__ void load(const T* row, int i, int d) {
+  // bytes from the row's beginning to piece p of the lane
+  static __device__ __forceinline__ uint32_t place(int i, int d, int p) {
+    if constexpr (DW >= 4) return 16u * (uint32_t)min(i * (DW / 4) + p, d * (int)sizeof(T) / 16 - 1);
+    return i * DW < d * (int)sizeof(T) / 4 ? 4u * (uint32_t)(i * DW) : 0u;
+  }
+  // (places: the lane's pieces, as above)
+  __device__ __forceinline__ void load(const void* base, uint32_t row, const uint32_t (&places)[DW >= 4 ? DW / 4 : 1]) {
     if constexpr (DW >= 4) {
 #pragma unroll
       for (int p = 0; p < DW / 4; ++p) {
-        const int piece = min(i * (DW / 4) + p, d * (int)sizeof(T) / 16 - 1);
-        const ar_u4 x = ((const ar_u4*)row)[piece];
+        const ar_u4 x = tree_at<ar_u4>(base, row + places[p]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[4 * p + e] = x[e];
       }
+    } else if constexpr (DW == 2) {
+      const ar_u2 x = tree_at<ar_u2>(base, row + places[0]);
+      w[0] = x[0];
+      w[1] = x[1];
     } else {
-      const int at = i * DW < d * (int)sizeof(T) / 4 ? i * DW : 0;   // (beyond the head: something that is not used)
-      if constexpr (DW == 2) {
-        const ar_u2 x = *(const ar_u2*)((const uint32_t*)row + at);
-        w[0] = x[0];
-        w[1] = x[1];
-      } else {
-        w[0] = ((const uint32_t*)row)[at];
-      }
+      w[0] = tree_at<uint32_t>(base, row + places[0]);
     }
   }
 };
@@ -79,13 +88,22 @@ __device__ __forceinline__ bool tree_clean(uint32_t& w) {
   }
 }
 
-// Eight scores of a lane as a bf16 operand.
-__device__ __forceinline__ ar_bf8 tree_pack(const float* p) {
-  ar_bf8 x;
+// Eight probabilities as the sum of two bf16 operands: the upper half of each number, and what that leaves, rounded (16 bits
+// in all).  Cut off rather than rounded, the first takes half the instructions.
+typedef float tr_f8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ void tree_split(const float (&p)[8], ar_bf8& hi, ar_bf8& lo) {
+  ar_u4 h;
+  tr_f8 rest;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = (__bf16)p[e];
-  return x;
+  for (int e = 0; e < 4; ++e) h[e] = __builtin_amdgcn_perm(__float_as_uint(p[2 * e + 1]), __float_as_uint(p[2 * e]), 0x07060302u);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) rest[e] = p[e] - __uint_as_float(__float_as_uint(p[e]) & 0xffff0000u);   // exact
+  hi = __builtin_bit_cast(ar_bf8, h);
+  lo = __builtin_convertvector(rest, ar_bf8);
 }
+
+typedef short tr_v4s __attribute__((ext_vector_type(4)));
+typedef tr_v4s __attribute__((address_space(3))) * tr_lds_v4s;
 
 template <typename T, int DP, int MT>
 struct TreeTile {
@@ -94,19 +112,19 @@ struct TreeTile {
   static constexpr int KT = 16 * NU, NE = 4 * NU;   // keys of a tile, and of a quad in it
   static constexpr int STEPS = DP * (int)sizeof(T) / 64;
   static constexpr int VW = DP / 16;
+  static constexpr int CH = 4 * STEPS;              // 16-byte pieces of a row
+  static constexpr int KL = KT * CH / kWave;        // loads of a wave for the tile's rows of K
+
+  // A row of K is kept in LDS where the operand that has it looks: the 16 rows of block u, row m of them with key
+  // (m / 4) NE + 4 u + m % 4.
+  static __device__ __forceinline__ int place(int key) { return (key % NE) / 4 * 16 + key / NE * 4 + key % 4; }
 
   // o[j] += v_j^T p for the keys of the tile; p[e]: probability of the quad's key e for the lane's query
   static __device__ __forceinline__ void add(const TreeV<T, VW> (&v)[NE], const float (&p)[MT][NE], ar_f4 (&o)[MT][VW]) {
     if constexpr (BF) {
       ar_bf8 hi[MT], lo[MT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        hi[m] = tree_pack(p[m]);
-        float rest[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) rest[e] = p[m][e] - (float)hi[m][e];   // exact
-        lo[m] = tree_pack(rest);
-      }
+      for (int m = 0; m < MT; ++m) tree_split(p[m], hi[m], lo[m]);
 #pragma unroll
       for (int w = 0; w < VW / 2; ++w) {
         ar_u4 a, b;
@@ -136,30 +154,154 @@ struct TreeTile {
   }
 };
 
-// The parts of a workgroup: [unit][row block] MT VW float4 a lane, and (maximum, sum) of 16 MT queries.
+// How the sequences are cut into splits: of equal length, whatever the lengths of the sequences, as many as the grid was
+// made for (every sequence's last one may be shorter, so there are up to b more).  From the lengths alone, by every wave
+// for itself; a split is found by its number among all, or a sequence's splits by the sequence.
+struct TreeCut {
+  int b, len, split, splits, slot0, per;   // splits of the sequence, the number of its first
+  static __device__ __forceinline__ int tiles(const TreeArgs& a, int len, int kt) { return (len + kt - 1) / kt + (a.t + kt - 1) / kt; }
+  static __device__ __forceinline__ int length(const TreeArgs& a, int b) {
+    return a.lengths ? min(max(a.lengths[b], 0), a.n) : a.n;
+  }
+  // tiles of a split (32 bits divide four times as fast as 64)
+  static __device__ __forceinline__ int share(const TreeArgs& a, int64_t all) {
+    const int x = all <= INT32_MAX ? (int)(((uint32_t)all + (uint32_t)a.splits - 1u) / (uint32_t)a.splits) : (int)((all + a.splits - 1) / a.splits);
+    return max(a.least, x);
+  }
+  // slot >= 0: the split of that number (false: there is none); else sequence `seq`
+  __device__ __forceinline__ bool find(const TreeArgs& a, int kt, int slot, int seq) {
+    if (!a.lengths || a.b == 1) {
+      len = length(a, 0);
+      const int64_t all = (int64_t)a.b * tiles(a, len, kt);
+      per = share(a, all);
+      splits = (tiles(a, len, kt) + per - 1) / per;
+      b = slot >= 0 ? slot / splits : seq;
+      slot0 = b * splits;
+      split = slot - slot0;
+      return b < a.b;
+    }
+    const int lane = lane_id();
+    long long all = 0;
+    for (int i = lane; i < a.b; i += kWave) all += tiles(a, length(a, i), kt);
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) all += __shfl_xor(all, off, kWave);
+    per = __builtin_amdgcn_readfirstlane(share(a, all));
+    int before = 0;
+    for (int base = 0; base < a.b; base += kWave) {
+      const int i = base + lane;
+      const int mine = i < a.b ? (tiles(a, length(a, min(i, a.b - 1)), kt) + per - 1) / per : 0;
+      const int end = before + wave_inclusive_sum(mine);
+      const unsigned long long hit = __ballot(slot >= 0 ? slot < end : i == seq);
+      if (hit) {
+        const int at = __ffsll(hit) - 1;
+        b = base + at;
+        splits = __builtin_amdgcn_readlane(mine, at);
+        slot0 = __builtin_amdgcn_readlane(end, at) - splits;
+        split = slot - slot0;
+        len = length(a, b);
+        return true;
+      }
+      before = __builtin_amdgcn_readlane(end, kWave - 1);
+    }
+    return false;
+  }
+};
+
+// What the workgroups of both kernels have in common: where they are and whose keys they read.
+template <typename T>
+struct TreePlace {
+  int rb, unit, b, M, len, begin, end;   // tiles of the split
+  const T *q, *kc, *vc, *kn, *vn;
+  __device__ __forceinline__ bool find(const TreeArgs& a, int kt) {   // false: nothing to do
+    // the row blocks of a unit (a split of a head) follow each other 8 workgroups apart: on one XCD, whose L2 then has the
+    // rows of K and V that the first of them brought
+    rb = (int)blockIdx.x % (8 * a.row_blocks) / 8;
+    unit = (int)blockIdx.x / (8 * a.row_blocks) * 8 + (int)blockIdx.x % 8;
+    if (unit >= a.units) return false;
+    TreeCut cut;
+    if (!cut.find(a, kt, unit / a.hc, 0)) return false;
+    b = cut.b;
+    len = cut.len;
+    begin = cut.split * cut.per;
+    end = min(TreeCut::tiles(a, len, kt), begin + cut.per);
+    const int hc = unit % a.hc, gc = a.hq / a.hc;
+    M = gc * a.t;
+    q = (const T*)a.q + ((int64_t)b * a.hq + (int64_t)hc * gc) * a.t * a.d;
+    kc = (const T*)a.k + b * a.kv_b + hc * a.kv_h;
+    vc = (const T*)a.v + b * a.kv_b + hc * a.kv_h;
+    const int64_t hn = (int64_t)b * a.hn + hc / (a.hc / a.hn);
+    kn = (const T*)a.k_new + hn * a.t * a.d;
+    vn = (const T*)a.v_new + hn * a.t * a.d;
+    return true;
+  }
+};
+
+// A tile's scores become probabilities: running maximum, sum, and the rescaling of o where the maximum has grown too much.
+template <int MT, int NE, int VW>
+__device__ __forceinline__ void tree_softmax(float (&p)[MT][NE], float (&top)[MT], float (&sum)[MT], ar_f4 (&o)[MT][VW], float scale_log2e) {
+  bool more = false;
+  float high[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    float x = p[m][0];
+#pragma unroll
+    for (int e = 1; e < NE; ++e) x = fmaxf(x, p[m][e]);
+    high[m] = ar_quad_max(x) * scale_log2e;
+    more = more | (high[m] > top[m] + kTrSlack);
+  }
+  if (__ballot(more)) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const float now = fmaxf(top[m], high[m]);
+      const float f = ar_exp2(top[m] - now);
+      top[m] = now;
+      sum[m] *= f;
+#pragma unroll
+      for (int j = 0; j < VW; ++j) o[m][j] *= f;
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      p[m][e] = ar_exp2(fmaf(p[m][e], scale_log2e, -top[m]));
+      sum[m] += p[m][e];
+    }
+}
+
+// Takes what a query does not see out of a tile that is not a whole one of the cache.
+template <int MT, int NE>
+__device__ __forceinline__ void tree_mask(float (&p)[MT][NE], const TreeArgs& a, int b, const int (&ti)[MT], int quad, int valid,
+                                          bool draft, int first) {
+  // (every byte is read, from a place that exists, and then counts or not: reading under a condition compiled to a
+  // branch per key, in which the masked score was lost)
+  const uint8_t* seen = a.mask + b * a.mask_b + (draft ? first : 0);
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      const int key = quad * NE + e;
+      const uint32_t byte = seen[(int64_t)ti[m] * a.t + (draft ? min(key, valid - 1) : 0)];
+      const bool sees = (key < valid) & (!draft | (byte != 0));
+      p[m][e] = sees ? p[m][e] : -INFINITY;
+    }
+}
+
+// Few queries: the four waves of a workgroup take the tiles of its split in turn, each for itself.  Bound by the reading of
+// K and V.
 template <typename T, int DP, int MT>
-__global__ __launch_bounds__(kTrThreads) void tree_part_kernel(TreeArgs a) {
+__global__ __launch_bounds__(kTrThreads, MT == 2 && DP == 128 ? 2 : 1) void tree_stream_kernel(TreeArgs a) {
   using Tile = TreeTile<T, DP, MT>;
   constexpr int NU = Tile::NU, KT = Tile::KT, NE = Tile::NE, STEPS = Tile::STEPS, VW = Tile::VW;
   constexpr int JC = 2;   // output blocks that the waves join at a time
-  __shared__ ar_f4 joint[kTrWaves][MT * JC][kWave];
+  constexpr int CH = Tile::CH, KL = Tile::KL;
+  constexpr int KB = KT * CH * kTrWaves, JB = kTrWaves * MT * JC * kWave;   // 16-byte pieces: of K, and of the joining
+  __shared__ ar_u4 smem[KB > JB ? KB : JB];
   __shared__ float ml[kTrWaves][MT][16][2];
   const int lane = lane_id(), wave = wave_id(), col = lane & 15, quad = lane >> 4;
-  // the row blocks of a unit (a split of a head) follow each other 8 workgroups apart: on one XCD, whose L2 then has the
-  // rows of K and V that the first of them brought
-  const int rb = (int)blockIdx.x % (8 * a.row_blocks) / 8;
-  const int unit = (int)blockIdx.x / (8 * a.row_blocks) * 8 + (int)blockIdx.x % 8;
-  if (unit >= a.units) return;
-  const int split = unit % a.S, head = unit / a.S, b = head / a.hc, hc = head % a.hc;
-  const int gc = a.hq / a.hc, M = gc * a.t, row0 = rb * 16 * MT;
-  const int len = a.lengths ? min(max(a.lengths[b], 0), a.n) : a.n;
-
-  const T* q = (const T*)a.q + ((int64_t)b * a.hq + (int64_t)hc * gc) * a.t * a.d;
-  const T* kc = (const T*)a.k + b * a.kv_b + hc * a.kv_h;
-  const T* vc = (const T*)a.v + b * a.kv_b + hc * a.kv_h;
-  const int64_t hn = (int64_t)b * a.hn + hc / (a.hc / a.hn);
-  const T* kn = (const T*)a.k_new + hn * a.t * a.d;
-  const T* vn = (const T*)a.v_new + hn * a.t * a.d;
+  TreePlace<T> at;
+  if (!at.find(a, KT)) return;
+  const int M = at.M, row0 = at.rb * 16 * MT, len = at.len;
   const int pieces = a.d * (int)sizeof(T) / 16;
 
   ar_u4 qf[MT][STEPS];
@@ -168,7 +310,7 @@ __global__ __launch_bounds__(kTrThreads) void tree_part_kernel(TreeArgs a) {
   for (int m = 0; m < MT; ++m) {
     const int row = min(row0 + 16 * m + col, M - 1);
     ti[m] = row % a.t;
-    ar_row(q + (int64_t)row * a.d, quad, pieces, qf[m]);
+    ar_row(at.q + (int64_t)row * a.d, quad, pieces, qf[m]);
   }
   ar_f4 o[MT][VW] = {};
   float top[MT], sum[MT];
@@ -177,91 +319,97 @@ __global__ __launch_bounds__(kTrThreads) void tree_part_kernel(TreeArgs a) {
     top[m] = kTrNone;
     sum[m] = 0.0f;
   }
-  const int cached = (len + KT - 1) / KT, tiles = cached + (a.t + KT - 1) / KT;
-  const int per = (tiles + a.S - 1) / a.S;
-  const int end = min(tiles, (split + 1) * per);
+  const int cached = (len + KT - 1) / KT, begin = at.begin, end = at.end;
   bool odd = false;
-  for (int tile = split * per + __builtin_amdgcn_readfirstlane(wave); tile < end; tile += kTrWaves) {
-    const bool draft = tile >= cached;
-    const int first = (draft ? tile - cached : tile) * KT;
-    const int valid = min(KT, (draft ? a.t : len) - first);
-    const int64_t step = draft ? a.d : a.kv_r;
-    const T* kt = (draft ? kn : kc) + first * step;
-    const T* vt = (draft ? vn : vc) + first * step;
-    ar_u4 kf[NU][STEPS];
+  // A wave reads whole rows, 64 / CH at a time; K and V of the next tile are on their way while this one is worked on.
+  ar_u4* k_s = smem + wave * KT * CH;
+  const int piece = lane % CH, krow = lane / CH;
+  ar_u4 kg[KL];
+  TreeV<T, VW> v[NE];
+  constexpr int E = (int)sizeof(T), RPL = kWave / CH;   // bytes of an element, rows of a load
+  constexpr int VP = TreeV<T, VW>::DW >= 4 ? TreeV<T, VW>::DW / 4 : 1;
+  uint32_t vplace[VP];
 #pragma unroll
-    for (int u = 0; u < NU; ++u)
-      ar_row(kt + min((col >> 2) * NE + 4 * u + (col & 3), valid - 1) * step, quad, pieces, kf[u]);
-    TreeV<T, VW> v[NE];
+  for (int i = 0; i < VP; ++i) vplace[i] = TreeV<T, VW>::place(col, a.d, i);
+  const uint32_t kplace = 16u * (uint32_t)min(piece, pieces - 1), krs = (uint32_t)a.kv_r * E;
+  const uint32_t kwhole = (uint32_t)krow * krs + kplace, vwhole = (uint32_t)(quad * NE) * krs;
+  // a whole tile of the cache: the wave's address and offsets that do not change
+  auto load_k = [&](int tile) {
+    const char* src = (const char*)at.kc + (int64_t)tile * KT * krs;
 #pragma unroll
-    for (int e = 0; e < NE; ++e) v[e].load(vt + min(quad * NE + e, valid - 1) * step, col, a.d);
-
+    for (int i = 0; i < KL; ++i) kg[i] = tree_at<ar_u4>(src + (int64_t)(i * RPL) * krs, kwhole);
+  };
+  auto load_v = [&](int tile) {
+    const char* src = (const char*)at.vc + (int64_t)tile * KT * krs;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) v[e].load(src + (int64_t)e * krs, vwhole, vplace);
+  };
+  // kg and v are the tile's; valid keys, the first of them drafted token `first` if draft
+  auto work = [&](auto is_whole, int valid, bool draft, int first, auto next_k, auto next_v) {
+    constexpr bool WHOLE = decltype(is_whole)::value;
+    ar_wave_sync();
+    if (pieces < CH) {   // (a head of a width between two of the kernels')
+#pragma unroll
+      for (int i = 0; i < KL; ++i) kg[i] = piece < pieces ? kg[i] : ar_u4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < KL; ++i) k_s[ar_place<CH>(Tile::place(i * RPL + krow), piece)] = kg[i];
+    ar_wave_sync();
+    next_k();
     float p[MT][NE];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int u = 0; u < NU; ++u) {
+      ar_u4 kf[STEPS];
 #pragma unroll
-      for (int u = 0; u < NU; ++u) {
+      for (int c = 0; c < STEPS; ++c) kf[c] = k_s[ar_place<CH>(16 * u + col, 4 * c + quad)];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
         ar_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < STEPS; ++c) s = ar_step<T>(kf[u][c], qf[m][c], s);
+        for (int c = 0; c < STEPS; ++c) s = ar_step<T>(kf[c], qf[m][c], s);
 #pragma unroll
         for (int r = 0; r < 4; ++r) p[m][4 * u + r] = s[r];
       }
-    const bool whole = !draft && valid == KT;
-    if (!whole) {
-      // (every byte is read, from a place that exists, and then counts or not: reading under a condition compiled to a
-      // branch per key, in which the masked score was lost)
-      const uint8_t* seen = a.mask + b * a.mask_b + (draft ? first : 0);
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int e = 0; e < NE; ++e) {
-          const int key = quad * NE + e;
-          const uint32_t byte = seen[(int64_t)ti[m] * a.t + (draft ? min(key, valid - 1) : 0)];
-          const bool sees = (key < valid) & (!draft | (byte != 0));
-          p[m][e] = sees ? p[m][e] : -INFINITY;
-        }
     }
-    bool more = false;
-    float high[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      float x = p[m][0];
-#pragma unroll
-      for (int e = 1; e < NE; ++e) x = fmaxf(x, p[m][e]);
-      high[m] = ar_quad_max(x) * a.scale_log2e;
-      more = more || high[m] > top[m] + kTrSlack;
-    }
-    if (__ballot(more)) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const float now = fmaxf(top[m], high[m]);
-        const float f = ar_exp2(top[m] - now);
-        top[m] = now;
-        sum[m] *= f;
-#pragma unroll
-        for (int j = 0; j < VW; ++j) o[m][j] *= f;
-      }
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        p[m][e] = ar_exp2(fmaf(p[m][e], a.scale_log2e, -top[m]));
-        sum[m] += p[m][e];
-      }
-    if (!whole) {
+    if constexpr (!WHOLE) tree_mask<MT, NE>(p, a, at.b, ti, quad, valid, draft, first);
+    tree_softmax<MT, NE, VW>(p, top, sum, o, a.scale_log2e);
+    if constexpr (!WHOLE) {
 #pragma unroll
       for (int e = 0; e < NE; ++e)
 #pragma unroll
         for (int w = 0; w < TreeV<T, VW>::DW; ++w) {
-          if (quad * NE + e >= valid) v[e].w[w] = 0;   // (a row that stands for one beyond the end)
+          v[e].w[w] = quad * NE + e < valid ? v[e].w[w] : 0u;   // (a row that stands for one beyond the end)
           // queries that do not see a drafted token must not meet what its V holds: the joining launch adds that
-          if (draft) odd = tree_clean<T>(v[e].w[w]) || odd;
+          if (draft) odd = tree_clean<T>(v[e].w[w]) | odd;
         }
     }
     Tile::add(v, p, o);
+    next_v();
+  };
+  int tile = begin + __builtin_amdgcn_readfirstlane(wave);
+  const int wholes = min(end, len / KT);
+  if (tile < wholes) {
+    load_k(tile);
+    load_v(tile);
   }
+  for (; tile < wholes; tile += kTrWaves) {   // (the next tile, or this one again)
+    const int next = tile + kTrWaves < wholes ? tile + kTrWaves : tile;
+    work(std::true_type{}, KT, false, 0, [&] { load_k(next); }, [&] { load_v(next); });
+  }
+  for (; tile < end; tile += kTrWaves) {      // the last tile of the cache, if it is not whole, and the drafted ones
+    const bool draft = tile >= cached;
+    const int first = (draft ? tile - cached : tile) * KT, valid = min(KT, (draft ? a.t : len) - first);
+    const uint32_t rs = draft ? (uint32_t)a.d * E : krs;
+    const char* ks = (const char*)(draft ? at.kn : at.kc) + (int64_t)first * rs;
+    const char* vs = (const char*)(draft ? at.vn : at.vc) + (int64_t)first * rs;
+#pragma unroll
+    for (int i = 0; i < KL; ++i) kg[i] = tree_at<ar_u4>(ks, (uint32_t)min(i * RPL + krow, valid - 1) * rs + kplace);
+#pragma unroll
+    for (int e = 0; e < NE; ++e) v[e].load(vs, (uint32_t)min(quad * NE + e, valid - 1) * rs, vplace);
+    work(std::false_type{}, valid, draft, first, [] {}, [] {});
+  }
+  __syncthreads();   // (the rows of K make room for the sums)
+  ar_f4(*joint)[MT * JC][kWave] = (ar_f4(*)[MT * JC][kWave])smem;
 
   // the four waves' sums, each over its own keys, to one maximum and together
 #pragma unroll
@@ -272,9 +420,9 @@ __global__ __launch_bounds__(kTrThreads) void tree_part_kernel(TreeArgs a) {
       ml[wave][m][col][1] = sum[m];
     }
   }
-  const int64_t at = (int64_t)unit * a.row_blocks + rb;
   odd = __syncthreads_or(odd);
-  if (threadIdx.x == 0) a.odd[at] = odd;
+  if (threadIdx.x == 0) a.odd[(int64_t)at.unit * a.row_blocks + at.rb] = odd;
+  const int64_t tile16 = (int64_t)at.unit * a.row_tiles + row0 / 16;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     float all = ml[0][m][col][0];
@@ -287,7 +435,7 @@ __global__ __launch_bounds__(kTrThreads) void tree_part_kernel(TreeArgs a) {
 #pragma unroll
     for (int j = 0; j < VW; ++j) o[m][j] *= f;
     if (wave == 0 && quad == 0 && row0 + 16 * m + col < M) {
-      float* dst = a.part_ml + (at * MT + m) * 32 + col * 2;
+      float* dst = a.part_ml + (tile16 + m) * 32 + col * 2;
       dst[0] = all;
       dst[1] = total;
     }
@@ -306,146 +454,437 @@ __global__ __launch_bounds__(kTrThreads) void tree_part_kernel(TreeArgs a) {
 #pragma unroll
       for (int w = 1; w < kTrWaves; ++w) x += joint[w][s][lane];
       const int m = s / JC, j = j0 + s % JC;
-      if (row0 + 16 * m + col < M) ((ar_f4*)a.part)[((at * MT + m) * VW + j) * kWave + lane] = x;
+      if (row0 + 16 * m + col < M) ((ar_f4*)a.part)[((tile16 + m) * VW + j) * kWave + lane] = x;
     }
     __syncthreads();
   }
 }
 
-// One workgroup per 16 queries of a cache head joins the S parts: wave -> (block j of the output, group of splits).
-template <typename T, int DP, int MT>
+constexpr int kTlWaves = 4, kTlThreads = kTlWaves * kWave;
+
+// Many queries: WR x WK waves, WR with 16 MT queries each that share the keys, WK groups of them with every WK-th tile of
+// the split; K and V of the groups' tiles pass through LDS, whole rows read ahead into registers, one barrier a tile.  Two
+// workgroups per CU, whose waves are at different places, so that one forms exponentials while the other multiplies (as
+// one workgroup of eight waves they did both at the same time: twice as slow).  V's operand is read transposed
+// (ds_read_b64_tr_b16: four keys of one element a lane).
+template <typename T, int DP, int WR>
+struct TreeShare {
+  static constexpr int MT = DP == 256 ? 1 : 2, WK = kTlWaves / WR;
+  using Tile = TreeTile<T, DP, MT>;
+  static constexpr int KT = Tile::KT, CH = Tile::CH, KL = Tile::KL;
+  static constexpr int ROWS = WR * 16 * MT;
+  static constexpr int TILE = 2 * KT * CH;                          // 16-byte pieces of a tile's K and V
+  static constexpr int LPW = (2 * KL + WR - 1) / WR;                // loads of a wave for a tile
+  static constexpr int AHEAD = LPW <= 4 ? 2 : 1;                    // steps whose rows are on their way
+  static constexpr int JC = 2, JOINT = WK > 1 ? kTlWaves * MT * JC * kWave : 0;
+  static constexpr int SMEM = 2 * WK * TILE > JOINT ? 2 * WK * TILE : JOINT;
+
+  // Where piece `piece` of V's row is: moved within the row so that what a transposing read takes (32 bytes of rows r ..
+  // r + 3 and r + 8 .. r + 11) or an fp32 operand (64 bytes of rows r, r + 4 ..) comes from different banks.
+  static __device__ __forceinline__ int v_place(int row, int piece) {
+    int x;
+    if constexpr (sizeof(T) == 4)
+      x = (4 * (row >> 2)) & (CH - 1);
+    else if constexpr (CH >= 16)
+      x = 2 * ((row & 3) | ((row >> 3) & 1) << 2);
+    else if constexpr (CH == 8)
+      x = 2 * (((row >> 1) & 1) | ((row >> 3) & 1) << 1);
+    else
+      x = 2 * ((row >> 3) & 1);
+    return row * CH + (piece ^ x);
+  }
+};
+
+template <typename T, int DP, int WR>
+__global__ __launch_bounds__(kTlThreads, 2) void tree_share_kernel(TreeArgs a) {
+  using Share = TreeShare<T, DP, WR>;
+  constexpr int MT = Share::MT, WK = Share::WK;
+  using Tile = TreeTile<T, DP, MT>;
+  constexpr int NU = Tile::NU, KT = Tile::KT, NE = Tile::NE, STEPS = Tile::STEPS, VW = Tile::VW, CH = Tile::CH, KL = Tile::KL;
+  constexpr int E = (int)sizeof(T), RPL = kWave / CH, LPW = Share::LPW, JC = Share::JC;
+  __shared__ ar_u4 smem[Share::SMEM];
+  __shared__ float ml[kTlWaves][MT][16][2];
+  TreePlace<T> at;
+  if (!at.find(a, KT)) return;
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), col = lane & 15, quad = lane >> 4;
+  const int wr = wave % WR, wk = wave / WR;
+  const int M = at.M, row0 = at.rb * Share::ROWS + wr * 16 * MT, len = at.len;
+  const int pieces = a.d * E / 16;
+  ar_u4 qf[MT][STEPS];
+  int ti[MT];   // drafted token of the lane's query
+  ar_f4 o[MT][VW] = {};
+  float top[MT], sum[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int row = min(row0 + 16 * m + col, M - 1);
+    ti[m] = row % a.t;
+    ar_row(at.q + (int64_t)row * a.d, quad, pieces, qf[m]);
+    top[m] = kTrNone;
+    sum[m] = 0.0f;
+  }
+  const int cached = (len + KT - 1) / KT, begin = at.begin, end = at.end, steps = (end - begin + WK - 1) / WK;
+  bool odd = false;
+  // this wave's share of a tile: loads l0 .. l0 + LPW of its K and then V rows
+  const int mine = wave % WK, l0 = wave / WK * LPW;
+  const int piece = lane % CH, krow = lane / CH;
+  const uint32_t place = 16u * (uint32_t)min(piece, pieces - 1), krs = (uint32_t)a.kv_r * E;
+  ar_u4 ring[Share::AHEAD][LPW];
+  auto load = [&](int step, ar_u4 (&g)[LPW]) {
+    // (always from a place that exists: loads under a condition were waited for one by one)
+    const int tile = min(begin + step * WK + mine, end - 1);
+    const bool draft = tile >= cached;
+    const int first = (draft ? tile - cached : tile) * KT, last = (draft ? a.t : len) - first - 1;
+    const uint32_t rs = draft ? (uint32_t)a.d * E : krs;
+    const char* ks = (const char*)(draft ? at.kn : at.kc) + (int64_t)first * rs;
+    const char* vs = (const char*)(draft ? at.vn : at.vc) + (int64_t)first * rs;
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) {
+      const int l = min(l0 + i, 2 * KL - 1);
+      g[i] = tree_at<ar_u4>(l < KL ? ks : vs, (uint32_t)min(l % KL * RPL + krow, last) * rs + place);
+    }
+  };
+  // Two versions of a step's work: of whole tiles of the cache, and with everything that the others need.
+  uint32_t to[LPW];   // where the loads go within a tile
+#pragma unroll
+  for (int i = 0; i < LPW; ++i) {
+    const int l = min(l0 + i, 2 * KL - 1), row = l % KL * RPL + krow;
+    to[i] = (uint32_t)(l < KL ? ar_place<CH>(Tile::place(row), piece) : KT * CH + Share::v_place(row, piece));
+  }
+  auto store = [&](auto is_whole, int step, ar_u4 (&g)[LPW]) {
+    const int tile = begin + step * WK + mine;
+    ar_u4* dst = smem + ((step & 1) * WK + mine) * Share::TILE;
+    if constexpr (!decltype(is_whole)::value) {
+      if (tile >= end) return;
+      const bool draft = tile >= cached;
+      const int valid = (draft ? a.t : len) - (draft ? tile - cached : tile) * KT;
+#pragma unroll
+      for (int i = 0; i < LPW; ++i) {
+        const int l = min(l0 + i, 2 * KL - 1), row = l % KL * RPL + krow;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {   // of V: zeros for a row that stands for one beyond the end
+          uint32_t x = ((l < KL) | (row < valid)) ? g[i][w] : 0u;
+          // queries that do not see a drafted token must not meet what its V holds: the joining launch adds that
+          const uint32_t kept = x;
+          const bool found = tree_clean<T>(x) & draft & (l >= KL);
+          odd = odd | found;
+          g[i][w] = found ? x : kept;
+        }
+      }
+    }
+    if (pieces < CH) {   // (a head of a width between two of the kernels')
+#pragma unroll
+      for (int i = 0; i < LPW; ++i) g[i] = piece < pieces ? g[i] : ar_u4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) dst[to[i]] = g[i];
+  };
+  uint32_t vat[Tile::BF ? VW : 1][2];   // bf16: where the lane's part of V's operands is
+  if constexpr (Tile::BF) {
+#pragma unroll
+    for (int j = 0; j < VW; ++j) {
+      // keys 8 quad .. + 3 and + 4 .. + 7 of elements 16 j ..: lane i of 16 points to key i / 4, elements 4 (i % 4) ..
+      const int row = 8 * quad + (col >> 2), x = 2 * j + ((col >> 1) & 1);
+      vat[j][0] = 16u * (uint32_t)Share::v_place(row, x) + 8u * (uint32_t)(col & 1);
+      vat[j][1] = 16u * (uint32_t)Share::v_place(row + 4, x) + 8u * (uint32_t)(col & 1);
+    }
+  }
+  auto work = [&](auto is_whole, int step) {
+    constexpr bool WHOLE = decltype(is_whole)::value;
+    const int tile = begin + step * WK + wk;
+    if constexpr (!WHOLE)
+      if (tile >= end) return;
+    const ar_u4* k_s = smem + ((step & 1) * WK + wk) * Share::TILE;
+    const ar_u4* v_s = k_s + KT * CH;
+    float p[MT][NE];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      ar_u4 kf[STEPS];
+#pragma unroll
+      for (int c = 0; c < STEPS; ++c) kf[c] = k_s[ar_place<CH>(16 * u + col, 4 * c + quad)];
+      ar_f4 s[MT] = {};
+#pragma unroll
+      for (int c = 0; c < STEPS; ++c)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) s[m] = ar_step<T>(kf[c], qf[m][c], s[m]);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[m][4 * u + r] = s[m][r];
+    }
+    if constexpr (!WHOLE) {
+      const bool draft = tile >= cached;
+      const int first = (draft ? tile - cached : tile) * KT, valid = min(KT, (draft ? a.t : len) - first);
+      if (draft || valid < KT) tree_mask<MT, NE>(p, a, at.b, ti, quad, valid, draft, first);
+    }
+    tree_softmax<MT, NE, VW>(p, top, sum, o, a.scale_log2e);
+    if constexpr (Tile::BF) {
+      ar_bf8 hi[MT], lo[MT];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) tree_split(p[m], hi[m], lo[m]);
+#pragma unroll
+      for (int j = 0; j < VW; ++j) {
+        const tr_v4s b0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_v4s)((const char*)v_s + vat[j][0]));
+        const tr_v4s b1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_v4s)((const char*)v_s + vat[j][1]));
+        const ar_bf8 v = __builtin_bit_cast(ar_bf8, __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) o[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, lo[m], o[m][j], 0, 0, 0);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) o[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, hi[m], o[m][j], 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VW; ++j)
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+          const float v = ((const float*)(v_s + Share::v_place(4 * quad + e, 4 * j + (col >> 2))))[col & 3];
+#pragma unroll
+          for (int m = 0; m < MT; ++m) o[m][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[m][e], o[m][j], 0, 0, 0);
+        }
+    }
+  };
+  constexpr int AHEAD = Share::AHEAD;
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) load(i, ring[i]);
+  store(std::false_type{}, 0, ring[0]);
+  __syncthreads();
+  const int wholes = (min(end, len / KT) - begin) / WK;   // steps that have whole tiles only
+  int step = 0;
+  for (; step + AHEAD < wholes; step += AHEAD) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      load(step + i + AHEAD, ring[i]);
+      work(std::true_type{}, step + i);
+      store(std::true_type{}, step + i + 1, ring[(i + 1) % AHEAD]);
+      __syncthreads();
+    }
+  }
+  for (; step < steps; step += AHEAD) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {   // (steps behind the last have no tile)
+      load(step + i + AHEAD, ring[i]);
+      work(std::false_type{}, step + i);
+      store(std::false_type{}, step + i + 1, ring[(i + 1) % AHEAD]);
+      __syncthreads();
+    }
+  }
+
+  odd = __syncthreads_or(odd);
+  if (threadIdx.x == 0) a.odd[(int64_t)at.unit * a.row_blocks + at.rb] = odd;
+  const int64_t tile16 = (int64_t)at.unit * a.row_tiles + row0 / 16;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) sum[m] = ar_quad_sum(sum[m]);
+  if constexpr (WK > 1) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+      if (quad == 0) {
+        ml[wave][m][col][0] = top[m];
+        ml[wave][m][col][1] = sum[m];
+      }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    float all = top[m], total = sum[m];
+    if constexpr (WK > 1) {
+      all = ml[wr][m][col][0];
+#pragma unroll
+      for (int w = 1; w < WK; ++w) all = fmaxf(all, ml[w * WR + wr][m][col][0]);
+      total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WK; ++w) total += ml[w * WR + wr][m][col][1] * ar_exp2(ml[w * WR + wr][m][col][0] - all);
+      const float f = ar_exp2(top[m] - all);
+#pragma unroll
+      for (int j = 0; j < VW; ++j) o[m][j] *= f;
+    }
+    if (wk == 0 && quad == 0 && row0 + 16 * m + col < M) {
+      float* dst = a.part_ml + (tile16 + m) * 32 + col * 2;
+      dst[0] = all;
+      dst[1] = total;
+    }
+  }
+  if constexpr (WK == 1) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < VW; ++j)
+        if (row0 + 16 * m + col < M) ((ar_f4*)a.part)[((tile16 + m) * VW + j) * kWave + lane] = o[m][j];
+  } else {
+    ar_f4(*joint)[MT * JC][kWave] = (ar_f4(*)[MT * JC][kWave])smem;
+    for (int j0 = 0; j0 < VW; j0 += JC) {
+#pragma unroll
+      for (int j = 0; j < VW; ++j)
+        if (j >= j0 && j < j0 + JC) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m) joint[wave][m * JC + (j & (JC - 1))][lane] = o[m][j];
+        }
+      __syncthreads();
+      for (int s = wk; s < MT * JC; s += WK) {
+        ar_f4 x = joint[wr][s][lane];
+#pragma unroll
+        for (int w = 1; w < WK; ++w) x += joint[w * WR + wr][s][lane];
+        const int m = s / JC, j = j0 + s % JC;
+        if (row0 + 16 * m + col < M) ((ar_f4*)a.part)[((tile16 + m) * VW + j) * kWave + lane] = x;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// A workgroup joins the splits' parts of 16 queries of a cache head, a quad of the lanes that hold them (a quarter of the
+// head): 16 threads with a query each for (block j of the output, every G-th split).  SHARED: which of the two kernels left
+// the parts, whose lanes have other elements.
+template <typename T, int DP, bool SHARED>
 __global__ __launch_bounds__(kTrCombThreads) void tree_join_kernel(TreeArgs a) {
-  constexpr int VW = DP / 16, NW = kTrCombThreads / kWave, G = NW / VW;
+  constexpr int VW = DP / 16, GROUPS = kTrCombThreads / 16, G = GROUPS / VW, KT = sizeof(T) == 2 ? 32 : 16, FIRST = 4;
   __shared__ float f_s[kTrMaxSplits][16];
-  __shared__ float red[kTrCombThreads / 16][16];
+  __shared__ float red[GROUPS][16];
   __shared__ float top_s[16], sum_s[16];
-  __shared__ ar_f4 joint[NW][kWave];
-  const int lane = lane_id(), wave = wave_id(), col = lane & 15;
-  const int rb = (int)blockIdx.x / MT % a.row_blocks, m = (int)blockIdx.x % MT, head = (int)blockIdx.x / MT / a.row_blocks;
-  const int gc = a.hq / a.hc, M = gc * a.t, row0 = rb * 16 * MT + 16 * m;
-  if (row0 >= M) return;
-  const int64_t at0 = (int64_t)head * a.S * a.row_blocks + rb;   // + split * row_blocks
-  const int c = threadIdx.x & 15, s0 = threadIdx.x >> 4;
-  const bool mine = row0 + c < M;
+  __shared__ ar_f4 joint[G][VW][16];
+  const int col = threadIdx.x & 15, group = threadIdx.x >> 4;
+  const int quad = (int)blockIdx.x & 3, tile = (int)(blockIdx.x >> 2) % a.row_tiles, head = (int)(blockIdx.x >> 2) / a.row_tiles;
+  const int M = a.hq / a.hc * a.t, row0 = 16 * tile, b = head / a.hc;
+  TreeCut cut;
+  cut.find(a, KT, -1, b);
+  const int S = min(cut.splits, kTrMaxSplits);
+  const int64_t unit0 = (int64_t)cut.slot0 * a.hc + head % a.hc;   // + split * hc
+  const bool mine = row0 + col < M;
+  // (the first parts are asked for before their weights are known)
+  const int j = group % VW, g = group / VW;
+  const ar_f4* part = (const ar_f4*)a.part + ((unit0 * a.row_tiles + tile) * VW + j) * kWave + quad * 16 + col;
+  const int64_t next = (int64_t)a.hc * a.row_tiles * VW * kWave;
+  ar_f4 early[FIRST];
+#pragma unroll
+  for (int i = 0; i < FIRST; ++i)
+    early[i] = mine ? part[min(g + i * G, S - 1) * next] : ar_f4{0.0f, 0.0f, 0.0f, 0.0f};
   float top = kTrNone;
   bool odd = false;
-  for (int s = s0; s < a.S; s += kTrCombThreads / 16) {
-    odd = odd || a.odd[at0 + (int64_t)s * a.row_blocks];
-    const float x = mine ? a.part_ml[((at0 + (int64_t)s * a.row_blocks) * MT + m) * 32 + c * 2] : kTrNone;
-    f_s[s][c] = x;
+  for (int s = group; s < S; s += GROUPS) {
+    odd = odd | (a.odd[(unit0 + (int64_t)s * a.hc) * a.row_blocks + row0 / a.rows] != 0);
+    const float x = mine ? a.part_ml[((unit0 + (int64_t)s * a.hc) * a.row_tiles + tile) * 32 + col * 2] : kTrNone;
+    f_s[s][col] = x;
     top = fmaxf(top, x);
   }
-  red[s0][c] = top;
+  red[group][col] = top;
   odd = __syncthreads_or(odd);
   if (threadIdx.x < 16) {
-    float x = red[0][c];
-    for (int i = 1; i < min(a.S, kTrCombThreads / 16); ++i) x = fmaxf(x, red[i][c]);
-    top_s[c] = x;
+    float x = red[0][col];
+    for (int i = 1; i < min(S, GROUPS); ++i) x = fmaxf(x, red[i][col]);
+    top_s[col] = x;
   }
   __syncthreads();
   float total = 0.0f;
-  for (int s = s0; s < a.S; s += kTrCombThreads / 16) {
-    const float f = ar_exp2(f_s[s][c] - top_s[c]);
-    f_s[s][c] = f;
-    if (mine) total += f * a.part_ml[((at0 + (int64_t)s * a.row_blocks) * MT + m) * 32 + c * 2 + 1];
+  for (int s = group; s < S; s += GROUPS) {
+    const float f = ar_exp2(f_s[s][col] - top_s[col]);
+    f_s[s][col] = f;
+    if (mine) total += f * a.part_ml[((unit0 + (int64_t)s * a.hc) * a.row_tiles + tile) * 32 + col * 2 + 1];
   }
-  red[s0][c] = total;
+  red[group][col] = total;
   __syncthreads();
   if (threadIdx.x < 16) {
-    float x = red[0][c];
-    for (int i = 1; i < min(a.S, kTrCombThreads / 16); ++i) x += red[i][c];
-    sum_s[c] = x;
+    float x = red[0][col];
+    for (int i = 1; i < min(S, GROUPS); ++i) x += red[i][col];
+    sum_s[col] = x;
   }
-  __syncthreads();
-  {
-    const int j = wave % VW, g = wave / VW;
-    ar_f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (row0 + col < M) {
-#pragma unroll 8
-      for (int s = g; s < a.S; s += G)
-        x += ((const ar_f4*)a.part)[(((at0 + (int64_t)s * a.row_blocks) * MT + m) * VW + j) * kWave + lane] * f_s[s][col];
-    }
-    joint[wave][lane] = x;
+  ar_f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < FIRST; ++i)
+    if (g + i * G < S) x += early[i] * f_s[g + i * G][col];
+  if (mine) {
+#pragma unroll 4
+    for (int s = g + FIRST * G; s < S; s += G) x += part[s * next] * f_s[s][col];
   }
+  joint[g][j][col] = x;
   __syncthreads();
   const int64_t row = (int64_t)head * M + row0;   // rows of all heads follow each other
-  for (int e = threadIdx.x; e < 16 * DP; e += kTrCombThreads) {
-    const int r = e / DP, x = e % DP;
-    if (x >= a.d || row0 + r >= M) continue;
-    const int j = x % VW, at = x / VW;   // output rows 4 quad + i of block j
+  for (int e = threadIdx.x; e < 16 * 4 * VW; e += kTrCombThreads) {
+    const int r = e / (4 * VW), y = e % (4 * VW);
+    const int blk = SHARED ? y / 4 : y % VW, i = SHARED ? y % 4 : y / VW;
+    const int d = SHARED ? 16 * blk + 4 * quad + i : 4 * VW * quad + y;
+    if (d >= a.d || row0 + r >= M) continue;
     float v = 0.0f;
 #pragma unroll
-    for (int g = 0; g < G; ++g) v += joint[g * VW + j][(at >> 2) * 16 + r][at & 3];
+    for (int h = 0; h < G; ++h) v += joint[h][blk][r][i];
     if (odd) {
-      const int b = head / a.hc, hn = head % a.hc / (a.hc / a.hn);
-      const T* vn = (const T*)a.v_new + ((int64_t)b * a.hn + hn) * a.t * a.d + x;
+      const int hn = head % a.hc / (a.hc / a.hn);
+      const T* vn = (const T*)a.v_new + ((int64_t)b * a.hn + hn) * a.t * a.d + d;
       const uint8_t* sees = a.mask + b * a.mask_b + (int64_t)((row0 + r) % a.t) * a.t;
-      for (int i = 0; i < a.t; ++i) {
-        const float y = ld_f32(vn, (int64_t)i * a.d);
-        if (sees[i] && !(fabsf(y) < INFINITY)) v += y;
+      for (int k = 0; k < a.t; ++k) {
+        const float z = ld_f32(vn, (int64_t)k * a.d);
+        if (sees[k] && !(fabsf(z) < INFINITY)) v += z;
       }
     }
-    st_f32((T*)a.out, (row + r) * a.d + x, sum_s[r] == 0.0f ? 0.0f : v / sum_s[r]);
+    st_f32((T*)a.out, (row + r) * a.d + d, sum_s[r] == 0.0f ? 0.0f : v / sum_s[r]);
   }
-  if (a.lse && threadIdx.x < 16 && mine)
-    a.lse[row + c] = sum_s[c] == 0.0f ? -INFINITY : (top_s[c] + log2f(sum_s[c])) * kLn2;
+  if (a.lse && quad == 0 && threadIdx.x < 16 && mine)
+    a.lse[row + col] = sum_s[col] == 0.0f ? -INFINITY : (top_s[col] + log2f(sum_s[col])) * kLn2;
 }
 
 // How a call is cut up, from its sizes alone.
 struct TreePlan {
-  int dp, mt, row_blocks, S, units;
-  int64_t part, ml, odd;   // words of 4 bytes
+  int dp, mt, wr;                    // wr = 0: tree_stream_kernel
+  int rows, row_blocks, row_tiles, splits, least, units;
+  int64_t part, ml, odd;             // words of 4 bytes
 };
-static TreePlan tree_plan(int b, int hq, int hc, int t, int64_t n, int d, int dtype) {
+static TreePlan tree_plan(int b, int hq, int hc, int t, int64_t n, int d, bool lengths, int dtype) {
   TreePlan p;
   p.dp = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256;
   const int64_t M = (int64_t)(hq / hc) * t;
-  p.mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-  if (p.dp == 256) p.mt = std::min(p.mt, dtype == LRQK_BF16 ? 2 : 1);   // (more queries' sums would not fit the registers)
-  p.row_blocks = (int)((M + 16 * p.mt - 1) / (16 * p.mt));
   const int kt = dtype == LRQK_BF16 ? 32 : 16;
   const int64_t tiles = (n + kt - 1) / kt + (t + kt - 1) / kt;
-  const int64_t heads = (int64_t)b * hc;
-  // two workgroups per CU, four tiles for each of a workgroup's waves at least
-  int64_t S = std::max<int64_t>(1, 512 / (heads * p.row_blocks));
-  S = std::min<int64_t>(S, (tiles + 4 * kTrWaves - 1) / (4 * kTrWaves));
-  p.S = (int)std::max<int64_t>(1, std::min<int64_t>(S, kTrMaxSplits));
-  p.units = (int)(heads * p.S);
-  const int64_t groups = (int64_t)p.units * p.row_blocks * p.mt;
+  int64_t groups_wanted, least;
+  if (M <= (p.dp == 256 ? 16 : 32)) {
+    p.mt = M <= 16 ? 1 : 2;
+    p.wr = 0;
+    p.rows = 16 * p.mt;
+    least = 4 * kTrWaves;   // four tiles for each of a workgroup's waves
+  } else {
+    p.mt = p.dp == 256 ? 1 : 2;
+    p.wr = M <= 32 * p.mt && p.dp != 256 ? 2 : 4;
+    p.rows = 16 * p.mt * p.wr;
+    least = 2 * kTlWaves / p.wr;
+  }
+  // two workgroups per CU; twice as many where the lengths may differ
+  groups_wanted = b > 1 && lengths ? 1024 : 512;
+  p.row_blocks = (int)((M + p.rows - 1) / p.rows);
+  p.row_tiles = p.row_blocks * (p.rows / 16);
+  p.splits = (int)std::max<int64_t>(b, groups_wanted / ((int64_t)hc * p.row_blocks));
+  p.least = (int)std::max<int64_t>(least, (tiles + kTrMaxSplits - 1) / kTrMaxSplits);
+  // the splits that there can be: the wanted ones and the sequences' shorter ones, or what the shortest splits make
+  const int64_t slots = std::min<int64_t>((int64_t)p.splits + b, b * ((tiles + p.least - 1) / p.least));
+  p.units = (int)(hc * slots);
+  const int64_t groups = (int64_t)p.units * p.row_tiles;
   p.part = groups * 16 * p.dp;
   p.ml = groups * 32;
   p.odd = (int64_t)p.units * p.row_blocks;
   return p;
 }
 
-template <typename T, int DP, int MT>
-static int tree_launch(const TreeArgs& a, hipStream_t st) {
-  const int64_t grid = (int64_t)(a.units + 7) / 8 * 8 * a.row_blocks;
-  hipLaunchKernelGGL((tree_part_kernel<T, DP, MT>), dim3((unsigned)grid), dim3(kTrThreads), 0, st, a);
-  LRQK_HIP_CHECK(hipGetLastError());
-  hipLaunchKernelGGL((tree_join_kernel<T, DP, MT>), dim3((unsigned)(a.units / a.S * a.row_blocks * MT)), dim3(kTrCombThreads), 0, st,
-                     a);
+template <typename T, int DP>
+static int tree_launch(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
+  const dim3 grid((unsigned)((int64_t)(a.units + 7) / 8 * 8 * a.row_blocks));
+  const dim3 join((unsigned)((int64_t)a.b * a.hc * a.row_tiles * 4));
+  if (p.wr == 0) {
+    if constexpr (DP < 256)
+      if (p.mt == 2) hipLaunchKernelGGL((tree_stream_kernel<T, DP, 2>), grid, dim3(kTrThreads), 0, st, a);
+    if (p.mt == 1) hipLaunchKernelGGL((tree_stream_kernel<T, DP, 1>), grid, dim3(kTrThreads), 0, st, a);
+    LRQK_HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL((tree_join_kernel<T, DP, false>), join, dim3(kTrCombThreads), 0, st, a);
+  } else {
+    if constexpr (DP < 256)
+      if (p.wr == 2) hipLaunchKernelGGL((tree_share_kernel<T, DP, 2>), grid, dim3(kTlThreads), 0, st, a);
+    if (p.wr == 4) hipLaunchKernelGGL((tree_share_kernel<T, DP, 4>), grid, dim3(kTlThreads), 0, st, a);
+    LRQK_HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL((tree_join_kernel<T, DP, true>), join, dim3(kTrCombThreads), 0, st, a);
+  }
   LRQK_HIP_CHECK(hipGetLastError());
   return LRQK_OK;
 }
-template <typename T, int DP>
-static int tree_launch_mt(const TreeArgs& a, int mt, hipStream_t st) {
-  if constexpr (DP == 256) {
-    if constexpr (sizeof(T) == 2)
-      if (mt == 2) return tree_launch<T, DP, 2>(a, st);
-    return tree_launch<T, DP, 1>(a, st);
-  } else {
-    if (mt == 1) return tree_launch<T, DP, 1>(a, st);
-    if (mt == 2) return tree_launch<T, DP, 2>(a, st);
-    return tree_launch<T, DP, 4>(a, st);
-  }
-}
 template <typename T>
 static int tree_launch_dp(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
-  if (p.dp == 32) return tree_launch_mt<T, 32>(a, p.mt, st);
-  if (p.dp == 64) return tree_launch_mt<T, 64>(a, p.mt, st);
-  if (p.dp == 128) return tree_launch_mt<T, 128>(a, p.mt, st);
-  return tree_launch_mt<T, 256>(a, p.mt, st);
+  if (p.dp == 32) return tree_launch<T, 32>(a, p, st);
+  if (p.dp == 64) return tree_launch<T, 64>(a, p, st);
+  if (p.dp == 128) return tree_launch<T, 128>(a, p, st);
+  return tree_launch<T, 256>(a, p, st);
 }
 
 static int tree_check(int b, int hq, int hc, int t, int64_t n, int d, int dtype) {
@@ -464,10 +903,10 @@ static int tree_check(int b, int hq, int hc, int t, int64_t n, int d, int dtype)
 
 using namespace lrqk;
 
-extern "C" int64_t lrqk_tree_attention_workspace(int b, int hq, int hc, int t, int64_t n, int d, int dtype) {
+extern "C" int64_t lrqk_tree_attention_workspace(int b, int hq, int hc, int t, int64_t n, int d, int have_lengths, int dtype) {
   const int rc = tree_check(b, hq, hc, t, n, d, dtype);
   if (rc) return rc;
-  const TreePlan p = tree_plan(b, hq, hc, t, n, d, dtype);
+  const TreePlan p = tree_plan(b, hq, hc, t, n, d, have_lengths != 0, dtype);
   return (p.part + p.ml + p.odd) * (int64_t)sizeof(float);
 }
 
@@ -486,13 +925,16 @@ extern "C" int lrqk_tree_attention(const void* q, const void* k_cache, const voi
                    (uintptr_t)v_new % 16 == 0 && (uintptr_t)workspace % 16 == 0 && kv_batch_stride % vec == 0 &&
                    kv_head_stride % vec == 0 && kv_row_stride % vec == 0,
                LRQK_EINVAL, "pointers and rows must be 16-byte aligned");
-  const TreePlan p = tree_plan(b, hq, hc, t, n, d, dtype);
+  LRQK_REQUIRE(kv_row_stride >= 0 && kv_row_stride <= (1 << 24), LRQK_ELIMIT, "kv_row_stride=%lld (at most 2^24 elements)",
+               (long long)kv_row_stride);
+  const TreePlan p = tree_plan(b, hq, hc, t, n, d, lengths != nullptr, dtype);
   const int64_t need = (p.part + p.ml + p.odd) * (int64_t)sizeof(float);
   LRQK_REQUIRE(workspace_bytes >= need, LRQK_EINVAL, "workspace of %lld bytes: %lld are needed", (long long)workspace_bytes,
                (long long)need);
   TreeArgs a{q, k_cache, v_cache, k_new, v_new, mask, lengths, out, lse, (float*)workspace, (float*)workspace + p.part,
              (int32_t*)workspace + p.part + p.ml,
-             kv_batch_stride, kv_head_stride, kv_row_stride, mask_batch_stride, (int)n, hq, hc, hn, t, d, p.S, p.row_blocks, p.units,
+             kv_batch_stride, kv_head_stride, kv_row_stride, mask_batch_stride, b, (int)n, hq, hc, hn, t, d, p.splits, p.least, p.row_blocks, p.rows,
+             p.row_tiles, p.units,
              scale * kLog2e};
   hipStream_t st = (hipStream_t)stream;
   if (dtype == LRQK_F32) return tree_launch_dp<float>(a, p, st);

@@ -676,7 +676,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if b * hq * t:
         lib = _lib.load()
         q, k_new, v_new, mask = q.contiguous(), k_new.contiguous(), v_new.contiguous(), mask.contiguous()
-        need = check(lib.lrqk_tree_attention_workspace(b, hq, hc, t, n, d, dt))
+        need = check(lib.lrqk_tree_attention_workspace(b, hq, hc, t, n, d, int(lengths is not None), dt))
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         _launch(q, lib.lrqk_tree_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *st, n, _ptr(lengths),
                 k_new.data_ptr(), v_new.data_ptr(), mask.data_ptr(), t * t if mask.dim() == 3 else 0, out.data_ptr(), _ptr(lse), b,

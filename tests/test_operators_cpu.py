@@ -121,9 +121,9 @@ def test_scratch_sizes():
     assert lib.lrqk_attention_weights_workspace(1, 32, 8, 64, 64, 128, 0, 1) >= 32 * 64 * 4
     assert lib.lrqk_evict_workspace(2, 8, 5000, 100) == 2 * 8 * 100 * 12
     assert lib.lrqk_evict_workspace(2, 8, 100, 5000) == 2 * 8 * 100 * 12
-    small, large = (lib.lrqk_tree_attention_workspace(1, 32, 8, t, 131072, 128, 1) for t in (1, 64))
+    small, large = (lib.lrqk_tree_attention_workspace(1, 32, 8, t, 131072, 128, 1, 1) for t in (1, 64))
     assert 0 < small <= large < 1 << 30
-    for fn, args in (("lrqk_tree_attention_workspace", (0, 32, 8, 1, 10, 128, 1)), ("lrqk_attention_weights_workspace", (1, 32, 7, 1, 10, 128, 1, 1)),
+    for fn, args in (("lrqk_tree_attention_workspace", (0, 32, 8, 1, 10, 128, 1, 1)), ("lrqk_attention_weights_workspace", (1, 32, 7, 1, 10, 128, 1, 1)),
                      ("lrqk_evict_workspace", (1, 1, 0, 1))):
         assert getattr(lib, fn)(*args) == EINVAL
 
