@@ -11,7 +11,7 @@
 // between the quads, and the probabilities are the operand of O^T = V^T P^T as they lie: the rows of K are dealt to the
 // lanes such that a quad's scores are those of successive keys, whose V rows the same quad loads, 16 lanes one whole row.
 // Bf16 V is transposed between those lanes' registers; bf16 probabilities are the sum of two bf16 numbers (16 bits), so
-// that the one rounding to bf16 is the output's.
+// that the one rounding to bf16 is the output's (but for very many queries: tree_share_kernel).
 #include <algorithm>
 #include <type_traits>
 
@@ -20,10 +20,9 @@
 namespace lrqk {
 
 constexpr int kTrWaves = 4, kTrThreads = kTrWaves * kWave;
-constexpr int kTrCombThreads = 512;
 constexpr int kTrMaxSplits = 256;
 constexpr float kTrNone = -3.0e38f;   // running maximum of a query that has seen no key yet
-constexpr float kTrSlack = 8.0f;      // a maximum may be exceeded by 2^8 before the sums are rescaled to the new one
+constexpr float kTrMuch = 4096.0f;    // a lane's probabilities of a tile may add up to this before the maximum is looked for
 
 struct TreeArgs {
   const void *q, *k, *v, *k_new, *v_new;
@@ -31,8 +30,10 @@ struct TreeArgs {
   const int32_t* lengths;   // or null: n each
   void* out;
   float* lse;               // or null
-  float *part, *part_ml;    // of 16 queries of a split: VW float4 a lane, and (maximum, sum) of each query
+  float *part, *part_ml;    // of 16 queries of a split: VW float4 a lane, and of each query the maximum, the sum and that of
+                            // the probabilities as they were multiplied (3 x 16)
   int32_t* odd;             // per workgroup of a split: whether its drafted rows of V hold infinities or NaN
+  int32_t* cut;             // of a sequence: the number of its first split, and how many it has
   int64_t kv_b, kv_h, kv_r; // elements between sequences, heads and rows of the cache
   int64_t mask_b;
   // splits: of all sequences together, for a cache head; least: tiles of a split, at least; rows: of a row block
@@ -156,7 +157,7 @@ struct TreeTile {
 
 // How the sequences are cut into splits: of equal length, whatever the lengths of the sequences, as many as the grid was
 // made for (every sequence's last one may be shorter, so there are up to b more).  From the lengths alone, by every wave
-// for itself; a split is found by its number among all, or a sequence's splits by the sequence.
+// for itself; a sequence's first workgroup leaves what the joining launch wants to know of it.
 struct TreeCut {
   int b, len, split, splits, slot0, per;   // splits of the sequence, the number of its first
   static __device__ __forceinline__ int tiles(const TreeArgs& a, int len, int kt) { return (len + kt - 1) / kt + (a.t + kt - 1) / kt; }
@@ -168,14 +169,13 @@ struct TreeCut {
     const int x = all <= INT32_MAX ? (int)(((uint32_t)all + (uint32_t)a.splits - 1u) / (uint32_t)a.splits) : (int)((all + a.splits - 1) / a.splits);
     return max(a.least, x);
   }
-  // slot >= 0: the split of that number (false: there is none); else sequence `seq`
-  __device__ __forceinline__ bool find(const TreeArgs& a, int kt, int slot, int seq) {
+  // the split of number `slot` of all; false: there is none
+  __device__ __forceinline__ bool find(const TreeArgs& a, int kt, int slot) {
     if (!a.lengths || a.b == 1) {
       len = length(a, 0);
-      const int64_t all = (int64_t)a.b * tiles(a, len, kt);
-      per = share(a, all);
+      per = share(a, (int64_t)a.b * tiles(a, len, kt));
       splits = (tiles(a, len, kt) + per - 1) / per;
-      b = slot >= 0 ? slot / splits : seq;
+      b = slot / splits;
       slot0 = b * splits;
       split = slot - slot0;
       return b < a.b;
@@ -191,7 +191,7 @@ struct TreeCut {
       const int i = base + lane;
       const int mine = i < a.b ? (tiles(a, length(a, min(i, a.b - 1)), kt) + per - 1) / per : 0;
       const int end = before + wave_inclusive_sum(mine);
-      const unsigned long long hit = __ballot(slot >= 0 ? slot < end : i == seq);
+      const unsigned long long hit = __ballot(slot < end);
       if (hit) {
         const int at = __ffsll(hit) - 1;
         b = base + at;
@@ -219,7 +219,11 @@ struct TreePlace {
     unit = (int)blockIdx.x / (8 * a.row_blocks) * 8 + (int)blockIdx.x % 8;
     if (unit >= a.units) return false;
     TreeCut cut;
-    if (!cut.find(a, kt, unit / a.hc, 0)) return false;
+    if (!cut.find(a, kt, unit / a.hc)) return false;
+    if (cut.split == 0 && unit % a.hc == 0 && rb == 0 && threadIdx.x == 0) {
+      a.cut[2 * cut.b] = cut.slot0;
+      a.cut[2 * cut.b + 1] = cut.splits;
+    }
     b = cut.b;
     len = cut.len;
     begin = cut.split * cut.per;
@@ -236,37 +240,45 @@ struct TreePlace {
   }
 };
 
-// A tile's scores become probabilities: running maximum, sum, and the rescaling of o where the maximum has grown too much.
+// A tile's scores x become probabilities p = 2^(x scale - top), and the running sums.  The maximum is not looked for: as
+// long as a lane's probabilities add up to little the one that is there serves, and where one of them does not (a larger
+// score, or the first) the tile is done again with the maximum, o and the sums rescaled to it.  (A maximum per tile was a
+// quarter of the vector instructions, which this kernel is bound by.)
 template <int MT, int NE, int VW>
-__device__ __forceinline__ void tree_softmax(float (&p)[MT][NE], float (&top)[MT], float (&sum)[MT], ar_f4 (&o)[MT][VW], float scale_log2e) {
+__device__ __forceinline__ void tree_softmax(const float (&x)[MT][NE], float (&p)[MT][NE], float (&top)[MT], float (&sum)[MT],
+                                             ar_f4 (&o)[MT][VW], float scale_log2e) {
+  float part[MT];
   bool more = false;
-  float high[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    float x = p[m][0];
 #pragma unroll
-    for (int e = 1; e < NE; ++e) x = fmaxf(x, p[m][e]);
-    high[m] = ar_quad_max(x) * scale_log2e;
-    more = more | (high[m] > top[m] + kTrSlack);
+    for (int e = 0; e < NE; ++e) {
+      p[m][e] = ar_exp2(fmaf(x[m][e], scale_log2e, -top[m]));
+      part[m] = e == 0 ? p[m][0] : part[m] + p[m][e];
+    }
+    more = more | !(part[m] <= kTrMuch);
   }
   if (__ballot(more)) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const float now = fmaxf(top[m], high[m]);
+      float high = x[m][0];
+#pragma unroll
+      for (int e = 1; e < NE; ++e) high = fmaxf(high, x[m][e]);
+      const float now = fmaxf(top[m], ar_quad_max(high) * scale_log2e);
       const float f = ar_exp2(top[m] - now);
       top[m] = now;
       sum[m] *= f;
 #pragma unroll
       for (int j = 0; j < VW; ++j) o[m][j] *= f;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        p[m][e] = ar_exp2(fmaf(x[m][e], scale_log2e, -now));
+        part[m] = e == 0 ? p[m][0] : part[m] + p[m][e];
+      }
     }
   }
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      p[m][e] = ar_exp2(fmaf(p[m][e], scale_log2e, -top[m]));
-      sum[m] += p[m][e];
-    }
+  for (int m = 0; m < MT; ++m) sum[m] += part[m];
 }
 
 // Takes what a query does not see out of a tile that is not a whole one of the cache.
@@ -356,7 +368,7 @@ __global__ __launch_bounds__(kTrThreads, MT == 2 && DP == 128 ? 2 : 1) void tree
     for (int i = 0; i < KL; ++i) k_s[ar_place<CH>(Tile::place(i * RPL + krow), piece)] = kg[i];
     ar_wave_sync();
     next_k();
-    float p[MT][NE];
+    float x[MT][NE], p[MT][NE];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       ar_u4 kf[STEPS];
@@ -368,11 +380,11 @@ __global__ __launch_bounds__(kTrThreads, MT == 2 && DP == 128 ? 2 : 1) void tree
 #pragma unroll
         for (int c = 0; c < STEPS; ++c) s = ar_step<T>(kf[c], qf[m][c], s);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[m][4 * u + r] = s[r];
+        for (int r = 0; r < 4; ++r) x[m][4 * u + r] = s[r];
       }
     }
-    if constexpr (!WHOLE) tree_mask<MT, NE>(p, a, at.b, ti, quad, valid, draft, first);
-    tree_softmax<MT, NE, VW>(p, top, sum, o, a.scale_log2e);
+    if constexpr (!WHOLE) tree_mask<MT, NE>(x, a, at.b, ti, quad, valid, draft, first);
+    tree_softmax<MT, NE, VW>(x, p, top, sum, o, a.scale_log2e);
     if constexpr (!WHOLE) {
 #pragma unroll
       for (int e = 0; e < NE; ++e)
@@ -435,9 +447,9 @@ __global__ __launch_bounds__(kTrThreads, MT == 2 && DP == 128 ? 2 : 1) void tree
 #pragma unroll
     for (int j = 0; j < VW; ++j) o[m][j] *= f;
     if (wave == 0 && quad == 0 && row0 + 16 * m + col < M) {
-      float* dst = a.part_ml + (tile16 + m) * 32 + col * 2;
+      float* dst = a.part_ml + (tile16 + m) * 48 + col;
       dst[0] = all;
-      dst[1] = total;
+      dst[16] = dst[32] = total;
     }
   }
   for (int j0 = 0; j0 < VW; j0 += JC) {
@@ -467,6 +479,13 @@ constexpr int kTlWaves = 4, kTlThreads = kTlWaves * kWave;
 // workgroups per CU, whose waves are at different places, so that one forms exponentials while the other multiplies (as
 // one workgroup of eight waves they did both at the same time: twice as slow).  V's operand is read transposed
 // (ds_read_b64_tr_b16: four keys of one element a lane).
+//
+// FINE: bf16 probabilities as the sum of two bf16 numbers, as in tree_stream_kernel.  Beyond 128 queries a cache head this
+// is bound by the products, and half of those with V are the second number's (64 drafts over 4 x 64K, 32 / 8 heads: 370
+// instead of 450 us without it; 25 drafts over 128K, bound by the reading: 106 instead of 111).  There the probabilities
+// are rounded to bf16, 2^-9 of each, independently of each other, and what they are divided by is the sum of the rounded
+// ones (one more block of o), so that a result is off by what its rounding to bf16 is off by once more; lse keeps the exact
+// ones' sum.
 template <typename T, int DP, int WR>
 struct TreeShare {
   static constexpr int MT = DP == 256 ? 1 : 2, WK = kTlWaves / WR;
@@ -495,7 +514,7 @@ struct TreeShare {
   }
 };
 
-template <typename T, int DP, int WR>
+template <typename T, int DP, int WR, bool FINE>
 __global__ __launch_bounds__(kTlThreads, 2) void tree_share_kernel(TreeArgs a) {
   using Share = TreeShare<T, DP, WR>;
   constexpr int MT = Share::MT, WK = Share::WK;
@@ -503,7 +522,7 @@ __global__ __launch_bounds__(kTlThreads, 2) void tree_share_kernel(TreeArgs a) {
   constexpr int NU = Tile::NU, KT = Tile::KT, NE = Tile::NE, STEPS = Tile::STEPS, VW = Tile::VW, CH = Tile::CH, KL = Tile::KL;
   constexpr int E = (int)sizeof(T), RPL = kWave / CH, LPW = Share::LPW, JC = Share::JC;
   __shared__ ar_u4 smem[Share::SMEM];
-  __shared__ float ml[kTlWaves][MT][16][2];
+  __shared__ float ml[kTlWaves][MT][16][3];
   TreePlace<T> at;
   if (!at.find(a, KT)) return;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), col = lane & 15, quad = lane >> 4;
@@ -512,7 +531,8 @@ __global__ __launch_bounds__(kTlThreads, 2) void tree_share_kernel(TreeArgs a) {
   const int pieces = a.d * E / 16;
   ar_u4 qf[MT][STEPS];
   int ti[MT];   // drafted token of the lane's query
-  ar_f4 o[MT][VW] = {};
+  constexpr int OB = VW + (FINE ? 0 : 1);   // blocks of o, the last one of the sums
+  ar_f4 o[MT][OB] = {};
   float top[MT], sum[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -529,6 +549,15 @@ __global__ __launch_bounds__(kTlThreads, 2) void tree_share_kernel(TreeArgs a) {
   const int piece = lane % CH, krow = lane / CH;
   const uint32_t place = 16u * (uint32_t)min(piece, pieces - 1), krs = (uint32_t)a.kv_r * E;
   ar_u4 ring[Share::AHEAD][LPW];
+  uint32_t from[LPW];   // of a whole tile of the cache: bytes from its first row of K or V
+#pragma unroll
+  for (int i = 0; i < LPW; ++i) from[i] = (uint32_t)(min(l0 + i, 2 * KL - 1) % KL * RPL + krow) * krs + place;
+  auto load_whole = [&](int step, ar_u4 (&g)[LPW]) {
+    const int64_t at_tile = (int64_t)(begin + step * WK + mine) * KT * krs;
+    const char *ks = (const char*)at.kc + at_tile, *vs = (const char*)at.vc + at_tile;
+#pragma unroll
+    for (int i = 0; i < LPW; ++i) g[i] = tree_at<ar_u4>(min(l0 + i, 2 * KL - 1) < KL ? ks : vs, from[i]);
+  };
   auto load = [&](int step, ar_u4 (&g)[LPW]) {
     // (always from a place that exists: loads under a condition were waited for one by one)
     const int tile = min(begin + step * WK + mine, end - 1);
@@ -548,11 +577,11 @@ __global__ __launch_bounds__(kTlThreads, 2) void tree_share_kernel(TreeArgs a) {
 #pragma unroll
   for (int i = 0; i < LPW; ++i) {
     const int l = min(l0 + i, 2 * KL - 1), row = l % KL * RPL + krow;
-    to[i] = (uint32_t)(l < KL ? ar_place<CH>(Tile::place(row), piece) : KT * CH + Share::v_place(row, piece));
+    to[i] = (uint32_t)(mine * Share::TILE) + (uint32_t)(l < KL ? ar_place<CH>(Tile::place(row), piece) : KT * CH + Share::v_place(row, piece));
   }
-  auto store = [&](auto is_whole, int step, ar_u4 (&g)[LPW]) {
+  auto store = [&](auto is_whole, auto buffer, int step, ar_u4 (&g)[LPW]) {
     const int tile = begin + step * WK + mine;
-    ar_u4* dst = smem + ((step & 1) * WK + mine) * Share::TILE;
+    ar_u4* dst = smem + decltype(buffer)::value * WK * Share::TILE;
     if constexpr (!decltype(is_whole)::value) {
       if (tile >= end) return;
       const bool draft = tile >= cached;
@@ -584,88 +613,126 @@ __global__ __launch_bounds__(kTlThreads, 2) void tree_share_kernel(TreeArgs a) {
     for (int j = 0; j < VW; ++j) {
       // keys 8 quad .. + 3 and + 4 .. + 7 of elements 16 j ..: lane i of 16 points to key i / 4, elements 4 (i % 4) ..
       const int row = 8 * quad + (col >> 2), x = 2 * j + ((col >> 1) & 1);
-      vat[j][0] = 16u * (uint32_t)Share::v_place(row, x) + 8u * (uint32_t)(col & 1);
-      vat[j][1] = 16u * (uint32_t)Share::v_place(row + 4, x) + 8u * (uint32_t)(col & 1);
+      vat[j][0] = 16u * (uint32_t)(wk * Share::TILE + KT * CH + Share::v_place(row, x)) + 8u * (uint32_t)(col & 1);
+      vat[j][1] = 16u * (uint32_t)(wk * Share::TILE + KT * CH + Share::v_place(row + 4, x)) + 8u * (uint32_t)(col & 1);
     }
   }
-  auto work = [&](auto is_whole, int step) {
+  uint32_t kat[STEPS];   // where the lane's part of K's operands is (block u: 16 rows further)
+#pragma unroll
+  for (int c = 0; c < STEPS; ++c) kat[c] = (uint32_t)(wk * Share::TILE + ar_place<CH>(col, 4 * c + quad));
+  auto work = [&](auto is_whole, auto buffer, int step) {
     constexpr bool WHOLE = decltype(is_whole)::value;
     const int tile = begin + step * WK + wk;
     if constexpr (!WHOLE)
       if (tile >= end) return;
-    const ar_u4* k_s = smem + ((step & 1) * WK + wk) * Share::TILE;
-    const ar_u4* v_s = k_s + KT * CH;
-    float p[MT][NE];
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      ar_u4 kf[STEPS];
-#pragma unroll
-      for (int c = 0; c < STEPS; ++c) kf[c] = k_s[ar_place<CH>(16 * u + col, 4 * c + quad)];
-      ar_f4 s[MT] = {};
+    const ar_u4* tile_s = smem + decltype(buffer)::value * WK * Share::TILE;   // (the buffer's offset is the instructions')
+    float x[MT][NE], p[MT][NE];
+    {
+      ar_u4 kf[NU][STEPS];
 #pragma unroll
       for (int c = 0; c < STEPS; ++c)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) s[m] = ar_step<T>(kf[c], qf[m][c], s[m]);
+        for (int u = 0; u < NU; ++u) kf[u][c] = (tile_s + 16 * u * CH)[kat[c]];   // (16 rows on, pieces change places alike)
+      ar_f4 s[NU][MT] = {};
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int c = 0; c < STEPS; ++c)   // (NU MT sums side by side: one waits for none of its own)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[m][4 * u + r] = s[m][r];
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) s[u][m] = ar_step<T>(kf[u][c], qf[m][c], s[u][m]);
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[m][4 * u + r] = s[u][m][r];
     }
     if constexpr (!WHOLE) {
       const bool draft = tile >= cached;
       const int first = (draft ? tile - cached : tile) * KT, valid = min(KT, (draft ? a.t : len) - first);
-      if (draft || valid < KT) tree_mask<MT, NE>(p, a, at.b, ti, quad, valid, draft, first);
+      if (draft || valid < KT) tree_mask<MT, NE>(x, a, at.b, ti, quad, valid, draft, first);
     }
-    tree_softmax<MT, NE, VW>(p, top, sum, o, a.scale_log2e);
+    constexpr int VB = VW < 4 ? VW : 4;   // blocks of V's operands at a time
+    auto operand = [&](int j) {
+      const tr_v4s b0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_v4s)((const char*)tile_s + vat[j][0]));
+      const tr_v4s b1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_v4s)((const char*)tile_s + vat[j][1]));
+      return __builtin_bit_cast(ar_bf8, __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    ar_bf8 v[Tile::BF ? VB : 1];
+    if constexpr (Tile::BF) {   // (the first ones are on their way while the exponentials are formed)
+#pragma unroll
+      for (int j = 0; j < VB; ++j) v[j] = operand(j);
+    }
+    tree_softmax<MT, NE, OB>(x, p, top, sum, o, a.scale_log2e);
     if constexpr (Tile::BF) {
       ar_bf8 hi[MT], lo[MT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) tree_split(p[m], hi[m], lo[m]);
+      for (int m = 0; m < MT; ++m) {
+        if constexpr (FINE) {
+          tree_split(p[m], hi[m], lo[m]);
+        } else {
+          tr_f8 y;
 #pragma unroll
-      for (int j = 0; j < VW; ++j) {
-        const tr_v4s b0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_v4s)((const char*)v_s + vat[j][0]));
-        const tr_v4s b1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_lds_v4s)((const char*)v_s + vat[j][1]));
-        const ar_bf8 v = __builtin_bit_cast(ar_bf8, __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7));
+          for (int e = 0; e < 8; ++e) y[e] = p[m][e];
+          hi[m] = __builtin_convertvector(y, ar_bf8);
+          const uint32_t one = 0x3f803f80u;
+          o[m][VW] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ar_bf8, ar_u4{one, one, one, one}), hi[m], o[m][VW], 0, 0, 0);
+        }
+      }
 #pragma unroll
-        for (int m = 0; m < MT; ++m) o[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, lo[m], o[m][j], 0, 0, 0);
+      for (int j0 = 0; j0 < VW; j0 += VB) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) o[m][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, hi[m], o[m][j], 0, 0, 0);
+        for (int j = 0; j < VB; ++j)
+#pragma unroll
+          for (int m = 0; m < MT; ++m) o[m][j0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[j], hi[m], o[m][j0 + j], 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < VB; ++j) {
+          if constexpr (FINE) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) o[m][j0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[j], lo[m], o[m][j0 + j], 0, 0, 0);
+          }
+          if (j0 + VB < VW) v[j] = operand(j0 + VB + j);
+        }
       }
     } else {
 #pragma unroll
       for (int j = 0; j < VW; ++j)
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
-          const float v = ((const float*)(v_s + Share::v_place(4 * quad + e, 4 * j + (col >> 2))))[col & 3];
+          const float v = ((const float*)(tile_s + wk * Share::TILE + KT * CH + Share::v_place(4 * quad + e, 4 * j + (col >> 2))))[col & 3];
 #pragma unroll
           for (int m = 0; m < MT; ++m) o[m][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[m][e], o[m][j], 0, 0, 0);
         }
     }
   };
   constexpr int AHEAD = Share::AHEAD;
+  using First = std::integral_constant<int, 0>;
+  using Second = std::integral_constant<int, 1>;
 #pragma unroll
   for (int i = 0; i < AHEAD; ++i) load(i, ring[i]);
-  store(std::false_type{}, 0, ring[0]);
+  store(std::false_type{}, First{}, 0, ring[0]);
   __syncthreads();
   const int wholes = (min(end, len / KT) - begin) / WK;   // steps that have whole tiles only
   int step = 0;
-  for (; step + AHEAD < wholes; step += AHEAD) {
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      load(step + i + AHEAD, ring[i]);
-      work(std::true_type{}, step + i);
-      store(std::true_type{}, step + i + 1, ring[(i + 1) % AHEAD]);
-      __syncthreads();
-    }
+  for (; step + 1 + AHEAD < wholes; step += 2) {
+    load_whole(step + AHEAD, ring[0]);
+    work(std::true_type{}, First{}, step);
+    store(std::true_type{}, Second{}, step + 1, ring[1 % AHEAD]);
+    __syncthreads();
+    load_whole(step + 1 + AHEAD, ring[1 % AHEAD]);
+    work(std::true_type{}, Second{}, step + 1);
+    store(std::true_type{}, First{}, step + 2, ring[0]);
+    __syncthreads();
   }
-  for (; step < steps; step += AHEAD) {
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {   // (steps behind the last have no tile)
-      load(step + i + AHEAD, ring[i]);
-      work(std::false_type{}, step + i);
-      store(std::false_type{}, step + i + 1, ring[(i + 1) % AHEAD]);
-      __syncthreads();
-    }
+  for (; step < steps; step += 2) {   // (steps behind the last have no tile)
+    load(step + AHEAD, ring[0]);
+    work(std::false_type{}, First{}, step);
+    store(std::false_type{}, Second{}, step + 1, ring[1 % AHEAD]);
+    __syncthreads();
+    load(step + 1 + AHEAD, ring[1 % AHEAD]);
+    work(std::false_type{}, Second{}, step + 1);
+    store(std::false_type{}, First{}, step + 2, ring[0]);
+    __syncthreads();
   }
 
   odd = __syncthreads_or(odd);
@@ -679,27 +746,33 @@ __global__ __launch_bounds__(kTlThreads, 2) void tree_share_kernel(TreeArgs a) {
       if (quad == 0) {
         ml[wave][m][col][0] = top[m];
         ml[wave][m][col][1] = sum[m];
+        ml[wave][m][col][2] = FINE ? sum[m] : o[m][OB - 1][0];   // (every row of that block is the sum)
       }
     __syncthreads();
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    float all = top[m], total = sum[m];
+    float all = top[m], total = sum[m], norm = FINE ? sum[m] : o[m][OB - 1][0];
     if constexpr (WK > 1) {
       all = ml[wr][m][col][0];
 #pragma unroll
       for (int w = 1; w < WK; ++w) all = fmaxf(all, ml[w * WR + wr][m][col][0]);
-      total = 0.0f;
+      total = norm = 0.0f;
 #pragma unroll
-      for (int w = 0; w < WK; ++w) total += ml[w * WR + wr][m][col][1] * ar_exp2(ml[w * WR + wr][m][col][0] - all);
+      for (int w = 0; w < WK; ++w) {
+        const float f = ar_exp2(ml[w * WR + wr][m][col][0] - all);
+        total += ml[w * WR + wr][m][col][1] * f;
+        norm += ml[w * WR + wr][m][col][2] * f;
+      }
       const float f = ar_exp2(top[m] - all);
 #pragma unroll
       for (int j = 0; j < VW; ++j) o[m][j] *= f;
     }
     if (wk == 0 && quad == 0 && row0 + 16 * m + col < M) {
-      float* dst = a.part_ml + (tile16 + m) * 32 + col * 2;
+      float* dst = a.part_ml + (tile16 + m) * 48 + col;
       dst[0] = all;
-      dst[1] = total;
+      dst[16] = total;
+      dst[32] = norm;
     }
   }
   if constexpr (WK == 1) {
@@ -733,20 +806,18 @@ __global__ __launch_bounds__(kTlThreads, 2) void tree_share_kernel(TreeArgs a) {
 // A workgroup joins the splits' parts of 16 queries of a cache head, a quad of the lanes that hold them (a quarter of the
 // head): 16 threads with a query each for (block j of the output, every G-th split).  SHARED: which of the two kernels left
 // the parts, whose lanes have other elements.
-template <typename T, int DP, bool SHARED>
-__global__ __launch_bounds__(kTrCombThreads) void tree_join_kernel(TreeArgs a) {
-  constexpr int VW = DP / 16, GROUPS = kTrCombThreads / 16, G = GROUPS / VW, KT = sizeof(T) == 2 ? 32 : 16, FIRST = 4;
+template <typename T, int DP, bool SHARED, int THREADS>
+__global__ __launch_bounds__(THREADS) void tree_join_kernel(TreeArgs a) {
+  constexpr int VW = DP / 16, GROUPS = THREADS / 16, G = GROUPS / VW, FIRST = 4;
   __shared__ float f_s[kTrMaxSplits][16];
-  __shared__ float red[GROUPS][16];
-  __shared__ float top_s[16], sum_s[16];
+  __shared__ float red[GROUPS][16], red2[GROUPS][16];
+  __shared__ float top_s[16], sum_s[16], norm_s[16];
   __shared__ ar_f4 joint[G][VW][16];
   const int col = threadIdx.x & 15, group = threadIdx.x >> 4;
   const int quad = (int)blockIdx.x & 3, tile = (int)(blockIdx.x >> 2) % a.row_tiles, head = (int)(blockIdx.x >> 2) / a.row_tiles;
   const int M = a.hq / a.hc * a.t, row0 = 16 * tile, b = head / a.hc;
-  TreeCut cut;
-  cut.find(a, KT, -1, b);
-  const int S = min(cut.splits, kTrMaxSplits);
-  const int64_t unit0 = (int64_t)cut.slot0 * a.hc + head % a.hc;   // + split * hc
+  const int S = a.cut[2 * b + 1];
+  const int64_t unit0 = (int64_t)a.cut[2 * b] * a.hc + head % a.hc;   // + split * hc
   const bool mine = row0 + col < M;
   // (the first parts are asked for before their weights are known)
   const int j = group % VW, g = group / VW;
@@ -756,11 +827,13 @@ __global__ __launch_bounds__(kTrCombThreads) void tree_join_kernel(TreeArgs a) {
 #pragma unroll
   for (int i = 0; i < FIRST; ++i)
     early[i] = mine ? part[min(g + i * G, S - 1) * next] : ar_f4{0.0f, 0.0f, 0.0f, 0.0f};
+  const float* ml = a.part_ml + (unit0 * a.row_tiles + tile) * 48 + col;
+  const int64_t ml_next = (int64_t)a.hc * a.row_tiles * 48;
   float top = kTrNone;
   bool odd = false;
   for (int s = group; s < S; s += GROUPS) {
     odd = odd | (a.odd[(unit0 + (int64_t)s * a.hc) * a.row_blocks + row0 / a.rows] != 0);
-    const float x = mine ? a.part_ml[((unit0 + (int64_t)s * a.hc) * a.row_tiles + tile) * 32 + col * 2] : kTrNone;
+    const float x = mine ? ml[s * ml_next] : kTrNone;
     f_s[s][col] = x;
     top = fmaxf(top, x);
   }
@@ -772,18 +845,23 @@ __global__ __launch_bounds__(kTrCombThreads) void tree_join_kernel(TreeArgs a) {
     top_s[col] = x;
   }
   __syncthreads();
-  float total = 0.0f;
+  float total = 0.0f, norm = 0.0f;
   for (int s = group; s < S; s += GROUPS) {
     const float f = ar_exp2(f_s[s][col] - top_s[col]);
     f_s[s][col] = f;
-    if (mine) total += f * a.part_ml[((unit0 + (int64_t)s * a.hc) * a.row_tiles + tile) * 32 + col * 2 + 1];
+    if (mine) {
+      total += f * ml[s * ml_next + 16];
+      norm += f * ml[s * ml_next + 32];
+    }
   }
   red[group][col] = total;
+  red2[group][col] = norm;
   __syncthreads();
-  if (threadIdx.x < 16) {
-    float x = red[0][col];
-    for (int i = 1; i < min(S, GROUPS); ++i) x += red[i][col];
-    sum_s[col] = x;
+  if (threadIdx.x < 32) {
+    const float(&r)[GROUPS][16] = threadIdx.x < 16 ? red : red2;
+    float x = r[0][col];
+    for (int i = 1; i < min(S, GROUPS); ++i) x += r[i][col];
+    (threadIdx.x < 16 ? sum_s : norm_s)[col] = x;
   }
   ar_f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -796,7 +874,7 @@ __global__ __launch_bounds__(kTrCombThreads) void tree_join_kernel(TreeArgs a) {
   joint[g][j][col] = x;
   __syncthreads();
   const int64_t row = (int64_t)head * M + row0;   // rows of all heads follow each other
-  for (int e = threadIdx.x; e < 16 * 4 * VW; e += kTrCombThreads) {
+  for (int e = threadIdx.x; e < 16 * 4 * VW; e += THREADS) {
     const int r = e / (4 * VW), y = e % (4 * VW);
     const int blk = SHARED ? y / 4 : y % VW, i = SHARED ? y % 4 : y / VW;
     const int d = SHARED ? 16 * blk + 4 * quad + i : 4 * VW * quad + y;
@@ -813,7 +891,7 @@ __global__ __launch_bounds__(kTrCombThreads) void tree_join_kernel(TreeArgs a) {
         if (sees[k] && !(fabsf(z) < INFINITY)) v += z;
       }
     }
-    st_f32((T*)a.out, (row + r) * a.d + d, sum_s[r] == 0.0f ? 0.0f : v / sum_s[r]);
+    st_f32((T*)a.out, (row + r) * a.d + d, norm_s[r] == 0.0f ? 0.0f : v / norm_s[r]);
   }
   if (a.lse && quad == 0 && threadIdx.x < 16 && mine)
     a.lse[row + col] = sum_s[col] == 0.0f ? -INFINITY : (top_s[col] + log2f(sum_s[col])) * kLn2;
@@ -822,13 +900,15 @@ __global__ __launch_bounds__(kTrCombThreads) void tree_join_kernel(TreeArgs a) {
 // How a call is cut up, from its sizes alone.
 struct TreePlan {
   int dp, mt, wr;                    // wr = 0: tree_stream_kernel
+  bool fine;
   int rows, row_blocks, row_tiles, splits, least, units;
-  int64_t part, ml, odd;             // words of 4 bytes
+  int64_t part, ml, odd, cut;        // words of 4 bytes
 };
 static TreePlan tree_plan(int b, int hq, int hc, int t, int64_t n, int d, bool lengths, int dtype) {
   TreePlan p;
   p.dp = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256;
   const int64_t M = (int64_t)(hq / hc) * t;
+  p.fine = dtype == LRQK_F32 || M <= 128;
   const int kt = dtype == LRQK_BF16 ? 32 : 16;
   const int64_t tiles = (n + kt - 1) / kt + (t + kt - 1) / kt;
   int64_t groups_wanted, least;
@@ -854,11 +934,20 @@ static TreePlan tree_plan(int b, int hq, int hc, int t, int64_t n, int d, bool l
   p.units = (int)(hc * slots);
   const int64_t groups = (int64_t)p.units * p.row_tiles;
   p.part = groups * 16 * p.dp;
-  p.ml = groups * 32;
+  p.ml = groups * 48;
   p.odd = (int64_t)p.units * p.row_blocks;
+  p.cut = 2 * (int64_t)b;
   return p;
 }
 
+// (few workgroups: more threads for the splits of each)
+template <typename T, int DP, bool SHARED>
+static void tree_join_launch(const TreeArgs& a, dim3 grid, hipStream_t st) {
+  if (grid.x <= 512)
+    hipLaunchKernelGGL((tree_join_kernel<T, DP, SHARED, 512>), grid, dim3(512), 0, st, a);
+  else
+    hipLaunchKernelGGL((tree_join_kernel<T, DP, SHARED, 256>), grid, dim3(256), 0, st, a);
+}
 template <typename T, int DP>
 static int tree_launch(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)(a.units + 7) / 8 * 8 * a.row_blocks));
@@ -868,13 +957,15 @@ static int tree_launch(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
       if (p.mt == 2) hipLaunchKernelGGL((tree_stream_kernel<T, DP, 2>), grid, dim3(kTrThreads), 0, st, a);
     if (p.mt == 1) hipLaunchKernelGGL((tree_stream_kernel<T, DP, 1>), grid, dim3(kTrThreads), 0, st, a);
     LRQK_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL((tree_join_kernel<T, DP, false>), join, dim3(kTrCombThreads), 0, st, a);
+    tree_join_launch<T, DP, false>(a, join, st);
   } else {
     if constexpr (DP < 256)
-      if (p.wr == 2) hipLaunchKernelGGL((tree_share_kernel<T, DP, 2>), grid, dim3(kTlThreads), 0, st, a);
-    if (p.wr == 4) hipLaunchKernelGGL((tree_share_kernel<T, DP, 4>), grid, dim3(kTlThreads), 0, st, a);
+      if (p.wr == 2) hipLaunchKernelGGL((tree_share_kernel<T, DP, 2, true>), grid, dim3(kTlThreads), 0, st, a);
+    if constexpr (sizeof(T) == 2)
+      if (p.wr == 4 && !p.fine) hipLaunchKernelGGL((tree_share_kernel<T, DP, 4, false>), grid, dim3(kTlThreads), 0, st, a);
+    if (p.wr == 4 && p.fine) hipLaunchKernelGGL((tree_share_kernel<T, DP, 4, true>), grid, dim3(kTlThreads), 0, st, a);
     LRQK_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL((tree_join_kernel<T, DP, true>), join, dim3(kTrCombThreads), 0, st, a);
+    tree_join_launch<T, DP, true>(a, join, st);
   }
   LRQK_HIP_CHECK(hipGetLastError());
   return LRQK_OK;
@@ -907,7 +998,7 @@ extern "C" int64_t lrqk_tree_attention_workspace(int b, int hq, int hc, int t, i
   const int rc = tree_check(b, hq, hc, t, n, d, dtype);
   if (rc) return rc;
   const TreePlan p = tree_plan(b, hq, hc, t, n, d, have_lengths != 0, dtype);
-  return (p.part + p.ml + p.odd) * (int64_t)sizeof(float);
+  return (p.part + p.ml + p.odd + p.cut) * (int64_t)sizeof(float);
 }
 
 extern "C" int lrqk_tree_attention(const void* q, const void* k_cache, const void* v_cache, int64_t kv_batch_stride,
@@ -928,11 +1019,11 @@ extern "C" int lrqk_tree_attention(const void* q, const void* k_cache, const voi
   LRQK_REQUIRE(kv_row_stride >= 0 && kv_row_stride <= (1 << 24), LRQK_ELIMIT, "kv_row_stride=%lld (at most 2^24 elements)",
                (long long)kv_row_stride);
   const TreePlan p = tree_plan(b, hq, hc, t, n, d, lengths != nullptr, dtype);
-  const int64_t need = (p.part + p.ml + p.odd) * (int64_t)sizeof(float);
+  const int64_t need = (p.part + p.ml + p.odd + p.cut) * (int64_t)sizeof(float);
   LRQK_REQUIRE(workspace_bytes >= need, LRQK_EINVAL, "workspace of %lld bytes: %lld are needed", (long long)workspace_bytes,
                (long long)need);
   TreeArgs a{q, k_cache, v_cache, k_new, v_new, mask, lengths, out, lse, (float*)workspace, (float*)workspace + p.part,
-             (int32_t*)workspace + p.part + p.ml,
+             (int32_t*)workspace + p.part + p.ml, (int32_t*)workspace + p.part + p.ml + p.odd,
              kv_batch_stride, kv_head_stride, kv_row_stride, mask_batch_stride, b, (int)n, hq, hc, hn, t, d, p.splits, p.least, p.row_blocks, p.rows,
              p.row_tiles, p.units,
              scale * kLog2e};

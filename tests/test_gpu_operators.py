@@ -223,9 +223,10 @@ def _tree64(q, kc, vc, kn, vn, mask, lengths, scale):
                 o = o + torch.where(sees[:, j:j + 1] & odd[j], v[j], 0.0)
             out[i, h] = o
             lse[i, h] = torch.where(some, (top + torch.log(l))[:, 0], -INF)
-            # numerator and denominator: the exponents, the sums (m + t addends, joined over waves and splits), and the
-            # 16 bits of a bf16 probability
-            each = 2 * ds + U * (m + t + 64) * 2 + (2.0 ** -16 if q.dtype == BF else 0.0)
+            # numerator and denominator: the exponents, the sums (m + t addends, joined over waves and splits), and a bf16
+            # probability's 16 bits, or 8 (half a step of the numerator's and of the denominator's) beyond 128 queries a head
+            few = hq // hc * t <= 128
+            each = 2 * ds + U * (m + t + 64) * 2 + (0.0 if q.dtype == FP else 2.0 ** -16 if few else 2 * HALF[BF])
             mag = w.nan_to_num(0) @ torch.where(odd, 0.0, v.abs())
             tol[i, h] = each[:, None] * mag + HALF[q.dtype] * o.nan_to_num(0, 0, 0).abs()
             tol_l[i, h] = ds + U * (m + t + 64) + 4 * U * lse[i, h].nan_to_num(0, 0, 0).abs()
