@@ -3,6 +3,8 @@ current stream; every computation below happens in liblrqk_hip.so."""
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 import threading
 from typing import Optional, Tuple
 
@@ -512,39 +514,54 @@ def decode_step(ws: Workspace, b_q, b_k, a_k, active_idx, k_act, v_act, kv_store
 # These calls take no workspace object: their scratch comes from torch for the call's stream, so that several streams and
 # captured graphs need not share any.
 
-def _launch(t: torch.Tensor, fn, *args) -> int:
-    """The library call on t's device and its current stream."""
-    if torch.cuda.current_device() == t.get_device():
-        return check(fn(*args, _stream(t)))
-    with torch.cuda.device(t.device):
-        return check(fn(*args, _stream(t)))
+# (A call of a few tokens is bound by its host time, so sizes, types and devices are compared as they are: no device objects,
+# no tuples, and the scratch sizes of a set of sizes are asked for once.)
+
+def _launch(dev: int, fn, *args) -> int:
+    """The library call on device ``dev`` and its current stream."""
+    if torch.cuda.current_device() == dev:
+        return check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
+    with torch.cuda.device(dev):
+        return check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
 
 
-def _on_one_gpu(first: torch.Tensor, *ts):
-    _need_cuda(first, *ts)
+def _on_one_gpu(first: torch.Tensor, *ts) -> int:
+    dev = first.get_device()
+    if dev < 0:
+        raise ValueError("tensor must live on the GPU")
     for t in ts:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors on {first.device} and {t.device}")
+    return dev
 
 
 def _expect(name: str, t: torch.Tensor, shape, dtype, contiguous: bool = True):
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+    if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"{name} is {tuple(t.shape)} {t.dtype}: {tuple(shape)} {dtype} is wanted")
     if contiguous and not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
 
 
 def _row_strides(name: str, t: torch.Tensor):
-    """Strides of a cache [b,H,n,d] whose rows are contiguous."""
+    """Strides of sequences, heads and rows of a tensor whose rows are contiguous."""
     s = t.stride()
-    if t.shape[3] > 1 and s[3] != 1:
+    if s[3] != 1 and t.shape[3] > 1:
         raise ValueError(f"the rows of {name} must be contiguous")
-    return s[0], s[1], s[2]
+    return s[:3]
 
 
 def _lengths(lengths: Optional[torch.Tensor], b: int):
     if lengths is not None:
         _expect("lengths", lengths, (b,), torch.int32)
+
+
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(entry: str, *sizes: int) -> int:
+    return check(getattr(_lib.load(), entry)(*sizes))
+
+
+def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
 
 
 class RotaryPlan:
@@ -603,12 +620,13 @@ def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positio
     its input or apart from both inputs; else new contiguous tensors.  ``transpose`` turns back: the gradient of the turn.
     Returns (q', k'), or q' without a k."""
     pos = positions if isinstance(positions, torch.Tensor) else None
-    _on_one_gpu(q, k, pos, plan.inv_freq)
+    dev = _on_one_gpu(q, k, pos, plan.inv_freq)
     b, hq, s, d = q.shape
-    hk = 0 if k is None else k.shape[1]
-    xs = (q,) if k is None else (q, k)
-    if k is not None and (tuple(k.shape) != (b, hk, s, d) or k.dtype != q.dtype):
-        raise ValueError(f"k is {tuple(k.shape)} {k.dtype} beside q {tuple(q.shape)} {q.dtype}")
+    hk = 0
+    if k is not None:
+        hk = k.shape[1]
+        if k.shape != (b, hk, s, d) or k.dtype != q.dtype:
+            raise ValueError(f"k is {tuple(k.shape)} {k.dtype} beside q {tuple(q.shape)} {q.dtype}")
     if plan.rotary_dim > d:
         raise ValueError(f"a plan of {plan.rotary_dim} elements for heads of {d}")
     dt = _dt(q)
@@ -621,10 +639,13 @@ def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positio
         _expect("positions", pos, (b, s) if pos.dim() == 2 else (s,), torch.int32, contiguous=False)
         if s > 1 and pos.stride(-1) != 1:
             raise ValueError("positions of a sequence must be contiguous")
-        pos_stride = pos.stride(0) if pos.dim() == 2 else 0
+        if pos.dim() == 2:
+            pos_stride = pos.stride(0)
     if out is None:
-        ys = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
+        xs = (q,) if k is None else (q, k)
         ys = tuple(out)[:len(xs)] if isinstance(out, (tuple, list)) else (out,)
         if len(ys) != len(xs) or any(y is None for y in ys):
             raise ValueError("out holds one tensor for q, and one for k if there is a k")
@@ -635,14 +656,15 @@ def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positio
                 raise ValueError("out has several elements in one place")
             if not _same_view(x, y) and not all(_apart(y, z) for z in xs):
                 raise ValueError("out overlaps an input and is not the view that is turned")
-    strides = []
-    for x, y in zip(xs, ys):
-        strides += [*_row_strides("q, k", x), *_row_strides("out", y)]
+        q_out, k_out = ys if k is not None else (ys[0], None)
+    strides = (*_row_strides("q", q), *_row_strides("out", q_out))
+    if k is not None:
+        strides += (*_row_strides("k", k), *_row_strides("out", k_out))
     if b * s > 0:
-        _launch(q, _lib.load().lrqk_rotary, q.data_ptr(), _ptr(k), ys[0].data_ptr(), ys[1].data_ptr() if hk else None,
-                (ctypes.c_int64 * len(strides))(*strides), _ptr(pos), pos_stride, first, plan.inv_freq.data_ptr(), plan.factor,
-                b, hq, hk, s, d, plan.rotary_dim, int(plan.interleaved), int(transpose), dt)
-    return ys if k is not None else ys[0]
+        _launch(dev, _lib.load().lrqk_rotary, q.data_ptr(), _ptr(k), q_out.data_ptr(), _ptr(k_out),
+                struct.pack(f"{len(strides)}q", *strides), _ptr(pos), pos_stride, first, plan.inv_freq.data_ptr(), plan.factor,
+                b, hq, hk, s, d, plan.rotary_dim, plan.interleaved, transpose, dt)
+    return q_out if k is None else (q_out, k_out)
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
@@ -655,30 +677,31 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     [t,t] or [b,t,t]: drafted token i sees j.  Hc = Hn for a dense cache, Hc = Hq for an active set (``engine.Kgpu``).
     ``scale`` (1 / sqrt(d) if None) is positive.  -> [b,Hq,t,d], zeros for a token that sees nothing; with ``return_lse``
     also fp32 [b,Hq,t], the logarithm of the sum of the exponentials (-inf for such a token)."""
-    _on_one_gpu(q, k_cache, v_cache, k_new, v_new, mask, lengths)
+    dev = _on_one_gpu(q, k_cache, v_cache, k_new, v_new, mask, lengths)
     b, hq, t, d = q.shape
-    hc, n, hn = k_cache.shape[1], k_cache.shape[2], k_new.shape[1]
-    dt = _dt(q)
-    _expect("k_cache", k_cache, (b, hc, n, d), q.dtype, contiguous=False)
-    _expect("v_cache", v_cache, (b, hc, n, d), q.dtype, contiguous=False)
-    _expect("k_new", k_new, (b, hn, t, d), q.dtype, contiguous=False)
-    _expect("v_new", v_new, (b, hn, t, d), q.dtype, contiguous=False)
+    _, hc, n, _ = k_cache.shape
+    hn = k_new.shape[1]
+    dt, dtype = _dt(q), q.dtype
+    _expect("k_cache", k_cache, (b, hc, n, d), dtype, contiguous=False)
+    _expect("v_cache", v_cache, (b, hc, n, d), dtype, contiguous=False)
+    _expect("k_new", k_new, (b, hn, t, d), dtype, contiguous=False)
+    _expect("v_new", v_new, (b, hn, t, d), dtype, contiguous=False)
     if hc == 0 or hn == 0 or hq % hc or hc % hn:
         raise ValueError(f"{hq} query heads, {hc} heads of the cache, {hn} of the drafted tokens: each a multiple of the next")
-    if tuple(mask.shape) not in ((t, t), (b, t, t)) or mask.dtype not in (torch.bool, torch.uint8):
+    if mask.shape not in ((b, t, t), (t, t)) or mask.dtype not in (torch.bool, torch.uint8):
         raise ValueError(f"mask is {tuple(mask.shape)} {mask.dtype}: bool or uint8 [t,t] or [b,t,t] is wanted")
     _lengths(lengths, b)
     st = _row_strides("k_cache", k_cache)
     if _row_strides("v_cache", v_cache) != st and n > 0:
         raise ValueError("k_cache and v_cache must have the same strides")
-    out = torch.empty((b, hq, t, d), dtype=q.dtype, device=q.device)
+    q = q.contiguous()
+    out = torch.empty_like(q)
     lse = torch.empty((b, hq, t), dtype=torch.float32, device=q.device) if return_lse else None
     if b * hq * t:
-        lib = _lib.load()
-        q, k_new, v_new, mask = q.contiguous(), k_new.contiguous(), v_new.contiguous(), mask.contiguous()
-        need = check(lib.lrqk_tree_attention_workspace(b, hq, hc, t, n, d, int(lengths is not None), dt))
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _launch(q, lib.lrqk_tree_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *st, n, _ptr(lengths),
+        k_new, v_new, mask = k_new.contiguous(), v_new.contiguous(), mask.contiguous()
+        need = _scratch_bytes("lrqk_tree_attention_workspace", b, hq, hc, t, n, d, lengths is not None, dt)
+        ws = _scratch(need, q)
+        _launch(dev, _lib.load().lrqk_tree_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *st, n, _ptr(lengths),
                 k_new.data_ptr(), v_new.data_ptr(), mask.data_ptr(), t * t if mask.dim() == 3 else 0, out.data_ptr(), _ptr(lse), b,
                 hq, hc, hn, t, d, d ** -0.5 if scale is None else float(scale), ws.data_ptr(), need, dt)
     return (out, lse) if return_lse else out
@@ -694,7 +717,7 @@ def attention_weights(q: torch.Tensor, k: torch.Tensor, lengths: Optional[torch.
     (``tree_attention(return_lse=True)``; a query of -inf adds nothing); without it they are formed here.  -> fp32 [b,Hc,n]:
     ``weights`` (0 if None) plus the sums over the query heads of each head and over the tokens, in ``out`` if that is given,
     else in place if there are weights."""
-    _on_one_gpu(q, k, lengths, lse, weights, out)
+    dev = _on_one_gpu(q, k, lengths, lse, weights, out)
     b, hq, t, d = q.shape
     hc, n = k.shape[1], k.shape[2]
     dt = _dt(q)
@@ -716,11 +739,10 @@ def attention_weights(q: torch.Tensor, k: torch.Tensor, lengths: Optional[torch.
         return out
     if t == 0:
         return out.copy_(weights) if weights is not None else out.zero_()
-    lib = _lib.load()
     q = q.contiguous()
-    need = check(lib.lrqk_attention_weights_workspace(b, hq, hc, t, n, d, int(lse is not None), dt))
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _launch(q, lib.lrqk_attention_weights, q.data_ptr(), k.data_ptr(), *_row_strides("k", k), n, _ptr(lengths), _ptr(lse),
+    need = _scratch_bytes("lrqk_attention_weights_workspace", b, hq, hc, t, n, d, lse is not None, dt)
+    ws = _scratch(need, q) if need else None
+    _launch(dev, _lib.load().lrqk_attention_weights, q.data_ptr(), k.data_ptr(), *_row_strides("k", k), n, _ptr(lengths), _ptr(lse),
             _ptr(weights), out.data_ptr(), b, hq, hc, t, d, d ** -0.5 if scale is None else float(scale), _ptr(ws), need, dt)
     return out
 
@@ -735,7 +757,7 @@ def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Te
     slot if that is one of the first ``budget``; the others move, in order, into the slots that became free.  In place, or
     into ``out`` = (weights, ids, k, v), buffers of at least min(budget, n) slots that are apart from the inputs; slots behind
     the tokens that stay are left as they were.  -> the new lengths, int32 [b]."""
-    _on_one_gpu(weights, ids, k, v, lengths, *(out or ()))
+    dev = _on_one_gpu(weights, ids, k, v, lengths, *(out or ()))
     b, h, n, d = k.shape
     dt = _dt(k)
     _expect("weights", weights, (b, h, n), torch.float32)
@@ -762,13 +784,11 @@ def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Te
     new = torch.empty((b,), dtype=torch.int32, device=k.device)
     if b * h * n == 0:
         return new.zero_()
-    lib = _lib.load()
     budget = min(budget, 2 ** 30)
-    recent = min(recent, budget)
-    need = check(lib.lrqk_evict_workspace(b, h, n, budget))
-    ws = torch.empty(need, dtype=torch.uint8, device=k.device)
-    _launch(k, lib.lrqk_evict, weights.data_ptr(), ids.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths), n, *ptrs, cap_out,
-            new.data_ptr(), b, h, d, budget, recent, ws.data_ptr(), need, dt)
+    need = _scratch_bytes("lrqk_evict_workspace", b, h, n, budget)
+    ws = _scratch(need, k)
+    _launch(dev, _lib.load().lrqk_evict, weights.data_ptr(), ids.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths), n, *ptrs,
+            cap_out, new.data_ptr(), b, h, d, budget, min(recent, budget), ws.data_ptr(), need, dt)
     return new
 
 
