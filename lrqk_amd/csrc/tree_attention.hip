@@ -805,69 +805,74 @@ __global__ __launch_bounds__(kTlThreads, 2) void tree_share_kernel(TreeArgs a) {
 
 // A workgroup joins the splits' parts of 16 queries of a cache head, a quad of the lanes that hold them (a quarter of the
 // head): 16 threads with a query each for (block j of the output, every G-th split).  SHARED: which of the two kernels left
-// the parts, whose lanes have other elements.
+// the parts, whose lanes have other elements.  Its time is a chain of reads that wait for each other and barriers, so the
+// reads are few in a row, and what 16 queries of all waves make is added up by every thread that wants it.
 template <typename T, int DP, bool SHARED, int THREADS>
 __global__ __launch_bounds__(THREADS) void tree_join_kernel(TreeArgs a) {
-  constexpr int VW = DP / 16, GROUPS = THREADS / 16, G = GROUPS / VW, FIRST = 4;
+  constexpr int VW = DP / 16, GROUPS = THREADS / 16, G = GROUPS / VW, FIRST = 4, NW = THREADS / kWave;
   __shared__ float f_s[kTrMaxSplits][16];
-  __shared__ float red[GROUPS][16], red2[GROUPS][16];
-  __shared__ float top_s[16], sum_s[16], norm_s[16];
+  __shared__ float red[3][NW][16];
   __shared__ ar_f4 joint[G][VW][16];
-  const int col = threadIdx.x & 15, group = threadIdx.x >> 4;
+  const int col = threadIdx.x & 15, group = threadIdx.x >> 4, wave = wave_id();
   const int quad = (int)blockIdx.x & 3, tile = (int)(blockIdx.x >> 2) % a.row_tiles, head = (int)(blockIdx.x >> 2) / a.row_tiles;
   const int M = a.hq / a.hc * a.t, row0 = 16 * tile, b = head / a.hc;
-  const int S = a.cut[2 * b + 1];
-  const int64_t unit0 = (int64_t)a.cut[2 * b] * a.hc + head % a.hc;   // + split * hc
+  const int slot0 = a.b == 1 ? 0 : a.cut[2 * b], slots = a.units / a.hc;
+  const int64_t unit0 = (int64_t)slot0 * a.hc + head % a.hc;   // + split * hc
   const bool mine = row0 + col < M;
-  // (the first parts are asked for before their weights are known)
+  // (the first parts are asked for before it is known how many there are: the scratch has room for `slots`, and what is
+  // behind the sequence's is not looked at)
   const int j = group % VW, g = group / VW;
   const ar_f4* part = (const ar_f4*)a.part + ((unit0 * a.row_tiles + tile) * VW + j) * kWave + quad * 16 + col;
   const int64_t next = (int64_t)a.hc * a.row_tiles * VW * kWave;
-  ar_f4 early[FIRST];
-#pragma unroll
-  for (int i = 0; i < FIRST; ++i)
-    early[i] = mine ? part[min(g + i * G, S - 1) * next] : ar_f4{0.0f, 0.0f, 0.0f, 0.0f};
   const float* ml = a.part_ml + (unit0 * a.row_tiles + tile) * 48 + col;
   const int64_t ml_next = (int64_t)a.hc * a.row_tiles * 48;
-  float top = kTrNone;
-  bool odd = false;
-  for (int s = group; s < S; s += GROUPS) {
-    odd = odd | (a.odd[(unit0 + (int64_t)s * a.hc) * a.row_blocks + row0 / a.rows] != 0);
-    const float x = mine ? ml[s * ml_next] : kTrNone;
-    f_s[s][col] = x;
-    top = fmaxf(top, x);
+  const int32_t* odd_at = a.odd + unit0 * a.row_blocks + row0 / a.rows;
+  ar_f4 early[FIRST];
+#pragma unroll
+  for (int i = 0; i < FIRST; ++i) early[i] = part[min(g + i * G, slots - 1 - slot0) * next];
+  // maximum, sums and flag of the thread's first split
+  const int s1 = min(group, slots - 1 - slot0);
+  const float top1 = ml[s1 * ml_next], sum1 = ml[s1 * ml_next + 16], norm1 = ml[s1 * ml_next + 32];
+  const int odd1 = odd_at[(int64_t)s1 * a.hc * a.row_blocks];
+  const int S = a.cut[2 * b + 1];
+  float top = (mine & (group < S)) ? top1 : kTrNone;
+  bool odd = (group < S) & (odd1 != 0);
+  for (int s = group + GROUPS; s < S; s += GROUPS) {
+    odd = odd | (odd_at[(int64_t)s * a.hc * a.row_blocks] != 0);
+    top = fmaxf(top, mine ? ml[s * ml_next] : kTrNone);
   }
-  red[group][col] = top;
+  top = ar_quad_max(top);
+  if (lane_id() < 16) red[0][wave][col] = top;
   odd = __syncthreads_or(odd);
-  if (threadIdx.x < 16) {
-    float x = red[0][col];
-    for (int i = 1; i < min(S, GROUPS); ++i) x = fmaxf(x, red[i][col]);
-    top_s[col] = x;
-  }
-  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < NW; ++w) top = fmaxf(top, red[0][w][col]);
   float total = 0.0f, norm = 0.0f;
-  for (int s = group; s < S; s += GROUPS) {
-    const float f = ar_exp2(f_s[s][col] - top_s[col]);
+  if (group < S) {
+    const float f = mine ? ar_exp2(top1 - top) : 0.0f;
+    f_s[group][col] = f;
+    total = mine ? f * sum1 : 0.0f;
+    norm = mine ? f * norm1 : 0.0f;
+  }
+  for (int s = group + GROUPS; s < S; s += GROUPS) {
+    const float f = mine ? ar_exp2(ml[s * ml_next] - top) : 0.0f;
     f_s[s][col] = f;
     if (mine) {
       total += f * ml[s * ml_next + 16];
       norm += f * ml[s * ml_next + 32];
     }
   }
-  red[group][col] = total;
-  red2[group][col] = norm;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    const float(&r)[GROUPS][16] = threadIdx.x < 16 ? red : red2;
-    float x = r[0][col];
-    for (int i = 1; i < min(S, GROUPS); ++i) x += r[i][col];
-    (threadIdx.x < 16 ? sum_s : norm_s)[col] = x;
+  total = ar_quad_sum(total);
+  norm = ar_quad_sum(norm);
+  if (lane_id() < 16) {
+    red[1][wave][col] = total;
+    red[2][wave][col] = norm;
   }
+  __syncthreads();
   ar_f4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int i = 0; i < FIRST; ++i)
-    if (g + i * G < S) x += early[i] * f_s[g + i * G][col];
   if (mine) {
+#pragma unroll
+    for (int i = 0; i < FIRST; ++i)
+      if (g + i * G < S) x += early[i] * f_s[g + i * G][col];
 #pragma unroll 4
     for (int s = g + FIRST * G; s < S; s += G) x += part[s * next] * f_s[s][col];
   }
@@ -879,9 +884,11 @@ __global__ __launch_bounds__(THREADS) void tree_join_kernel(TreeArgs a) {
     const int blk = SHARED ? y / 4 : y % VW, i = SHARED ? y % 4 : y / VW;
     const int d = SHARED ? 16 * blk + 4 * quad + i : 4 * VW * quad + y;
     if (d >= a.d || row0 + r >= M) continue;
-    float v = 0.0f;
+    float v = 0.0f, all = 0.0f;
 #pragma unroll
     for (int h = 0; h < G; ++h) v += joint[h][blk][r][i];
+#pragma unroll
+    for (int w = 0; w < NW; ++w) all += red[2][w][r];
     if (odd) {
       const int hn = head % a.hc / (a.hc / a.hn);
       const T* vn = (const T*)a.v_new + ((int64_t)b * a.hn + hn) * a.t * a.d + d;
@@ -891,10 +898,14 @@ __global__ __launch_bounds__(THREADS) void tree_join_kernel(TreeArgs a) {
         if (sees[k] && !(fabsf(z) < INFINITY)) v += z;
       }
     }
-    st_f32((T*)a.out, (row + r) * a.d + d, norm_s[r] == 0.0f ? 0.0f : v / norm_s[r]);
+    st_f32((T*)a.out, (row + r) * a.d + d, all == 0.0f ? 0.0f : v / all);
   }
-  if (a.lse && quad == 0 && threadIdx.x < 16 && mine)
-    a.lse[row + col] = sum_s[col] == 0.0f ? -INFINITY : (top_s[col] + log2f(sum_s[col])) * kLn2;
+  if (a.lse && quad == 0 && threadIdx.x < 16 && mine) {
+    float all = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) all += red[1][w][col];
+    a.lse[row + col] = all == 0.0f ? -INFINITY : (top + log2f(all)) * kLn2;
+  }
 }
 
 // How a call is cut up, from its sizes alone.
