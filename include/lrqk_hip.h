@@ -297,7 +297,7 @@ int lrqk_tree_attention(const void* q, const void* k_cache, const void* v_cache,
  * out[b][hc][j] = weights[b][hc][j] (0 if NULL; may be out) + the sum over the hq / hc query heads of the cache head and
  * over the queries i with j <= length - t + i of exp(scale q_i.k_j - lse_i), j < n; tokens behind the length get nothing.
  * q: [b][hq][t][d], k: rows of d elements by strides as above.  lse: fp32 [b][hq][t] as lrqk_tree_attention leaves it
- * (a query of -inf adds nothing), or NULL: of the keys that the query sees here.  weights, out: fp32 [b][hc][n].
+ * (a query of -inf adds nothing, whatever q and k hold), or NULL: of the keys that the query sees here.  weights, out: fp32 [b][hc][n].
  * Deterministic: no atomics.  Workspace as above (with lse none is needed). */
 int64_t lrqk_attention_weights_workspace(int b, int hq, int hc, int t, int64_t n, int d, int have_lse, int dtype);
 int lrqk_attention_weights(const void* q, const void* k, int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,

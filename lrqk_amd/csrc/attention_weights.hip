@@ -308,6 +308,7 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_columns_kernel(WeightAr
     } next[2];
     struct {
       int base, stop, at;
+      bool none;   // some of its queries saw nothing: they give nothing, whatever they hold
     } now{};
     int h = packed ? 0 : begin / per, tt = packed ? begin : t0 + begin % per, left = end - begin;
     auto load = [&](Next& x) {   // the next tile (behind the last one that one again)
@@ -325,11 +326,10 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_columns_kernel(WeightAr
       x.lse = lse[min(x.base + (int)(threadIdx.x % kAwTile), x.stop - 1)];
     };
     auto store = [&](auto buffer, Next& x) {
-      now = {x.base, x.stop, x.at};
-      Tile::store(smem + decltype(buffer)::value * Tile::SIZE, pieces, x.g);
       const float l = x.lse * a.lse_scale;
-      if (threadIdx.x < kAwTile)   // (a query that saw nothing gives nothing)
-        ((float*)lse_s[decltype(buffer)::value])[threadIdx.x] = l == -INFINITY ? INFINITY : l;
+      now = {x.base, x.stop, x.at, __any(l == -INFINITY) != 0};
+      Tile::store(smem + decltype(buffer)::value * Tile::SIZE, pieces, x.g);
+      if (threadIdx.x < kAwTile) ((float*)lse_s[decltype(buffer)::value])[threadIdx.x] = l;
     };
     if (begin < end) {
       load(next[0]);
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_columns_kernel(WeightAr
       const ar_u4* rows = smem + decltype(buffer)::value * Tile::SIZE;
       const int base = now.base, stop = now.stop, at = now.at;
       if (first >= len || (!packed && behind + at + kAwTile - 1 < first)) return;   // (no query sees a key of the wave)
-      const bool whole = base + kAwTile <= stop && first + KEYS - 1 <= behind + at;
+      const bool whole = base + kAwTile <= stop && first + KEYS - 1 <= behind + at && !now.none;
       auto add = [&](auto is_whole) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
@@ -372,7 +372,7 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_columns_kernel(WeightAr
 #pragma unroll
               for (int r = 0; r < 4; ++r) {
                 const int i = 16 * u + 4 * quad + r, last = behind + (packed ? (base + i) % a.t : at + i);
-                const bool sees = (base + i < stop) & (first + 16 * j + col <= last);
+                const bool sees = (base + i < stop) & (first + 16 * j + col <= last) & (l2[r] != -INFINITY);
                 p[r] = sees ? p[r] : 0.0f;
               }
             }
@@ -439,12 +439,14 @@ __global__ __launch_bounds__(kAwThreads, DP * (int)sizeof(T) <= 512 ? 2 : 1) voi
   float l2[NT];
   int last[NT];   // last key that the lane's query sees
   ar_u4 qf[NT][STEPS];
+  bool nones = false;
 #pragma unroll
   for (int m = 0; m < NT; ++m) {
     const int row = min(16 * m + col, M - 1);
-    const float l = a.lse[(int64_t)head * M + row] * a.lse_scale;
-    l2[m] = l == -INFINITY ? INFINITY : l;   // (a query that saw nothing gives nothing)
-    last[m] = 16 * m + col < M ? behind + row % a.t : -1;
+    l2[m] = a.lse[(int64_t)head * M + row] * a.lse_scale;
+    const bool none = l2[m] == -INFINITY;   // (a query that saw nothing gives nothing, whatever it holds)
+    last[m] = ((16 * m + col < M) & !none) ? behind + row % a.t : -1;
+    nones = nones | none;
     ar_row(q + (int64_t)row * a.d, quad, pieces, qf[m]);
   }
   const float* had = a.weights ? a.weights + (int64_t)head * a.n : nullptr;
@@ -452,7 +454,7 @@ __global__ __launch_bounds__(kAwThreads, DP * (int)sizeof(T) <= 512 ? 2 : 1) voi
   const int tiles = (a.n + kAwTile - 1) / kAwTile;
   const int tile0 = (int)(blockIdx.x / a.heads) * a.per + wave, end = min(tiles, (int)(blockIdx.x / a.heads + 1) * a.per);
   // (few queries see a part of the keys of the last tiles, and of the smaller heads' tiles have rows that are none)
-  const int wholes = M == 16 * NT ? max(0, behind + 1) / kAwTile : 0;
+  const int wholes = M == 16 * NT && !__any(nones) ? max(0, behind + 1) / kAwTile : 0;
   const int piece = lane % CH, krow = lane / CH, keys = max(len, 1);
   ar_u4 g[LOADS];
   float w = 0.0f;

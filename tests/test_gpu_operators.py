@@ -601,3 +601,374 @@ def test_evict_refusals(ops):
             bad()
     with pytest.raises(_lib.LrqkError):
         ops.evict(w, ids, k[..., :5].contiguous(), v[..., :5].contiguous(), n, 5, 1)
+
+
+# ----------------------------------------------------------------------------------------------------------- more sizes
+
+@pytest.mark.parametrize("b", [65, 150])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_tree_attention_many_sequences(ops, dtype, b):
+    """More sequences than a wave has lanes, lengths of every kind: the splits' places are counted over all of them."""
+    print("tree many", dtype, b, flush=True)
+    lengths = torch.randint(0, 600, (b,), generator=_gen(b), dtype=torch.int32)
+    lengths[::7], lengths[3::11] = 0, 600
+    lengths = lengths.to(DEV)
+    for t, hq in ((2, 2), (20, 2)):
+        q, kc, vc, kn, vn, mask = _tree_inputs(b, dtype, b, hq, 1, 1, t, 600, 32)
+        _check_tree(ops, q, kc, vc, kn, vn, mask, lengths, what=t)
+    _check_tree(ops, q, kc, vc, kn, vn, mask, None)
+
+
+@pytest.mark.parametrize("t,hq", [(16, 1), (17, 1), (8, 4), (11, 3), (32, 2), (13, 5), (32, 4), (43, 3)])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_tree_attention_at_the_kernels_borders(ops, dtype, t, hq):
+    """16 and 17, 32 and 33, 64 and 65, 128 and 129 queries a cache head."""
+    print("tree borders", dtype, t, hq, flush=True)
+    for d in (64, 256):
+        q, kc, vc, kn, vn, mask = _tree_inputs(t, dtype, 2, hq, 1, 1, t, 333, d)
+        _check_tree(ops, q, kc, vc, kn, vn, mask, torch.tensor([333, 160], dtype=torch.int32, device=DEV), what=d)
+
+
+def test_tree_attention_refuses_rows_too_far_apart(ops):
+    from lrqk_amd import _lib
+    q, _, _, kn, vn, mask = _tree_inputs(1, BF, 1, 1, 1, 1, 2, 1, 8)
+    far = torch.empty(2 ** 24 + 16, dtype=BF, device=DEV).as_strided((1, 1, 2, 8), (0, 0, 2 ** 24 + 8, 1))
+    with pytest.raises(_lib.LrqkError):
+        ops.tree_attention(q, far, far, kn, vn, mask)
+
+
+@pytest.mark.parametrize("t,hq", [(16, 1), (17, 1), (16, 2), (11, 3), (16, 4), (13, 5), (40, 4)])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_attention_weights_at_the_kernels_borders(ops, dtype, t, hq):
+    """16 and 17, 32 and 33, 64 and 65 queries a cache head, with the sums of the attention and without."""
+    print("weights borders", dtype, t, hq, flush=True)
+    g = _gen(t)
+    for d in (32, 64, 128, 256):
+        q, k = _randn(g, 2, 2 * hq, t, d, dtype=dtype, scale=2.0), _randn(g, 2, 2, 300, d, dtype=dtype)
+        lengths = torch.tensor([300, 20], dtype=torch.int32, device=DEV)
+        _check_weights(ops, q, k, lengths, what=d)
+        _check_weights(ops, q, k, lengths, lse=_randn(g, 2, 2 * hq, t) + 3.0, weights=torch.rand((2, 2, 300), generator=g).to(DEV), what=d)
+
+
+def test_attention_weights_far_rows(ops):
+    """Rows and heads whose distances pass 32 bits of elements."""
+    print("weights far", flush=True)
+    g = _gen(11)
+    step, n = 2 ** 24 + 64, 150
+    place = torch.empty(step * n + 2 ** 32 + 128, dtype=BF, device=DEV)
+    for strides in ((0, 64, step, 1), (0, 2 ** 32 + 64, 64, 1)):
+        k = place.as_strided((1, 2, n, 64), strides)
+        k.copy_(_randn(g, 1, 2, n, 64, dtype=BF))
+        for t in (3, 40):
+            q = _randn(g, 1, 4, t, 64, dtype=BF, scale=2.0)
+            assert torch.equal(ops.attention_weights(q, k), ops.attention_weights(q, k.contiguous()))
+            _check_weights(ops, q, k)
+
+
+@pytest.mark.parametrize("n", [4095, 4096, 4097, 12288, 12289, 32768, 32769])
+def test_evict_lengths_around_the_kernels_borders(ops, n):
+    print("evict borders", n, flush=True)
+    g = _gen(n)
+    for over in (127, 128, 129, n // 2):
+        _check_evict(ops, *_cache(g, 1, 2, n, 8, BF), None, n - over, 30, what=over)
+    _check_evict(ops, *_cache(g, 2, 1, n, 16, FP), torch.tensor([n, n - 100], dtype=torch.int32, device=DEV), n - 128, 0)
+
+
+def test_evict_writes_the_lengths_in_place(ops):
+    """The library's own entry with the new lengths in the place of the old ones, many tokens over the budget and few."""
+    from lrqk_amd import _lib
+    print("evict aliased", flush=True)
+    lib, g = _lib.load(), _gen(4)
+    for n, budget in ((1000, 900), (1000, 300)):
+        held = _cache(g, 3, 2, n, 16, BF)
+        lengths = torch.tensor([n, 500, budget - 1], dtype=torch.int32, device=DEV)
+        want = [x.clone() for x in held]
+        new = ops.evict(*want, lengths, budget, 9)
+        need = lib.lrqk_evict_workspace(3, 2, n, budget)
+        ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+        rc = lib.lrqk_evict(*(x.data_ptr() for x in held), lengths.data_ptr(), n, None, None, None, None, n, lengths.data_ptr(), 3, 2, 16,
+                            budget, 9, ws.data_ptr(), need, _lib.BF16, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0 and torch.equal(lengths, new)
+        assert all(torch.equal(x, y) for x, y in zip(held, want))
+
+
+def test_evict_far_rows(ops):
+    """A head of more than 2^31 elements: tokens that move from behind them, one by one and many."""
+    print("evict far", flush=True)
+    n, d = 2 ** 23 + 200, 256
+    g = _gen(6)
+    order = torch.randperm(n, generator=g)
+    weights = order.float().to(DEV).view(1, 1, n)                  # (distinct, and exact in fp32)
+    ids = torch.arange(n, dtype=torch.int32, device=DEV).view(1, 1, n)
+    k = torch.empty((1, 1, n, d), dtype=BF, device=DEV)
+    marks = (torch.arange(n, device=DEV) % 251).to(BF)
+    k.copy_(marks[None, None, :, None].expand(1, 1, n, d))
+    v = -k
+    for budget, in_place in ((1000, False), (n - 100, True)):
+        slots = torch.arange(n)
+        top = torch.where(slots >= n - 8, n + slots, order)        # the 8 newest come first
+        stay = torch.zeros(n, dtype=torch.bool)
+        stay[top.topk(budget).indices] = True
+        source = slots[:budget].clone()
+        source[~stay[:budget]] = slots[budget:][stay[budget:]]
+        source = source.to(DEV)
+        want = weights[0, 0, source], ids[0, 0, source], marks[source]
+        if in_place:
+            out = weights, ids, k, v
+            assert ops.evict(*out, None, budget, 8).tolist() == [budget]
+        else:
+            out = tuple(torch.empty((1, 1, budget, *x.shape[3:]), dtype=x.dtype, device=DEV) for x in (weights, ids, k, v))
+            assert ops.evict(weights, ids, k, v, None, budget, 8, out=out).tolist() == [budget]
+        assert torch.equal(out[0][0, 0, :budget], want[0]) and torch.equal(out[1][0, 0, :budget], want[1])
+        for i in (0, 127, d - 1):
+            assert torch.equal(out[2][0, 0, :budget, i], want[2]) and torch.equal(out[3][0, 0, :budget, i], -want[2])
+
+
+# ------------------------------------------------------------------------------------------------------- all of them
+
+def _tree_of(parents):
+    """(depths, mask) of a tree whose token i follows token parents[i] (-1: the cache)"""
+    t = len(parents)
+    depth, mask = [0] * t, torch.eye(t, dtype=torch.bool)
+    for i, p in enumerate(parents):
+        if p >= 0:
+            depth[i] = depth[p] + 1
+            mask[i] |= mask[p]
+    return torch.tensor(depth, dtype=torch.int32), mask
+
+
+class _Budgeted:
+    """One layer's cache as a decoder of drafted tokens holds it."""
+
+    def __init__(self, b, hc, room, d, dtype):
+        self.k, self.v = (torch.zeros((b, hc, room, d), dtype=dtype, device=DEV) for _ in range(2))
+        self.weights = torch.zeros((b, hc, room), device=DEV)
+        self.ids = torch.zeros((b, hc, room), dtype=torch.int32, device=DEV)
+        self.lengths = torch.zeros(b, dtype=torch.int32, device=DEV)     # tokens that are held
+        self.seen = torch.zeros(b, dtype=torch.int32, device=DEV)        # tokens that there were
+
+    def append(self, paths, k_new, v_new):
+        """The drafted tokens ``paths[i]`` of sequence i, in order."""
+        for i, p in enumerate(paths):
+            n, s, m = int(self.lengths[i]), int(self.seen[i]), len(p)
+            self.k[i, :, n:n + m], self.v[i, :, n:n + m] = k_new[i][:, p], v_new[i][:, p]
+            self.ids[i, :, n:n + m] = torch.arange(s, s + m, dtype=torch.int32, device=DEV)
+            self.weights[i, :, n:n + m] = 0.0
+            self.lengths[i] += m
+            self.seen[i] += m
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("hq,hc,d,rd", [(8, 2, 128, 128), (6, 6, 64, 32), (4, 1, 96, 96)])
+def test_a_decoder_of_drafts_over_a_budget(ops, dtype, hq, hc, d, rd):
+    """Prompt, then rounds of: turn the drafts, attend, accept a path of each sequence, add its attention up, evict.  Every
+    call is held to its formula in 64 bits on what it was given."""
+    print("together", dtype, hq, hc, d, flush=True)
+    b, budget, recent, prompt = 3, 60, 10, 75
+    g = _gen(d)
+    plan = ops.RotaryPlan(rd, 1e4, False, {"type": "yarn", "factor": 4.0, "original_context": 64}, DEV)
+    cache = _Budgeted(b, hc, 100, d, dtype)
+
+    def heads(t):
+        return [_randn(g, b, t, h, d, dtype=dtype, scale=s).transpose(1, 2) for h, s in ((hq, 2.0), (hc, 1.0), (hc, 1.0))]
+
+    # the prompt is a tree without branches over an empty cache; its keys are turned into their slots
+    q, k, v = heads(prompt)
+    q1, k1 = ops.rotary(plan, q, k, 0, out=(torch.empty((b, hq, prompt, d), dtype=dtype, device=DEV), cache.k[:, :, :prompt]))
+    for x, y in ((q, q1), (k, k1)):
+        _check_rotary(plan, x, y, torch.arange(prompt, dtype=torch.int32, device=DEV))
+    chain = torch.ones((prompt, prompt), dtype=torch.bool, device=DEV).tril()
+    out, lse = _check_tree(ops, q1, cache.k, cache.v, k1, v, chain, cache.lengths)
+    cache.append([list(range(prompt))] * b, k1, v)
+    cache.weights = _check_weights(ops, q1, cache.k, cache.lengths, lse, weights=cache.weights)
+    # what a column of the attention matrix adds up to in all is the number of rows
+    assert torch.allclose(cache.weights.sum(-1), torch.full((b, hc), float(prompt * hq // hc), device=DEV), rtol=1e-4)
+    held = cache.weights, cache.ids, cache.k, cache.v
+    _check_evict(ops, *held, cache.lengths, budget, recent)                       # (ends in place)
+    cache.lengths = torch.full((b,), budget, dtype=torch.int32, device=DEV)
+    for step, (parents, paths) in enumerate((([-1, 0, 0, 1, 1, 2, -1, 6], ([0, 1, 4], [6], [0, 2, 5])), ([-1], ([0], [0], [0])),
+                                             ([-1, -1, 1, 2, 3, 4], ([0], [1, 2, 3, 4, 5], [1])),
+                                             ([-1, 0, 1, 2, 0, 4, 4, -1, 7, 8, 9, 10], ([0, 1, 2, 3], [7, 8, 9, 10, 11], [0, 4, 6])))):
+        t = len(parents)
+        depth, mask = _tree_of(parents)
+        q, k, v = heads(t)
+        pos = cache.seen[:, None] + depth.to(DEV)
+        q1, k1 = ops.rotary(plan, q, k, pos)
+        _check_rotary(plan, q, q1, pos)
+        _check_rotary(plan, k, k1, pos)
+        out, lse = _check_tree(ops, q1, cache.k, cache.v, k1, v, mask.to(DEV), cache.lengths, what=step)
+        cache.append(paths, k1, v)
+        # the accepted queries are the sequences' last tokens: shorter paths lie right in a block of the longest, and what is
+        # in front of them has sums of -inf and adds nothing
+        most = max(map(len, paths))
+        q_last, lse_last = torch.full((b, hq, most, d), NAN, dtype=dtype, device=DEV), torch.full((b, hq, most), -INF, device=DEV)
+        for i, p in enumerate(paths):
+            q_last[i, :, most - len(p):], lse_last[i, :, most - len(p):] = q1[i][:, p], lse[i][:, p]
+        q_clean = q_last.nan_to_num(0)
+        got = _check_weights(ops, q_clean, cache.k, cache.lengths, lse_last, weights=cache.weights.clone())
+        before = cache.weights.sum(-1)
+        assert ops.attention_weights(q_last, cache.k, cache.lengths, lse_last, weights=cache.weights) is cache.weights
+        assert torch.equal(cache.weights, got)
+        gained = torch.tensor([[len(p) * hq / hc] for p in paths], device=DEV)
+        assert torch.allclose(cache.weights.sum(-1) - before, gained.expand(b, hc), rtol=1e-3)
+        held = cache.weights, cache.ids, cache.k, cache.v
+        old = cache.lengths
+        _check_evict(ops, *held, old, budget, recent)
+        cache.lengths = old.clamp(max=budget)
+
+
+def test_accepted_drafts_attend_as_a_whole_sequence(ops):
+    """Chains of drafts, accepted one after another, have what causal attention over the whole sequence gives, and their
+    tokens' sums are its columns'; all from the unturned inputs in 64 bits."""
+    print("whole sequence", flush=True)
+    b, hq, hc, d, total = 1, 4, 2, 64, 60
+    g = _gen(12)
+    plan = ops.RotaryPlan(64, 1e4, True, None, DEV)
+    q, k, v = (_randn(g, b, h, total, d) for h in (hq, hc, hc))
+    cache = _Budgeted(b, hc, total, d, FP)
+    outs, lses, at = [], [], 0
+    for m in (30, 1, 7, 1, 16, 5):
+        part = slice(at, at + m)
+        q1, k1 = ops.rotary(plan, q[:, :, part], k[:, :, part], at)
+        tree = torch.ones((m, m), dtype=torch.bool, device=DEV).tril()
+        out, lse = ops.tree_attention(q1, cache.k, cache.v, k1, v[:, :, part].contiguous(), tree, cache.lengths, return_lse=True)
+        cache.append([list(range(m))], k1, v[:, :, part])
+        ops.attention_weights(q1, cache.k, cache.lengths, lse, weights=cache.weights)
+        outs.append(out)
+        lses.append(lse)
+        at += m
+    pos = torch.arange(total, dtype=torch.int32, device=DEV)
+    (q64, eq), (k64, ek) = _rotary64(plan, q, pos), _rotary64(plan, k, pos)
+    # the turned rows' roundings reach the scores, and the exponents, through the products with the other side
+    eq, ek = eq + HALF[FP] * q64.abs(), ek + HALF[FP] * k64.abs()
+    causal = torch.ones((total, total), dtype=torch.bool, device=DEV).tril()
+    for h in range(hq):
+        x, y, z = q64[0, h], k64[0, h * hc // hq], v[0, h * hc // hq].double()
+        s = torch.where(causal, x @ y.T * d ** -0.5, -INF)
+        ds = d ** -0.5 * (eq[0, h] @ y.abs().T + x.abs() @ ek[0, h * hc // hq].T + U * (d + 4) * (x.abs() @ y.abs().T)).amax(-1) + 4 * U
+        p = torch.softmax(s, -1)
+        tol = (2 * ds + U * 2 * (total + 64))[:, None] * (p @ z.abs()) + HALF[FP] * (p @ z).abs()
+        _within(torch.cat(outs, 2)[0, h], p @ z, tol, h)
+        lse = torch.logsumexp(s, -1)
+        _within(torch.cat(lses, 2)[0, h], lse, ds + U * (total + 64) + 4 * U * lse.abs(), h)
+    for hh in range(hc):
+        exact, tol = 0.0, 0.0
+        for h in range(hh * hq // hc, (hh + 1) * hq // hc):
+            x, y = q64[0, h], k64[0, hh]
+            s = torch.where(causal, x @ y.T * d ** -0.5, -INF)
+            ds = d ** -0.5 * (eq[0, h] @ y.abs().T + x.abs() @ ek[0, hh].T + U * (d + 4) * (x.abs() @ y.abs().T)).amax(-1) + 4 * U
+            p, lse = torch.softmax(s, -1), torch.logsumexp(s, -1)
+            exact = exact + p.sum(0)
+            tol = tol + (p * (2 * ds + U * (total + 64) + 8 * U * (1 + lse.abs()))[:, None]).sum(0) + U * 80 * p.sum(0)
+        _within(cache.weights[0, hh], exact, tol, hh)
+
+
+def _round(ops, plan, q, k, v, mask, cache):
+    """A round on fixed buffers, as it is captured: all drafts are accepted, and the cache goes to other buffers."""
+    t = q.shape[2]
+    pos = cache["seen"][:, None] + torch.arange(t, dtype=torch.int32, device=DEV)
+    q1, k1 = ops.rotary(plan, q, k, pos)
+    out, lse = ops.tree_attention(q1, cache["k"], cache["v"], k1, v, mask, cache["lengths"], return_lse=True)
+    at = (cache["lengths"][:, None] + torch.arange(t, device=DEV))[:, None]
+    rows = at[..., None].expand(-1, k.shape[1], -1, k.shape[3]).long()
+    cache["k"].scatter_(2, rows, k1)
+    cache["v"].scatter_(2, rows, v)
+    cache["ids"].scatter_(2, rows[..., 0], pos[:, None].expand(-1, k.shape[1], -1))
+    cache["weights"].scatter_(2, rows[..., 0], torch.zeros_like(rows[..., 0], dtype=torch.float32))
+    cache["lengths"] += t
+    cache["seen"] += t
+    ops.attention_weights(q1, cache["k"], cache["lengths"], lse, weights=cache["weights"])
+    cache["lengths"].copy_(ops.evict(cache["weights"], cache["ids"], cache["k"], cache["v"], cache["lengths"], 900, 16))
+    return out
+
+
+def _start(g, dtype, b=2, hc=2, room=1024, d=64):
+    weights, ids, k, v = _cache(g, b, hc, room, d, dtype)
+    return {"weights": weights, "ids": ids, "k": k, "v": v, "lengths": torch.tensor([890, 300], dtype=torch.int32, device=DEV),
+            "seen": torch.tensor([890, 300], dtype=torch.int32, device=DEV)}
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("t,hq", [(1, 2), (5, 8), (40, 8)])
+def test_rounds_replayed_from_graphs(ops, dtype, t, hq):
+    """Two captured rounds, replayed in turn with the lengths growing, an eager round of a third cache between the replays:
+    the same bits as eager rounds."""
+    print("graphs", dtype, t, hq, flush=True)
+    g = _gen(t)
+    plan = ops.RotaryPlan(64, 1e4, False, None, DEV)
+    mask = torch.ones((t, t), dtype=torch.bool, device=DEV).tril()
+
+    def inputs():
+        return [_randn(g, 2, h, t, 64, dtype=dtype) for h in (hq, 2, 2)]
+    caches = [_start(g, dtype) for _ in range(2)]
+    eager = [{n: x.clone() for n, x in c.items()} for c in caches]
+    third = _start(g, dtype)
+    fixed = [inputs() for _ in range(2)]
+    scrap = _start(g, dtype)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _round(ops, plan, *fixed[0], mask, scrap)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for x, c in zip(fixed, caches):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_round(ops, plan, *x, mask, c))
+        graphs.append(graph)
+    for _ in range(5):
+        for x, e, c, graph, out in zip(fixed, eager, caches, graphs, outs):
+            new = inputs()
+            for a, z in zip(x, new):
+                a.copy_(z)
+            graph.replay()
+            _round(ops, plan, *inputs(), mask, third)
+            torch.cuda.synchronize()
+            want = _round(ops, plan, *new, mask, e)
+            assert torch.equal(out, want)
+            assert all(torch.equal(c[n], e[n]) for n in c)
+
+
+def test_two_streams_at_once(ops):
+    """The same calls on two streams at once and on one after the other have the same bits."""
+    print("streams", flush=True)
+    g = _gen(30)
+    plan = ops.RotaryPlan(64, 1e4, False, None, DEV)
+    t = 12
+    mask = torch.ones((t, t), dtype=torch.bool, device=DEV).tril()
+    x = [[_randn(g, 2, h, t, 64, dtype=BF) for h in (8, 2, 2)] for _ in range(2)]
+    caches = [_start(g, BF) for _ in range(2)]
+    alone = [{n: y.clone() for n, y in c.items()} for c in caches]
+    want = [[_round(ops, plan, *x[i], mask, alone[i]) for _ in range(6)] for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(_round(ops, plan, *x[i], mask, caches[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want[i]))
+        assert all(torch.equal(caches[i][n], alone[i][n]) for n in alone[i])
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("t", [4, 16, 64, 200])
+def test_attention_weights_of_queries_that_saw_nothing(ops, dtype, t):
+    """Sums of -inf beside ordinary ones: such queries add nothing, NaN and infinities in them included."""
+    print("weights none", dtype, t, flush=True)
+    g = _gen(t)
+    q, k = _randn(g, 2, 4, t, 64, dtype=dtype, scale=2.0), _randn(g, 2, 2, 500, 64, dtype=dtype)
+    lse = _randn(g, 2, 4, t) + 3.0
+    none = (torch.rand((2, 4, t), generator=g) < 0.2).to(DEV)
+    none[1] = True
+    lse = torch.where(none, -INF, lse)
+    lengths = torch.tensor([500, 440], dtype=torch.int32, device=DEV)
+    want = _check_weights(ops, q, k, lengths, lse)
+    assert not want[1].any()
+    for odd in (NAN, INF):
+        assert torch.equal(ops.attention_weights(torch.where(none[..., None], torch.tensor(odd, dtype=dtype, device=DEV), q), k, lengths, lse), want)
+    k[1] = NAN
+    assert torch.equal(ops.attention_weights(q, k, lengths, lse), want)
