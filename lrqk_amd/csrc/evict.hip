@@ -6,20 +6,25 @@
 //
 //   select   one workgroup per head: the budget-th largest 32-bit key by a radix search over histograms in LDS (11, 11 and 10
 //            bits; ties by slot), then the list source[slot] of the slots that stay.  The keys of up to 32768 tokens are in
-//            registers; of more they are formed again for every pass.
+//            registers; of more they are formed again for every look.
 //   move     rows of K and V, weights and ids.  In place and with few tokens over the budget select does that too.
 //
-// Bound by the latency of one workgroup's passes (32768 tokens: 256 KB to one CU), not by the memory.
+// Bound by the instructions of the one workgroup, not by the memory: a wave's instruction takes its SIMD 4 cycles, so each
+// one that looks at every key of 32768 takes 0.25 us.  8 heads of 32768 tokens down to 2112: select 22 us (reads 3, keys and
+// the first histogram 4, the others 4, counting 3, the lists 5), move 5 us.  32 heads of 2117 tokens down to 2112, in place
+// and in one launch: 10 us, most of it the chain of barriers.  (Several workgroups a head would have to wait for each other
+// four times, as launches of some 4 us each.  A wave's slots one behind the other need no table of counts, but then one
+// or two waves have all slots in front of `keep`, which cost most: 24 us.  Copies of a histogram per wave instead of per
+// lane: no difference.)
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 
 namespace lrqk {
 
 constexpr int kEvThreads = 1024, kEvWaves = kEvThreads / kWave;
-constexpr int kEvPer = 4;                       // slots of a thread per trip: 16 bytes of weights and of ids
-constexpr int kEvTrip = kEvThreads * kEvPer;
-constexpr int kEvBins = 2048, kEvCopies = 4;    // of a histogram, and how many share the waves' additions
+constexpr int kEvBins = 2048, kEvCopies = 4;    // of a histogram, and how many share a wave's additions
 constexpr int kEvMoveThreads = 256;
 constexpr int kEvFew = 128;                     // tokens over the budget whose rows select moves itself
 
@@ -33,10 +38,11 @@ struct EvictMove {
   int cap, cap_out, chunks;   // slots of a head; 16-byte pieces of a row
 };
 
-// Order of the tokens: the newest in front of everything, then NaN, then by weight.
+// Order of the tokens: the newest in front of everything, then NaN, then by weight.  (No id is above the newest one, so
+// that their difference has 32 bits.)
 __device__ __forceinline__ uint32_t evict_key(float w, int32_t id, int32_t newest, int recent) {
-  if ((int64_t)id > (int64_t)newest - recent) return 0xffffffffu;
-  return w != w ? 0xfffffffeu : score_key(w);
+  const uint32_t k = w != w ? 0xfffffffeu : score_key(w);
+  return (uint32_t)newest - (uint32_t)id < (uint32_t)recent ? 0xffffffffu : k;
 }
 
 __device__ __forceinline__ int evict_len(const int32_t* lengths, int b, int cap) {
@@ -60,31 +66,9 @@ __device__ __forceinline__ uint32_t evict_scan(uint32_t v, uint32_t* scratch, ui
   return base + incl - v;
 }
 
-// The same for N values a thread, all threads' first ones in front of the second ones.  scratch: 129 words.  Three
-// barriers, however many.
-template <int N>
-__device__ __forceinline__ void evict_scan_trips(uint32_t (&v)[N], uint32_t* scratch, uint32_t& total) {
-  static_assert(N * kEvWaves <= 2 * kWave, "two sums a lane");
-  uint32_t incl[N];
-#pragma unroll
-  for (int t = 0; t < N; ++t) {
-    incl[t] = (uint32_t)wave_inclusive_sum((int)v[t]);
-    if (lane_id() == kWave - 1) scratch[t * kEvWaves + wave_id()] = incl[t];
-  }
-  __syncthreads();
-  if (wave_id() == 0) {
-    const int i = 2 * lane_id();
-    const uint32_t a = i < N * kEvWaves ? scratch[i] : 0u, b = i < N * kEvWaves ? scratch[i + 1] : 0u;
-    const uint32_t end = (uint32_t)wave_inclusive_sum((int)(a + b));
-    scratch[i] = end - a - b;
-    scratch[i + 1] = end - b;
-    if (lane_id() == kWave - 1) scratch[2 * kWave] = end;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int t = 0; t < N; ++t) v[t] = scratch[t * kEvWaves + wave_id()] + incl[t] - v[t];
-  total = scratch[2 * kWave];
-  __syncthreads();
+// `base` and the lanes of `mask` in front of this one.
+__device__ __forceinline__ uint32_t evict_place(unsigned long long mask, uint32_t base) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, base));
 }
 
 __device__ __forceinline__ void evict_row(const EvictMove& m, int h, int from_slot, int to_slot, int sub, int step) {
@@ -102,16 +86,19 @@ __device__ __forceinline__ void evict_row(const EvictMove& m, int h, int from_sl
   }
 }
 
-// TRIPS: trips whose keys are in registers (0: none).  source: [bh][budget]; holes, movers: [bh][budget] scratch.  lg: 2^lg
-// threads move a row, where this launch moves them (few).
-template <int TRIPS>
+// A block of slots is CHUNKS rounds of a piece of 64 slots for each wave, whose keys are in registers.  MANY: more slots
+// than the largest block has, and the keys are formed again for every look at them.  source: [bh][budget]; holes, movers:
+// [bh][budget] scratch.  lg: 2^lg threads move a row, where this launch moves them (few).
+template <int CHUNKS, bool MANY>
 __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictMove m, const int32_t* lengths, int32_t* new_lengths, int heads,
                                                                   int budget, int recent, int32_t* source, int32_t* holes,
                                                                   int32_t* movers, int few, int lg) {
-  __shared__ uint32_t hist[kEvCopies][kEvBins];
-  __shared__ uint32_t scratch[2 * kWave + 1];
+  static_assert(CHUNKS <= kWave, "a lane for the counts of each round");
+  __shared__ uint4 hist[kEvBins];   // (four copies of a bin side by side)
+  __shared__ uint32_t scratch[kEvWaves];
+  __shared__ uint32_t counts[CHUNKS][kEvWaves + 1];   // (rows in different banks)
   __shared__ uint32_t pick_s[3];
-  const int h = blockIdx.x, tid = threadIdx.x;
+  const int h = blockIdx.x, tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id());
   const int n = evict_len(lengths, h / heads, m.cap);
   const int keep = min(n, budget);
   int32_t* src = source + (int64_t)h * budget;
@@ -124,109 +111,68 @@ __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictMove m, c
   }
   const float* w = m.w + (int64_t)h * m.cap;
   const int32_t* id = m.ids + (int64_t)h * m.cap;
-  const bool wide = m.cap % 4 == 0 && (uintptr_t)m.w % 16 == 0 && (uintptr_t)m.ids % 16 == 0;
-  const int trips = TRIPS > 0 ? TRIPS : (n + kEvTrip - 1) / kEvTrip;
-  // weights and ids of the thread's slots of a trip (behind the n-th: the last one's)
-  auto read = [&](int trip, float (&x)[kEvPer], int32_t (&y)[kEvPer]) {
-    const int i0 = trip * kEvTrip + tid * kEvPer;
-    if (wide && i0 + kEvPer <= n) {
-      const float4 a = *(const float4*)(w + i0);
-      const int4 b = *(const int4*)(id + i0);
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-      y[0] = b.x; y[1] = b.y; y[2] = b.z; y[3] = b.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < kEvPer; ++j) {
-        x[j] = w[min(i0 + j, n - 1)];
-        y[j] = id[min(i0 + j, n - 1)];
-      }
-    }
-  };
-  constexpr int HELD = TRIPS > 0 ? TRIPS : 1;
-  constexpr bool ONCE = TRIPS > 0 && TRIPS <= 3;   // (there is room for the ids too until the newest one is known)
-  uint32_t key[HELD][kEvPer];
-  int32_t held_id[ONCE ? TRIPS : 1][kEvPer];
+  const int blocks = MANY ? (n + CHUNKS * kEvThreads - 1) / (CHUNKS * kEvThreads) : 1;
+  // first slot of a round's piece (up to 2^30 slots and a block more)
+  auto first_slot = [&](int block, int c) { return (block * CHUNKS + c) * kEvThreads + wave * kWave; };
+  uint32_t key[CHUNKS];
   int32_t newest = INT32_MIN;
-  if constexpr (ONCE) {
+  {
+    int32_t y[CHUNKS];
+    auto read = [&](int block) {   // (of a slot behind the n-th the last one)
 #pragma unroll
-    for (int t = 0; t < TRIPS; ++t) {
-      float x[kEvPer];
-      read(t, x, held_id[t]);
-#pragma unroll
-      for (int j = 0; j < kEvPer; ++j) {
-        key[t][j] = __float_as_uint(x[j]);
-        newest = max(newest, held_id[t][j]);
+      for (int c = 0; c < CHUNKS; ++c) {
+        const int slot = min(first_slot(block, c) + lane, n - 1);
+        y[c] = id[slot];
+        if constexpr (!MANY) key[c] = __float_as_uint(w[slot]);
       }
-    }
-  } else {
-#pragma unroll 4
-    for (int t = 0; t < trips; ++t) {
-      const int i0 = t * kEvTrip + tid * kEvPer;
-      if (wide && i0 + kEvPer <= n) {
-        const int4 y = *(const int4*)(id + i0);
-        newest = max(max(max(newest, y.x), y.y), max(y.z, y.w));
-      } else {
 #pragma unroll
-        for (int j = 0; j < kEvPer; ++j) newest = max(newest, id[min(i0 + j, n - 1)]);
-      }
-    }
-  }
-  newest = (int32_t)(wave_reduce_u32((uint32_t)newest ^ 0x80000000u, [](uint32_t a, uint32_t b) { return max(a, b); }) ^ 0x80000000u);
-  if (lane_id() == 0) scratch[wave_id()] = (uint32_t)newest;
-  __syncthreads();
-  newest = (int32_t)scratch[0];
+      for (int c = 0; c < CHUNKS; ++c) newest = max(newest, y[c]);
+    };
+    for (int block = 0; block < blocks; ++block) read(block);
+    newest = (int32_t)(wave_reduce_u32((uint32_t)newest ^ 0x80000000u, [](uint32_t a, uint32_t b) { return max(a, b); }) ^ 0x80000000u);
+    if (lane == 0) scratch[wave] = (uint32_t)newest;
+    __syncthreads();
 #pragma unroll
-  for (int i = 1; i < kEvWaves; ++i) newest = max(newest, (int32_t)scratch[i]);
-  // (0: no slot; the smallest key of a token, -inf's, is 0x007fffff)
-  if constexpr (TRIPS > 0) {
+    for (int i = 0; i < kEvWaves; ++i) newest = max(newest, (int32_t)scratch[i]);
+    if constexpr (!MANY) {
 #pragma unroll
-    for (int t = 0; t < TRIPS; ++t) {
-      float x[kEvPer];
-      int32_t y[kEvPer];
-      if constexpr (!ONCE) read(t, x, y);
-#pragma unroll
-      for (int j = 0; j < kEvPer; ++j) {
-        const bool in = t * kEvTrip + tid * kEvPer + j < n;
-        const uint32_t k = ONCE ? evict_key(__uint_as_float(key[t][j]), held_id[ONCE ? t : 0][j], newest, recent) : evict_key(x[j], y[j], newest, recent);
-        key[t][j] = in ? k : 0u;
+      for (int c = 0; c < CHUNKS; ++c) {   // (0: no slot; the smallest key of a token, -inf's, is 0x007fffff)
+        const uint32_t k = evict_key(__uint_as_float(key[c]), y[c], newest, recent);
+        key[c] = first_slot(0, c) + lane < n ? k : 0u;
       }
     }
   }
-  auto keys = [&](int t, uint32_t (&k)[kEvPer]) {
-    if constexpr (TRIPS == 0) {
-      float x[kEvPer];
-      int32_t y[kEvPer];
-      read(t, x, y);
+  auto form = [&](int block) {
+    if constexpr (MANY) {
+      int32_t y[CHUNKS];
 #pragma unroll
-      for (int j = 0; j < kEvPer; ++j) {
-        const bool in = t * kEvTrip + tid * kEvPer + j < n;
-        const uint32_t v = evict_key(x[j], y[j], newest, recent);
-        k[j] = in ? v : 0u;
+      for (int c = 0; c < CHUNKS; ++c) {
+        const int slot = min(first_slot(block, c) + lane, n - 1);
+        key[c] = __float_as_uint(w[slot]);
+        y[c] = id[slot];
+      }
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        const uint32_t k = evict_key(__uint_as_float(key[c]), y[c], newest, recent);
+        key[c] = first_slot(block, c) + lane < n ? k : 0u;
       }
     }
   };
 
-  uint32_t prefix = 0, high = 0, need = (uint32_t)keep, equal = 0;   // the need-th largest of the keys that begin with `prefix`
+  uint32_t prefix = 0, need = (uint32_t)keep, equal = 0;   // the need-th largest of the `equal` keys that begin with `prefix`
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    for (int i = tid; i < kEvCopies * kEvBins; i += kEvThreads) (&hist[0][0])[i] = 0;
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t limit = pass == 1 ? 1u << 21 : 1u << 10;
+    for (int i = tid; i < kEvBins; i += kEvThreads) hist[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    uint32_t* mine = hist[wave_id() & (kEvCopies - 1)];
-    auto count = [&](const uint32_t (&k)[kEvPer]) {
+    uint32_t* mine = (uint32_t*)hist + (lane & (kEvCopies - 1));
+    for (int block = 0; block < blocks; ++block) {
+      form(block);
 #pragma unroll
-      for (int j = 0; j < kEvPer; ++j)
-        if (k[j] != 0u && (k[j] & high) == prefix) atomicAdd(&mine[(k[j] >> shift) & (bins - 1)], 1u);
-    };
-    if constexpr (TRIPS > 0) {
-#pragma unroll
-      for (int t = 0; t < TRIPS; ++t) count(key[t]);
-    } else {
-#pragma unroll 2
-      for (int t = 0; t < trips; ++t) {
-        uint32_t k[kEvPer];
-        keys(t, k);
-        count(k);
+      for (int c = 0; c < CHUNKS; ++c) {   // (what is no slot is in the first bins, which are behind all tokens)
+        const uint32_t rest = key[c] ^ prefix;
+        if (pass == 0 ? first_slot(block, c) < n : rest < limit) atomicAdd(&mine[kEvCopies * (rest >> shift)], 1u);
       }
     }
     __syncthreads();
@@ -234,10 +180,8 @@ __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictMove m, c
     uint32_t c[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int bin = kEvBins - 1 - (2 * tid + j);
-      c[j] = 0;
-#pragma unroll
-      for (int i = 0; i < kEvCopies; ++i) c[j] += hist[i][bin];
+      const uint4 four = hist[kEvBins - 1 - (2 * tid + j)];
+      c[j] = (four.x + four.y) + (four.z + four.w);
     }
     uint32_t total;
     uint32_t before = evict_scan(c[0] + c[1], scratch, total);
@@ -252,87 +196,104 @@ __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictMove m, c
     }
     __syncthreads();
     prefix |= pick_s[0] << shift;
-    high |= (uint32_t)(bins - 1) << shift;
     need = pick_s[1];
     equal = pick_s[2];
+    if (need == equal) break;   // (all that begin with it stay: mostly two passes)
   }
-  // every key above `prefix` stays, and the first `need` of the `equal` ones that have it
+  // Every key from `prefix` on stays, or where fewer are needed than have it, the first `need` of those.  Lane c has the
+  // counts of the wave's round c, and the table of all waves' says what is in front of its piece.
   int32_t* hole = holes + (int64_t)h * budget;
   int32_t* mover = movers + (int64_t)h * budget;
-  uint32_t ties = 0, nh = 0, nm = 0;
-  const bool rank_ties = need < equal;
-  auto tied = [&](int t, const uint32_t (&k)[kEvPer]) {
-    uint32_t mine = 0;
+  uint32_t moved = 0;   // (as many movers as holes)
+  auto list = [&](auto has_ties) {
+    constexpr bool TIES = decltype(has_ties)::value;
+    uint32_t ties = 0, nh = 0, nm = 0;   // of the blocks before
+    // two numbers of lane c, in 16 bits each: their sums over the pieces in front of the wave's of round c
+    auto in_front = [&](uint32_t mine, uint32_t& low, uint32_t& high) {
+      if (lane < CHUNKS) counts[lane][wave] = mine;
+      __syncthreads();
+      uint32_t before = 0, all = 0;
 #pragma unroll
-    for (int j = 0; j < kEvPer; ++j) mine += ((k[j] == prefix) & (t * kEvTrip + tid * kEvPer + j < n)) ? 1u : 0u;
-    return mine;
-  };
-  // which of the slots' tokens stay (a bit each), and how many holes (low half) and movers (high half) that makes; rank: of
-  // the first tie
-  auto decide = [&](int t, const uint32_t (&k)[kEvPer], uint32_t rank, uint32_t& bits) {
-    uint32_t packed = 0;
-    bits = 0;
+      for (int i = 0; i < kEvWaves; ++i) {
+        const uint32_t x = counts[min(lane, CHUNKS - 1)][i];
+        before += i < wave ? x : 0u;
+        all += x;
+      }
+      all = lane < CHUNKS ? all : 0u;   // (of a round: at most 1024 in each half)
+      const uint32_t ends = (uint32_t)wave_inclusive_sum((int)(all & 0xffffu)), highs = (uint32_t)wave_inclusive_sum((int)(all >> 16));
+      const uint32_t at = low, at_high = high;
+      low = at + ends - (all & 0xffffu) + (before & 0xffffu);
+      high = at_high + highs - (all >> 16) + (before >> 16);
+      __syncthreads();
+      return make_uint2(at + (uint32_t)__builtin_amdgcn_readlane((int)ends, kWave - 1),
+                        at_high + (uint32_t)__builtin_amdgcn_readlane((int)highs, kWave - 1));
+    };
+    for (int block = 0; block < blocks; ++block) {
+      form(block);
+      uint32_t rank = ties;   // of the first tie of lane c's piece
+      if constexpr (TIES) {
+        int mine = 0;
+        uint32_t none = 0;
 #pragma unroll
-    for (int j = 0; j < kEvPer; ++j) {
-      const int slot = t * kEvTrip + tid * kEvPer + j;
-      const bool in = slot < n, tie = in & (k[j] == prefix), stay = in & ((k[j] > prefix) | (tie & (rank < need)));
-      rank += (rank_ties & tie) ? 1u : 0u;
-      bits |= stay ? 1u << j : 0u;
-      packed += (in & (slot < keep) & !stay) ? 1u : 0u;
-      packed += (stay & (slot >= keep)) ? 0x10000u : 0u;
-    }
-    return packed;
-  };
-  auto emit = [&](int t, uint32_t bits, uint32_t ah, uint32_t am) {
+        for (int c = 0; c < CHUNKS; ++c) {
+          const int tied = __popcll(__ballot(key[c] == prefix));
+          mine = lane == c ? tied : mine;
+        }
+        ties = in_front((uint32_t)mine, rank, none).x;
+      }
+      auto stays = [&](int c) -> bool {
+        if constexpr (!TIES) return key[c] >= prefix;
+        const uint32_t r = evict_place(__ballot(key[c] == prefix), (uint32_t)__builtin_amdgcn_readlane((int)rank, c));
+        return (key[c] > prefix) | ((key[c] == prefix) & (r < need));
+      };
+      int mine = 0;
 #pragma unroll
-    for (int j = 0; j < kEvPer; ++j) {
-      const int slot = t * kEvTrip + tid * kEvPer + j;
-      if (slot >= n) continue;
-      if (slot < keep) {
-        if (!(bits >> j & 1u)) hole[ah++] = slot;
-        else if (!few) src[slot] = slot;
-      } else if (bits >> j & 1u) {
-        mover[am++] = slot;
+      for (int c = 0; c < CHUNKS; ++c) {
+        const int first = first_slot(block, c);
+        const bool stay = stays(c);
+        int both;
+        if (first >= keep)
+          both = __popcll(__ballot(stay)) << 16;
+        else
+          both = __popcll(__ballot((first + lane < keep) & !stay)) + (__popcll(__ballot((first + lane >= keep) & stay)) << 16);
+        mine = lane == c ? both : mine;
+      }
+      uint32_t ah = nh, am = nm;
+      const uint2 ends = in_front((uint32_t)mine, ah, am);
+      nh = ends.x;
+      nm = ends.y;
+      auto put = [&](int32_t* to, bool which, uint32_t at, int slot) {
+        const unsigned long long mask = __ballot(which);
+        if (mask && which) to[evict_place(mask, at)] = slot;
+      };
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        const int first = first_slot(block, c);
+        const bool stay = stays(c);
+        const uint32_t mover_at = (uint32_t)__builtin_amdgcn_readlane((int)am, c);
+        if (first >= keep) {
+          put(mover, stay, mover_at, first + lane);
+        } else {
+          const bool front = first + lane < keep;
+          put(hole, front & !stay, (uint32_t)__builtin_amdgcn_readlane((int)ah, c), first + lane);
+          put(mover, stay & !front, mover_at, first + lane);
+          if (!few && (stay & front)) src[first + lane] = first + lane;
+        }
       }
     }
+    moved = nm;
   };
-  if constexpr (TRIPS > 0) {   // (up to 32767 holes and as many movers: the halves hold them)
-    uint32_t at[TRIPS], bits[TRIPS], total;
-#pragma unroll
-    for (int t = 0; t < TRIPS; ++t) at[t] = 0;
-    if (rank_ties) {
-#pragma unroll
-      for (int t = 0; t < TRIPS; ++t) at[t] = tied(t, key[t]);
-      evict_scan_trips<TRIPS>(at, scratch, total);
-    }
-#pragma unroll
-    for (int t = 0; t < TRIPS; ++t) at[t] = decide(t, key[t], at[t], bits[t]);
-    evict_scan_trips<TRIPS>(at, scratch, total);
-#pragma unroll
-    for (int t = 0; t < TRIPS; ++t) emit(t, bits[t], at[t] & 0xffffu, at[t] >> 16);
-    nh = total & 0xffffu;
-  } else {
-    for (int t = 0; t < trips; ++t) {
-      uint32_t k[kEvPer], rank = 0, bits, total;
-      keys(t, k);
-      if (rank_ties) {
-        rank = ties + evict_scan(tied(t, k), scratch, total);
-        ties += total;
-      }
-      const uint32_t at = evict_scan(decide(t, k, rank, bits), scratch, total);
-      emit(t, bits, nh + (at & 0xffffu), nm + (at >> 16));
-      nh += total & 0xffffu;
-      nm += total >> 16;
-    }
-  }
+  if (need < equal)
+    list(std::true_type{});
+  else
+    list(std::false_type{});
   __threadfence_block();
   __syncthreads();
-  // (nh == nm: keep slots hold keep tokens)
   if (!few) {
-    for (uint32_t i = tid; i < nh; i += kEvThreads) src[hole[i]] = mover[i];
+    for (uint32_t i = tid; i < moved; i += kEvThreads) src[hole[i]] = mover[i];
     return;
   }
-  for (uint32_t i = tid >> lg; i < nh; i += kEvThreads >> lg) evict_row(m, h, mover[i], hole[i], tid & ((1 << lg) - 1), 1 << lg);
+  for (uint32_t i = tid >> lg; i < moved; i += kEvThreads >> lg) evict_row(m, h, mover[i], hole[i], tid & ((1 << lg) - 1), 1 << lg);
   if (h % heads == 0 && tid == 0) new_lengths[h / heads] = keep;
 }
 
@@ -398,20 +359,12 @@ extern "C" int lrqk_evict(float* weights, int32_t* ids, void* k, void* v, const 
   while ((1 << lg) < m.chunks && (1 << lg) < kWave) ++lg;
   // (not where the new lengths take the place of the old ones, which the workgroups of the other heads still want to see)
   const int few = in_place && cap - budget <= kEvFew && new_lengths != lengths ? 1 : 0;
-  const int trips = (cap + kEvTrip - 1) / kEvTrip;
   const dim3 grid((unsigned)bh), block(kEvThreads);
-  if (trips <= 1)
-    hipLaunchKernelGGL((evict_select_kernel<1>), grid, block, 0, st, m, lengths, new_lengths, heads, budget, recent, source, holes, movers,
-                       few, lg);
-  else if (trips <= 3)
-    hipLaunchKernelGGL((evict_select_kernel<3>), grid, block, 0, st, m, lengths, new_lengths, heads, budget, recent, source, holes, movers,
-                       few, lg);
-  else if (trips <= 8)
-    hipLaunchKernelGGL((evict_select_kernel<8>), grid, block, 0, st, m, lengths, new_lengths, heads, budget, recent, source, holes, movers,
-                       few, lg);
-  else
-    hipLaunchKernelGGL((evict_select_kernel<0>), grid, block, 0, st, m, lengths, new_lengths, heads, budget, recent, source, holes, movers,
-                       few, lg);
+  auto select = cap <= 4 * kEvThreads    ? evict_select_kernel<4, false>
+                : cap <= 12 * kEvThreads ? evict_select_kernel<12, false>
+                : cap <= 32 * kEvThreads ? evict_select_kernel<32, false>
+                                         : evict_select_kernel<32, true>;
+  hipLaunchKernelGGL(select, grid, block, 0, st, m, lengths, new_lengths, heads, budget, recent, source, holes, movers, few, lg);
   LRQK_HIP_CHECK(hipGetLastError());
   if (few) return LRQK_OK;
   const int rpb = kEvMoveThreads >> lg;
