@@ -4,8 +4,8 @@ Only the call pattern matters here: every layer calls ``cache.update(q, k, v, la
 as the reference's patched attention does (lrqk_attention.py:2254-2290, 2326-2344) -- raw K/V
 and ordinary causal attention over the prompt, the active set ``[b,Hq,k+L,d]`` and exact
 single-query attention per decoded token.  Projections, norms, rotary embedding, SwiGLU and the
-prompt attention are plain PyTorch-ROCm library calls on random-initialised weights; the
-cache path (factorisation, selection, fetch, decode attention) is the HIP library.
+prompt attention are plain PyTorch-ROCm library calls on random-initialised weights (scaled or
+interleaved rotary positions: the HIP library's); the cache path (factorisation, selection, fetch, decode attention) is the HIP library.
 
 ``cache=None`` runs the same module with a dense K/V cache; with ``k + lite`` at least as long as
 the whole sequence the LRQK run returns every cached token (the growing-prefix branch,
@@ -36,6 +36,8 @@ class DecoderConfig:
     vocab: int = 128256
     rope_theta: float = 5e5
     rms_eps: float = 1e-5
+    rope_interleaved: bool = False           # pairs of neighbours; else halves
+    rope_scaling: Optional[dict] = None      # as ops.RotaryPlan takes it
 
 
 LLAMA3_8B = DecoderConfig()
@@ -79,6 +81,9 @@ class LlamaShapeDecoder:
                 wg=w(c.hidden, c.intermediate), wu=w(c.hidden, c.intermediate), wd=w(c.intermediate, c.hidden)))
         half = c.head_dim // 2
         self.inv_freq = 1.0 / (c.rope_theta ** (torch.arange(0, half, device=self.device, dtype=torch.float32) / half))
+        self.rope = None   # (else the library turns q and k, in one launch)
+        if c.rope_interleaved or c.rope_scaling is not None:
+            self.rope = ops.RotaryPlan(c.head_dim, c.rope_theta, c.rope_interleaved, c.rope_scaling, self.device)
         self.ws = ops.Workspace()
         self.dense: Optional[List[Tuple[torch.Tensor, torch.Tensor]]] = None
         self.progress = None   # optional callable(str), called once per layer while the prompt is processed
@@ -123,7 +128,10 @@ class LlamaShapeDecoder:
             q = (hcur @ L["wq"]).view(b, s, c.heads, c.head_dim).transpose(1, 2)
             k = (hcur @ L["wk"]).view(b, s, c.kv_heads, c.head_dim).transpose(1, 2)
             v = (hcur @ L["wv"]).view(b, s, c.kv_heads, c.head_dim).transpose(1, 2).contiguous()
-            q, k = self._rope(q, pos0).contiguous(), self._rope(k, pos0).contiguous()
+            if self.rope is None:
+                q, k = self._rope(q, pos0).contiguous(), self._rope(k, pos0).contiguous()
+            else:
+                q, k = ops.rotary(self.rope, q, k, pos0)
             if cache is None:
                 if self.dense[li] is None:
                     self.dense[li] = (k, v)

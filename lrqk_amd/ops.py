@@ -617,7 +617,7 @@ def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
 def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positions, transpose: bool = False, out=None):
     """q [b,Hq,s,d] and k [b,Hk,s,d] (or None) turned to ``positions``: int32 [s] or [b,s] on the GPU, or the first one of
     s that follow each other.  Any strides, rows contiguous.  ``out``: (q', k') to write to, each of them any view that is
-    its input or apart from both inputs; else new contiguous tensors.  ``transpose`` turns back: the gradient of the turn.
+    its input or apart from both inputs, and that share no element; else new contiguous tensors.  ``transpose`` turns back: the gradient of the turn.
     Returns (q', k'), or q' without a k."""
     pos = positions if isinstance(positions, torch.Tensor) else None
     dev = _on_one_gpu(q, k, pos, plan.inv_freq)
@@ -656,6 +656,8 @@ def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positio
                 raise ValueError("out has several elements in one place")
             if not _same_view(x, y) and not all(_apart(y, z) for z in xs):
                 raise ValueError("out overlaps an input and is not the view that is turned")
+        if k is not None and ys[0].data_ptr() == ys[1].data_ptr() and q.numel() and k.numel():
+            raise ValueError("out of q and of k are in one place")
         q_out, k_out = ys if k is not None else (ys[0], None)
     strides = (*_row_strides("q", q), *_row_strides("out", q_out))
     if k is not None:

@@ -138,3 +138,28 @@ def test_selection_path_against_oracle_run(dec, oracle):
                 assert common >= 15, (li, step, sorted(ra), sorted(ro))
     print("   tokens identical; smallest agreement of a head's resident set with the oracle run: %d of 16" % worst,
           flush=True)
+
+
+def _turned(dec, **rope):
+    cfg = dec.DecoderConfig(layers=2, hidden=64, heads=4, kv_heads=2, head_dim=16, intermediate=128, vocab=97, rope_theta=1e4, **rope)
+    return dec.LlamaShapeDecoder(cfg, torch.float32, DEV, seed=3)
+
+
+def test_scaled_positions_over_both_caches(dec):
+    """The library's rotary positions in the decoder: a factor of one is the plain decoder, and a scaled, interleaved one
+    decodes the same tokens over the dense cache and over the one that keeps every token."""
+    print("decoder: scaled positions", flush=True)
+    ids = torch.randint(0, 97, (2, 24), generator=torch.Generator().manual_seed(0)).to(DEV)
+    plain, one = _model(dec), _turned(dec, rope_scaling={"type": "linear", "factor": 1.0})
+    a, b = plain.forward(ids, 0, None), one.forward(ids, 0, None)
+    # fp32 angles of up to 24 rad are off by 24 * 2^-22, which is what a turned element is off by, relative to its pair; two
+    # layers and the norms pass that on a few dozen times at most
+    assert float((a - b).abs().max()) <= 40 * 24 * 2.0 ** -22 * float(a.abs().max())
+    m = _turned(dec, rope_interleaved=True, rope_scaling={"type": "yarn", "factor": 4.0, "original_context": 16})
+    dense, *_ = m.generate(ids, 8, None)
+    cache = m.new_cache(r=4, num_active_tokens=20, lite_tokens=12, max_iter=(2, 2), tol=(1e-8, 1e-8), max_sequence_length=16)
+    got, *_ = m.generate(ids, 8, cache)
+    assert torch.equal(got.cpu(), dense.cpu())
+    # (a model of small random weights hardly looks at positions: its tokens need not differ, but its logits do)
+    m.dense = plain.dense = None
+    assert not torch.equal(m.forward(ids, 0, None), plain.forward(ids, 0, None))

@@ -972,3 +972,12 @@ def test_attention_weights_of_queries_that_saw_nothing(ops, dtype, t):
         assert torch.equal(ops.attention_weights(torch.where(none[..., None], torch.tensor(odd, dtype=dtype, device=DEV), q), k, lengths, lse), want)
     k[1] = NAN
     assert torch.equal(ops.attention_weights(q, k, lengths, lse), want)
+
+
+def test_rotary_refuses_one_place_for_both(ops):
+    plan = ops.RotaryPlan(64, 1e4, False, None, DEV)
+    q, y = torch.zeros(1, 2, 3, 64, device=DEV), torch.zeros(1, 2, 3, 64, device=DEV)
+    with pytest.raises(ValueError):
+        ops.rotary(plan, q, q, 0, out=(q, q))
+    with pytest.raises(ValueError):
+        ops.rotary(plan, q, q.clone(), 0, out=(y, y))
