@@ -981,3 +981,21 @@ def test_rotary_refuses_one_place_for_both(ops):
         ops.rotary(plan, q, q, 0, out=(q, q))
     with pytest.raises(ValueError):
         ops.rotary(plan, q, q.clone(), 0, out=(y, y))
+
+
+@pytest.mark.parametrize("n", [32769, 36864, 36865, 100000])
+def test_evict_longer_than_a_workgroup(ops, n):
+    """Heads that several workgroups look through: ties over all of them, sequences of every length beside each other, the
+    newest tokens anywhere."""
+    print("evict wide", n, flush=True)
+    g = _gen(n)
+    w, ids, k, v = _cache(g, 3, 2, n, 8, BF)
+    lengths = torch.tensor([n, 0, n - 4097], dtype=torch.int32, device=DEV)
+    ids = ids.gather(2, torch.rand((3, 2, n), generator=g).argsort(-1).to(DEV))
+    for budget, recent in ((1, 0), (2112, 64), (n // 2, 5000), (n - 1, 1), (n + 5, 3)):
+        for x in (w, (w * 3).floor(), torch.zeros_like(w)):
+            held = [y.clone() for y in (x, ids, k, v)]
+            _check_evict(ops, *held, lengths, budget, recent, what=(budget, recent))
+    odd = w.clone()
+    odd[:, :, ::3], odd[:, :, 1::3] = NAN, -INF
+    _check_evict(ops, odd, ids, k, v, None, n // 2, 100)
