@@ -94,7 +94,9 @@ struct WeightTile {
   }
 };
 
-// Item (head, part, group of 64 NT rows) of a workgroup: its queries' maximum and sum over its part of the keys.
+// Item (head, part, group of 64 NT rows) of a workgroup: its queries' maximum and sum over its part of the keys.  Bound by
+// the exponentials (16 cycles of a SIMD for a wave's 64, and 8 more for scaling and adding, beside 2 16x16x32 products' 16):
+// 8192 tokens of 32 / 8 heads of 128, 275 GFLOP in 315 to 360 us, and `merge` 8.
 template <typename T, int DP, int NT>
 __global__ __launch_bounds__(kAwThreads, 2) void weights_rows_kernel(WeightArgs a) {
   using Tile = WeightTile<T, DP>;
@@ -269,7 +271,8 @@ __global__ __launch_bounds__(kAwThreads) void weights_merge_kernel(WeightArgs a,
   a.lse2[row] = sum == 0.0f ? -INFINITY : top + log2f(sum);
 }
 
-// 64 NT keys and a chunk of the queries a workgroup.
+// 64 NT keys and a chunk of the queries a workgroup.  Bound as the rows are: 8192 tokens, 342 to 380 us, and `sum` 5.  (Keys in
+// registers and queries through LDS: the other way round a wave's sums would be rows' and cross the lanes for every tile.)
 template <typename T, int DP, int NT>
 __global__ __launch_bounds__(kAwThreads, 2) void weights_columns_kernel(WeightArgs a) {
   using Tile = WeightTile<T, DP>;
@@ -421,9 +424,13 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_columns_kernel(WeightAr
   }
 }
 
-// All queries of a cache head, up to 16 NT, and every fourth tile of 32 keys of a split for each of the four waves.
+// All queries of a cache head, up to 16 NT, and every fourth tile of 32 keys of a split for each of the four waves.  Bound
+// by the reading of the keys: 5 tokens over 2 x 64K, 32 / 8 heads of 128 bf16 elements, 268 MB in 57 us, 4.7 TB/s.  (Four
+// workgroups per CU take 128 registers a thread; with 136 three fit, and the fourth ran alone: 49 instead of 46 us for 32
+// queries a cache head over 64K.)  The two kernels of many queries take 58 + 5 us for 16, 32 or 64 queries a cache head over
+// 64K keys where this one takes 44, 46 and 51, and 18 + 5 for 64 over 8K instead of 12.
 template <typename T, int DP, int NT>
-__global__ __launch_bounds__(kAwThreads, DP * (int)sizeof(T) <= 512 ? 2 : 1) void weights_stream_kernel(WeightArgs a) {
+__global__ __launch_bounds__(kAwThreads, DP * (int)sizeof(T) <= 256 && NT <= 2 ? 4 : DP * (int)sizeof(T) <= 512 ? 2 : 1) void weights_stream_kernel(WeightArgs a) {
   using Tile = WeightTile<T, DP>;
   constexpr int STEPS = Tile::STEPS, CH = Tile::CH, NU = kAwTile / 16, LOADS = kAwTile * CH / kWave;
   __shared__ ar_u4 smem[kAwWaves][kAwTile * CH];
@@ -532,7 +539,7 @@ static WeightPlan weights_plan(int b, int hq, int hc, int t, int64_t n, int d, i
   const int64_t M = (int64_t)(hq / hc) * t, heads = (int64_t)b * hc;
   const int row = p.dp * (int)elem_size(dtype);
   p.nt = row <= 256 ? 4 : row <= 512 ? 2 : 1;
-  p.few = M <= (row <= 256 ? 64 : row <= 512 ? 32 : 16);   // (what a wave has room for)
+  p.few = M <= (row <= 256 ? 64 : row <= 512 ? 32 : 16);   // (what a wave has room for; both kernels measured at weights_stream_kernel)
   if (p.few) {
     // four workgroups per CU, two tiles for each of a workgroup's waves at least
     const int64_t tiles = (n + kAwTile - 1) / kAwTile, splits = std::max<int64_t>(1, 1024 / heads);

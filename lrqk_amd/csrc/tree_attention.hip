@@ -300,7 +300,9 @@ __device__ __forceinline__ void tree_mask(float (&p)[MT][NE], const TreeArgs& a,
 }
 
 // Few queries: the four waves of a workgroup take the tiles of its split in turn, each for itself.  Bound by the reading of
-// K and V.
+// K and V: a token over 32K of 8 cache heads of 128 bf16 elements, 134 MB in 27 us, 5.0 TB/s, and the join 6.  (Of few tokens
+// by the chain of the first reads: 2112 of 32 heads, 10 us.)  Up to 32 queries a cache head: tree_share_kernel takes 58 us
+// for 16 or 32 of them where this one takes 51 (32K tokens, after 256 MB of writes), of fp32 40 instead of 29 and 35 (8K).
 template <typename T, int DP, int MT>
 __global__ __launch_bounds__(kTrThreads, MT == 2 && DP == 128 ? 2 : 1) void tree_stream_kernel(TreeArgs a) {
   using Tile = TreeTile<T, DP, MT>;
@@ -481,8 +483,9 @@ constexpr int kTlWaves = 4, kTlThreads = kTlWaves * kWave;
 // (ds_read_b64_tr_b16: four keys of one element a lane).
 //
 // FINE: bf16 probabilities as the sum of two bf16 numbers, as in tree_stream_kernel.  Beyond 128 queries a cache head this
-// is bound by the products, and half of those with V are the second number's (64 drafts over 4 x 64K, 32 / 8 heads: 370
-// instead of 450 us without it; 25 drafts over 128K, bound by the reading: 106 instead of 111).  There the probabilities
+// is bound by the products, and half of those with V are the second number's (64 drafts over 4 x 64K, 32 / 8 heads: 195 to
+// 230 instead of 230 to 285 us without it, as the clock holds; 1.1 PFLOP/s at best; 25 drafts over 128K, bound by the reading:
+// 108 instead of 112).  There the probabilities
 // are rounded to bf16, 2^-9 of each, independently of each other, and what they are divided by is the sum of the rounded
 // ones (one more block of o), so that a result is off by what its rounding to bf16 is off by once more; lse keeps the exact
 // ones' sum.
@@ -951,7 +954,8 @@ static TreePlan tree_plan(int b, int hq, int hc, int t, int64_t n, int d, bool l
   return p;
 }
 
-// (few workgroups: more threads for the splits of each)
+// (few workgroups: more threads for the splits of each.  64 workgroups 7 us instead of 10, 256 workgroups 10.6 instead of
+// 12.6; 1024 workgroups 10.6 instead of 9.8)
 template <typename T, int DP, bool SHARED>
 static void tree_join_launch(const TreeArgs& a, dim3 grid, hipStream_t st) {
   if (grid.x <= 512)
