@@ -545,16 +545,18 @@ static WeightPlan weights_plan(int b, int hq, int hc, int t, int64_t n, int d, i
     const int64_t tiles = (n + kAwTile - 1) / kAwTile, splits = std::max<int64_t>(1, 1024 / heads);
     p.few_per = (int)std::max<int64_t>(2 * kAwWaves, (tiles + splits - 1) / splits);
   }
-  // two thousand workgroups of keys and chunks of queries (half of a prompt's have little to do), eight tiles of queries
-  // for each
+  // two thousand workgroups of keys and chunks of queries (half of a prompt's have little to do; one thousand: no faster),
+  // eight tiles of queries for each
   const int64_t blocks = (n + 16 * p.nt * kAwWaves - 1) / (16 * p.nt * kAwWaves), items = (M + 15) / 16;
   p.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(2048 / (blocks * heads), items / 16));
   if (!p.few) p.part = heads * n * p.chunks;
   if (have_lse) return p;
-  p.rows_nt = (int)std::min<int64_t>(p.nt, M <= 64 ? 1 : M <= 128 ? 2 : 4);
+  // (lse over 8192 keys: 64 queries a cache head 7.8 us with 16 a wave, 12.7 with 64; 128 9.0 and 13; 1024 34 and 29)
+  p.rows_nt = M <= 128 ? 1 : p.nt;
   p.groups = (int)((M + 64 * p.rows_nt - 1) / (64 * p.rows_nt));
   // parts of one length, however many keys a group of queries sees (a prompt's first ones few): four thousand, with eight
-  // tiles of 32 keys at least.  (One part a group, 8K tokens: a quarter of the GPU waited for the longest ones.)
+  // tiles of 32 keys at least.  (One part a group, 8K tokens: a quarter of the GPU waited for the longest ones; two thousand
+  // parts: 368 instead of 359 us.)
   const int64_t tiles = (n + kAwTile - 1) / kAwTile;
   const int64_t parts = std::max<int64_t>(1, std::min<int64_t>((tiles + 7) / 8, 4096 / (heads * p.groups)));
   p.per = (int)((tiles + parts - 1) / parts);
@@ -570,7 +572,7 @@ static int weights_rows_launch(const WeightArgs& a, const WeightPlan& p, int hea
   constexpr int MOST = DP * (int)sizeof(T) <= 256 ? 4 : DP * (int)sizeof(T) <= 512 ? 2 : 1;
   if constexpr (MOST >= 4)
     if (p.rows_nt == 4) hipLaunchKernelGGL((weights_rows_kernel<T, DP, 4>), grid, dim3(kAwThreads), 0, st, a);
-  if constexpr (MOST >= 2)
+  if constexpr (MOST == 2)
     if (p.rows_nt == 2) hipLaunchKernelGGL((weights_rows_kernel<T, DP, 2>), grid, dim3(kAwThreads), 0, st, a);
   if (p.rows_nt == 1) hipLaunchKernelGGL((weights_rows_kernel<T, DP, 1>), grid, dim3(kAwThreads), 0, st, a);
   LRQK_HIP_CHECK(hipGetLastError());

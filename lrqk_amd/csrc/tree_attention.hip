@@ -933,11 +933,12 @@ static TreePlan tree_plan(int b, int hq, int hc, int t, int64_t n, int d, bool l
     least = 4 * kTrWaves;   // four tiles for each of a workgroup's waves
   } else {
     p.mt = p.dp == 256 ? 1 : 2;
-    p.wr = M <= 32 * p.mt && p.dp != 256 ? 2 : 4;
+    p.wr = M <= 32 * p.mt && p.dp != 256 ? 2 : 4;   // (64 queries over 32K: 33 us with two waves of them, 35 with four; fp32, 4K: 29, 32)
     p.rows = 16 * p.mt * p.wr;
     least = 2 * kTlWaves / p.wr;
   }
-  // two workgroups per CU; twice as many where the lengths may differ
+  // Two workgroups per CU (25 drafts over 128K: 112 + 10 us for the join, four per CU 129 + 16); four where the lengths may
+  // differ (64 drafts over 4 sequences of 4 .. 32K: 130 + 17, two per CU 160 + 13; one token over 16 of 2 .. 16K: 110 and 121).
   groups_wanted = b > 1 && lengths ? 1024 : 512;
   p.row_blocks = (int)((M + p.rows - 1) / p.rows);
   p.row_tiles = p.row_blocks * (p.rows / 16);
