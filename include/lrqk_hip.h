@@ -283,8 +283,9 @@ int lrqk_rotary(const void* q, const void* k, void* q_out, void* k_out, const in
  * for all).  hc = hn: a dense cache; hc = hq: the active set (k_act, v_act), whose tokens every query head picks itself.
  * q, out: [b][hq][t][d]; lse (or NULL): fp32 [b][hq][t], log of the sum of exp(scale q.k).  A query that sees nothing
  * gives zeros and -inf.  What a masked drafted token or a row behind the length holds, infinities and NaN included, does
- * not matter.  Strides in elements, the same for k_cache and v_cache, multiples of 16 bytes.  Head widths up to 256
- * elements, t up to 1024.
+ * not matter; a cached value that is not finite leaves its element of the outputs not finite (a NaN perhaps for an
+ * infinity).  Strides in elements, the same for k_cache and v_cache, multiples of 16 bytes, rows at most 2^24 elements
+ * apart.  Head widths up to 256 elements, t up to 1024, n up to 2^30, b * hq up to 65535.
  * These calls take no ctx: their scratch is the caller's (lrqk_*_workspace bytes of device memory, 16-byte aligned,
  * contents of no meaning before and after), so that calls on several streams and captured graphs need not share any. */
 int64_t lrqk_tree_attention_workspace(int b, int hq, int hc, int t, int64_t n, int d, int have_lengths, int dtype);
@@ -297,8 +298,9 @@ int lrqk_tree_attention(const void* q, const void* k_cache, const void* v_cache,
  * out[b][hc][j] = weights[b][hc][j] (0 if NULL; may be out) + the sum over the hq / hc query heads of the cache head and
  * over the queries i with j <= length - t + i of exp(scale q_i.k_j - lse_i), j < n; tokens behind the length get nothing.
  * q: [b][hq][t][d], k: rows of d elements by strides as above.  lse: fp32 [b][hq][t] as lrqk_tree_attention leaves it
- * (a query of -inf adds nothing, whatever q and k hold), or NULL: of the keys that the query sees here.  weights, out: fp32 [b][hc][n].
- * Deterministic: no atomics.  Workspace as above (with lse none is needed). */
+ * (a query of -inf adds nothing, whatever q and k hold), or NULL: of the keys that the query sees here.  weights, out:
+ * fp32 [b][hc][n].  Deterministic: no atomics.  Workspace as above (none where its size is 0).  Limits: head widths up to
+ * 256 elements, n up to 2^30, b * hq up to 65535. */
 int64_t lrqk_attention_weights_workspace(int b, int hq, int hc, int t, int64_t n, int d, int have_lse, int dtype);
 int lrqk_attention_weights(const void* q, const void* k, int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,
                            int64_t n, const int32_t* lengths, const float* lse, const float* weights, float* out, int b, int hq,
@@ -307,9 +309,8 @@ int lrqk_attention_weights(const void* q, const void* k, int64_t k_batch_stride,
 /* No counterpart in the reference.  Eviction from a cache by those weights: of the first lengths[sequence] tokens (cap if
  * NULL) of every head, min(length, budget) stay -- those whose ids are within `recent` of the head's largest one (of the
  * lowest slots, if ids that repeat make them more than the budget), then those of the largest weights (NaN in front; equal
- * ones: of the lowest slots).  A token that stays and is in the first
- * min(length, budget) slots keeps its slot; the others that stay move, in order, into the slots that became free, in
- * order.  weights fp32, ids int32 [b][heads][cap], k, v [b][heads][cap][d].  In place where weights_out, ids_out, k_out,
+ * ones: of the lowest slots).  A token that stays and is in the first min(length, budget) slots keeps its slot; the others
+ * that stay move, in order, into the slots that became free, in order.  weights fp32, ids int32 [b][heads][cap], k, v [b][heads][cap][d].  In place where weights_out, ids_out, k_out,
  * v_out are NULL; otherwise those ([b][heads][cap_out], rows of d) take the tokens that stay and the inputs keep theirs.
  * Slots behind the tokens that stay are left as they were.  new_lengths int32 [b] (may be lengths). */
 int64_t lrqk_evict_workspace(int b, int heads, int cap, int budget);

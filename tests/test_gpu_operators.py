@@ -401,6 +401,8 @@ def _weights64(q, k, lengths, lse, scale, weights):
             big = torch.where(at == -INF, 0.0, at).abs()
             each = ds + (ds + U * (m + 64) if lse is None else 0.0) + 4 * U * (1 + big)
             tol[i, h * hc // hq, :m] += (p * each[:, None]).sum(0) + U * (64 + t // 64) * p.sum(0)
+            # fp32 has no normal number below 2^-126: each of the t exponentials below it is off by that at most, being 0 instead
+            tol[i, h * hc // hq, :m] += t * 2.0 ** -126
     return out, tol + 2.0 ** -24 * out.abs()
 
 
@@ -999,3 +1001,22 @@ def test_evict_longer_than_a_workgroup(ops, n):
     odd = w.clone()
     odd[:, :, ::3], odd[:, :, 1::3] = NAN, -INF
     _check_evict(ops, odd, ids, k, v, None, n // 2, 100)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("t,hq", [(3, 2), (40, 1), (70, 2)])
+def test_scores_that_rise_and_fall(ops, dtype, t, hq):
+    """Scores that rise from tile to tile, fall, lie far below zero or jump once: the running maximum is found wherever it
+    is looked for, by both operators."""
+    print("scores", dtype, t, hq, flush=True)
+    n, d = 1200, 64
+    q, kc, vc, kn, vn, mask = _tree_inputs(9, dtype, 1, hq, 1, 1, t, n, d)
+    q[..., 0] = 1.0
+    for name, ramp in (("rise", torch.linspace(-300, 300, n)), ("fall", torch.linspace(300, -300, n)), ("low", torch.full((n,), -5000.0)),
+                       ("high", torch.full((n,), 5000.0)), ("jump", torch.where(torch.arange(n) == 777, 900.0, -900.0))):
+        k = kc.clone()
+        k[..., 0] = ramp.to(DEV).to(dtype)
+        for scale in (1.0, 0.125):
+            out, _ = _check_tree(ops, q, k, vc, kn, vn, mask, scale=scale, what=(name, scale))
+            assert bool(torch.isfinite(out).all())
+            _check_weights(ops, q, k, scale=scale, what=(name, scale))
