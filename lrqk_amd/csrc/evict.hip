@@ -52,7 +52,9 @@ __device__ __forceinline__ int evict_len(const int32_t* lengths, int b, int cap)
   return lengths ? min(max(lengths[b], 0), cap) : cap;
 }
 
-// Sums over the workgroup's threads in order: of what stands in front of the thread, and of all.  Two barriers.
+// Sums over the workgroup's threads in order: of what stands in front of the thread, and of all.  Two barriers (AGAIN: the
+// next one may use the same scratch at once), or one.
+template <bool AGAIN = true>
 __device__ __forceinline__ uint32_t evict_scan(uint32_t v, uint32_t* scratch, uint32_t& total) {
   const uint32_t incl = (uint32_t)wave_inclusive_sum((int)v);
   if (lane_id() == kWave - 1) scratch[wave_id()] = incl;
@@ -64,7 +66,7 @@ __device__ __forceinline__ uint32_t evict_scan(uint32_t v, uint32_t* scratch, ui
     base += w < wave_id() ? c : 0u;
     all += c;
   }
-  __syncthreads();
+  if (AGAIN) __syncthreads();
   total = all;
   return base + incl - v;
 }
@@ -90,14 +92,15 @@ __device__ __forceinline__ void evict_row(const EvictMove& m, int h, int from_sl
 }
 
 // Digit `pass` of the need-th largest key from a histogram (sums of a bin: count(bin)): two bins a thread, the largest
-// first.  `equal`: keys that begin like it; `need` counts among those from here on.
+// first.  `equal`: keys that begin like it; `need` counts among those from here on.  Two barriers: the first, within the
+// next one's sums, keeps the picked numbers until they have been read.
 template <typename F>
 __device__ __forceinline__ void evict_pick(F count, int shift, uint32_t& prefix, uint32_t& need, uint32_t& equal, uint32_t* scratch,
                                            uint32_t* pick_s) {
   const int bin = kEvBins - 1 - 2 * (int)threadIdx.x;
   const uint32_t c[2] = {count(bin), count(bin - 1)};
   uint32_t total;
-  uint32_t before = evict_scan(c[0] + c[1], scratch, total);
+  uint32_t before = evict_scan<false>(c[0] + c[1], scratch, total);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     if (before < need && need <= before + c[j]) {
@@ -111,7 +114,6 @@ __device__ __forceinline__ void evict_pick(F count, int shift, uint32_t& prefix,
   prefix |= pick_s[0] << shift;
   need = pick_s[1];
   equal = pick_s[2];
-  __syncthreads();
 }
 __device__ __forceinline__ int evict_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
 
@@ -231,6 +233,7 @@ __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictMove m, c
   __shared__ uint4 hist[kEvBins];   // (four copies of a bin side by side)
   __shared__ uint32_t scratch[kEvWaves];
   __shared__ uint32_t counts[CHUNKS][kEvWaves + 1];   // (rows in different banks)
+  __shared__ int32_t few_s[2][kEvFew];
   __shared__ uint32_t pick_s[3];
   const int h = blockIdx.x, tid = threadIdx.x;
   const int n = evict_len(lengths, h / heads, m.cap);
@@ -245,6 +248,7 @@ __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictMove m, c
   }
   const float* w = m.w + (int64_t)h * m.cap;
   const int32_t* id = m.ids + (int64_t)h * m.cap;
+  for (int i = tid; i < kEvBins; i += kEvThreads) hist[i] = make_uint4(0, 0, 0, 0);
   uint32_t key[CHUNKS];
   {
     int32_t y[CHUNKS], newest = INT32_MIN;
@@ -266,20 +270,20 @@ __global__ __launch_bounds__(kEvThreads) void evict_select_kernel(EvictMove m, c
   uint32_t prefix = 0, need = (uint32_t)keep, equal = 0;   // the need-th largest of the `equal` keys that begin with `prefix`
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
-    for (int i = tid; i < kEvBins; i += kEvThreads) hist[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
     evict_count<CHUNKS>(key, pass, __builtin_amdgcn_readfirstlane(wave_id()) * kWave, n, prefix, hist);
     __syncthreads();
     evict_pick(
-        [&](int bin) {
+        [&](int bin) {   // (and cleared for the next pass)
           const uint4 four = hist[bin];
+          hist[bin] = make_uint4(0, 0, 0, 0);
           return (four.x + four.y) + (four.z + four.w);
         },
         evict_shift(pass), prefix, need, equal, scratch, pick_s);
     if (need == equal) break;   // (all that begin with it stay: mostly two passes)
   }
-  int32_t* hole = holes + (int64_t)h * budget;
-  int32_t* mover = movers + (int64_t)h * budget;
+  // (few: as many movers at most as there are slots behind `keep`; and LDS is nearer)
+  int32_t* hole = few ? few_s[0] : holes + (int64_t)h * budget;
+  int32_t* mover = few ? few_s[1] : movers + (int64_t)h * budget;
   uint32_t ties = 0, nh = 0, moved = 0;   // (as many movers as holes)
   if (need < equal)
     evict_lists<CHUNKS, true>(key, 0, keep, prefix, need, ties, nh, moved, counts, few ? nullptr : src, hole, mover);
