@@ -10,9 +10,8 @@
 // sines and cosines of a tile of tokens once, into LDS, and turns all heads of those tokens with them: one sine per 40
 // pairs of a prompt with 32 + 8 heads.
 //
-// 32768 tokens of 32 + 8 heads of 128 bf16 elements, from the projections' layout into the heads': 671 MB in 135 to 138 us,
-// 4.9 TB/s, what a large copy reaches.  (Tiles of 16 tokens 154 us, of 8 147, of 2 144; 4093 tokens of 28 + 4 heads of 128 fp32
-// elements 30 to 32 us with any of them.)  One token: 4 us, a launch.
+// 32768 tokens of 32 + 8 heads of 128 bf16 elements, from the projections' layout into the heads': 671 MB in 133 to 136 us,
+// 4.9 TB/s, what a large copy reaches.  One token: 4 us, a launch.
 #include <math.h>
 
 #include <algorithm>
@@ -22,7 +21,6 @@
 namespace lrqk {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotTokens = 4;        // tokens of a workgroup
 constexpr int kRotMaxHalf = 128;     // pairs of a head
 constexpr double kTwoPi = 6.283185307179586476925286766559;
 
@@ -42,6 +40,7 @@ struct RotArgs {
   int64_t s;
   int half, rest;       // pairs, elements behind them
   int groups;           // of heads
+  int tokens;           // of a workgroup
   bool interleaved, transpose;
 };
 
@@ -72,8 +71,8 @@ struct RotVec {
 template <typename T, int V, bool INTERLEAVED>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a, int sub_log2) {
   extern __shared__ float2 cs[];  // [tokens][half]
-  const int64_t t0 = (int64_t)blockIdx.x * kRotTokens;
-  const int tokens = (int)min((int64_t)kRotTokens, a.s - t0);
+  const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
+  const int tokens = (int)min((int64_t)a.tokens, a.s - t0);
   const int64_t b = blockIdx.z;
   for (int e = threadIdx.x; e < tokens * a.half; e += kRotThreads) {
     const int t = e / a.half, i = e - t * a.half;
@@ -154,9 +153,9 @@ static int rotary_launch(const RotArgs& a, int b, bool vec, hipStream_t st) {
   const int pieces = (a.interleaved && vec ? 2 * a.half / V : a.half / V) + a.rest / V;
   int lg = 0;
   while ((1 << lg) < pieces && (1 << lg) < kRotThreads) ++lg;
-  const int64_t tiles = (a.s + kRotTokens - 1) / kRotTokens;
+  const int64_t tiles = (a.s + a.tokens - 1) / a.tokens;
   const dim3 grid((unsigned)tiles, (unsigned)a.groups, (unsigned)b);
-  const size_t lds = sizeof(float2) * kRotTokens * (size_t)std::max(a.half, 1);
+  const size_t lds = sizeof(float2) * a.tokens * (size_t)std::max(a.half, 1);
   if (a.interleaved) {
     if (vec)
       hipLaunchKernelGGL((rotary_kernel<T, VEC, true>), grid, dim3(kRotThreads), lds, st, a, lg);
@@ -254,7 +253,13 @@ extern "C" int lrqk_rotary(const void* q, const void* k, void* q_out, void* k_ou
   a.interleaved = interleaved != 0;
   a.transpose = transpose != 0;
   // as many groups of heads as give the launch a thousand workgroups, four heads each at least
-  const int64_t tiles = (s + kRotTokens - 1) / kRotTokens;
+  // Tiles of up to 40 KB, 64 tokens and 32 KB of sines and cosines.  (32K tokens of 32 + 8 heads of 128 bf16 elements: 2 tokens
+  // 129 us, 4 133, 16 158; 128K of 8 heads: 4 tokens 179, 16 109, 64 134; 256K of one: 4 tokens 124, 64 52; 8K of 28 + 4 fp32:
+  // 2 tokens 41, 4 47; 8K of 128 heads: 1 token 103, 4 114.)
+  const int64_t bytes = (int64_t)(hq + hk) * d * elem_size(dtype);
+  a.tokens = 64;
+  while (a.tokens > 1 && (a.tokens * bytes > 40 * 1024 || a.tokens * a.half > 4096)) a.tokens /= 2;
+  const int64_t tiles = (s + a.tokens - 1) / a.tokens;
   a.groups = (int)std::max<int64_t>(1, std::min<int64_t>((hq + hk + 3) / 4, 1024 / (tiles * b)));
   hipStream_t st = (hipStream_t)stream;
   if (dtype == LRQK_F32) return rotary_launch<float>(a, b, vok, st);

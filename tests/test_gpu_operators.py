@@ -1020,3 +1020,19 @@ def test_scores_that_rise_and_fall(ops, dtype, t, hq):
             out, _ = _check_tree(ops, q, k, vc, kn, vn, mask, scale=scale, what=(name, scale))
             assert bool(torch.isfinite(out).all())
             _check_weights(ops, q, k, scale=scale, what=(name, scale))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("b,hq,hk,s,d,rd", [(1, 1, 0, 300, 16, 16), (2, 3, 1, 130, 64, 48), (1, 70, 2, 9, 256, 256), (1, 8, 8, 257, 256, 256),
+                                            (2, 300, 20, 5, 128, 128), (1, 2, 2, 4097, 8, 8)])
+def test_rotary_over_many_tiles(ops, dtype, b, hq, hk, s, d, rd):
+    """Tiles of one token to 64, the last one not whole."""
+    print("rotary tiles", dtype, b, hq, hk, s, d, flush=True)
+    g = _gen(s)
+    for interleaved in (False, True):
+        plan = ops.RotaryPlan(rd, 1e4, interleaved, None, DEV)
+        q, k = _randn(g, b, s, hq, d, dtype=dtype).transpose(1, 2), _randn(g, b, hk, s, d, dtype=dtype) if hk else None
+        pos = torch.randint(0, 100000, (b, s), generator=g, dtype=torch.int32).to(DEV)
+        y = ops.rotary(plan, q, k, pos)
+        for x, z in zip((q, k), y) if hk else ((q, y),):
+            _check_rotary(plan, x, z, pos, what=interleaved)
