@@ -296,9 +296,9 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_columns_kernel(WeightAr
 #pragma unroll
   for (int j = 0; j < NT; ++j) sum[j] = part[j] = 0.0f;
   if (first0 < len) {   // (the same for all waves)
-    // tiles of queries: of one query head each, from the first that sees a key of the workgroup; or, of few queries a head,
-    // of several heads
-    const bool packed = a.t < 16;
+    // tiles of queries: of one query head each, from the first that sees a key of the workgroup; or, of heads with less than a
+    // tile, of several heads (16 tokens of 128 heads over 64K of one: 78 us instead of 174; from 32 tokens on no faster)
+    const bool packed = a.t < kAwTile;
     const int t0 = packed ? 0 : max(0, first0 - behind) / kAwTile;
     const int per = packed ? 1 : (a.t + kAwTile - 1) / kAwTile - t0;
     const int items = packed ? (M + kAwTile - 1) / kAwTile : gc * per;
