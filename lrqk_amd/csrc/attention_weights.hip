@@ -9,7 +9,7 @@
 //            a sum of its own for its query and meets the other lanes at the end only.  Few queries: the keys are split
 //            and `merge` joins the parts.
 //   columns  sums: a wave has 16 NT keys and walks over the queries that see them, S = Q K^T, so that a lane's sums are
-//            those of its keys; chunks of the queries, which `sum` adds up.
+//            those of its keys; chunks of the queries, which `sum` adds up where there are several.
 //   stream   the same for up to 64 queries of a cache head (rows of 256 bytes): a wave has all of them and streams keys, S^T = K Q^T, whose
 //            rows it adds up across the lanes.
 //
@@ -416,11 +416,12 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_columns_kernel(WeightAr
     }
   }
   if (first >= a.n) return;
-  float* out = a.part + (int64_t)chunk * a.heads * a.n + row;
+  float* out = (a.chunks == 1 ? a.out : a.part + (int64_t)chunk * a.heads * a.n) + row;
+  const float* had = a.chunks == 1 && a.weights ? a.weights + row : nullptr;
 #pragma unroll
   for (int j = 0; j < NT; ++j) {
     sum[j] = ar_quad_sum(sum[j] + part[j]);
-    if (quad == 0 && first + 16 * j + col < a.n) out[16 * j + col] = sum[j];
+    if (quad == 0 && first + 16 * j + col < a.n) out[16 * j + col] = had ? had[16 * j + col] + sum[j] : sum[j];
   }
 }
 
@@ -549,7 +550,7 @@ static WeightPlan weights_plan(int b, int hq, int hc, int t, int64_t n, int d, i
   // eight tiles of queries for each
   const int64_t blocks = (n + 16 * p.nt * kAwWaves - 1) / (16 * p.nt * kAwWaves), items = (M + 15) / 16;
   p.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(2048 / (blocks * heads), items / 16));
-  if (!p.few) p.part = heads * n * p.chunks;
+  if (!p.few && p.chunks > 1) p.part = heads * n * p.chunks;
   if (have_lse) return p;
   // (lse over 8192 keys: 64 queries a cache head 7.8 us with 16 a wave, 12.7 with 64; 128 9.0 and 13; 1024 34 and 29)
   p.rows_nt = M <= 128 ? 1 : p.nt;
@@ -608,6 +609,7 @@ static int weights_launch(WeightArgs a, const WeightPlan& p, int heads, hipStrea
   hipLaunchKernelGGL((weights_columns_kernel<T, DP, NT>), dim3((unsigned)((int64_t)(a.n + KEYS - 1) / KEYS * p.chunks * heads)),
                      dim3(kAwThreads), 0, st, a);
   LRQK_HIP_CHECK(hipGetLastError());
+  if (p.chunks == 1) return LRQK_OK;   // (the columns have added to the weights themselves)
   const int64_t count = (int64_t)heads * a.n;
   hipLaunchKernelGGL(weights_sum_kernel, dim3((unsigned)((count + kAwThreads - 1) / kAwThreads)), dim3(kAwThreads), 0, st, a, count);
   LRQK_HIP_CHECK(hipGetLastError());
