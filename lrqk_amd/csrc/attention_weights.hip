@@ -539,7 +539,11 @@ static WeightPlan weights_plan(int b, int hq, int hc, int t, int64_t n, int d, i
   p.dp = d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256;
   const int64_t M = (int64_t)(hq / hc) * t, heads = (int64_t)b * hc;
   const int row = p.dp * (int)elem_size(dtype);
-  p.nt = row <= 256 ? 4 : row <= 512 ? 2 : 1;
+  const int most = row <= 256 ? 4 : row <= 512 ? 2 : 1;   // 16 keys, or queries, that a wave has registers for
+  // 64 keys a wave where the products are many (8K prompt of 32 / 8 heads of 128: 352 us with 64, 362 with 32; 512 tokens over
+  // 64K: 395, 420), 32 where workgroups that load while others multiply count for more (4K prompt: 133, 106; 512 tokens over
+  // 8K: 68, 63; 200 over 32K: 115, 108; 200 over 1K: 29, 19)
+  p.nt = heads * M * (n - t / 2) >= (int64_t)1 << 29 ? most : std::min(most, 2);
   p.few = M <= (row <= 256 ? 64 : row <= 512 ? 32 : 16);   // (what a wave has room for; both kernels measured at weights_stream_kernel)
   if (p.few) {
     // four workgroups per CU, two tiles for each of a workgroup's waves at least
@@ -552,8 +556,9 @@ static WeightPlan weights_plan(int b, int hq, int hc, int t, int64_t n, int d, i
   p.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(2048 / (blocks * heads), items / 16));
   if (!p.few && p.chunks > 1) p.part = heads * n * p.chunks;
   if (have_lse) return p;
-  // (lse over 8192 keys: 64 queries a cache head 7.8 us with 16 a wave, 12.7 with 64; 128 9.0 and 13; 1024 34 and 29)
-  p.rows_nt = M <= 128 ? 1 : p.nt;
+  // (lse over 8192 keys: 64 queries a cache head 7.8 us with 16 a wave, 12.7 with 64; 128 9.0 and 13; 1024 34 and 29;
+  // both passes of an 8K prompt: 665 us with 64, 694 with 32)
+  p.rows_nt = M <= 128 ? 1 : most;
   p.groups = (int)((M + 64 * p.rows_nt - 1) / (64 * p.rows_nt));
   // parts of one length, however many keys a group of queries sees (a prompt's first ones few): four thousand, with eight
   // tiles of 32 keys at least.  (One part a group, 8K tokens: a quarter of the GPU waited for the longest ones; two thousand
@@ -605,9 +610,14 @@ static int weights_launch(WeightArgs a, const WeightPlan& p, int heads, hipStrea
     LRQK_HIP_CHECK(hipGetLastError());
     return LRQK_OK;
   }
-  constexpr int NT = DP * (int)sizeof(T) <= 256 ? 4 : DP * (int)sizeof(T) <= 512 ? 2 : 1, KEYS = 16 * NT * kAwWaves;
-  hipLaunchKernelGGL((weights_columns_kernel<T, DP, NT>), dim3((unsigned)((int64_t)(a.n + KEYS - 1) / KEYS * p.chunks * heads)),
-                     dim3(kAwThreads), 0, st, a);
+  const int keys = 16 * p.nt * kAwWaves;
+  const dim3 grid((unsigned)((int64_t)(a.n + keys - 1) / keys * p.chunks * heads));
+  constexpr int ROW = DP * (int)sizeof(T);
+  if constexpr (ROW <= 256)
+    if (p.nt == 4) hipLaunchKernelGGL((weights_columns_kernel<T, DP, 4>), grid, dim3(kAwThreads), 0, st, a);
+  if constexpr (ROW <= 512)
+    if (p.nt == 2) hipLaunchKernelGGL((weights_columns_kernel<T, DP, 2>), grid, dim3(kAwThreads), 0, st, a);
+  if constexpr (ROW > 512) hipLaunchKernelGGL((weights_columns_kernel<T, DP, 1>), grid, dim3(kAwThreads), 0, st, a);
   LRQK_HIP_CHECK(hipGetLastError());
   if (p.chunks == 1) return LRQK_OK;   // (the columns have added to the weights themselves)
   const int64_t count = (int64_t)heads * a.n;

@@ -1036,3 +1036,14 @@ def test_rotary_over_many_tiles(ops, dtype, b, hq, hk, s, d, rd):
         y = ops.rotary(plan, q, k, pos)
         for x, z in zip((q, k), y) if hk else ((q, y),):
             _check_rotary(plan, x, z, pos, what=interleaved)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (BF, 64), (BF, 24), (FP, 64), (FP, 128)])
+def test_attention_weights_of_many_products(ops, dtype, d):
+    """Where a wave takes 64 keys at a time: many tokens over a long cache."""
+    print("weights many", dtype, d, flush=True)
+    g = _gen(d)
+    q, k = _randn(g, 1, 32, 2050, d, dtype=dtype, scale=2.0), _randn(g, 1, 8, 10007, d, dtype=dtype)
+    lengths = torch.tensor([10001], dtype=torch.int32, device=DEV)
+    for lse in (None, _randn(g, 1, 32, 2050) + 6.0):
+        _check_weights(ops, q, k, lengths, lse, weights=torch.rand((1, 8, 10007), generator=g).to(DEV))
