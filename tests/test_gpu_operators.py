@@ -1047,3 +1047,25 @@ def test_attention_weights_of_many_products(ops, dtype, d):
     lengths = torch.tensor([10001], dtype=torch.int32, device=DEV)
     for lse in (None, _randn(g, 1, 32, 2050) + 6.0):
         _check_weights(ops, q, k, lengths, lse, weights=torch.rand((1, 8, 10007), generator=g).to(DEV))
+
+
+@pytest.mark.parametrize("d", [8, 32, 48, 64, 128, 200, 256])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_tree_attention_of_every_kernel_and_width(ops, dtype, d):
+    """10, 30, 60, 120 and 150 queries a cache head at every width, lengths that end in a tile."""
+    print("tree all", dtype, d, flush=True)
+    for t, hq in ((5, 2), (15, 2), (30, 2), (60, 2), (50, 3)):
+        q, kc, vc, kn, vn, mask = _tree_inputs(d + t, dtype, 2, hq, 1, 1, t, 470, d)
+        _check_tree(ops, q, kc, vc, kn, vn, mask, torch.tensor([467, 75], dtype=torch.int32, device=DEV), what=t)
+
+
+@pytest.mark.parametrize("t", [1, 3, 4, 5, 7, 8, 9, 12, 31, 32, 33, 63, 65, 127, 257])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_tree_masks_of_odd_lengths(ops, dtype, t):
+    """A row of the mask begins anywhere and ends in the middle of a quad's keys: every byte of it counts at its place."""
+    print("tree odd masks", dtype, t, flush=True)
+    for hq in (1, 6):
+        for density in (0.05, 0.9):
+            q, kc, vc, kn, vn, mask = _tree_inputs(t, dtype, 2, hq, 1, 1, t, 20, 32, density)
+            _check_tree(ops, q, kc, vc, kn, vn, mask, torch.tensor([0, 13], dtype=torch.int32, device=DEV), what=(hq, density))
+            _check_tree(ops, q, kc, vc, kn, vn, mask[1], None, what=(hq, density))
