@@ -317,7 +317,7 @@ __device__ __forceinline__ void tree_mask(float (&p)[MT][NE], const TreeArgs& a,
 }
 
 // Few queries: the four waves of a workgroup take the tiles of its split in turn, each for itself.  Bound by the reading of
-// K and V: a token over 32K of 8 cache heads of 128 bf16 elements, 134 MB in 27 us, 5.0 TB/s, and the join 6.  (Of few tokens
+// K and V: a token over 32K of 8 cache heads of 128 bf16 elements, 134 MB in 27 us, 5.0 TB/s, and the join 5.  (Of few tokens
 // by the chain of the first reads: 2112 of 32 heads, 10 us.)  Up to 32 queries a cache head: tree_share_kernel takes 58 us
 // for 16 or 32 of them where this one takes 51 (32K tokens, after 256 MB of writes), of fp32 40 instead of 29 and 35 (8K).
 template <typename T, int DP, int MT>
@@ -823,26 +823,31 @@ __global__ __launch_bounds__(kTlThreads, 2) void tree_share_kernel(TreeArgs a) {
   }
 }
 
-// A workgroup joins the splits' parts of 16 queries of a cache head, a quad of the lanes that hold them (a quarter of the
-// head): 16 threads with a query each for (block j of the output, every G-th split).  SHARED: which of the two kernels left
+// Blocks of 16 elements of the head that a workgroup of the join has.
+constexpr int tree_join_blocks(int blocks, int threads) { return threads == 512 && blocks > 4 ? 4 : blocks; }
+
+// A workgroup joins the splits' parts of 16 queries of a cache head, VB blocks of a quad of the lanes that hold them (a
+// quarter of the head): 16 threads with a query each for (block j, every G-th split).  SHARED: which of the two kernels left
 // the parts, whose lanes have other elements.  Its time is a chain of reads that wait for each other and barriers, so the
 // reads are few in a row, and what 16 queries of all waves make is added up by every thread that wants it.
 template <typename T, int DP, bool SHARED, int THREADS>
 __global__ __launch_bounds__(THREADS) void tree_join_kernel(TreeArgs a) {
-  constexpr int VW = DP / 16, GROUPS = THREADS / 16, G = GROUPS / VW, FIRST = 4, NW = THREADS / kWave;
+  constexpr int VW = DP / 16, VB = tree_join_blocks(VW, THREADS), JS = VW / VB;
+  constexpr int GROUPS = THREADS / 16, G = GROUPS / VB, FIRST = 4, NW = THREADS / kWave;
   __shared__ float f_s[kTrMaxSplits][16];
   __shared__ float red[3][NW][16];
-  __shared__ ar_f4 joint[G][VW][16];
+  __shared__ ar_f4 joint[G][VB][16];
   const int col = threadIdx.x & 15, group = threadIdx.x >> 4, wave = wave_id();
-  const int quad = (int)blockIdx.x & 3, tile = (int)(blockIdx.x >> 2) % a.row_tiles, head = (int)(blockIdx.x >> 2) / a.row_tiles;
+  const int quad = (int)blockIdx.x & 3, j0 = (int)(blockIdx.x >> 2) % JS * VB, place = (int)(blockIdx.x >> 2) / JS;
+  const int tile = place % a.row_tiles, head = place / a.row_tiles;
   const int M = a.hq / a.hc * a.t, row0 = 16 * tile, b = head / a.hc;
   const int slot0 = a.b == 1 ? 0 : a.cut[2 * b], slots = a.units / a.hc;
   const int64_t unit0 = (int64_t)slot0 * a.hc + head % a.hc;   // + split * hc
   const bool mine = row0 + col < M;
   // (the first parts are asked for before it is known how many there are: the scratch has room for `slots`, and what is
   // behind the sequence's is not looked at)
-  const int j = group % VW, g = group / VW;
-  const ar_f4* part = (const ar_f4*)a.part + ((unit0 * a.row_tiles + tile) * VW + j) * kWave + quad * 16 + col;
+  const int j = group % VB, g = group / VB;
+  const ar_f4* part = (const ar_f4*)a.part + ((unit0 * a.row_tiles + tile) * VW + j0 + j) * kWave + quad * 16 + col;
   const int64_t next = (int64_t)a.hc * a.row_tiles * VW * kWave;
   const float* ml = a.part_ml + (unit0 * a.row_tiles + tile) * 48 + col;
   const int64_t ml_next = (int64_t)a.hc * a.row_tiles * 48;
@@ -899,10 +904,10 @@ __global__ __launch_bounds__(THREADS) void tree_join_kernel(TreeArgs a) {
   joint[g][j][col] = x;
   __syncthreads();
   const int64_t row = (int64_t)head * M + row0;   // rows of all heads follow each other
-  for (int e = threadIdx.x; e < 16 * 4 * VW; e += THREADS) {
-    const int r = e / (4 * VW), y = e % (4 * VW);
-    const int blk = SHARED ? y / 4 : y % VW, i = SHARED ? y % 4 : y / VW;
-    const int d = SHARED ? 16 * blk + 4 * quad + i : 4 * VW * quad + y;
+  for (int e = threadIdx.x; e < 16 * 4 * VB; e += THREADS) {
+    const int r = e / (4 * VB), y = e % (4 * VB);
+    const int blk = SHARED ? y / 4 : y % VB, i = SHARED ? y % 4 : y / VB;
+    const int d = SHARED ? 16 * (j0 + blk) + 4 * quad + i : 4 * VW * quad + VW * i + j0 + blk;
     if (d >= a.d || row0 + r >= M) continue;
     float v = 0.0f, all = 0.0f;
 #pragma unroll
@@ -920,7 +925,7 @@ __global__ __launch_bounds__(THREADS) void tree_join_kernel(TreeArgs a) {
     }
     st_f32((T*)a.out, (row + r) * a.d + d, all == 0.0f ? 0.0f : v / all);
   }
-  if (a.lse && quad == 0 && threadIdx.x < 16 && mine) {
+  if (a.lse && quad == 0 && j0 == 0 && threadIdx.x < 16 && mine) {
     float all = 0.0f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) all += red[1][w][col];
@@ -972,12 +977,12 @@ static TreePlan tree_plan(int b, int hq, int hc, int t, int64_t n, int d, bool l
   return p;
 }
 
-// (few workgroups: more threads for the splits of each.  64 workgroups 7 us instead of 10, 256 workgroups 10.6 instead of
-// 12.6; 1024 workgroups 10.6 instead of 9.8)
+// (few workgroups: more threads for the splits of each, and more workgroups.  Of 64 workgroups 6.5 us instead of 10, of 256
+// 10.3 instead of 12.6; of 1024 13.4 instead of 9.9)
 template <typename T, int DP, bool SHARED>
 static void tree_join_launch(const TreeArgs& a, dim3 grid, hipStream_t st) {
   if (grid.x <= 512)
-    hipLaunchKernelGGL((tree_join_kernel<T, DP, SHARED, 512>), grid, dim3(512), 0, st, a);
+    hipLaunchKernelGGL((tree_join_kernel<T, DP, SHARED, 512>), dim3(grid.x * (DP / 16 / tree_join_blocks(DP / 16, 512))), dim3(512), 0, st, a);
   else
     hipLaunchKernelGGL((tree_join_kernel<T, DP, SHARED, 256>), grid, dim3(256), 0, st, a);
 }
