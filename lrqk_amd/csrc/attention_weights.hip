@@ -533,6 +533,8 @@ struct WeightPlan {
   int dp, rows_nt, groups, parts, per, nt, chunks, few_per;
   bool few;
   int64_t lse2, part;   // floats
+  int64_t part_at() const { return (lse2 + 3) / 4 * 4; }
+  int64_t bytes() const { return (part_at() + part) * (int64_t)sizeof(float); }
 };
 static WeightPlan weights_plan(int b, int hq, int hc, int t, int64_t n, int d, int dtype, bool have_lse) {
   WeightPlan p{};
@@ -543,7 +545,7 @@ static WeightPlan weights_plan(int b, int hq, int hc, int t, int64_t n, int d, i
   // 64 keys a wave where the products are many (8K prompt of 32 / 8 heads of 128: 352 us with 64, 362 with 32; 512 tokens over
   // 64K: 395, 420), 32 where workgroups that load while others multiply count for more (4K prompt: 133, 106; 512 tokens over
   // 8K: 68, 63; 200 over 32K: 115, 108; 200 over 1K: 29, 19)
-  p.nt = heads * M * (n - t / 2) >= (int64_t)1 << 29 ? most : std::min(most, 2);
+  p.nt = (double)heads * (double)M * (double)(n - t / 2) >= 0x1p29 ? most : std::min(most, 2);
   p.few = M <= (row <= 256 ? 64 : row <= 512 ? 32 : 16);   // (what a wave has room for; both kernels measured at weights_stream_kernel)
   if (p.few) {
     // four workgroups per CU, two tiles for each of a workgroup's waves at least
@@ -653,7 +655,7 @@ extern "C" int64_t lrqk_attention_weights_workspace(int b, int hq, int hc, int t
   const int rc = weights_check(b, hq, hc, t, n, d, dtype);
   if (rc) return rc;
   const WeightPlan p = weights_plan(b, hq, hc, t, n, d, dtype, have_lse != 0);
-  return (p.lse2 + p.part) * (int64_t)sizeof(float);
+  return p.bytes();
 }
 
 extern "C" int lrqk_attention_weights(const void* q, const void* k, int64_t k_batch_stride, int64_t k_head_stride, int64_t k_row_stride,
@@ -669,14 +671,14 @@ extern "C" int lrqk_attention_weights(const void* q, const void* k, int64_t k_ba
                    k_head_stride % vec == 0 && k_row_stride % vec == 0,
                LRQK_EINVAL, "pointers and rows must be 16-byte aligned");
   const WeightPlan p = weights_plan(b, hq, hc, t, n, d, dtype, lse != nullptr);
-  const int64_t need = (p.lse2 + p.part) * (int64_t)sizeof(float);
+  const int64_t need = p.bytes();
   LRQK_REQUIRE(workspace_bytes >= need && (workspace || need == 0), LRQK_EINVAL, "workspace of %lld bytes: %lld are needed", (long long)workspace_bytes,
                (long long)need);
   // (a launch's workgroups are counted in 31 bits; no memory holds what would need more)
   const int64_t places = std::max((int64_t)p.groups * std::max(p.parts, 1), (n + 63) / 64 * p.chunks);
   LRQK_REQUIRE(places * b * hc <= INT32_MAX, LRQK_ELIMIT, "%lld keys of %d heads and %d queries are more than a launch has places for",
                (long long)n, b * hc, t);
-  WeightArgs a{q, k, lengths, lse, kLog2e, (float*)workspace, (float*)workspace + p.lse2, weights, out, k_batch_stride, k_head_stride,
+  WeightArgs a{q, k, lengths, lse, kLog2e, (float*)workspace, (float*)workspace + p.part_at(), weights, out, k_batch_stride, k_head_stride,
                k_row_stride, (int)n, hq, hc, t, d, p.parts, p.per, p.groups, p.chunks, (uint32_t)(b * hc), scale * kLog2e};
   hipStream_t st = (hipStream_t)stream;
   if (dtype == LRQK_F32) return weights_launch_dp<float>(a, p, b * hc, st);
