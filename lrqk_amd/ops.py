@@ -693,8 +693,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if mask.shape not in ((b, t, t), (t, t)) or mask.dtype not in (torch.bool, torch.uint8):
         raise ValueError(f"mask is {tuple(mask.shape)} {mask.dtype}: bool or uint8 [t,t] or [b,t,t] is wanted")
     _lengths(lengths, b)
-    st = _row_strides("k_cache", k_cache)
-    if _row_strides("v_cache", v_cache) != st and n > 0:
+    st, sv = _row_strides("k_cache", k_cache), _row_strides("v_cache", v_cache)
+    if sv != st and n > 0 and any(x != y and m > 1 for x, y, m in zip(st, sv, k_cache.shape)):   # (one of a kind has no stride)
         raise ValueError("k_cache and v_cache must have the same strides")
     q = q.contiguous()
     out = torch.empty_like(q)
@@ -778,6 +778,8 @@ def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Te
         for name, y, shape, dtype in zip(("weights", "ids", "k", "v"), out, ((b, h, cap_out),) * 2 + ((b, h, cap_out, d),) * 2,
                                          (torch.float32, torch.int32, k.dtype, k.dtype)):
             _expect("out " + name, y, shape, dtype)
+        if out[2].data_ptr() == out[3].data_ptr() and out[2].numel():
+            raise ValueError("out of k and of v are in one place")
         if cap_out < min(budget, n):
             raise ValueError(f"out has {cap_out} slots for min(budget={budget}, {n}) tokens")
         if not all(_apart(x, y) for x in (weights, ids, k, v) for y in out):

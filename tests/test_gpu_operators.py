@@ -1069,3 +1069,66 @@ def test_tree_masks_of_odd_lengths(ops, dtype, t):
             q, kc, vc, kn, vn, mask = _tree_inputs(t, dtype, 2, hq, 1, 1, t, 20, 32, density)
             _check_tree(ops, q, kc, vc, kn, vn, mask, torch.tensor([0, 13], dtype=torch.int32, device=DEV), what=(hq, density))
             _check_tree(ops, q, kc, vc, kn, vn, mask[1], None, what=(hq, density))
+
+
+def test_strides_of_one_sequence_or_head_do_not_count(ops):
+    """K and V of one sequence out of batches of different sizes, of one head out of different ones, of one token."""
+    print("tree single strides", flush=True)
+    q, kc, vc, kn, vn, mask = _tree_inputs(2, BF, 1, 4, 2, 2, 3, 40, 32)
+    ref = ops.tree_attention(q, kc, vc, kn, vn, mask)
+    wide = torch.zeros((40, 2, 80, 32), dtype=BF, device=DEV)
+    wide = wide.as_strided((1, 2, 40, 32), (8, kc.stride(1), 32, 1))
+    wide.copy_(vc)
+    assert torch.equal(ops.tree_attention(q, kc, wide, kn, vn, mask), ref)
+    one = torch.zeros((1, 3, 40, 32), dtype=BF, device=DEV)[:, 1:2].copy_(vc[:, :1])
+    assert torch.equal(ops.tree_attention(q[:, :2], kc[:, :1], one, kn[:, :1], vn[:, :1], mask), ref[:, :2])
+    with pytest.raises(ValueError):
+        ops.tree_attention(q, kc, torch.cat((vc, vc), 3)[..., :32], kn, vn, mask)
+
+
+def test_evict_refuses_one_place_for_k_and_v(ops):
+    w, ids, k, v = _cache(_gen(0), 1, 1, 20, 16, BF)
+    out = [x[:, :, :8].clone() for x in (w, ids, k)]
+    with pytest.raises(ValueError):
+        ops.evict(w, ids, k, v, None, 8, 2, out=(*out, out[2]))
+
+
+def test_the_long_forms_replayed_from_a_graph(ops):
+    """A prompt's weights, wide drafts and the eviction of a long head, captured together and replayed with other inputs and
+    lengths, eager work between the replays."""
+    print("graph, long forms", flush=True)
+    g = _gen(77)
+    n, t = 40000, 200
+    mask = torch.ones((t, t), dtype=torch.bool, device=DEV).tril()
+    q, k, v = _randn(g, 2, 4, t, 64, dtype=BF), _randn(g, 2, 2, t, 64, dtype=BF), _randn(g, 2, 2, t, 64, dtype=BF)
+    w, ids, kc, vc = _cache(g, 2, 2, n, 64, BF)
+    lengths = torch.tensor([n, n - 3000], dtype=torch.int32, device=DEV)
+    out = [torch.zeros((2, 2, 2112, *x.shape[3:]), dtype=x.dtype, device=DEV) for x in (w, ids, kc, vc)]
+
+    def work():
+        a, lse = ops.tree_attention(q, kc, vc, k, v, mask, lengths, return_lse=True)
+        prompt = ops.attention_weights(q, k)
+        ops.attention_weights(q, kc, lengths, lse, weights=w)
+        new = ops.evict(w, ids, kc, vc, lengths, 2112, 64, out=tuple(out))
+        return a, lse, prompt, new
+    kept = w.clone()
+    work()
+    w.copy_(kept)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work()
+    for i in range(4):
+        q.copy_(_randn(g, 2, 4, t, 64, dtype=BF))
+        lengths.copy_(torch.tensor([n - 1000 * i, 2000 + 9000 * i], dtype=torch.int32))
+        w.copy_(kept)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [x.clone() for x in (*got, w, *out)]
+        w.copy_(kept)
+        eager = (*work(), w, *out)
+        torch.cuda.synchronize()
+        keep = [min(int(m), 2112) for m in lengths]
+        for x, y in zip(replayed[:5], eager[:5]):
+            assert torch.equal(x, y)
+        for x, y in zip(replayed[5:], eager[5:]):
+            assert all(torch.equal(x[b, :, :keep[b]], y[b, :, :keep[b]]) for b in range(2))
