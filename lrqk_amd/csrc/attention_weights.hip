@@ -95,8 +95,8 @@ struct WeightTile {
 };
 
 // Item (head, part, group of 64 NT rows) of a workgroup: its queries' maximum and sum over its part of the keys.  Bound by
-// the exponentials (16 cycles of a SIMD for a wave's 64, and 8 more for scaling and adding, beside 2 16x16x32 products' 16):
-// 8192 tokens of 32 / 8 heads of 128, 275 GFLOP in 315 to 360 us, and `merge` 8.
+// the exponentials beside the products: 8192 tokens of 32 / 8 heads of 128, 275 GFLOP in 321 to 350 us, the vector ALUs 59 %
+// busy, the matrix cores 37 %; `merge` 8.
 template <typename T, int DP, int NT>
 __global__ __launch_bounds__(kAwThreads, 2) void weights_rows_kernel(WeightArgs a) {
   using Tile = WeightTile<T, DP>;
@@ -271,8 +271,10 @@ __global__ __launch_bounds__(kAwThreads) void weights_merge_kernel(WeightArgs a,
   a.lse2[row] = sum == 0.0f ? -INFINITY : top + log2f(sum);
 }
 
-// 64 NT keys and a chunk of the queries a workgroup.  Bound as the rows are: 8192 tokens, 342 to 380 us, and `sum` 5.  (Keys in
-// registers and queries through LDS: the other way round a wave's sums would be rows' and cross the lanes for every tile.)
+// 64 NT keys and a chunk of the queries a workgroup.  Bound as the rows are: 8192 tokens, 352 to 390 us, vector ALUs 51 %,
+// matrix cores 33 %, no bank conflicts, and `sum` 5.  (Keys in registers and queries through LDS: the other way round a wave's
+// sums would be rows' and cross the lanes for every tile.  Products of 16 keys placed between the exponentials of the 16 before:
+// no difference; 64 queries a tile, half the barriers: 425 us, the registers do not hold them.)
 template <typename T, int DP, int NT>
 __global__ __launch_bounds__(kAwThreads, 2) void weights_columns_kernel(WeightArgs a) {
   using Tile = WeightTile<T, DP>;
