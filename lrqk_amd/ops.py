@@ -604,7 +604,8 @@ class RotaryPlan:
 
 
 def _same_view(x: torch.Tensor, y: torch.Tensor) -> bool:
-    return x.data_ptr() == y.data_ptr() and x.shape == y.shape and x.stride() == y.stride()
+    return (x.data_ptr() == y.data_ptr() and x.shape == y.shape and
+            all(a == b or n < 2 for n, a, b in zip(x.shape, x.stride(), y.stride())))
 
 
 def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
@@ -614,11 +615,51 @@ def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
     return x.numel() == 0 or y.numel() == 0 or end(x) <= y.data_ptr() or end(y) <= x.data_ptr()
 
 
+def _once(x: torch.Tensor) -> bool:
+    """Whether every element of a view has a place of its own (a view that cannot be made by slicing and permuting counts as one
+    that has not)."""
+    inner = 1
+    for stride, n in sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1):
+        if stride < inner:
+            return False
+        inner += (n - 1) * stride
+    return True
+
+
+def _blocks_meet(shift: int, x: int, y: int, dims) -> bool:
+    """Whether a block of x bytes and one of y bytes, ``shift`` behind it, meet.  dims: what both consist of, (bytes between
+    slabs, slabs of x, slabs of y), longest first; without any a block is whole."""
+    if shift >= x or -shift >= y:
+        return False
+    if not dims:
+        return True
+    step, nx, ny = dims[0]
+    x, y = x - (nx - 1) * step, y - (ny - 1) * step
+    # a slab of y lies j steps from one of x: those j at which they reach each other, as far as whole slabs go
+    first, last = max(1 - nx, (-y - shift) // step + 1), min(ny - 1, -((shift - x) // step) - 1)
+    return last - first > 3 or any(_blocks_meet(shift + j * step, x, y, dims[1:]) for j in range(first, last + 1))
+
+
+def _meet(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether two views have memory in common.  Views that lie between each other, as the parts of one projection do, are told
+    apart where their dimensions have the same strides; otherwise views whose ranges meet count as meeting."""
+    if _apart(x, y):
+        return False
+    e, dims = x.element_size(), []
+    if x.dim() == y.dim() and y.element_size() == e:
+        for nx, ny, sx, sy in zip(x.shape, y.shape, x.stride(), y.stride()):
+            step = sx if nx > 1 else sy
+            if max(nx, ny) > 1 and step > 0 and (sx == sy or min(nx, ny) == 1):
+                dims.append((step * e, nx, ny))
+    size = [t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) for t in (x, y)]
+    return _blocks_meet(y.data_ptr() - x.data_ptr(), *size, sorted(dims, reverse=True))
+
+
 def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positions, transpose: bool = False, out=None):
     """q [b,Hq,s,d] and k [b,Hk,s,d] (or None) turned to ``positions``: int32 [s] or [b,s] on the GPU, or the first one of
-    s that follow each other.  Any strides, rows contiguous.  ``out``: (q', k') to write to, each of them any view that is
-    its input or apart from both inputs, and that share no element; else new contiguous tensors.  ``transpose`` turns back: the gradient of the turn.
-    Returns (q', k'), or q' without a k."""
+    s that follow each other.  Any strides, rows contiguous.  ``out``: (q', k') to write to, each of them its input or a view
+    that has no element in common with an input, and none with the other (parts of one projection may lie between each other);
+    else new contiguous tensors.  ``transpose`` turns back: the gradient of the turn.  Returns (q', k'), or q' without a k."""
     pos = positions if isinstance(positions, torch.Tensor) else None
     dev = _on_one_gpu(q, k, pos, plan.inv_freq)
     b, hq, s, d = q.shape
@@ -650,14 +691,15 @@ def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positio
         if len(ys) != len(xs) or any(y is None for y in ys):
             raise ValueError("out holds one tensor for q, and one for k if there is a k")
         _on_one_gpu(q, *ys)
-        for x, y in zip(xs, ys):
+        for i, (x, y) in enumerate(zip(xs, ys)):
             _expect("out", y, x.shape, x.dtype, contiguous=False)
-            if any(n > 1 and st == 0 for n, st in zip(y.shape, y.stride())):
+            if not _once(y):
                 raise ValueError("out has several elements in one place")
-            if not _same_view(x, y) and not all(_apart(y, z) for z in xs):
+            others = xs[1 - i:2 - i] if _same_view(x, y) else xs
+            if any(z is not None and _meet(y, z) for z in (*others, pos, plan.inv_freq)):
                 raise ValueError("out overlaps an input and is not the view that is turned")
-        if k is not None and ys[0].data_ptr() == ys[1].data_ptr() and q.numel() and k.numel():
-            raise ValueError("out of q and of k are in one place")
+        if k is not None and _meet(*ys):
+            raise ValueError("out of q and out of k overlap")
         q_out, k_out = ys if k is not None else (ys[0], None)
     strides = (*_row_strides("q", q), *_row_strides("out", q_out))
     if k is not None:

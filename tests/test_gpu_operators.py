@@ -1132,3 +1132,38 @@ def test_the_long_forms_replayed_from_a_graph(ops):
             assert torch.equal(x, y)
         for x, y in zip(replayed[5:], eager[5:]):
             assert all(torch.equal(x[b, :, :keep[b]], y[b, :, :keep[b]]) for b in range(2))
+
+
+def test_rotary_refuses_outputs_that_overlap(ops):
+    """An input turned in place while the other one is read from the same memory, outputs shifted into each other, an output
+    over the positions."""
+    plan = ops.RotaryPlan(64, 1e4, False, None, DEV)
+    q, k = torch.zeros(1, 2, 3, 64, device=DEV), torch.zeros(1, 2, 3, 64, device=DEV)
+    flat, fresh = torch.zeros(2 * 384, device=DEV), torch.zeros(1, 2, 3, 64, device=DEV)
+    low, high = flat[:384].view(1, 2, 3, 64), flat[4:388].view(1, 2, 3, 64)
+    pos = flat[:3].view(torch.int32)
+    for bad in (lambda: ops.rotary(plan, q, q, 0, out=(q, fresh)), lambda: ops.rotary(plan, q, q, 0, out=(fresh, q)),
+                lambda: ops.rotary(plan, q, q[:, 1:], 0, out=(q, fresh[:, 1:])), lambda: ops.rotary(plan, q, k, 0, out=(low, high)),
+                lambda: ops.rotary(plan, low, k, 0, out=(low, high)), lambda: ops.rotary(plan, q, k, 0, out=(high, low)),
+                lambda: ops.rotary(plan, q, None, pos, out=low),
+                lambda: ops.rotary(plan, q, None, 0, out=flat.as_strided((1, 2, 3, 64), (384, 64, 32, 1)))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_rotary_of_one_projection_in_place(ops):
+    """q and k between each other in memory, however the projection lays them out, in place and into each other's kind."""
+    print("rotary in one buffer", flush=True)
+    g = _gen(31)
+    plan = ops.RotaryPlan(64, 1e4, False, None, DEV)
+    for layout in ((0, 2, 1, 3), (0, 1, 2, 3), (2, 0, 1, 3)):   # of [b, heads, s, d] in memory
+        back = [layout.index(i) for i in range(4)]
+        for dtype in (BF, FP):
+            x = _randn(g, 2, 7, 9, 64, dtype=dtype).permute(layout).contiguous().permute(back)
+            y = torch.zeros_like(x, memory_format=torch.preserve_format)
+            a, b = ops.rotary(plan, x[:, :4], x[:, 4:6], 11)
+            ops.rotary(plan, x[:, :4], x[:, 4:6], 11, out=(y[:, :4], y[:, 4:6]))
+            assert torch.equal(y[:, :4], a) and torch.equal(y[:, 4:6], b) and not y[:, 6].any()
+            kept = x[:, 6].clone()
+            ops.rotary(plan, x[:, :4], x[:, 4:6], 11, out=(x[:, :4], x[:, 4:6]))
+            assert torch.equal(x[:, :4], a) and torch.equal(x[:, 4:6], b) and torch.equal(x[:, 6], kept)

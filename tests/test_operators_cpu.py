@@ -135,3 +135,44 @@ def test_tensors_off_the_gpu_are_refused():
                  lambda: ops.attention_weights(t, t), lambda: ops.evict(t[..., 0], t[..., 0].int(), t, t, None, 2, 1)):
         with pytest.raises(ValueError):
             call()
+
+
+def _places(x):
+    """Byte addresses of a view's elements."""
+    at = torch.zeros((), dtype=torch.int64)
+    for n, s in zip(x.shape, x.stride()):
+        at = at[..., None] + torch.arange(n) * s
+    return set((x.data_ptr() + at.flatten() * x.element_size()).tolist())
+
+
+def test_views_that_meet():
+    """Two views have memory in common exactly if an element of one is an element of the other, for all ways of cutting one
+    buffer that a caller has; views across each other may count as meeting though they do not."""
+    flat = torch.zeros(4096)
+    qkv = flat[:2 * 5 * 7 * 4].view(2, 5, 7, 4)                                 # [b, s, heads, d]
+    q, k, v = qkv[:, :, :4].transpose(1, 2), qkv[:, :, 4:6].transpose(1, 2), qkv[:, :, 6:].transpose(1, 2)
+    heads = flat[:2 * 7 * 5 * 4].view(2, 7, 5, 4)                               # [b, heads, s, d]
+    time = flat[:5 * 2 * 7 * 4].view(5, 2, 7, 4).permute(1, 2, 0, 3)            # [s, b, heads, d]
+    pair = flat[:2 * 5 * 3 * 2 * 4].view(2, 5, 3, 2, 4)                         # k and v of a head side by side
+    views = [q, k, v, heads[:, :4], heads[:, 4:6], heads[:, 6:], time[:, :4], time[:, 4:6], pair[..., 0, :].transpose(1, 2),
+             pair[..., 1, :].transpose(1, 2), pair[:, :, :2, 1].transpose(1, 2), qkv[:, :3, :4].transpose(1, 2), qkv[:, 3:, :4].transpose(1, 2),
+             q[:1], q[1:], q[:, :, ::2], q[:, :, 1::2], q[..., :2], q[..., 2:], q[..., 1:3], flat[1:281].view(2, 5, 7, 4)[:, :, :4].transpose(1, 2)]
+    exact = 0
+    for x in views:
+        for y in views:
+            common = bool(_places(x) & _places(y))
+            assert ops._meet(x, y) >= common
+            exact += ops._meet(x, y) == common
+    assert exact >= 0.9 * len(views) ** 2
+    for x, y in ((q, k), (k, v), (q, v), (heads[:, :4], heads[:, 4:6]), (time[:, :4], time[:, 4:6]), (views[8], views[9]), (views[9], views[8]),
+                 (views[8], views[10]), (views[11], views[12]), (q[..., :2], q[..., 2:]), (q[:, :, ::2], q[:, :, 1::2])):
+        assert not ops._meet(x, y) and not ops._meet(y, x)
+    shifted = flat[4:4 + q.numel()].view(2, 4, 5, 4)
+    assert ops._meet(flat[:q.numel()].view(2, 4, 5, 4), shifted) and ops._meet(q, q) and ops._meet(q, q.clone().copy_(q)) is False
+    assert ops._meet(flat[:8].view(torch.int32), flat[:8]) and not ops._meet(flat[:0], flat)
+
+
+def test_views_whose_elements_have_a_place_each():
+    x = torch.zeros(3, 4, 5, 6)
+    assert all(ops._once(y) for y in (x, x.transpose(1, 2), x[:, 1:3, ::2], x[..., 2:4], x[:, :1].expand(3, 1, 5, 6), x.permute(2, 0, 3, 1), x[:0]))
+    assert not any(ops._once(y) for y in (x[:, :1].expand(3, 4, 5, 6), x.as_strided((3, 4), (2, 1)), x.as_strided((3, 4), (3, 1))))
