@@ -608,11 +608,20 @@ def _same_view(x: torch.Tensor, y: torch.Tensor) -> bool:
             all(a == b or n < 2 for n, a, b in zip(x.shape, x.stride(), y.stride())))
 
 
-def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
-    """Whether one of the two ends before the other begins."""
-    def end(t):
-        return t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-    return x.numel() == 0 or y.numel() == 0 or end(x) <= y.data_ptr() or end(y) <= x.data_ptr()
+def _range(x: torch.Tensor) -> Tuple[int, int]:
+    """Where a view's memory begins and ends."""
+    begin = x.data_ptr()
+    if x.is_contiguous() or x.numel() == 0:
+        return begin, begin + x.nbytes
+    return begin, begin + x.element_size() * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
+
+
+def _crosses(place: Tuple[int, int], x: Optional[torch.Tensor]) -> bool:
+    """Whether a view's range meets another one."""
+    if x is None or x.data_ptr() >= place[1]:
+        return False
+    begin, end = _range(x)
+    return max(begin, place[0]) < end and place[0] < place[1]
 
 
 def _once(x: torch.Tensor) -> bool:
@@ -643,7 +652,8 @@ def _blocks_meet(shift: int, x: int, y: int, dims) -> bool:
 def _meet(x: torch.Tensor, y: torch.Tensor) -> bool:
     """Whether two views have memory in common.  Views that lie between each other, as the parts of one projection do, are told
     apart where their dimensions have the same strides; otherwise views whose ranges meet count as meeting."""
-    if _apart(x, y):
+    at_x, at_y = _range(x), _range(y)
+    if not _crosses(at_x, y):
         return False
     e, dims = x.element_size(), []
     if x.dim() == y.dim() and y.element_size() == e:
@@ -651,8 +661,7 @@ def _meet(x: torch.Tensor, y: torch.Tensor) -> bool:
             step = sx if nx > 1 else sy
             if max(nx, ny) > 1 and step > 0 and (sx == sy or min(nx, ny) == 1):
                 dims.append((step * e, nx, ny))
-    size = [t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) for t in (x, y)]
-    return _blocks_meet(y.data_ptr() - x.data_ptr(), *size, sorted(dims, reverse=True))
+    return _blocks_meet(at_y[0] - at_x[0], at_x[1] - at_x[0], at_y[1] - at_y[0], sorted(dims, reverse=True))
 
 
 def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positions, transpose: bool = False, out=None):
@@ -760,7 +769,7 @@ def attention_weights(q: torch.Tensor, k: torch.Tensor, lengths: Optional[torch.
     contiguous; a token sees those up to itself.  lse fp32 [b,Hq,t]: the logarithms of its sums that the attention left
     (``tree_attention(return_lse=True)``; a query of -inf adds nothing); without it they are formed here.  -> fp32 [b,Hc,n]:
     ``weights`` (0 if None) plus the sums over the query heads of each head and over the tokens, in ``out`` if that is given,
-    else in place if there are weights."""
+    else in place if there are weights.  That place may be the weights' own, and is apart from the other inputs."""
     dev = _on_one_gpu(q, k, lengths, lse, weights, out)
     b, hq, t, d = q.shape
     hc, n = k.shape[1], k.shape[2]
@@ -773,12 +782,16 @@ def attention_weights(q: torch.Tensor, k: torch.Tensor, lengths: Optional[torch.
         _expect("lse", lse, (b, hq, t), torch.float32)
     if weights is not None:
         _expect("weights", weights, (b, hc, n), torch.float32)
-    if out is None:
-        out = weights if weights is not None else torch.empty((b, hc, n), dtype=torch.float32, device=q.device)
-    else:
+    given = out is not None or weights is not None
+    if out is not None:
         _expect("out", out, (b, hc, n), torch.float32)
-        if weights is not None and not _same_view(out, weights) and not _apart(out, weights):
-            raise ValueError("out overlaps weights")
+    else:
+        out = weights if given else torch.empty((b, hc, n), dtype=torch.float32, device=q.device)
+    if given:   # (the caller's place, or the weights')
+        place = _range(out)
+        others = (q, k, lse, lengths) if weights is None or _same_view(out, weights) else (q, k, lse, lengths, weights)
+        if any(_crosses(place, x) for x in others):
+            raise ValueError("the place of the sums overlaps an input")
     if out.numel() == 0:
         return out
     if t == 0:
@@ -824,7 +837,7 @@ def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Te
             raise ValueError("out of k and of v are in one place")
         if cap_out < min(budget, n):
             raise ValueError(f"out has {cap_out} slots for min(budget={budget}, {n}) tokens")
-        if not all(_apart(x, y) for x in (weights, ids, k, v) for y in out):
+        if any(_crosses(_range(x), y) for x in (weights, ids, k, v) for y in out):
             raise ValueError("out overlaps an input: leave it out to evict in place")
         ptrs = tuple(y.data_ptr() for y in out)
     new = torch.empty((b,), dtype=torch.int32, device=k.device)

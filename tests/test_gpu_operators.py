@@ -1167,3 +1167,18 @@ def test_rotary_of_one_projection_in_place(ops):
             kept = x[:, 6].clone()
             ops.rotary(plan, x[:, :4], x[:, 4:6], 11, out=(x[:, :4], x[:, 4:6]))
             assert torch.equal(x[:, :4], a) and torch.equal(x[:, 4:6], b) and torch.equal(x[:, 6], kept)
+
+
+def test_attention_weights_refuse_a_place_that_is_read(ops):
+    """The sums over what the kernels still read: queries, keys, lse, lengths; as out and as weights."""
+    flat = torch.zeros(4096, device=DEV)
+    q, k, lse = flat[:1536].view(1, 4, 6, 64), flat[1536:2688].view(1, 2, 9, 64), flat[2688:2712].view(1, 4, 6)
+    lengths = flat[2712:2713].view(torch.int32)
+    for at in (0, 1530, 1536, 2680, 2688, 2700, 2712):
+        place = flat[at:at + 18].view(1, 2, 9)
+        for where in (dict(out=place), dict(weights=place), dict(weights=torch.zeros_like(place), out=place)):
+            with pytest.raises(ValueError):
+                ops.attention_weights(q, k, lengths, lse, **where)
+    free = flat[3000:3018].view(1, 2, 9)
+    ops.attention_weights(q, k, lengths, lse, weights=free)
+    assert not free.any()   # (no tokens)
