@@ -664,6 +664,18 @@ def _meet(x: torch.Tensor, y: torch.Tensor) -> bool:
     return _blocks_meet(at_y[0] - at_x[0], at_x[1] - at_x[0], at_y[1] - at_y[0], sorted(dims, reverse=True))
 
 
+def _undisturbed(ranges) -> bool:
+    """Of (begin, bytes, written): whether what is written meets nothing else."""
+    reach = wrote = 0   # ends of what begins further in front
+    for begin, size, written in sorted(ranges):
+        if size and begin < (reach if written else wrote):
+            return False
+        reach = max(reach, begin + size)
+        if written:
+            wrote = max(wrote, begin + size)
+    return True
+
+
 def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positions, transpose: bool = False, out=None):
     """q [b,Hq,s,d] and k [b,Hk,s,d] (or None) turned to ``positions``: int32 [s] or [b,s] on the GPU, or the first one of
     s that follow each other.  Any strides, rows contiguous.  ``out``: (q', k') to write to, each of them its input or a view
@@ -812,14 +824,15 @@ def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Te
     ``lengths[i]`` tokens (int32 [b]; n if None).  The tokens whose ids are within ``recent`` of their head's largest one
     stay, and of the others those with the largest weights (equal ones: of the lowest slots).  A token that stays keeps its
     slot if that is one of the first ``budget``; the others move, in order, into the slots that became free.  In place, or
-    into ``out`` = (weights, ids, k, v), buffers of at least min(budget, n) slots that are apart from the inputs; slots behind
-    the tokens that stay are left as they were.  -> the new lengths, int32 [b]."""
+    into ``out`` = (weights, ids, k, v), buffers of at least min(budget, n) slots that are apart from the inputs and from each
+    other; slots behind the tokens that stay are left as they were.  -> the new lengths, int32 [b]."""
     dev = _on_one_gpu(weights, ids, k, v, lengths, *(out or ()))
     b, h, n, d = k.shape
     dt = _dt(k)
     _expect("weights", weights, (b, h, n), torch.float32)
     _expect("ids", ids, (b, h, n), torch.int32)
-    _expect("k", k, (b, h, n, d), k.dtype)
+    if not k.is_contiguous():
+        raise ValueError("k must be contiguous")
     _expect("v", v, (b, h, n, d), k.dtype)
     _lengths(lengths, b)
     budget, recent, cap_out = int(budget), int(recent), n
@@ -833,21 +846,34 @@ def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Te
         for name, y, shape, dtype in zip(("weights", "ids", "k", "v"), out, ((b, h, cap_out),) * 2 + ((b, h, cap_out, d),) * 2,
                                          (torch.float32, torch.int32, k.dtype, k.dtype)):
             _expect("out " + name, y, shape, dtype)
-        if out[2].data_ptr() == out[3].data_ptr() and out[2].numel():
-            raise ValueError("out of k and of v are in one place")
         if cap_out < min(budget, n):
             raise ValueError(f"out has {cap_out} slots for min(budget={budget}, {n}) tokens")
-        if any(_crosses(_range(x), y) for x in (weights, ids, k, v) for y in out):
-            raise ValueError("out overlaps an input: leave it out to evict in place")
         ptrs = tuple(y.data_ptr() for y in out)
-    new = torch.empty((b,), dtype=torch.int32, device=k.device)
-    if b * h * n == 0:
+    new = torch.empty_like(lengths) if lengths is not None else torch.empty((b,), dtype=torch.int32, device=k.device)
+    slots = b * h * n
+    if slots == 0:
         return new.zero_()
+    # (all are contiguous, so that ranges say it: asked for tensor by tensor this took longer than the kernels)
+    held = w_at, i_at, k_at, v_at = weights.data_ptr(), ids.data_ptr(), k.data_ptr(), v.data_ptr()
+    l_at, l_bytes = (0, 0) if lengths is None else (lengths.data_ptr(), 4 * b)
+    row = d * k.element_size()
+    word, rows = 4 * slots, row * slots
+    if out is None:   # (one tensor as keys and values: every row is moved to one place)
+        apart = (abs(w_at - i_at) >= word and (k_at == v_at or abs(k_at - v_at) >= rows) and
+                 not -word < w_at - k_at < rows and not -word < w_at - v_at < rows and
+                 not -word < i_at - k_at < rows and not -word < i_at - v_at < rows and
+                 not -l_bytes < l_at - w_at < word and not -l_bytes < l_at - i_at < word and
+                 not -l_bytes < l_at - k_at < rows and not -l_bytes < l_at - v_at < rows)
+    else:
+        ranges = [(w_at, word, False), (i_at, word, False), (k_at, rows, False), (v_at, rows, False), (l_at, l_bytes, False)]
+        apart = _undisturbed(ranges + [(p, b * h * cap_out * size, True) for p, size in zip(ptrs, (4, 4, row, row))])
+    if not apart:
+        raise ValueError("what is written overlaps something else (in place: leave out away)")
     budget = min(budget, 2 ** 30)
     need = _scratch_bytes("lrqk_evict_workspace", b, h, n, budget)
     ws = _scratch(need, k)
-    _launch(dev, _lib.load().lrqk_evict, weights.data_ptr(), ids.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(lengths), n, *ptrs,
-            cap_out, new.data_ptr(), b, h, d, budget, min(recent, budget), ws.data_ptr(), need, dt)
+    _launch(dev, _lib.load().lrqk_evict, *held, l_at or None, n, *ptrs, cap_out, new.data_ptr(),
+            b, h, d, budget, min(recent, budget), ws.data_ptr(), need, dt)
     return new
 
 

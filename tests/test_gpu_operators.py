@@ -1182,3 +1182,34 @@ def test_attention_weights_refuse_a_place_that_is_read(ops):
     free = flat[3000:3018].view(1, 2, 9)
     ops.attention_weights(q, k, lengths, lse, weights=free)
     assert not free.any()   # (no tokens)
+
+
+def test_evict_refuses_outputs_that_overlap(ops):
+    """Outputs shifted into each other, the weights' over the ids', one over the lengths, and in place caches over each other;
+    one tensor as keys and values is none of these."""
+    print("evict overlaps", flush=True)
+    g = _gen(5)
+    w, ids, k, v = _cache(g, 1, 2, 20, 64, BF)
+    n = torch.tensor([20], dtype=torch.int32, device=DEV)
+    flat, rows = torch.zeros(64, device=DEV), torch.zeros(4096, dtype=BF, device=DEV)
+    ok = (torch.zeros(1, 2, 9, device=DEV), torch.zeros(1, 2, 9, dtype=torch.int32, device=DEV), k[:, :, :9].clone(), v[:, :, :9].clone())
+    low, high = rows[:1152].view(1, 2, 9, 64), rows[64:1216].view(1, 2, 9, 64)
+    numbers = flat[9:27].view(torch.int32).view(1, 2, 9)
+    for out in ((*ok[:2], low, high), (*ok[:2], high, low), (flat[:18].view(1, 2, 9), numbers, *ok[2:]),
+                (flat[18:36].view(1, 2, 9), numbers, *ok[2:]), (rows[:36].view(torch.float32).view(1, 2, 9), ok[1], low, ok[3]),
+                (w.view(-1)[3:21].view(1, 2, 9), *ok[1:]), (ok[0], ok[1], k.view(-1)[64:1216].view(1, 2, 9, 64), ok[3])):
+        with pytest.raises(ValueError):
+            ops.evict(w, ids, k, v, n, 9, 1, out=out)
+    with pytest.raises(ValueError):
+        ops.evict(w, ids, k, v, numbers.view(-1)[4:5], 9, 1, out=(ok[0], numbers, *ok[2:]))
+    both = torch.zeros(2560 + 64, dtype=BF, device=DEV)
+    for held in ((w, ids, both[:2560].view(1, 2, 20, 64), both[64:].view(1, 2, 20, 64)), (w, w.view(torch.int32), k, v)):
+        with pytest.raises(ValueError):
+            ops.evict(*held, n, 9, 1)
+    with pytest.raises(ValueError):
+        ops.evict(w, ids, k, v, ids.view(-1)[7:8], 9, 1)
+    one, apart = [x.clone() for x in (w, ids, k, k)], [x.clone() for x in (w, ids, k, k)]
+    one[3] = one[2]
+    ops.evict(*one, n, 9, 1)
+    ops.evict(*apart, n, 9, 1)
+    assert all(torch.equal(x[:, :, :9], y[:, :, :9]) for x, y in zip(one, apart))

@@ -176,3 +176,14 @@ def test_views_whose_elements_have_a_place_each():
     x = torch.zeros(3, 4, 5, 6)
     assert all(ops._once(y) for y in (x, x.transpose(1, 2), x[:, 1:3, ::2], x[..., 2:4], x[:, :1].expand(3, 1, 5, 6), x.permute(2, 0, 3, 1), x[:0]))
     assert not any(ops._once(y) for y in (x[:, :1].expand(3, 4, 5, 6), x.as_strided((3, 4), (2, 1)), x.as_strided((3, 4), (3, 1))))
+
+
+def test_what_is_written_meets_nothing_else():
+    """Against all pairs: a written range and any other one with a byte in common."""
+    import random
+    rng = random.Random(0)
+    for _ in range(3000):
+        ranges = [(rng.randrange(40), rng.choice((0, 1, 3, 8)), rng.random() < 0.5) for _ in range(rng.randrange(1, 7))]
+        meets = any(max(x[0], y[0]) < min(x[0] + x[1], y[0] + y[1]) and (x[2] or y[2])
+                    for i, x in enumerate(ranges) for y in ranges[:i])
+        assert ops._undisturbed(ranges) is not meets, ranges
