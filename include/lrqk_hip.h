@@ -284,8 +284,8 @@ int lrqk_rotary(const void* q, const void* k, void* q_out, void* k_out, const in
  * q, out: [b][hq][t][d]; lse (or NULL): fp32 [b][hq][t], log of the sum of exp(scale q.k).  A query that sees nothing
  * gives zeros and -inf.  What a masked drafted token or a row behind the length holds, infinities and NaN included, does
  * not matter; a cached value that is not finite leaves its element of the outputs not finite (a NaN perhaps for an
- * infinity).  Strides in elements, the same for k_cache and v_cache, multiples of 16 bytes, rows at most 2^24 elements
- * apart.  Head widths up to 256 elements, t up to 1024, n up to 2^30, b * hq up to 65535.
+ * infinity).  Strides in elements, the same for k_cache and v_cache, multiples of 16 bytes (0 for a single sequence, head
+ * or row, here and in the calls below), rows at most 2^24 elements apart.  Head widths up to 256 elements, t up to 1024, n up to 2^30, b * hq up to 65535.
  * These calls take no ctx: their scratch is the caller's (lrqk_*_workspace bytes of device memory, 16-byte aligned,
  * contents of no meaning before and after), so that calls on several streams and captured graphs need not share any. */
 int64_t lrqk_tree_attention_workspace(int b, int hq, int hc, int t, int64_t n, int d, int have_lengths, int dtype);

@@ -543,11 +543,13 @@ def _expect(name: str, t: torch.Tensor, shape, dtype, contiguous: bool = True):
 
 
 def _row_strides(name: str, t: torch.Tensor):
-    """Strides of sequences, heads and rows of a tensor whose rows are contiguous."""
-    s = t.stride()
-    if s[3] != 1 and t.shape[3] > 1:
+    """Strides of sequences, heads and rows of a tensor whose rows are contiguous; 0 where there is one of a kind, whose stride
+    leads to nothing and may be anything."""
+    b, h, r, d = t.stride()
+    nb, nh, nr, nd = t.shape
+    if d != 1 and nd > 1:
         raise ValueError(f"the rows of {name} must be contiguous")
-    return s[:3]
+    return b if nb > 1 else 0, h if nh > 1 else 0, r if nr > 1 else 0
 
 
 def _lengths(lengths: Optional[torch.Tensor], b: int):
@@ -757,7 +759,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise ValueError(f"mask is {tuple(mask.shape)} {mask.dtype}: bool or uint8 [t,t] or [b,t,t] is wanted")
     _lengths(lengths, b)
     st, sv = _row_strides("k_cache", k_cache), _row_strides("v_cache", v_cache)
-    if sv != st and n > 0 and any(x != y and m > 1 for x, y, m in zip(st, sv, k_cache.shape)):   # (one of a kind has no stride)
+    if sv != st and n > 0:
         raise ValueError("k_cache and v_cache must have the same strides")
     q = q.contiguous()
     out = torch.empty_like(q)

@@ -1213,3 +1213,21 @@ def test_evict_refuses_outputs_that_overlap(ops):
     ops.evict(*one, n, 9, 1)
     ops.evict(*apart, n, 9, 1)
     assert all(torch.equal(x[:, :, :9], y[:, :, :9]) for x, y in zip(one, apart))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_odd_strides_of_a_single_sequence_head_or_token(ops, dtype):
+    """A stride that leads to nothing may be anything: no multiple of 16 bytes, or more than rows may be apart."""
+    print("single strides", dtype, flush=True)
+    for b, h, n in ((1, 2, 40), (2, 1, 40), (2, 2, 1), (1, 1, 40), (1, 2, 1), (1, 1, 1)):
+        q, kc, vc, kn, vn, mask = _tree_inputs(b + 2 * h + n, dtype, b, 2 * h, h, h, 3, n, 64)
+        odd = tuple(s if m > 1 else far for m, s, far in zip(kc.shape, kc.stride(), (13, 7, (1 << 25) + 1, 1)))
+        k, v = kc.as_strided(kc.shape, odd), vc.as_strided(vc.shape, odd)
+        assert torch.equal(ops.tree_attention(q, k, v, kn, vn, mask), ops.tree_attention(q, kc, vc, kn, vn, mask))
+        lse = torch.full((b, 2 * h, 3), 4.0, device=DEV)
+        for given in (None, lse):
+            assert torch.equal(ops.attention_weights(q, k, lse=given), ops.attention_weights(q, kc, lse=given))
+        plan = ops.RotaryPlan(64, 1e4, False, None, DEV)
+        y = torch.empty_like(kc)
+        ops.rotary(plan, k, None, 5, out=y.as_strided(y.shape, odd))
+        assert torch.equal(y, ops.rotary(plan, kc, None, 5))
