@@ -535,6 +535,9 @@ struct WeightPlan {
   int dp, rows_nt, groups, parts, per, nt, chunks, few_per;
   bool few;
   int64_t lse2, part;   // floats
+  int64_t keys_blocks(int64_t n) const { return (n + 16 * nt * kAwWaves - 1) / (16 * nt * kAwWaves); }
+  // workgroups of the largest launch, for a head (that of few queries has a thousand; the joining ones less than these)
+  int64_t most_blocks(int64_t n) const { return std::max((int64_t)groups * parts, few ? 0 : keys_blocks(n) * chunks); }
   int64_t part_at() const { return (lse2 + 3) / 4 * 4; }
   int64_t bytes() const { return (part_at() + part) * (int64_t)sizeof(float); }
 };
@@ -556,7 +559,7 @@ static WeightPlan weights_plan(int b, int hq, int hc, int t, int64_t n, int d, i
   }
   // two thousand workgroups of keys and chunks of queries (half of a prompt's have little to do; one thousand: no faster),
   // eight tiles of queries for each
-  const int64_t blocks = (n + 16 * p.nt * kAwWaves - 1) / (16 * p.nt * kAwWaves), items = (M + 15) / 16;
+  const int64_t blocks = p.keys_blocks(n), items = (M + 15) / 16;
   p.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(2048 / (blocks * heads), items / 16));
   if (!p.few && p.chunks > 1) p.part = heads * n * p.chunks;
   if (have_lse) return p;
@@ -614,8 +617,7 @@ static int weights_launch(WeightArgs a, const WeightPlan& p, int heads, hipStrea
     LRQK_HIP_CHECK(hipGetLastError());
     return LRQK_OK;
   }
-  const int keys = 16 * p.nt * kAwWaves;
-  const dim3 grid((unsigned)((int64_t)(a.n + keys - 1) / keys * p.chunks * heads));
+  const dim3 grid((unsigned)(p.keys_blocks(a.n) * p.chunks * heads));
   constexpr int ROW = DP * (int)sizeof(T);
   if constexpr (ROW <= 256)
     if (p.nt == 4) hipLaunchKernelGGL((weights_columns_kernel<T, DP, 4>), grid, dim3(kAwThreads), 0, st, a);
@@ -676,10 +678,8 @@ extern "C" int lrqk_attention_weights(const void* q, const void* k, int64_t k_ba
   const int64_t need = p.bytes();
   LRQK_REQUIRE(workspace_bytes >= need && (workspace || need == 0), LRQK_EINVAL, "workspace of %lld bytes: %lld are needed", (long long)workspace_bytes,
                (long long)need);
-  // (a launch's workgroups are counted in 31 bits; no memory holds what would need more)
-  const int64_t places = std::max((int64_t)p.groups * std::max(p.parts, 1), (n + 63) / 64 * p.chunks);
-  LRQK_REQUIRE(places * b * hc <= INT32_MAX, LRQK_ELIMIT, "%lld keys of %d heads and %d queries are more than a launch has places for",
-               (long long)n, b * hc, t);
+  LRQK_REQUIRE(p.most_blocks(n) * b * hc <= kMaxThreads / kAwThreads, LRQK_ELIMIT,
+               "%lld keys of %d heads and %d queries are more than a launch has places for", (long long)n, b * hc, t);
   WeightArgs a{q, k, lengths, lse, kLog2e, (float*)workspace, (float*)workspace + p.part_at(), weights, out, k_batch_stride, k_head_stride,
                k_row_stride, (int)n, hq, hc, t, d, p.parts, p.per, p.groups, p.chunks, (uint32_t)(b * hc), scale * kLog2e};
   hipStream_t st = (hipStream_t)stream;

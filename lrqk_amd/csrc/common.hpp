@@ -9,6 +9,7 @@
 namespace lrqk {
 
 constexpr int kWave = 64;
+constexpr int64_t kMaxThreads = (int64_t(1) << 32) - 1;  // of a launch, along an axis of the grid
 
 int set_error(int code, const char* fmt, ...);
 

@@ -260,6 +260,7 @@ extern "C" int lrqk_rotary(const void* q, const void* k, void* q_out, void* k_ou
   a.tokens = 64;
   while (a.tokens > 1 && (a.tokens * bytes > 40 * 1024 || a.tokens * a.half > 4096)) a.tokens /= 2;
   const int64_t tiles = (s + a.tokens - 1) / a.tokens;
+  LRQK_REQUIRE(tiles <= kMaxThreads / kRotThreads, LRQK_ELIMIT, "%lld tokens are more than a launch has places for", (long long)s);
   a.groups = (int)std::max<int64_t>(1, std::min<int64_t>((hq + hk + 3) / 4, 1024 / (tiles * b)));
   hipStream_t st = (hipStream_t)stream;
   if (dtype == LRQK_F32) return rotary_launch<float>(a, b, vok, st);

@@ -990,6 +990,7 @@ template <typename T, int DP>
 static int tree_launch(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)(a.units + 7) / 8 * 8 * a.row_blocks));
   const dim3 join((unsigned)((int64_t)a.b * a.hc * a.row_tiles * 4));
+  // (of the most heads and drafts, 65535 and 1024: 2^23 and 2^24 - 256 workgroups, of 256 threads each; a launch may have 2^32 - 1 threads)
   if (p.wr == 0) {
     if constexpr (DP < 256)
       if (p.mt == 2) hipLaunchKernelGGL((tree_stream_kernel<T, DP, 2>), grid, dim3(kTrThreads), 0, st, a);

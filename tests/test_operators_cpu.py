@@ -187,3 +187,13 @@ def test_what_is_written_meets_nothing_else():
         meets = any(max(x[0], y[0]) < min(x[0] + x[1], y[0] + y[1]) and (x[2] or y[2])
                     for i, x in enumerate(ranges) for y in ranges[:i])
         assert ops._undisturbed(ranges) is not meets, ranges
+
+
+@pytest.mark.parametrize("fn,good,changed", [
+    ("lrqk_rotary", ROTARY, dict(s=(1 << 31) - 1)), ("lrqk_rotary", ROTARY, dict(s=(1 << 31) - 1, d=2, rotary_dim=2, hq=1, hk=0)),
+    ("lrqk_attention_weights", WEIGHTS, dict(hq=32, hc=32, t=100, n=1 << 30, lse=P)),       # the columns' launch
+    ("lrqk_attention_weights", WEIGHTS, dict(b=1023, hq=64, hc=64, t=1 << 20, n=1024))])    # that of the rows
+def test_more_workgroups_than_a_launch_has_are_refused(fn, good, changed):
+    """2^32 threads along an axis are too many, which the limits of the single sizes allow."""
+    assert _call(fn, good, **changed) == ELIMIT
+    assert b"places" in _lib.load().lrqk_last_error()
