@@ -542,6 +542,12 @@ def _expect(name: str, t: torch.Tensor, shape, dtype, contiguous: bool = True):
         raise ValueError(f"{name} must be contiguous")
 
 
+def _in_32_bits(*sizes: int):
+    """The library takes these sizes as 32-bit numbers: a larger one would reach it as another."""
+    if max(sizes) >> 31:
+        raise ValueError(f"a size of {max(sizes)} is beyond 32 bits")
+
+
 def _row_strides(name: str, t: torch.Tensor):
     """Strides of sequences, heads and rows of a tensor whose rows are contiguous; 0 where there is one of a kind, whose stride
     leads to nothing and may be anything."""
@@ -691,6 +697,7 @@ def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positio
         hk = k.shape[1]
         if k.shape != (b, hk, s, d) or k.dtype != q.dtype:
             raise ValueError(f"k is {tuple(k.shape)} {k.dtype} beside q {tuple(q.shape)} {q.dtype}")
+    _in_32_bits(b, hq, hk, d)
     if plan.rotary_dim > d:
         raise ValueError(f"a plan of {plan.rotary_dim} elements for heads of {d}")
     dt = _dt(q)
@@ -748,6 +755,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     b, hq, t, d = q.shape
     _, hc, n, _ = k_cache.shape
     hn = k_new.shape[1]
+    _in_32_bits(b, hq, hc, hn, t, d)
     dt, dtype = _dt(q), q.dtype
     _expect("k_cache", k_cache, (b, hc, n, d), dtype, contiguous=False)
     _expect("v_cache", v_cache, (b, hc, n, d), dtype, contiguous=False)
@@ -787,6 +795,7 @@ def attention_weights(q: torch.Tensor, k: torch.Tensor, lengths: Optional[torch.
     dev = _on_one_gpu(q, k, lengths, lse, weights, out)
     b, hq, t, d = q.shape
     hc, n = k.shape[1], k.shape[2]
+    _in_32_bits(b, hq, hc, t, d)
     dt = _dt(q)
     _expect("k", k, (b, hc, n, d), q.dtype, contiguous=False)
     if hc == 0 or hq % hc:
@@ -830,6 +839,7 @@ def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Te
     other; slots behind the tokens that stay are left as they were.  -> the new lengths, int32 [b]."""
     dev = _on_one_gpu(weights, ids, k, v, lengths, *(out or ()))
     b, h, n, d = k.shape
+    _in_32_bits(b, h, n, d)
     dt = _dt(k)
     _expect("weights", weights, (b, h, n), torch.float32)
     _expect("ids", ids, (b, h, n), torch.int32)
@@ -845,6 +855,7 @@ def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Te
         if len(out) != 4 or out[2].dim() != 4:
             raise ValueError("out holds weights, ids, k and v")
         cap_out = out[2].shape[2]
+        _in_32_bits(cap_out)
         for name, y, shape, dtype in zip(("weights", "ids", "k", "v"), out, ((b, h, cap_out),) * 2 + ((b, h, cap_out, d),) * 2,
                                          (torch.float32, torch.int32, k.dtype, k.dtype)):
             _expect("out " + name, y, shape, dtype)

@@ -197,3 +197,25 @@ def test_more_workgroups_than_a_launch_has_are_refused(fn, good, changed):
     """2^32 threads along an axis are too many, which the limits of the single sizes allow."""
     assert _call(fn, good, **changed) == ELIMIT
     assert b"places" in _lib.load().lrqk_last_error()
+
+
+FAR = (1 << 32) + 3
+
+
+@pytest.mark.parametrize("call", [
+    lambda x: ops.rotary(ops.RotaryPlan(2, device="cpu"), x(FAR, 1, 1, 2), None, 0), lambda x: ops.rotary(ops.RotaryPlan(2, device="cpu"), x(1, FAR, 1, 2), None, 0),
+    lambda x: ops.rotary(ops.RotaryPlan(2, device="cpu"), x(1, 1, 1, FAR), None, 0),
+    lambda x: ops.rotary(ops.RotaryPlan(2, device="cpu"), x(1, 1, 1, 2), x(1, FAR, 1, 2), 0),
+    lambda x: ops.tree_attention(x(1, 1, FAR, 8), *[x(1, 1, 5, 8)] * 2, *[x(1, 1, FAR, 8)] * 2, x(1, 1).bool().expand(FAR, FAR)),
+    lambda x: ops.tree_attention(x(FAR, 1, 3, 8), *[x(FAR, 1, 5, 8)] * 2, *[x(FAR, 1, 3, 8)] * 2, x(3, 3).bool()),
+    lambda x: ops.attention_weights(x(1, 1, FAR, 8), x(1, 1, 5, 8)), lambda x: ops.attention_weights(x(1, FAR, 2, 8), x(1, 1, 5, 8)),
+    lambda x: ops.attention_weights(x(1, FAR, 2, 8), x(1, FAR, 5, 8)),
+    lambda x: ops.evict(x(1, 1, FAR), x(1, 1, FAR).int(), *[x(1, 1, FAR, 8)] * 2, None, 9, 1),
+    lambda x: ops.evict(x(1, 1, 20), x(1, 1, 20).int(), *[x(1, 1, 20, 8)] * 2, None, 9, 1,
+                        out=(x(1, 1, FAR), x(1, 1, FAR).int(), *[x(1, 1, FAR, 8)] * 2))])
+def test_sizes_beyond_32_bits_do_not_reach_the_library_as_others(monkeypatch, call):
+    """(Tensors without memory: the call is refused before anything looks at what they hold.)"""
+    monkeypatch.setattr(ops, "_on_one_gpu", lambda *ts: 0)
+    monkeypatch.setattr(ops, "_launch", lambda *args: pytest.fail("reached the library"))
+    with pytest.raises(ValueError, match="beyond 32 bits"):
+        call(lambda *shape: torch.empty(shape, device="meta"))
