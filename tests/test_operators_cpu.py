@@ -206,7 +206,7 @@ FAR = (1 << 32) + 3
     lambda x: ops.rotary(ops.RotaryPlan(2, device="cpu"), x(FAR, 1, 1, 2), None, 0), lambda x: ops.rotary(ops.RotaryPlan(2, device="cpu"), x(1, FAR, 1, 2), None, 0),
     lambda x: ops.rotary(ops.RotaryPlan(2, device="cpu"), x(1, 1, 1, FAR), None, 0),
     lambda x: ops.rotary(ops.RotaryPlan(2, device="cpu"), x(1, 1, 1, 2), x(1, FAR, 1, 2), 0),
-    lambda x: ops.tree_attention(x(1, 1, FAR, 8), *[x(1, 1, 5, 8)] * 2, *[x(1, 1, FAR, 8)] * 2, x(1, 1).bool().expand(FAR, FAR)),
+    lambda x: ops.tree_attention(x(1, 1, FAR, 8), *[x(1, 1, 5, 8)] * 2, *[x(1, 1, FAR, 8)] * 2, x(3, 3).bool()),
     lambda x: ops.tree_attention(x(FAR, 1, 3, 8), *[x(FAR, 1, 5, 8)] * 2, *[x(FAR, 1, 3, 8)] * 2, x(3, 3).bool()),
     lambda x: ops.attention_weights(x(1, 1, FAR, 8), x(1, 1, 5, 8)), lambda x: ops.attention_weights(x(1, FAR, 2, 8), x(1, 1, 5, 8)),
     lambda x: ops.attention_weights(x(1, FAR, 2, 8), x(1, FAR, 5, 8)),
