@@ -495,9 +495,17 @@ static EvictPlan evict_plan(int64_t bh, int cap, int budget) {
   return p;
 }
 
-extern "C" int64_t lrqk_evict_workspace(int b, int heads, int cap, int budget) {
+static int evict_check(int b, int heads, int cap, int budget) {
   LRQK_REQUIRE(b > 0 && heads > 0 && cap > 0 && budget > 0, LRQK_EINVAL, "bad sizes b=%d heads=%d cap=%d budget=%d", b, heads, cap,
                budget);
+  LRQK_REQUIRE((int64_t)b * heads <= 65535, LRQK_ELIMIT, "%d sequences of %d heads: at most 65535 heads in all", b, heads);
+  LRQK_REQUIRE(cap <= (1 << 30), LRQK_ELIMIT, "cap=%d", cap);
+  return LRQK_OK;
+}
+
+extern "C" int64_t lrqk_evict_workspace(int b, int heads, int cap, int budget) {
+  const int rc = evict_check(b, heads, cap, budget);
+  if (rc) return rc;
   return evict_plan((int64_t)b * heads, cap, budget).words * (int64_t)sizeof(int32_t);
 }
 
@@ -505,10 +513,9 @@ extern "C" int lrqk_evict(float* weights, int32_t* ids, void* k, void* v, const 
                           int32_t* ids_out, void* k_out, void* v_out, int cap_out, int32_t* new_lengths, int b, int heads, int d,
                           int budget, int recent, void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
   LRQK_REQUIRE(dtype == LRQK_F32 || dtype == LRQK_BF16, LRQK_EINVAL, "dtype=%d", dtype);
-  LRQK_REQUIRE(b > 0 && heads > 0 && d > 0 && cap > 0 && budget > 0, LRQK_EINVAL, "bad sizes b=%d heads=%d d=%d cap=%d budget=%d",
-               b, heads, d, cap, budget);
-  LRQK_REQUIRE((int64_t)b * heads <= 65535, LRQK_ELIMIT, "%d sequences of %d heads: at most 65535 heads in all", b, heads);
-  LRQK_REQUIRE(cap <= (1 << 30), LRQK_ELIMIT, "cap=%d", cap);
+  LRQK_REQUIRE(d > 0, LRQK_EINVAL, "bad sizes d=%d", d);
+  const int rc = evict_check(b, heads, cap, budget);
+  if (rc) return rc;
   LRQK_REQUIRE(recent >= 0 && recent <= budget, LRQK_EINVAL, "recent=%d outside 0..budget=%d", recent, budget);
   LRQK_REQUIRE(weights && ids && k && v && new_lengths && workspace, LRQK_EINVAL, "null pointer");
   const bool in_place = weights_out == nullptr;

@@ -219,3 +219,11 @@ def test_sizes_beyond_32_bits_do_not_reach_the_library_as_others(monkeypatch, ca
     monkeypatch.setattr(ops, "_launch", lambda *args: pytest.fail("reached the library"))
     with pytest.raises(ValueError, match="beyond 32 bits"):
         call(lambda *shape: torch.empty(shape, device="meta"))
+
+
+def test_scratch_of_more_than_an_eviction_takes():
+    """The sizes that lrqk_evict refuses, for which the scratch's were formed beyond the integers' ends."""
+    lib = _lib.load()
+    for sizes in ((1, 1, (1 << 31) - 1, 10), (1, 1, (1 << 30) + 1, 10), (40000, 2, 100, 10), ((1 << 31) - 1, (1 << 31) - 1, 1 << 30, 9)):
+        assert lib.lrqk_evict_workspace(*sizes) == ELIMIT
+    assert lib.lrqk_evict_workspace(1, 1, 1 << 30, (1 << 31) - 1) >= 12 << 30
