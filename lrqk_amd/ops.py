@@ -558,6 +558,12 @@ def _row_strides(name: str, t: torch.Tensor):
     return b if nb > 1 else 0, h if nh > 1 else 0, r if nr > 1 else 0
 
 
+def _rows16(x: torch.Tensor) -> torch.Tensor:
+    """x, or a copy of it where its rows do not follow each other or begin between two 16-byte pieces."""
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
 def _lengths(lengths: Optional[torch.Tensor], b: int):
     if lengths is not None:
         _expect("lengths", lengths, (b,), torch.int32)
@@ -769,11 +775,11 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     st, sv = _row_strides("k_cache", k_cache), _row_strides("v_cache", v_cache)
     if sv != st and n > 0:
         raise ValueError("k_cache and v_cache must have the same strides")
-    q = q.contiguous()
+    q = _rows16(q)
     out = torch.empty_like(q)
     lse = torch.empty((b, hq, t), dtype=torch.float32, device=q.device) if return_lse else None
     if b * hq * t:
-        k_new, v_new, mask = k_new.contiguous(), v_new.contiguous(), mask.contiguous()
+        k_new, v_new, mask = _rows16(k_new), _rows16(v_new), mask.contiguous()
         need = _scratch_bytes("lrqk_tree_attention_workspace", b, hq, hc, t, n, d, lengths is not None, dt)
         ws = _scratch(need, q)
         _launch(dev, _lib.load().lrqk_tree_attention, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *st, n, _ptr(lengths),
@@ -819,7 +825,7 @@ def attention_weights(q: torch.Tensor, k: torch.Tensor, lengths: Optional[torch.
         return out
     if t == 0:
         return out.copy_(weights) if weights is not None else out.zero_()
-    q = q.contiguous()
+    q = _rows16(q)
     need = _scratch_bytes("lrqk_attention_weights_workspace", b, hq, hc, t, n, d, lse is not None, dt)
     ws = _scratch(need, q) if need else None
     _launch(dev, _lib.load().lrqk_attention_weights, q.data_ptr(), k.data_ptr(), *_row_strides("k", k), n, _ptr(lengths), _ptr(lse),

@@ -1231,3 +1231,19 @@ def test_odd_strides_of_a_single_sequence_head_or_token(ops, dtype):
         y = torch.empty_like(kc)
         ops.rotary(plan, k, None, 5, out=y.as_strided(y.shape, odd))
         assert torch.equal(y, ops.rotary(plan, kc, None, 5))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_new_rows_that_begin_between_two_pieces(ops, dtype):
+    """Queries, keys and values of the new tokens anywhere in a larger buffer."""
+    print("odd places", dtype, flush=True)
+    q, kc, vc, kn, vn, mask = _tree_inputs(8, dtype, 2, 4, 2, 2, 3, 50, 64)
+
+    def odd(x):
+        y = torch.zeros(x.numel() + 1, dtype=x.dtype, device=DEV)[1:].view(x.shape).copy_(x)
+        assert y.is_contiguous() and y.data_ptr() % 16
+        return y
+    for a, b in zip(ops.tree_attention(odd(q), kc, vc, odd(kn), odd(vn), odd(mask), return_lse=True),
+                    ops.tree_attention(q, kc, vc, kn, vn, mask, return_lse=True)):
+        assert torch.equal(a, b)
+    assert torch.equal(ops.attention_weights(odd(q), kc), ops.attention_weights(q, kc))
