@@ -27,6 +27,7 @@ constexpr int kAwWaves = 4, kAwThreads = kAwWaves * kWave;
 constexpr float kAwNone = -3.0e38f;    // maximum of no scores
 constexpr float kAwMuch = 4096.0f;      // a lane's exponentials of a tile may add up to this before the maximum is looked for
 constexpr int kAwTile = 32;             // rows of a tile that is walked over
+constexpr int kAwPart = 16;             // tiles of which a lane's sum is one number, before it joins the others
 
 struct WeightArgs {
   const void *q, *k;
@@ -142,14 +143,17 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_rows_kernel(WeightArgs 
   }
   int last[NT];   // last key that the lane's query sees
   int most = -1, least = a.n;
-  float top[NT], sum[NT];
+  float top[NT], part_sum[NT];
+  double sum[NT];   // of kAwPart tiles at a time: thousands of addends to one fp32 number would lose its last bits
+  int held = 0;
 #pragma unroll
   for (int m = 0; m < NT; ++m) {
     last[m] = behind + min(row0 + 16 * m + col, M - 1) % a.t;
     most = max(most, last[m]);
     least = min(least, last[m]);
     top[m] = kAwNone;
-    sum[m] = 0.0f;
+    part_sum[m] = 0.0f;
+    sum[m] = 0.0;
   }
   // keys that a query of the wave sees, and that all of them see
   most = (int)wave_reduce_u32((uint32_t)(most + 1), [](uint32_t x, uint32_t y) { return max(x, y); });
@@ -204,7 +208,9 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_rows_kernel(WeightArgs 
 #pragma unroll
         for (int e = 1; e < NE; ++e) now = fmaxf(now, x[m][e]);
         now = fmaxf(top[m], now * a.scale_log2e);
-        sum[m] *= ar_exp2(top[m] - now);
+        const float f = ar_exp2(top[m] - now);
+        part_sum[m] *= f;
+        sum[m] *= f;
         top[m] = now;
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
@@ -214,7 +220,15 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_rows_kernel(WeightArgs 
       }
     }
 #pragma unroll
-    for (int m = 0; m < NT; ++m) sum[m] += add[m];
+    for (int m = 0; m < NT; ++m) part_sum[m] += add[m];
+    if (++held == kAwPart) {
+      held = 0;
+#pragma unroll
+      for (int m = 0; m < NT; ++m) {
+        sum[m] += part_sum[m];
+        part_sum[m] = 0.0f;
+      }
+    }
   };
   load(begin, g[0]);
   load(begin + 1, g[1]);
@@ -235,7 +249,7 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_rows_kernel(WeightArgs 
 #pragma unroll
   for (int m = 0; m < NT; ++m) {
     const float all = ar_quad_max(top[m]);
-    const float total = ar_quad_sum(sum[m] * ar_exp2(top[m] - all));
+    const float total = ar_quad_sum((float)(sum[m] + part_sum[m]) * ar_exp2(top[m] - all));
     const int row = row0 + 16 * m + col;
     if (quad != 0 || row >= M) continue;
     const int64_t at = (int64_t)head * M + row;
@@ -389,7 +403,7 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_columns_kernel(WeightAr
         add(std::true_type{});
       else
         add(std::false_type{});
-      if (++held == 16) {   // (sums of sums: thousands of addends to one fp32 number would lose its last bits)
+      if (++held == kAwPart) {   // (sums of sums, as above)
         held = 0;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {

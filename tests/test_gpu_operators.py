@@ -1247,3 +1247,31 @@ def test_new_rows_that_begin_between_two_pieces(ops, dtype):
                     ops.tree_attention(q, kc, vc, kn, vn, mask, return_lse=True)):
         assert torch.equal(a, b)
     assert torch.equal(ops.attention_weights(odd(q), kc), ops.attention_weights(q, kc))
+
+
+@pytest.mark.parametrize("b,t", [(2112, 1), (513, 1024)])
+def test_attention_weights_of_thousands_of_tiles_in_one_part(ops, b, t):
+    """So many heads that each walks over all its keys in one part, 4096 tiles that all add the same number to a lane's sum:
+    every addition then rounds the same way, and the error may not grow with the tiles."""
+    print("weights, one part", b, t, flush=True)
+    n = 131072
+    a = torch.linspace(0.02, 1.5, b, dtype=torch.float64).to(BF).to(DEV)   # logit of the first tile; of the others 0
+    q, k = torch.zeros((b, 1, t, 8), dtype=BF, device=DEV), torch.zeros((1, 1, n, 8), dtype=BF, device=DEV)
+    q[..., 0] = a[:, None, None]
+    k[:, :, :32, 0] = 1.0
+    got = ops.attention_weights(q, k.expand(b, 1, n, 8), scale=1.0)
+    e = a.double().exp()
+    seen = torch.arange(n - t + 1, n + 1, dtype=torch.float64, device=DEV)
+    each = 1.0 / (32 * e[:, None] + seen - 32)                           # [b,t]: of a key of the later tiles
+    # sums of 17 (in units of 2: 2^-19): of base 2 the logarithm 2 units, its sum with the maximum and the exponent half of one;
+    # the exponential 2 units of 2^-23.  Additions, half of 2^-23 each: 8 exponentials of a tile, 32 tiles, and 16 of the parts,
+    # those of the maximum's change and the waves' lanes; of the columns 8 a tile and as many of the parts.
+    tol = math.log(2) * 3 * 2.0 ** -19 + 2 * 2.0 ** -23 + (8 + 32 + 16 + 48) * 2.0 ** -24
+    for first in range(0, b, 64):
+        w = each[first:first + 64]
+        exact = torch.empty((w.shape[0], n), dtype=torch.float64, device=DEV)
+        exact[:, :n - t + 1] = w.sum(1, keepdim=True)
+        exact[:, n - t:] = w.flip(1).cumsum(1).flip(1)
+        exact[:, :32] *= e[first:first + 64, None]
+        off = ((got[first:first + 64, 0].double() - exact) / exact).abs().max()
+        assert float(off) <= tol, (first, float(off), tol)
