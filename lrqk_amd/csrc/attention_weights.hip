@@ -389,7 +389,7 @@ __global__ __launch_bounds__(kAwThreads, 2) void weights_columns_kernel(WeightAr
             for (int r = 0; r < 4; ++r) p[r] = ar_exp2(fmaf(s[j][r], a.scale_log2e, -l2[r]));
             if constexpr (!decltype(is_whole)::value) {
 #pragma unroll
-              for (int r = 0; r < 4; ++r) {
+              for (int r = 0; r < 4; ++r) {   // (& and not &&: no branch, see tree_mask)
                 const int i = 16 * u + 4 * quad + r, last = behind + (packed ? (base + i) % a.t : at + i);
                 const bool sees = (base + i < stop) & (first + 16 * j + col <= last) & (l2[r] != -INFINITY);
                 p[r] = sees ? p[r] : 0.0f;

@@ -285,8 +285,12 @@ __device__ __forceinline__ void tree_softmax(const float (&x)[MT][NE], float (&p
 template <int MT, int NE>
 __device__ __forceinline__ void tree_mask(float (&p)[MT][NE], const TreeArgs& a, int b, const int (&ti)[MT], int quad, int valid,
                                           bool draft, int first) {
-  // (the bytes are read, from a place that exists, and then count or not: reading under a condition compiled to a branch per
-  // key, in which the masked score was lost.  1024 drafts alone: a quad's bytes in one load 78 us, one by one 99)
+  // The bytes are read, from a place that exists, and then count or not.  As if (key >= valid || (draft && !seen[key])) p = -inf
+  // the assignment is lost (clang 22 of ROCm 7.2.0): the scores are elements of a vector, the compiler makes the vector with
+  // -inf in front of the condition, and in the block of the inner one it copies the unmasked vector over it, for the lanes
+  // that see the key and for those that do not.  All that is left of the assignment is an empty block, which
+  // tests/test_csrc_cpu.py looks for in the whole library.  Conditions of & and | have no blocks.  (1024 drafts alone: a quad's
+  // bytes in one load 78 us, one by one 99.)
   static_assert(NE == 4 || NE == 8, "bytes of a word");
   const uint8_t* masks = a.mask + b * a.mask_b;
   const int key0 = quad * NE;   // the lane's first key of the tile

@@ -57,3 +57,42 @@ def test_gram_pass_is_compiled_for_the_rows_that_reach_it():
     names = subprocess.run(["nm", "-C", LIB], check=True, capture_output=True, text=True).stdout
     assert set(re.findall(r"lrqk::als_gram_vec_kernel<([^>]*)>", names)) == {
         "float, 8", "float, 16", "float, 32", "lrqk::bf16_t, 8"}
+
+
+OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
+
+
+def _empty_blocks(asm):
+    """Blocks under an exec mask that hold nothing: what is left of an assignment under a condition whose value was formed in
+    front of it, and may have been overwritten since."""
+    lines = [x for x in (re.sub(r"\s*(//|;).*", "", line).strip() for line in asm.splitlines()) if x and not x.startswith(".")]
+    found = []
+    for i, line in enumerate(lines[:-1]):
+        m = re.match(r"s_and_saveexec_b64 (\S+), ", line)
+        if m and lines[i + 1] == f"s_or_b64 exec, exec, {m.group(1)}":
+            found.append(i)
+    return found
+
+
+def test_empty_blocks_are_found():
+    block = """
+      s_or_b64 exec, exec, s[0:1]
+      s_and_saveexec_b64 s[2:3], s[4:5]   // 0000: 00000000
+      {}
+      s_or_b64 exec, exec, s[2:3]
+      s_and_saveexec_b64 vcc, s[4:5]
+      s_or_b64 exec, exec, s[2:3]"""
+    assert not _empty_blocks(block.format("v_mov_b32_e32 v1, s0"))
+    assert len(_empty_blocks(block.format(""))) == len(_empty_blocks(block.format(".LBB0_5:"))) == 1
+
+
+@pytest.mark.skipif(not os.path.exists(LIB) or not os.path.exists(OBJDUMP), reason="needs the built library and llvm-objdump")
+def test_no_conditional_assignment_is_lost(tmp_path):
+    """In all device code of the library: a masked score was once left unmasked by such a block."""
+    lib = shutil.copy(LIB, tmp_path / "lib.so")
+    subprocess.run([OBJDUMP, "--offloading", lib], check=True, capture_output=True, timeout=60, cwd=tmp_path)
+    parts = sorted(p for p in tmp_path.iterdir() if "amdgcn" in p.name)
+    assert len(parts) >= 10
+    for part in parts:
+        asm = subprocess.run([OBJDUMP, "-d", part], check=True, capture_output=True, text=True, timeout=120).stdout
+        assert not _empty_blocks(asm), part.name
