@@ -542,20 +542,20 @@ def _expect(name: str, t: torch.Tensor, shape, dtype, contiguous: bool = True):
         raise ValueError(f"{name} must be contiguous")
 
 
-def _in_32_bits(*sizes: int):
-    """The library takes these sizes as 32-bit numbers: a larger one would reach it as another."""
-    if max(sizes) >> 31:
-        raise ValueError(f"a size of {max(sizes)} is beyond 32 bits")
+def _too_large(*sizes: int):
+    """The library takes sizes as 32-bit numbers: a larger one would reach it as another."""
+    raise ValueError(f"a size of {max(sizes)} is beyond 32 bits")
 
 
-def _row_strides(name: str, t: torch.Tensor):
-    """Strides of sequences, heads and rows of a tensor whose rows are contiguous; 0 where there is one of a kind, whose stride
-    leads to nothing and may be anything."""
-    b, h, r, d = t.stride()
-    nb, nh, nr, nd = t.shape
-    if d != 1 and nd > 1:
+def _row_strides(name: str, t: torch.Tensor, b: int, h: int, n: int, d: int):
+    """Strides of sequences, heads and rows of a tensor of these sizes whose rows are contiguous; 0 where there is one of a kind,
+    whose stride leads to nothing and may be anything."""
+    s = t.stride()
+    if s[3] != 1 and d > 1:
         raise ValueError(f"the rows of {name} must be contiguous")
-    return b if nb > 1 else 0, h if nh > 1 else 0, r if nr > 1 else 0
+    if b == 1 or h == 1 or n == 1:
+        return s[0] if b > 1 else 0, s[1] if h > 1 else 0, s[2] if n > 1 else 0
+    return s[:3]
 
 
 def _rows16(x: torch.Tensor) -> torch.Tensor:
@@ -617,40 +617,28 @@ class RotaryPlan:
         self.inv_freq = freq.to(device)
 
 
-def _same_view(x: torch.Tensor, y: torch.Tensor) -> bool:
-    return (x.data_ptr() == y.data_ptr() and x.shape == y.shape and
-            all(a == b or n < 2 for n, a, b in zip(x.shape, x.stride(), y.stride())))
+# Whether views share memory is asked of their layouts and of how far apart they begin: for the buffers of a loop the same
+# question every time, so that its answer is kept (a layout is b, heads, tokens, elements and their strides but the last, 1).
 
-
-def _range(x: torch.Tensor) -> Tuple[int, int]:
-    """Where a view's memory begins and ends."""
-    begin = x.data_ptr()
-    if x.is_contiguous() or x.numel() == 0:
-        return begin, begin + x.nbytes
-    return begin, begin + x.element_size() * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
-
-
-def _crosses(place: Tuple[int, int], x: Optional[torch.Tensor]) -> bool:
-    """Whether a view's range meets another one."""
-    if x is None or x.data_ptr() >= place[1]:
-        return False
-    begin, end = _range(x)
-    return max(begin, place[0]) < end and place[0] < place[1]
-
-
-def _once(x: torch.Tensor) -> bool:
+@functools.lru_cache(maxsize=1024)
+def _once(shape, strides) -> bool:
     """Whether every element of a view has a place of its own (a view that cannot be made by slicing and permuting counts as one
     that has not)."""
     inner = 1
-    for stride, n in sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1):
+    for stride, n in sorted((s, n) for s, n in zip((*strides, 1), shape) if n > 1):
         if stride < inner:
             return False
         inner += (n - 1) * stride
     return True
 
 
+def _reach(shape, strides) -> int:
+    """Elements from a view's first to behind its last."""
+    return 1 + sum((n - 1) * s for n, s in zip(shape, (*strides, 1)))
+
+
 def _blocks_meet(shift: int, x: int, y: int, dims) -> bool:
-    """Whether a block of x bytes and one of y bytes, ``shift`` behind it, meet.  dims: what both consist of, (bytes between
+    """Whether a block of x elements and one of y, ``shift`` behind it, meet.  dims: what both consist of, (elements between
     slabs, slabs of x, slabs of y), longest first; without any a block is whole."""
     if shift >= x or -shift >= y:
         return False
@@ -663,19 +651,47 @@ def _blocks_meet(shift: int, x: int, y: int, dims) -> bool:
     return last - first > 3 or any(_blocks_meet(shift + j * step, x, y, dims[1:]) for j in range(first, last + 1))
 
 
-def _meet(x: torch.Tensor, y: torch.Tensor) -> bool:
-    """Whether two views have memory in common.  Views that lie between each other, as the parts of one projection do, are told
-    apart where their dimensions have the same strides; otherwise views whose ranges meet count as meeting."""
-    at_x, at_y = _range(x), _range(y)
-    if not _crosses(at_x, y):
-        return False
-    e, dims = x.element_size(), []
-    if x.dim() == y.dim() and y.element_size() == e:
-        for nx, ny, sx, sy in zip(x.shape, y.shape, x.stride(), y.stride()):
-            step = sx if nx > 1 else sy
-            if max(nx, ny) > 1 and step > 0 and (sx == sy or min(nx, ny) == 1):
-                dims.append((step * e, nx, ny))
-    return _blocks_meet(at_y[0] - at_x[0], at_x[1] - at_x[0], at_y[1] - at_y[0], sorted(dims, reverse=True))
+@functools.lru_cache(maxsize=1024)
+def _views_meet(shift: int, e: int, shape_x, strides_x, shape_y, strides_y) -> bool:
+    """Whether two views of elements of e bytes, the second of which begins ``shift`` bytes behind the first, have memory in
+    common.  Views that lie between each other, as the parts of one projection do, are told apart where their dimensions
+    have the same strides; otherwise views whose ranges meet count as meeting."""
+    dims = []
+    for nx, ny, sx, sy in zip(shape_x, shape_y, (*strides_x, 1), (*strides_y, 1)):
+        step = sx if nx > 1 else sy
+        if max(nx, ny) > 1 and step > 0 and (sx == sy or min(nx, ny) == 1):
+            dims.append((step, nx, ny))
+    x, y = _reach(shape_x, strides_x), _reach(shape_y, strides_y)
+    # (views that begin within each other's elements: what an element covers reaches into the next one)
+    return any(_blocks_meet(at, x, y, sorted(dims, reverse=True)) for at in {shift // e, -(-shift // e)})
+
+
+def _refuse_overlaps(e: int, b: int, s: int, d: int, views, heads, strides, pos, pos_stride: int, freq):
+    """q, q', k, k' of a turn, with three strides each: an output is its input or meets none, and not the other output."""
+    places = []   # where a view begins and ends; its layout
+    for i, (x, h) in enumerate(zip(views, heads)):
+        if x is None or h == 0:
+            places.append(None)
+            continue
+        sb, sh, ss = st = strides[3 * i:3 * i + 3]
+        at = x.data_ptr()
+        places.append((at, at + e * ((b - 1) * sb + (h - 1) * sh + (s - 1) * ss + d), (b, h, s, d), st))
+
+    def meet(x, y):
+        return x is not None and x[0] < y[1] and y[0] < x[1] and _views_meet(y[0] - x[0], e, *x[2:], *y[2:])
+    q, q_out, k, k_out = places
+    for x, y, other in ((q, q_out, k), (k, k_out, q)):
+        if y is None:
+            continue
+        if not _once(*y[2:]):
+            raise ValueError("out has several elements in one place")
+        if (x[0] != y[0] or x[3] != y[3]) and meet(x, y) or meet(other, y):
+            raise ValueError("out overlaps an input and is not the view that is turned")
+        if freq.data_ptr() < y[1] and y[0] < freq.data_ptr() + freq.nbytes or pos is not None and (
+                pos.data_ptr() < y[1] and y[0] < pos.data_ptr() + 4 * ((b - 1) * pos_stride + s)):
+            raise ValueError("out overlaps the positions or the plan")
+    if k_out is not None and meet(q_out, k_out):
+        raise ValueError("out of q and out of k overlap")
 
 
 def _undisturbed(ranges) -> bool:
@@ -703,7 +719,8 @@ def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positio
         hk = k.shape[1]
         if k.shape != (b, hk, s, d) or k.dtype != q.dtype:
             raise ValueError(f"k is {tuple(k.shape)} {k.dtype} beside q {tuple(q.shape)} {q.dtype}")
-    _in_32_bits(b, hq, hk, d)
+    if (b | hq | hk | d) >> 31:
+        _too_large(b, hq, hk, d)
     if plan.rotary_dim > d:
         raise ValueError(f"a plan of {plan.rotary_dim} elements for heads of {d}")
     dt = _dt(q)
@@ -722,24 +739,20 @@ def rotary(plan: RotaryPlan, q: torch.Tensor, k: Optional[torch.Tensor], positio
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
-        xs = (q,) if k is None else (q, k)
-        ys = tuple(out)[:len(xs)] if isinstance(out, (tuple, list)) else (out,)
-        if len(ys) != len(xs) or any(y is None for y in ys):
+        ys = tuple(out)[:1 if k is None else 2] if isinstance(out, (tuple, list)) else (out,)
+        if len(ys) != (1 if k is None else 2) or any(y is None for y in ys):
             raise ValueError("out holds one tensor for q, and one for k if there is a k")
         _on_one_gpu(q, *ys)
-        for i, (x, y) in enumerate(zip(xs, ys)):
-            _expect("out", y, x.shape, x.dtype, contiguous=False)
-            if not _once(y):
-                raise ValueError("out has several elements in one place")
-            others = xs[1 - i:2 - i] if _same_view(x, y) else xs
-            if any(z is not None and _meet(y, z) for z in (*others, pos, plan.inv_freq)):
-                raise ValueError("out overlaps an input and is not the view that is turned")
-        if k is not None and _meet(*ys):
-            raise ValueError("out of q and out of k overlap")
         q_out, k_out = ys if k is not None else (ys[0], None)
-    strides = (*_row_strides("q", q), *_row_strides("out", q_out))
+        if q_out is not q:
+            _expect("out", q_out, q.shape, q.dtype, contiguous=False)
+        if k_out is not k:
+            _expect("out", k_out, k.shape, k.dtype, contiguous=False)
+    strides = (*_row_strides("q", q, b, hq, s, d), *_row_strides("out", q_out, b, hq, s, d))
     if k is not None:
-        strides += (*_row_strides("k", k), *_row_strides("out", k_out))
+        strides += (*_row_strides("k", k, b, hk, s, d), *_row_strides("out", k_out, b, hk, s, d))
+    if out is not None and b * s * d > 0:
+        _refuse_overlaps(q.element_size(), b, s, d, (q, q_out, k, k_out), (hq, hq, hk, hk), strides, pos, pos_stride, plan.inv_freq)
     if b * s > 0:
         _launch(dev, _lib.load().lrqk_rotary, q.data_ptr(), _ptr(k), q_out.data_ptr(), _ptr(k_out),
                 struct.pack(f"{len(strides)}q", *strides), _ptr(pos), pos_stride, first, plan.inv_freq.data_ptr(), plan.factor,
@@ -761,7 +774,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     b, hq, t, d = q.shape
     _, hc, n, _ = k_cache.shape
     hn = k_new.shape[1]
-    _in_32_bits(b, hq, hc, hn, t, d)
+    if (b | hq | hc | hn | t | d) >> 31:
+        _too_large(b, hq, hc, hn, t, d)
     dt, dtype = _dt(q), q.dtype
     _expect("k_cache", k_cache, (b, hc, n, d), dtype, contiguous=False)
     _expect("v_cache", v_cache, (b, hc, n, d), dtype, contiguous=False)
@@ -772,7 +786,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     if mask.shape not in ((b, t, t), (t, t)) or mask.dtype not in (torch.bool, torch.uint8):
         raise ValueError(f"mask is {tuple(mask.shape)} {mask.dtype}: bool or uint8 [t,t] or [b,t,t] is wanted")
     _lengths(lengths, b)
-    st, sv = _row_strides("k_cache", k_cache), _row_strides("v_cache", v_cache)
+    st, sv = _row_strides("k_cache", k_cache, b, hc, n, d), _row_strides("v_cache", v_cache, b, hc, n, d)
     if sv != st and n > 0:
         raise ValueError("k_cache and v_cache must have the same strides")
     q = _rows16(q)
@@ -801,7 +815,8 @@ def attention_weights(q: torch.Tensor, k: torch.Tensor, lengths: Optional[torch.
     dev = _on_one_gpu(q, k, lengths, lse, weights, out)
     b, hq, t, d = q.shape
     hc, n = k.shape[1], k.shape[2]
-    _in_32_bits(b, hq, hc, t, d)
+    if (b | hq | hc | t | d) >> 31:
+        _too_large(b, hq, hc, t, d)
     dt = _dt(q)
     _expect("k", k, (b, hc, n, d), q.dtype, contiguous=False)
     if hc == 0 or hq % hc:
@@ -811,25 +826,31 @@ def attention_weights(q: torch.Tensor, k: torch.Tensor, lengths: Optional[torch.
         _expect("lse", lse, (b, hq, t), torch.float32)
     if weights is not None:
         _expect("weights", weights, (b, hc, n), torch.float32)
-    given = out is not None or weights is not None
+    fresh = out is None and weights is None
     if out is not None:
         _expect("out", out, (b, hc, n), torch.float32)
     else:
-        out = weights if given else torch.empty((b, hc, n), dtype=torch.float32, device=q.device)
-    if given:   # (the caller's place, or the weights')
-        place = _range(out)
-        others = (q, k, lse, lengths) if weights is None or _same_view(out, weights) else (q, k, lse, lengths, weights)
-        if any(_crosses(place, x) for x in others):
-            raise ValueError("the place of the sums overlaps an input")
-    if out.numel() == 0:
+        out = torch.empty((b, hc, n), dtype=torch.float32, device=q.device) if fresh else weights
+    w_at, out_at = _ptr(weights), out.data_ptr()
+    if w_at is not None and 0 < abs(w_at - out_at) < 4 * b * hc * n:
+        raise ValueError("out overlaps weights")
+    if b * n == 0:
         return out
     if t == 0:
         return out.copy_(weights) if weights is not None else out.zero_()
-    q = _rows16(q)
+    q, strides = _rows16(q), _row_strides("k", k, b, hc, n, d)
+    q_at, k_at, l_at, lse_at = q.data_ptr(), k.data_ptr(), _ptr(lengths), _ptr(lse)
+    if not fresh:   # (all contiguous but k)
+        e, end = q.element_size(), out_at + 4 * b * hc * n
+        k_end = k_at + e * ((b - 1) * strides[0] + (hc - 1) * strides[1] + (n - 1) * strides[2] + d)
+        if (q_at < end and out_at < q_at + e * b * hq * t * d or k_at < end and out_at < k_end or
+                l_at is not None and l_at < end and out_at < l_at + 4 * b or
+                lse_at is not None and lse_at < end and out_at < lse_at + 4 * b * hq * t):
+            raise ValueError("the place of the sums overlaps an input")
     need = _scratch_bytes("lrqk_attention_weights_workspace", b, hq, hc, t, n, d, lse is not None, dt)
     ws = _scratch(need, q) if need else None
-    _launch(dev, _lib.load().lrqk_attention_weights, q.data_ptr(), k.data_ptr(), *_row_strides("k", k), n, _ptr(lengths), _ptr(lse),
-            _ptr(weights), out.data_ptr(), b, hq, hc, t, d, d ** -0.5 if scale is None else float(scale), _ptr(ws), need, dt)
+    _launch(dev, _lib.load().lrqk_attention_weights, q_at, k_at, *strides, n, l_at, lse_at, w_at, out_at, b, hq,
+            hc, t, d, d ** -0.5 if scale is None else float(scale), _ptr(ws), need, dt)
     return out
 
 
@@ -845,7 +866,8 @@ def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Te
     other; slots behind the tokens that stay are left as they were.  -> the new lengths, int32 [b]."""
     dev = _on_one_gpu(weights, ids, k, v, lengths, *(out or ()))
     b, h, n, d = k.shape
-    _in_32_bits(b, h, n, d)
+    if (b | h | n | d) >> 31:
+        _too_large(b, h, n, d)
     dt = _dt(k)
     _expect("weights", weights, (b, h, n), torch.float32)
     _expect("ids", ids, (b, h, n), torch.int32)
@@ -861,7 +883,8 @@ def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Te
         if len(out) != 4 or out[2].dim() != 4:
             raise ValueError("out holds weights, ids, k and v")
         cap_out = out[2].shape[2]
-        _in_32_bits(cap_out)
+        if cap_out >> 31:
+            _too_large(cap_out)
         for name, y, shape, dtype in zip(("weights", "ids", "k", "v"), out, ((b, h, cap_out),) * 2 + ((b, h, cap_out, d),) * 2,
                                          (torch.float32, torch.int32, k.dtype, k.dtype)):
             _expect("out " + name, y, shape, dtype)
