@@ -268,7 +268,8 @@ int lrqk_attention_static(const void* q, const void* k_act, const void* v_act, i
  * rotary_dim elements of a head -- elements i and i + rotary_dim / 2, or 2 i and 2 i + 1 if interleaved -- becomes
  * factor (x cos a - y sin a, y cos a + x sin a), a = position * freq[i] (formed and reduced in fp64; freq on the device);
  * the others are copied.  transpose: by -a, the gradient of the turn.  strides (host): elements between sequences, heads
- * and tokens of q, q_out, k, k_out, three each; rows are contiguous.  An output may be its input (with its strides).
+ * and tokens of q, q_out, k, k_out, three each; rows are contiguous.  An output may be its input (with its strides), and has nothing in common with
+ * the other tensors, whose ranges this entry does not compare.
  * positions: int32 [b][s], sequences pos_stride apart (0: one for all), or NULL: first, first + 1, ... */
 int lrqk_rotary_frequencies(int rotary_dim, double theta, int scaling, double factor, double p0, double p1,
                             double original_context, double* freq, double* result_factor);
@@ -284,8 +285,13 @@ int lrqk_rotary(const void* q, const void* k, void* q_out, void* k_out, const in
  * q, out: [b][hq][t][d]; lse (or NULL): fp32 [b][hq][t], log of the sum of exp(scale q.k).  A query that sees nothing
  * gives zeros and -inf.  What a masked drafted token or a row behind the length holds, infinities and NaN included, does
  * not matter; a cached value that is not finite leaves its element of the outputs not finite (a NaN perhaps for an
- * infinity).  Strides in elements, the same for k_cache and v_cache, multiples of 16 bytes (0 for a single sequence, head
- * or row, here and in the calls below), rows at most 2^24 elements apart.  Head widths up to 256 elements, t up to 1024, n up to 2^30, b * hq up to 65535.
+ * infinity).
+ * What probabilities are held in for the product with V: fp32, of fp32 tensors.  Of bf16 tensors two bf16 numbers each, off by
+ * up to 2^-15 of them; beyond 128 queries a cache head (hq / hc * t) one bf16 number, off by up to 2^-8, which moves an output
+ * by up to 2^-8 of the mean of |v - out| besides its own rounding.  lse is that of the fp32 numbers.
+ * Strides in elements, the same for k_cache and v_cache, multiples of 16 bytes (0 for a single sequence, head or row, here
+ * and in the calls below), rows at most 2^24 elements apart.  Head widths up to 256 elements, t up to 1024, n up to 2^30,
+ * b * hq up to 65535.
  * These calls take no ctx: their scratch is the caller's (lrqk_*_workspace bytes of device memory, 16-byte aligned,
  * contents of no meaning before and after), so that calls on several streams and captured graphs need not share any. */
 int64_t lrqk_tree_attention_workspace(int b, int hq, int hc, int t, int64_t n, int d, int have_lengths, int dtype);
@@ -310,8 +316,10 @@ int lrqk_attention_weights(const void* q, const void* k, int64_t k_batch_stride,
  * NULL) of every head, min(length, budget) stay -- those whose ids are within `recent` of the head's largest one (of the
  * lowest slots, if ids that repeat make them more than the budget), then those of the largest weights (NaN in front; equal
  * ones: of the lowest slots).  A token that stays and is in the first min(length, budget) slots keeps its slot; the others
- * that stay move, in order, into the slots that became free, in order.  weights fp32, ids int32 [b][heads][cap], k, v [b][heads][cap][d].  In place where weights_out, ids_out, k_out,
- * v_out are NULL; otherwise those ([b][heads][cap_out], rows of d) take the tokens that stay and the inputs keep theirs.
+ * that stay move, in order, into the slots that became free, in order.
+ * weights fp32, ids int32 [b][heads][cap], k, v [b][heads][cap][d].  In place where weights_out, ids_out, k_out, v_out are
+ * NULL; otherwise those ([b][heads][cap_out], rows of d) take the tokens that stay and the inputs keep theirs.  What is
+ * written has nothing in common with anything else (this entry looks at where tensors begin, not at their ranges).
  * Slots behind the tokens that stay are left as they were.  new_lengths int32 [b] (may be lengths). */
 int64_t lrqk_evict_workspace(int b, int heads, int cap, int budget);
 int lrqk_evict(float* weights, int32_t* ids, void* k, void* v, const int32_t* lengths, int cap, float* weights_out,

@@ -96,7 +96,7 @@ struct WeightTile {
 };
 
 // Item (head, part, group of 64 NT rows) of a workgroup: its queries' maximum and sum over its part of the keys.  Bound by
-// the exponentials beside the products: 8192 tokens of 32 / 8 heads of 128, 275 GFLOP in 321 to 350 us, the vector ALUs 59 %
+// the exponentials beside the products: 8192 tokens of 32 / 8 heads of 128, 275 GFLOP in 313 to 350 us, the vector ALUs 59 %
 // busy, the matrix cores 37 %; `merge` 8.
 template <typename T, int DP, int NT>
 __global__ __launch_bounds__(kAwThreads, 2) void weights_rows_kernel(WeightArgs a) {

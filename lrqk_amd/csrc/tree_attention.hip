@@ -10,8 +10,8 @@
 // workgroup.  S^T = K Q^T leaves a query in a lane's column, so maximum, sum and rescaling need no exchange but two
 // between the quads, and the probabilities are the operand of O^T = V^T P^T as they lie: the rows of K are dealt to the
 // lanes such that a quad's scores are those of successive keys, whose V rows the same quad loads, 16 lanes one whole row.
-// Bf16 V is transposed between those lanes' registers; bf16 probabilities are the sum of two bf16 numbers (16 bits), so
-// that the one rounding to bf16 is the output's (but for very many queries: tree_share_kernel).
+// Bf16 V is transposed between those lanes' registers; bf16 probabilities are the sum of two bf16 numbers (off by up to
+// 2^-15 of them), so that the one rounding to bf16 is the output's (but for very many queries: tree_share_kernel).
 #include <algorithm>
 #include <type_traits>
 
@@ -504,12 +504,12 @@ constexpr int kTlWaves = 4, kTlThreads = kTlWaves * kWave;
 // (ds_read_b64_tr_b16: four keys of one element a lane).
 //
 // FINE: bf16 probabilities as the sum of two bf16 numbers, as in tree_stream_kernel.  Beyond 128 queries a cache head this
-// is bound by the products, and half of those with V are the second number's (64 drafts over 4 x 64K, 32 / 8 heads: 195 to
-// 230 instead of 230 to 285 us without it, as the clock holds; 1.1 PFLOP/s at best; 25 drafts over 128K, bound by the reading:
-// 108 instead of 112).  There the probabilities
-// are rounded to bf16, 2^-9 of each, independently of each other, and what they are divided by is the sum of the rounded
-// ones (one more block of o), so that a result is off by what its rounding to bf16 is off by once more; lse keeps the exact
-// ones' sum.
+// is bound by the products, and half of those with V are the second number's (64 drafts over 4 x 64K, 32 / 8 heads, three
+// ragged sets of lengths: 311, 222 and 226 us a call without it, 372, 258 and 276 with it; 25 drafts over 128K, bound by the
+// reading: 108 instead of 112).  There a probability is rounded to bf16, by up to 2^-8 of it, each for itself, and what they
+// are divided by is the sum of the rounded ones (one more block of o), so that an output moves by up to 2^-8 of the mean of
+// |v - out|, and by its own rounding; lse keeps the exact ones' sum.  Those 64 drafts: 0.00215 of the output's norm off a
+// result in 64 bits, 0.00166 with two numbers, which is the output's rounding alone.
 template <typename T, int DP, int WR>
 struct TreeShare {
   static constexpr int MT = DP == 256 ? 1 : 2, WK = kTlWaves / WR;

@@ -768,7 +768,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     q [b,Hq,t,d]; k_cache, v_cache [b,Hc,n,d], of which sequence i has ``lengths[i]`` tokens (int32 [b] on the GPU; all n if
     None), any strides that both share, rows contiguous; k_new, v_new [b,Hn,t,d] of the drafted tokens; mask bool or uint8
     [t,t] or [b,t,t]: drafted token i sees j.  Hc = Hn for a dense cache, Hc = Hq for an active set (``engine.Kgpu``).
-    ``scale`` (1 / sqrt(d) if None) is positive.  -> [b,Hq,t,d], zeros for a token that sees nothing; with ``return_lse``
+    ``scale`` (1 / sqrt(d) if None) is positive.  Probabilities meet bf16 values as two bf16 numbers each, and beyond 128
+    queries a cache head (Hq / Hc * t) as one: an output then moves by up to 2^-8 of the mean of |v - out| (pass float32
+    tensors where that is too much), lse not at all.  -> [b,Hq,t,d], zeros for a token that sees nothing; with ``return_lse``
     also fp32 [b,Hq,t], the logarithm of the sum of the exponentials (-inf for such a token)."""
     dev = _on_one_gpu(q, k_cache, v_cache, k_new, v_new, mask, lengths)
     b, hq, t, d = q.shape
