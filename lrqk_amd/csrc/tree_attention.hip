@@ -21,6 +21,7 @@ namespace lrqk {
 
 constexpr int kTrWaves = 4, kTrThreads = kTrWaves * kWave;
 constexpr int kTrMaxSplits = 256;
+constexpr int kTrLong = 512;          // tiles of a split, at most, for each row block (tree_plan)
 constexpr float kTrNone = -3.0e38f;   // running maximum of a query that has seen no key yet
 constexpr float kTrMuch = 4096.0f;    // a lane's probabilities of a tile may add up to this before the maximum is looked for
 
@@ -37,7 +38,8 @@ struct TreeArgs {
   int64_t kv_b, kv_h, kv_r; // elements between sequences, heads and rows of the cache
   int64_t mask_b;
   // splits: of all sequences together, for a cache head; least: tiles of a split, at least; rows: of a row block
-  int b, n, hq, hc, hn, t, d, splits, least, row_blocks, rows, row_tiles, units;
+  // most: tiles of a split, at most
+  int b, n, hq, hc, hn, t, d, splits, least, most, row_blocks, rows, row_tiles, units;
   float scale_log2e;
 };
 
@@ -167,7 +169,7 @@ struct TreeCut {
   // tiles of a split (32 bits divide four times as fast as 64)
   static __device__ __forceinline__ int share(const TreeArgs& a, int64_t all) {
     const int x = all <= INT32_MAX ? (int)(((uint32_t)all + (uint32_t)a.splits - 1u) / (uint32_t)a.splits) : (int)((all + a.splits - 1) / a.splits);
-    return max(a.least, x);
+    return max(a.least, min(x, a.most));
   }
   // the split of number `slot` of all; false: there is none
   __device__ __forceinline__ bool find(const TreeArgs& a, int kt, int slot) {
@@ -941,7 +943,7 @@ __global__ __launch_bounds__(THREADS) void tree_join_kernel(TreeArgs a) {
 struct TreePlan {
   int dp, mt, wr;                    // wr = 0: tree_stream_kernel
   bool fine;
-  int rows, row_blocks, row_tiles, splits, least, units;
+  int rows, row_blocks, row_tiles, splits, least, most, units;
   int64_t part, ml, odd, cut;        // words of 4 bytes
 };
 static TreePlan tree_plan(int b, int hq, int hc, int t, int64_t n, int d, bool lengths, int dtype) {
@@ -970,8 +972,15 @@ static TreePlan tree_plan(int b, int hq, int hc, int t, int64_t n, int d, bool l
   p.row_tiles = p.row_blocks * (p.rows / 16);
   p.splits = (int)std::max<int64_t>(b, groups_wanted / ((int64_t)hc * p.row_blocks));
   p.least = (int)std::max<int64_t>(least, (tiles + kTrMaxSplits - 1) / kTrMaxSplits);
-  // the splits that there can be: the wanted ones and the sequences' shorter ones, or what the shortest splits make
-  const int64_t slots = std::min<int64_t>((int64_t)p.splits + b, b * ((tiles + p.least - 1) / p.least));
+  // Where the heads alone fill the GPU a split would be all of a sequence, and one fp32 number the sum over all its keys: with
+  // 131072 that round alike lse was 1.2e-4 off and an output 2e-3 (fp32; the matrix cores cut off), with splits of up to 512
+  // tiles 2.4e-6 and 8e-6.  Their scratch is 1 % of K and V; more row blocks, which have as much each, have longer splits.  Of
+  // a whole cache they are of one length: 64 drafts over 64 sequences of 32K, 1027 tiles as 1024 and 3, took 3.8 ms instead of 2.6.
+  const int64_t longest = std::max<int64_t>(p.least, (int64_t)kTrLong * p.row_blocks), parts = (tiles + longest - 1) / longest;
+  p.most = (int)((tiles + parts - 1) / parts);
+  // the splits that there can be: the wanted ones and the sequences' shorter ones, or those of the longest splits; or what the
+  // shortest make
+  const int64_t slots = std::min<int64_t>(std::max<int64_t>((int64_t)p.splits + b, b * parts), b * ((tiles + p.least - 1) / p.least));
   p.units = (int)(hc * slots);
   const int64_t groups = (int64_t)p.units * p.row_tiles;
   p.part = groups * 16 * p.dp;
@@ -994,7 +1003,7 @@ template <typename T, int DP>
 static int tree_launch(const TreeArgs& a, const TreePlan& p, hipStream_t st) {
   const dim3 grid((unsigned)((int64_t)(a.units + 7) / 8 * 8 * a.row_blocks));
   const dim3 join((unsigned)((int64_t)a.b * a.hc * a.row_tiles * 4));
-  // (of the most heads and drafts, 65535 and 1024: 2^23 and 2^24 - 256 workgroups, of 256 threads each; a launch may have 2^32 - 1 threads)
+  // (of the most heads and drafts, 65535 and 1024: 2^24 - 256 workgroups of 256 threads; a launch may have 2^32 - 1 threads)
   if (p.wr == 0) {
     if constexpr (DP < 256)
       if (p.mt == 2) hipLaunchKernelGGL((tree_stream_kernel<T, DP, 2>), grid, dim3(kTrThreads), 0, st, a);
@@ -1065,9 +1074,11 @@ extern "C" int lrqk_tree_attention(const void* q, const void* k_cache, const voi
   const int64_t need = (p.part + p.ml + p.odd + p.cut) * (int64_t)sizeof(float);
   LRQK_REQUIRE(workspace_bytes >= need, LRQK_EINVAL, "workspace of %lld bytes: %lld are needed", (long long)workspace_bytes,
                (long long)need);
+  LRQK_REQUIRE(((int64_t)p.units + 7) / 8 * 8 * p.row_blocks <= kMaxThreads / kTrThreads, LRQK_ELIMIT,
+               "%lld tokens of %d heads and %d drafts are more than a launch has places for", (long long)n, b * hc, t);
   TreeArgs a{q, k_cache, v_cache, k_new, v_new, mask, lengths, out, lse, (float*)workspace, (float*)workspace + p.part,
              (int32_t*)workspace + p.part + p.ml, (int32_t*)workspace + p.part + p.ml + p.odd,
-             kv_batch_stride, kv_head_stride, kv_row_stride, mask_batch_stride, b, (int)n, hq, hc, hn, t, d, p.splits, p.least, p.row_blocks, p.rows,
+             kv_batch_stride, kv_head_stride, kv_row_stride, mask_batch_stride, b, (int)n, hq, hc, hn, t, d, p.splits, p.least, p.most, p.row_blocks, p.rows,
              p.row_tiles, p.units,
              scale * kLog2e};
   hipStream_t st = (hipStream_t)stream;

@@ -1275,3 +1275,32 @@ def test_attention_weights_of_thousands_of_tiles_in_one_part(ops, b, t):
         exact[:, :32] *= e[first:first + 64, None]
         off = ((got[first:first + 64, 0].double() - exact) / exact).abs().max()
         assert float(off) <= tol, (first, float(off), tol)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("b,t", [(2112, 1), (1030, 33), (1030, 65), (1030, 130)])
+def test_tree_attention_of_heads_that_fill_the_gpu(ops, dtype, b, t):
+    """So many heads that each could walk over its keys in one part, whose exponentials are all the same number: every addition
+    then rounds the same way (the matrix cores cut off), and the error may not grow with the cache."""
+    print("tree, one part", dtype, b, t, flush=True)
+    n, g = 131072, _gen(t)
+    a = torch.linspace(0.02, 1.5, b, dtype=torch.float64).to(BF).to(DEV)   # logit of the first 32 keys; of the others 0
+    q, kn = torch.zeros((b, 1, t, 8), dtype=dtype, device=DEV), torch.zeros((b, 1, t, 8), dtype=dtype, device=DEV)
+    k, v = torch.zeros((1, 1, n, 8), dtype=dtype, device=DEV), torch.rand((1, 1, n, 8), generator=g).to(dtype).to(DEV)
+    q[..., 0], k[:, :, :32, 0], v[..., 0] = a[:, None, None].to(dtype), 1.0, 1.0
+    mask = torch.zeros((t, t), dtype=torch.bool, device=DEV)
+    out, lse = ops.tree_attention(q, k.expand(b, 1, n, 8), v.expand(b, 1, n, 8), kn, kn, mask, scale=1.0, return_lse=True)
+    e = a.double().exp()[:, None]
+    total = 32 * e + (n - 32)
+    exact = (e * v[0, 0, :32].double().sum(0) + v[0, 0, 32:].double().sum(0)) / total
+    # a split has 512 tiles for each 128 queries: a lane adds up so many numbers to one that grows, so that half of them count,
+    # half of 2^-23 each, and 8 of a tile, 16 and 64 of the joins
+    tiles = 512 * (2 if t > 128 else 1)
+    of_sum = (tiles / 2 + 8 + 16 + 64) * 2.0 ** -24
+    # log of base 2 (17: a unit is 2^-19), 2 units, its sum with the maximum half of one, times ln 2; the product's rounding
+    assert float((lse.double() - total.log()[..., None]).abs().max()) <= of_sum + math.log(2) * 2.5 * 2.0 ** -19 + 2.0 ** -21
+    # the product with V: a split's keys, 4 (fp32) or 32 (bf16) a step, each step up to a unit of a sum that grows; bf16 values
+    # times two numbers, and the output's rounding
+    steps = tiles * (16 / 4 if dtype == FP else 2)
+    tol = of_sum + (steps / 2 + 64) * U + (2.0 ** -15 if dtype == BF else 0.0) + (2.0 ** -8 if dtype == BF and t > 128 else 0.0) + HALF[dtype]
+    assert float(((out[:, 0].double() - exact[:, None]) / exact[:, None]).abs().max()) <= tol
