@@ -617,8 +617,8 @@ class RotaryPlan:
         self.inv_freq = freq.to(device)
 
 
-# Whether views share memory is asked of their layouts and of how far apart they begin: for the buffers of a loop the same
-# question every time, so that its answer is kept (a layout is b, heads, tokens, elements and their strides but the last, 1).
+# Whether views share memory is asked of their layouts (b, heads, tokens, elements, and their strides but the last, which is 1)
+# and of how far apart they begin.
 
 @functools.lru_cache(maxsize=1024)
 def _once(shape, strides) -> bool:
@@ -630,11 +630,6 @@ def _once(shape, strides) -> bool:
             return False
         inner += (n - 1) * stride
     return True
-
-
-def _reach(shape, strides) -> int:
-    """Elements from a view's first to behind its last."""
-    return 1 + sum((n - 1) * s for n, s in zip(shape, (*strides, 1)))
 
 
 def _blocks_meet(shift: int, x: int, y: int, dims) -> bool:
@@ -652,18 +647,27 @@ def _blocks_meet(shift: int, x: int, y: int, dims) -> bool:
 
 
 @functools.lru_cache(maxsize=1024)
-def _views_meet(shift: int, e: int, shape_x, strides_x, shape_y, strides_y) -> bool:
-    """Whether two views of elements of e bytes, the second of which begins ``shift`` bytes behind the first, have memory in
-    common.  Views that lie between each other, as the parts of one projection do, are told apart where their dimensions
-    have the same strides; otherwise views whose ranges meet count as meeting."""
+def _common(shape_x, strides_x, shape_y, strides_y):
+    """Elements from the first of a view to behind the last, of two views, and the dimensions that have the same stride in both as
+    _blocks_meet takes them."""
     dims = []
     for nx, ny, sx, sy in zip(shape_x, shape_y, (*strides_x, 1), (*strides_y, 1)):
         step = sx if nx > 1 else sy
         if max(nx, ny) > 1 and step > 0 and (sx == sy or min(nx, ny) == 1):
             dims.append((step, nx, ny))
-    x, y = _reach(shape_x, strides_x), _reach(shape_y, strides_y)
+    reach = [1 + sum((n - 1) * s for n, s in zip(shape, (*strides, 1))) for shape, strides in ((shape_x, strides_x), (shape_y, strides_y))]
+    return (*reach, sorted(dims, reverse=True))
+
+
+def _views_meet(shift: int, e: int, shape_x, strides_x, shape_y, strides_y) -> bool:
+    """Whether two views of elements of e bytes, the second of which begins ``shift`` bytes behind the first, have memory in
+    common.  Views that lie between each other, as the parts of one projection do, are told apart where their dimensions
+    have the same strides; otherwise views whose ranges meet count as meeting."""
+    x, y, dims = _common(shape_x, strides_x, shape_y, strides_y)
+    if shift % e == 0:
+        return _blocks_meet(shift // e, x, y, dims)
     # (views that begin within each other's elements: what an element covers reaches into the next one)
-    return any(_blocks_meet(at, x, y, sorted(dims, reverse=True)) for at in {shift // e, -(-shift // e)})
+    return _blocks_meet(shift // e, x, y, dims) or _blocks_meet(shift // e + 1, x, y, dims)
 
 
 def _refuse_overlaps(e: int, b: int, s: int, d: int, views, heads, strides, pos, pos_stride: int, freq):
@@ -678,19 +682,22 @@ def _refuse_overlaps(e: int, b: int, s: int, d: int, views, heads, strides, pos,
         places.append((at, at + e * ((b - 1) * sb + (h - 1) * sh + (s - 1) * ss + d), (b, h, s, d), st))
 
     def meet(x, y):
-        return x is not None and x[0] < y[1] and y[0] < x[1] and _views_meet(y[0] - x[0], e, *x[2:], *y[2:])
+        return x is not None and y is not None and x[0] < y[1] and y[0] < x[1] and _views_meet(y[0] - x[0], e, *x[2:], *y[2:])
     q, q_out, k, k_out = places
-    for x, y, other in ((q, q_out, k), (k, k_out, q)):
+    f_at, p_at = freq.data_ptr(), 0 if pos is None else pos.data_ptr()
+    f_end, p_end = f_at + freq.nbytes, 0 if pos is None else p_at + 4 * ((b - 1) * pos_stride + s)
+    for y in (q_out, k_out):
         if y is None:
             continue
         if not _once(*y[2:]):
             raise ValueError("out has several elements in one place")
-        if (x[0] != y[0] or x[3] != y[3]) and meet(x, y) or meet(other, y):
-            raise ValueError("out overlaps an input and is not the view that is turned")
-        if freq.data_ptr() < y[1] and y[0] < freq.data_ptr() + freq.nbytes or pos is not None and (
-                pos.data_ptr() < y[1] and y[0] < pos.data_ptr() + 4 * ((b - 1) * pos_stride + s)):
+        if f_at < y[1] and y[0] < f_end or p_at < y[1] and y[0] < p_end:
             raise ValueError("out overlaps the positions or the plan")
-    if k_out is not None and meet(q_out, k_out):
+    in_place = q == q_out and k == k_out   # (then one pair is left)
+    if (q != q_out and meet(q, q_out)) or (k != k_out and meet(k, k_out)) or meet(k, q_out) or (
+            not in_place and meet(q, k_out)):
+        raise ValueError("out overlaps an input and is not the view that is turned")
+    if not in_place and meet(q_out, k_out):
         raise ValueError("out of q and out of k overlap")
 
 

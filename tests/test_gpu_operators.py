@@ -1304,3 +1304,19 @@ def test_tree_attention_of_heads_that_fill_the_gpu(ops, dtype, b, t):
     steps = tiles * (16 / 4 if dtype == FP else 2)
     tol = of_sum + (steps / 2 + 64) * U + (2.0 ** -15 if dtype == BF else 0.0) + (2.0 ** -8 if dtype == BF and t > 128 else 0.0) + HALF[dtype]
     assert float(((out[:, 0].double() - exact[:, None]) / exact[:, None]).abs().max()) <= tol
+
+
+def test_rotary_in_place_is_held_to_every_rule(ops):
+    """Both in place: keys that lie in several heads' or tokens' place, the positions under either, queries and keys shifted."""
+    plan = ops.RotaryPlan(64, 1e4, False, None, DEV)
+    flat = torch.zeros(2048, device=DEV)
+    q, k = flat[:384].view(1, 2, 3, 64), flat[384:768].view(1, 2, 3, 64)
+    pos = torch.zeros(3, dtype=torch.int32, device=DEV)
+    a, b = ops.rotary(plan, q, k, pos, out=(q, k))
+    assert a is q and b is k
+    one = flat[1024:1088].view(1, 1, 1, 64).expand(1, 2, 3, 64)
+    shifted = flat[380:764].view(1, 2, 3, 64)
+    for x, y, p in ((q, one, pos), (one, k, pos), (q, k, flat[382:385].view(torch.int32)), (q, k, flat[3:6].view(torch.int32)), (q, shifted, pos),
+                    (shifted, q, pos), (q, q, pos)):
+        with pytest.raises(ValueError):
+            ops.rotary(plan, x, y, p, out=(x, y))
