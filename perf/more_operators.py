@@ -1,0 +1,513 @@
+"""Operators of a drafted generation whose cache is held in 8 bits, as cases that can be timed and compared.
+
+A round of such a generation attends with a tree of drafted tokens over the cache, verifies the drafts against the target's
+probabilities, and writes the keys and values of the accepted ones behind the sequence.  A case is one of
+
+  append     keys and values written into the cache: of a whole prompt, or of the accepted path of a tree
+  attention  attention of ``t`` tokens over the cached ones and, in a tree, over each other
+  verify     the accepted path of a tree of drafts and the token that follows it, from given random numbers
+
+The cache has blocks of 64 tokens of a head, each with one scale for its keys and one for its values: codes * scale.  Keys are
+held as [64, width], values as [width, 64], the width rounded up to 64, 128 or 256.  The tokens of the block that is not
+complete yet, and of the one before it, are kept as they came: token p in row p % 128 of a tail.
+
+Head counts, head widths, contexts and the vocabulary are those of ``lrqk_amd.synth.WORKLOADS``, of
+``lrqk_amd.decoder.DecoderConfig`` and of the tests.
+"""
+import math
+
+import torch
+
+own = False
+
+DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}
+CODES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
+BLOCK, TAIL = 64, 128
+QUERY_SCALE = 2.5   # logits of a trained model spread over several units, so the attention has peaks
+
+
+def _append(name, batch, heads, head_dim, dtype, kind, t, n):
+    return {"name": name, "op": "append", "batch": batch, "heads": heads, "head_dim": head_dim, "dtype": dtype, "kind": kind,
+            "t": t, "n": n}   # n: what is cached already, at most; 0: a prompt
+
+
+def _attention(name, batch, heads, cache_heads, head_dim, dtype, kind, t, n, ragged, tree):
+    return {"name": name, "op": "attention", "batch": batch, "heads": heads, "cache_heads": cache_heads, "head_dim": head_dim,
+            "dtype": dtype, "kind": kind, "t": t, "n": n, "ragged": ragged, "tree": tree}
+
+
+def _verify(name, batch, s, children, vocab, dtype, drafted):
+    return {"name": name, "op": "verify", "batch": batch, "s": s, "children": children, "vocab": vocab, "dtype": dtype,
+            "drafted": drafted}   # children: of a node, at most; drafted: there are probabilities that the drafts were drawn from
+
+
+def listed():
+    return [
+        # a long prompt, as the projections leave it
+        _append("append prompt 32K", 1, 8, 128, "bf16", "int8", 32768, 0),
+        # a prompt of odd length of the 28 / 4 head shape
+        _append("append prompt 4K fp32", 1, 4, 128, "fp32", "fp8", 4093, 0),
+        # what four sequences accepted of 16 drafts each and the token in front of them
+        _append("append drafts 4x2K", 4, 8, 128, "bf16", "int8", 17, 2112),
+        # a single token over a dense cache
+        _attention("token 32K", 1, 32, 8, 128, "bf16", "int8", 1, 32768, False, False),
+        # a generated token of each of sixteen sequences of different lengths
+        _attention("token 16x8K", 16, 32, 8, 128, "bf16", "fp8", 1, 8192, True, False),
+        # a few drafts over a short fp32 cache of odd length
+        _attention("tree 4K fp32", 1, 28, 4, 128, "fp32", "int8", 7, 4091, False, True),
+        # a usual tree over the longest context
+        _attention("tree 128K", 1, 32, 8, 128, "bf16", "fp8", 25, 131071, False, True),
+        # wide trees of four sequences of different lengths
+        _attention("tree 4x64K", 4, 32, 8, 128, "bf16", "int8", 64, 65536, True, True),
+        # nothing drafted: a token drawn from its distribution, the smallest call
+        _verify("sample token", 1, 1, 1, 128256, "fp32", False),
+        # eight drafts in a row of each of eight sequences
+        _verify("chain 8x8", 8, 9, 1, 128256, "fp32", True),
+        # a usual tree of four sequences, several drafts behind a token
+        _verify("tree 4x25", 4, 26, 4, 128256, "fp32", True),
+        # drafts that were looked up in the context, without probabilities of their own
+        _verify("lookup 16x16", 16, 17, 2, 128256, "bf16", False),
+    ]
+
+
+def _log(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    op = rng.choice(("append", "append", "attention", "attention", "attention", "verify", "verify"))
+    heads, kv_heads = rng.choice(((32, 8), (28, 4), (16, 8), (24, 3)))
+    head_dim = rng.choice((128, 128, 128, 64))
+    dtype, kind = rng.choice(("bf16", "bf16", "bf16", "fp32")), rng.choice(("int8", "fp8"))
+    batch = rng.choice((1, 1, 2, 3, 4))
+    if op == "append":
+        if rng.random() < 0.5:
+            case = _append("", batch, kv_heads, head_dim, dtype, kind, _log(rng, 1, 32768 // batch // (2 if dtype == "fp32" else 1)), 0)
+        else:
+            case = _append("", batch, kv_heads, head_dim, dtype, kind, rng.randint(1, 64), _log(rng, 64, 8192))
+    elif op == "attention":
+        own_heads = rng.random() < 0.2   # every query head has a cache of its own
+        tree = rng.random() < 0.7
+        t = _log(rng, 1, 64) if tree else 1
+        n = _log(rng, 64, (8192 if own_heads else 131072 if dtype == "bf16" else 32768) // batch)
+        case = _attention("", batch, heads, heads if own_heads else kv_heads, head_dim, dtype, kind, t, n,
+                          batch > 1 and rng.random() < 0.7, tree)
+    else:
+        s = rng.randint(1, 32)
+        case = _verify("", rng.choice((1, 2, 3, 4, 8)), s, rng.choice((1, 1, 2, 4)), _log(rng, 1000, 128256),
+                       rng.choice(("fp32", "fp32", "bf16")), rng.random() < 0.7)
+    return {k: v for k, v in case.items() if k != "name"}
+
+
+# ------------------------------------------------------------------------------------------------------------- inputs
+
+def _randn(gen, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(shape, generator=gen, device="cuda") * scale).to(dtype)
+
+
+def _keys(gen, b, h, n, d, dtype):
+    """[b,h,n,d]; some elements of a trained model's keys are larger than others throughout."""
+    return (torch.randn((b, h, n, d), generator=gen, device="cuda") * torch.exp(0.4 * _randn(gen, 1, h, 1, d))).to(dtype)
+
+
+def _width(d):
+    return 64 if d <= 64 else 128 if d <= 128 else 256
+
+
+def _parents(gen, batch, s, children):
+    """int32 [batch,s]: nodes in an order in which parents stand in front of their children, of which a node has at most
+    ``children``.  Node 0 is the root, whose parent is -1."""
+    i = torch.arange(s, device="cuda")
+    if children == 1:
+        return (i - 1).to(torch.int32).repeat(batch, 1)
+    # a wide tree, every node in turn with its children, or a deep one, each group of children below the first of the group before
+    wide = (i - 1).clamp(min=0) // children
+    deep = ((i - 1).clamp(min=0) // children * children - children + 1).clamp(min=0)
+    parents = torch.where(torch.rand((batch, 1), generator=gen, device="cuda") < 0.5, deep, wide)
+    return torch.where(i == 0, i - 1, parents).to(torch.int32)
+
+
+def _ancestors(parents):
+    """bool [batch,s,s]: a node sees itself and those between it and the root."""
+    batch, s = parents.shape
+    sees = torch.eye(s, device="cuda").repeat(batch, 1, 1)
+    step = torch.zeros((batch, s, s + 1), device="cuda").scatter_(2, (parents.long() + 1)[..., None], 1.0)[..., 1:]
+    for _ in range(max(1, (s - 1).bit_length())):
+        sees, step = ((sees + torch.matmul(step, sees)) > 0).float(), torch.matmul(step, step)
+    return sees.bool()
+
+
+def _empty_cache(b, h, capacity, d, dtype, kind):
+    """The cache as a dict of its buffers, on a tree that lacks it, or as the framework holds it."""
+    if own:
+        from lrqk_amd import ops
+        return ops.ByteCache(b, h, capacity, d, dtype=dtype, kind=kind, device="cuda")
+    blocks, w = -(-capacity // BLOCK), _width(d)
+    return {"k": torch.zeros((b, h, blocks, BLOCK, w), dtype=CODES[kind], device="cuda"),
+            "v": torch.zeros((b, h, blocks, w, BLOCK), dtype=CODES[kind], device="cuda"),
+            "k_scale": torch.ones((b, h, blocks), device="cuda"), "v_scale": torch.ones((b, h, blocks), device="cuda"),
+            "k_tail": torch.zeros((b, h, TAIL, d), dtype=dtype, device="cuda"),
+            "v_tail": torch.zeros((b, h, TAIL, d), dtype=dtype, device="cuda")}
+
+
+def _buffers(cache):
+    return cache if isinstance(cache, dict) else {x: getattr(cache, x) for x in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail")}
+
+
+def _fill(cache, k, v, lengths):
+    """Puts the first ``lengths`` of the rows k, v [b,h,n,d] into the cache."""
+    hold = _buffers(cache)
+    n, d = k.shape[2:]
+    kind = "int8" if hold["k"].dtype == torch.int8 else "fp8"
+    whole = n // BLOCK * BLOCK
+    at = (lengths.long()[:, None] - 1) // TAIL * TAIL + torch.arange(TAIL, device="cuda")   # the tail's tokens
+    at = torch.where(at >= lengths[:, None], at - TAIL, at).clamp(min=0)
+    for x, name in ((k, "k"), (v, "v")):
+        if whole:
+            codes, scale = _codes(x[:, :, :whole].reshape(*x.shape[:2], whole // BLOCK, BLOCK, d), kind, torch.float32)
+            hold[name + "_scale"][:, :, :whole // BLOCK] = scale
+            room = hold[name][:, :, :whole // BLOCK]
+            if name == "k":
+                room[..., :d] = codes
+            else:
+                room[..., :d, :] = codes.transpose(-1, -2)
+        hold[name + "_tail"].copy_(x.gather(2, at[:, None, :, None].expand(-1, x.shape[1], -1, d)))
+    return cache
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    b, op = case["batch"], case["op"]
+    if op == "verify":
+        s, vocab, dt = case["s"], case["vocab"], DTYPES[case["dtype"]]
+        parents = _parents(gen, b, s, case["children"])
+        # a few tokens have most of the probability; the drafting model's logits are near the target's
+        logits = 0.22 * _randn(gen, b, s, vocab) ** 3
+        target = torch.softmax(logits, -1)
+        guess = torch.softmax(logits + _randn(gen, b, s, vocab, scale=0.7), -1)
+        up = parents.long().clamp(min=0)
+        drawn_from = guess if case["drafted"] else target   # (a lookup finds what is likely)
+        tokens = torch.multinomial(drawn_from.gather(1, up[..., None].expand(-1, -1, vocab)).flatten(0, 1), 1, generator=gen)
+        return {"op": op, "case": case, "tokens": tokens.view(b, s).to(torch.int32), "target": target.to(dt),
+                "draft": guess.to(dt) if case["drafted"] else None, "uniforms": torch.rand((b, s), generator=gen, device="cuda"),
+                "parents": parents, "mask": _ancestors(parents)}
+    d, t, n, dt = case["head_dim"], case["t"], case["n"], DTYPES[case["dtype"]]
+    lengths = torch.full((b,), n, dtype=torch.int32, device="cuda")
+    if op == "append":
+        h = case["heads"]
+        # as a projection leaves them: all heads of a token side by side
+        k, v = (_keys(gen, b, t, h, d, dt).transpose(1, 2) for _ in range(2))
+        cache, path, counts = _empty_cache(b, h, n + t, d, dt, case["kind"]), None, None
+        if n:
+            lengths = torch.randint(max(1, n // 2), n + 1, (b,), generator=gen, device="cuda", dtype=torch.int32)
+            _fill(cache, *(_keys(gen, b, h, n, d, dt) for _ in range(2)), lengths)
+            # some of the drafts, in order, the first token among them
+            kept = torch.rand((b, t), generator=gen, device="cuda") < 0.5
+            kept[:, 0] = True
+            counts = kept.sum(-1).to(torch.int32)
+            path = (~kept).to(torch.uint8).sort(dim=-1, stable=True).indices.to(torch.int32)
+        return {"op": op, "case": case, "cache": cache, "k": k, "v": v, "lengths": lengths, "path": path, "counts": counts}
+    hq, hc = case["heads"], case["cache_heads"]
+    if case["ragged"]:
+        lengths[1:] = torch.randint(max(1, n // 8), n + 1, (b - 1,), generator=gen, device="cuda", dtype=torch.int32)
+    cache = _fill(_empty_cache(b, hc, n + t, d, dt, case["kind"]), _keys(gen, b, hc, n, d, dt), _randn(gen, b, hc, n, d, dtype=dt), lengths)
+    state = {"op": op, "case": case, "cache": cache, "lengths": lengths, "k_new": None, "v_new": None, "mask": None,
+             "q": _randn(gen, b, hq, t, d, dtype=dt, scale=QUERY_SCALE)}
+    if case["tree"]:
+        state["k_new"], state["v_new"] = _keys(gen, b, hc, t, d, dt), _randn(gen, b, hc, t, d, dtype=dt)
+        state["mask"] = _ancestors(_parents(gen, b, t, 3))
+    return state
+
+
+# --------------------------------------------------------------------------------------------------------- plain forms
+
+def _codes(x, kind, bits):
+    """Codes and fp32 scales of blocks [..., 64, d]; ``bits``: the type that quotients are formed in before they are rounded."""
+    x = x.float()
+    x = torch.where(torch.isnan(x), torch.zeros_like(x), x)
+    largest = torch.where(torch.isinf(x), torch.zeros_like(x), x).abs().amax((-1, -2))
+    if kind == "int8":
+        scale = (largest / 127.0).clamp(min=2.0 ** -100)
+        return torch.round(x.to(bits) / scale.to(bits)[..., None, None]).clamp(-127, 127).to(torch.int8), scale
+    part, power = torch.frexp(largest)   # part in [0.5, 1)
+    scale = torch.ldexp(torch.ones_like(largest), (power - torch.where(part <= 0.875, 9, 8)).clamp(min=-100))
+    return (x / scale[..., None, None]).clamp(-448, 448).to(torch.float8_e4m3fn), scale
+
+
+def _plain_append(state):
+    hold, lengths = state["cache"], state["lengths"]
+    b, h, t, d = state["k"].shape
+    kind = state["case"]["kind"]
+    count = torch.full_like(lengths, t) if state["counts"] is None else state["counts"]
+    new = lengths + count
+    blocks = hold["k"].shape[2]
+    # of the blocks that something was written to, at most so many
+    most = min(blocks, (t + BLOCK - 1) // BLOCK + 1)
+    first = lengths.long() // BLOCK
+    block = first[:, None] + torch.arange(most, device="cuda")                       # [b,most]
+    token = block[..., None] * BLOCK + torch.arange(BLOCK, device="cuda")            # [b,most,64]
+    fresh = token >= lengths[:, None, None]
+    index = (token - lengths[:, None, None]).clamp(0, t - 1).flatten(1)
+    if state["path"] is not None:
+        index = state["path"].long().gather(1, index)
+    ended = (block + 1) * BLOCK <= new[:, None]
+    # the tail's rows have the newest token that belongs there
+    row = torch.arange(TAIL, device="cuda")
+    newest = (new.long()[:, None] - 1 - row) // TAIL * TAIL + row                    # the last token of this row
+    written = newest >= lengths[:, None]
+    source = (newest - lengths[:, None]).clamp(0, t - 1)
+    if state["path"] is not None:
+        source = state["path"].long().gather(1, source)
+    place = block.clamp(max=blocks - 1)
+    ended = ended & (block < blocks)
+    for x, name in ((state["k"], "k"), (state["v"], "v")):
+        tail = hold[name + "_tail"]
+        old = tail.gather(2, (token % TAIL).flatten(1)[:, None, :, None].expand(-1, h, -1, d))
+        got = x.gather(2, index[:, None, :, None].expand(-1, h, -1, d))
+        rows = torch.where(fresh.flatten(1)[:, None, :, None], got, old).view(b, h, most, BLOCK, d)
+        codes, scale = _codes(rows, kind, torch.float64)
+        if name == "v":
+            codes = codes.transpose(-1, -2)
+        room = torch.zeros((b, h, most, *hold[name].shape[-2:]), dtype=codes.dtype, device="cuda")
+        room[..., :codes.shape[-2], :codes.shape[-1]] = codes
+        # (bytes are gathered and scattered: indexing has no 8-bit floats)
+        to = place[:, None, :].expand(-1, h, -1)
+        held, bytes_ = hold[name].view(torch.uint8).flatten(3), room.view(torch.uint8).flatten(3)
+        wide = to[..., None].expand(-1, -1, -1, held.shape[-1])
+        keep = ended[:, None, :, None]
+        # a block that is not complete puts back what is there; the places behind the last block are its own again
+        spare = torch.cat((held, held[:, :, :1]), 2)
+        spare.scatter_(2, torch.where(keep, wide, blocks), bytes_)
+        held.copy_(spare[:, :, :blocks])
+        scales = torch.cat((hold[name + "_scale"], hold[name + "_scale"][:, :, :1]), 2)
+        scales.scatter_(2, torch.where(ended[:, None, :], to, blocks), scale)
+        hold[name + "_scale"].copy_(scales[:, :, :blocks])
+        late = x.gather(2, source[:, None, :, None].expand(-1, h, -1, d))
+        tail.copy_(torch.where(written[:, None, :, None], late, tail))
+    return (*hold.values(), new)
+
+
+def _plain_rows(hold, name, lengths, n):
+    """fp32 [b,h,n,d]: the cached rows, those of the block that is not complete from the tail."""
+    tail = hold[name + "_tail"]
+    b, h, _, d = tail.shape
+    codes = hold[name].transpose(-1, -2) if name == "v" else hold[name]
+    rows = (codes[..., :d].float() * hold[name + "_scale"][..., None, None]).reshape(b, h, -1, d)[:, :, :n]
+    at = torch.arange(n, device="cuda")
+    late = tail.float().index_select(2, at % TAIL)
+    return torch.where((at >= lengths[:, None] // BLOCK * BLOCK)[:, None, :, None], late, rows)
+
+
+def _plain_attention(state):
+    q, lengths, case = state["q"], state["lengths"], state["case"]
+    b, hq, t, d = q.shape
+    hc, n = case["cache_heads"], case["n"]
+    x = (q.float() / math.sqrt(d)).view(b, hc, hq // hc * t, d)
+    seen = torch.arange(n, device="cuda") < lengths[:, None, None, None]
+    k, v = (_plain_rows(state["cache"], name, lengths, n) for name in ("k", "v"))
+    s = torch.matmul(x, k.transpose(-1, -2)).masked_fill_(~seen, -math.inf).view(b, hq, t, n)
+    if state["mask"] is not None:
+        e = torch.matmul(x, state["k_new"].float().transpose(-1, -2)).view(b, hq, t, t).masked_fill_(~state["mask"][:, None], -math.inf)
+        s = torch.cat((s, e), -1)
+        v = torch.cat((torch.where(seen[..., 0, :, None], v, torch.zeros_like(v)), state["v_new"].float()), 2)
+    top = s.amax(-1, keepdim=True)
+    s = s.sub_(torch.where(top == -math.inf, torch.zeros_like(top), top)).exp_()
+    total = s.sum(-1, keepdim=True)
+    out = torch.matmul(s.view(b, hc, hq // hc * t, -1), v).view(b, hq, t, d)
+    out = torch.where(total > 0, out / total, torch.zeros_like(out))
+    return out.to(q.dtype), (top + torch.log(total))[..., 0]
+
+
+def _plain_verify(state):
+    q, parents, tokens = state["target"].double(), state["parents"].long(), state["tokens"].long()
+    b, s, vocab = q.shape
+    at = torch.arange(s, device="cuda")
+    up = parents.clamp(min=0)
+    drafted = at > 0
+    # rank of a node among its parent's children, and how many of them there are
+    siblings = (parents[:, :, None] == parents[:, None, :]) & drafted[:, None] & drafted
+    rank = (siblings & (at[:, None] > at)).sum(-1)
+    children = torch.zeros_like(parents).scatter_add_(1, up, drafted.long().expand(b, -1))
+    q_at = q.flatten(1).gather(1, up * vocab + tokens)
+    u = state["uniforms"].double()
+    ranks = state["case"]["children"]
+    if state["draft"] is not None:
+        p = state["draft"].double()
+        p_at = p.flatten(1).gather(1, up * vocab + tokens)
+        cut, mass, cuts, masses = torch.zeros_like(u), torch.ones_like(u), [], []
+        for _ in range(ranks):   # what is left of every distribution behind that many refused children
+            cuts.append(cut)
+            masses.append(mass)
+            cut = cut + mass
+            mass = (q - cut[..., None] * p).clamp_(min=0).sum(-1)
+        cuts = torch.stack((*cuts, cut), -1)
+        mine = up * (ranks + 1) + rank
+        left = (q_at - cuts.flatten(1).gather(1, mine) * p_at).clamp(min=0)
+        taken = u * p_at * torch.stack((*masses, mass), -1).flatten(1).gather(1, mine) < left
+    else:
+        again = (siblings & (at[:, None] > at) & (tokens[:, :, None] == tokens[:, None, :])).any(-1)
+        own_mass = torch.where(again, torch.zeros_like(q_at), q_at)
+        before = (siblings & (at[:, None] > at)).double()
+        left = own_mass
+        taken = u * (1 - torch.matmul(before, own_mass[..., None])[..., 0]) < left
+    taken = taken & drafted
+    # of a node's children the first that is accepted; of those the ones whose ancestors were too
+    chosen = taken & ~((siblings & (at[:, None] > at)) & taken[:, None, :]).any(-1)
+    chosen = chosen | (at == 0)
+    on_path = (~state["mask"] | chosen[:, None, :]).all(-1)
+    order = torch.where(on_path, at, s).sort(-1).values
+    path = torch.where(order < s, order, -1).to(torch.int32)
+    counts = on_path.sum(-1)
+    end = path.long().gather(1, (counts - 1)[:, None])
+    row = q.gather(1, end[..., None].expand(-1, -1, vocab))[:, 0]
+    if state["draft"] is not None:
+        cut = cuts.flatten(1).gather(1, end * (ranks + 1) + children.gather(1, end))
+        row = (row - cut * p.gather(1, end[..., None].expand(-1, -1, vocab))[:, 0]).clamp(min=0)
+    else:
+        refused = (parents == end) & drafted
+        row = torch.cat((row, row[:, :1]), -1).scatter(1, torch.where(refused, tokens, vocab), 0.0)[:, :vocab]
+    sums = row.cumsum(-1)
+    token = (sums > u[:, :1] * sums[:, -1:]).to(torch.uint8).argmax(-1)
+    return path, counts.to(torch.int32), token.to(torch.int32)
+
+
+def run(state):
+    op = state["op"]
+    if own:
+        from lrqk_amd import ops
+        if op == "append":
+            new = ops.byte_append(state["cache"], state["k"], state["v"], state["lengths"], counts=state["counts"], path=state["path"])
+            return (*_buffers(state["cache"]).values(), new)
+        if op == "attention":
+            return ops.byte_attention(state["q"], state["cache"], state["lengths"], state["k_new"], state["v_new"], state["mask"],
+                                      return_lse=True)
+        return ops.verify_drafts(state["tokens"], state["target"], state["uniforms"], draft=state["draft"], parents=state["parents"])
+    return {"append": _plain_append, "attention": _plain_attention, "verify": _plain_verify}[op](state)
+
+
+# ------------------------------------------------------------------------------------------------------------ 64 bits
+
+def _exact_append(case, state):
+    hold = {k: v.double() for k, v in _buffers(state["cache"]).items()}
+    b, h, t, d = state["k"].shape
+    new = state["lengths"].clone()
+    for i in range(b):
+        n = int(state["lengths"][i])
+        m = t if state["counts"] is None else int(state["counts"][i])
+        new[i] = n + m
+        take = torch.arange(t, device="cuda") if state["path"] is None else state["path"][i].long()
+        for x, name in ((state["k"], "k"), (state["v"], "v")):
+            begin = n // BLOCK * BLOCK
+            kept = torch.arange(begin, n, device="cuda") % TAIL
+            rows = torch.cat((hold[name + "_tail"][i][:, kept], x[i][:, take[:m]].double()), 1)   # from token `begin`
+            for j in range(rows.shape[1] // BLOCK):
+                part = rows[:, BLOCK * j:BLOCK * (j + 1)]
+                top = part.abs().amax((1, 2))
+                if case["kind"] == "int8":
+                    scale = torch.clamp(top.float() / 127.0, min=2.0 ** -100)
+                    code = torch.round(part / scale.double()[:, None, None])
+                else:
+                    scale = 2.0 ** torch.clamp(torch.ceil(torch.log2(top / 448.0)), min=-100)
+                    # a step of 2^-3 of the power of two below the value, 2^-9 where that is smaller
+                    y = part / scale[:, None, None]
+                    step = 2.0 ** (torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3)
+                    code = torch.round(y / step) * step
+                hold[name + "_scale"][i, :, begin // BLOCK + j] = scale.double()
+                if name == "k":
+                    hold[name][i, :, begin // BLOCK + j, :, :d] = code
+                else:
+                    hold[name][i, :, begin // BLOCK + j, :d] = code.transpose(1, 2)
+            last = torch.arange(max(n, n + m - TAIL), n + m, device="cuda")
+            hold[name + "_tail"][i][:, last % TAIL] = x[i][:, take[last - n]].double()
+    return (*hold.values(), new)
+
+
+def _exact_attention(case, state):
+    b, hq, t, d = state["q"].shape
+    out = torch.zeros((b, hq, t, d), dtype=torch.float64, device="cuda")
+    lse = torch.full((b, hq, t), -math.inf, dtype=torch.float64, device="cuda")
+    group, hold = hq // case["cache_heads"], _buffers(state["cache"])
+    for i in range(b):
+        n = int(state["lengths"][i])
+        whole = n // BLOCK
+        late = torch.arange(whole * BLOCK, n, device="cuda") % TAIL
+        for h in range(hq):
+            c = h // group
+            k = hold["k"][i, c, :whole, :, :d].double() * hold["k_scale"][i, c, :whole, None, None].double()
+            v = hold["v"][i, c, :whole, :d].double() * hold["v_scale"][i, c, :whole, None, None].double()
+            k = torch.cat((k.reshape(-1, d), hold["k_tail"][i, c][late].double()))
+            v = torch.cat((v.transpose(1, 2).reshape(-1, d), hold["v_tail"][i, c][late].double()))
+            if state["mask"] is not None:
+                k, v = torch.cat((k, state["k_new"][i, c].double())), torch.cat((v, state["v_new"][i, c].double()))
+            s = state["q"][i, h].double() @ k.T * d ** -0.5
+            if state["mask"] is not None:
+                s[:, n:][~state["mask"][i]] = -math.inf
+            lse[i, h] = torch.logsumexp(s, -1)
+            out[i, h] = torch.softmax(s, -1) @ v
+    return out, lse
+
+
+def _exact_verify(case, state):
+    b, s, vocab = state["target"].shape
+    tokens, parents = state["tokens"].tolist(), state["parents"].tolist()
+    path = torch.full((b, s), -1, dtype=torch.int32)
+    counts, following = torch.zeros(b, dtype=torch.int32), torch.zeros(b, dtype=torch.int32)
+    for i in range(b):
+        u = state["uniforms"][i].double().tolist()
+        at, count = 0, 0
+        while True:
+            path[i, count] = at
+            count += 1
+            left, mass, accepted = state["target"][i, at].double(), 1.0, None
+            for c in (c for c in range(1, s) if parents[i][c] == at):
+                x = tokens[i][c]
+                p = torch.zeros(vocab, dtype=torch.float64, device="cuda")
+                if state["draft"] is None:
+                    p[x] = 1.0
+                else:
+                    p = state["draft"][i, at].double()
+                if u[c] * float(p[x]) * mass < float(left[x]):
+                    accepted = c
+                    break
+                if state["draft"] is None:
+                    mass -= float(left[x])
+                    left = left.clone()
+                    left[x] = 0.0
+                else:
+                    left = (left - mass * p).clamp(min=0)
+                    mass = float(left.sum())
+            if accepted is None:
+                break
+            at = accepted
+        counts[i] = count
+        sums = left.cumsum(0)
+        following[i] = int(torch.nonzero(sums > u[0] * sums[-1])[0])
+    return path, counts, following
+
+
+def exact(case, seed):
+    """What run() returns for these inputs, in 64 bits."""
+    return {"append": _exact_append, "attention": _exact_attention, "verify": _exact_verify}[case["op"]](case, prepare(case, seed))
+
+
+# --------------------------------------------------------------------------------------------------------------- work
+
+def work(case):
+    e = 4 if case["dtype"] == "fp32" else 2
+    b, op = case["batch"], case["op"]
+    if op == "verify":   # the probabilities of the drafts, and the rows behind the last accepted one
+        rows, vocab, s = (2 if case["drafted"] else 1), case["vocab"], case["s"]
+        return {"bytes": b * (rows * (vocab + s) * e + 16 * s), "flops": 3.0 * b * vocab}
+    d, t, n = case["head_dim"], case["t"], case["n"]
+    if op == "append":
+        elements = 2.0 * b * case["heads"] * d
+        if n == 0:   # read once; complete blocks coded, the last two kept
+            whole = t // BLOCK * BLOCK
+            return {"bytes": elements * (t * e + whole + min(t, TAIL) * e), "flops": 3.0 * elements * whole}
+        count = (t + 1) / 2   # (of the drafts about half) read and kept, coded in the end
+        return {"bytes": elements * count * (3 * e + 1), "flops": 3.0 * elements * count}
+    hq, hc = case["heads"], case["cache_heads"]
+    m = n * (1 + (b - 1) * 9 / 16) / b if case["ragged"] else n   # (of sequences of different lengths the mean)
+    new = t if case["tree"] else 0
+    return {"bytes": b * (2 * hc * m * (d + 4 / BLOCK) + 2 * hc * (new + BLOCK / 2) * d * e + 2 * hq * t * d * e + 4 * hq * t + new * t),
+            "flops": 4.0 * b * hq * t * (m + new) * d}
