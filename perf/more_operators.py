@@ -227,10 +227,12 @@ def _codes(x, kind, bits):
     x = torch.where(torch.isnan(x), torch.zeros_like(x), x)
     largest = torch.where(torch.isinf(x), torch.zeros_like(x), x).abs().amax((-1, -2))
     if kind == "int8":
-        scale = (largest / 127.0).clamp(min=2.0 ** -100)
+        scale = (largest.double() / 127.0).float().clamp(min=2.0 ** -100)   # (in 32 bits torch would multiply with 1 / 127)
         return torch.round(x.to(bits) / scale.to(bits)[..., None, None]).clamp(-127, 127).to(torch.int8), scale
     part, power = torch.frexp(largest)   # part in [0.5, 1)
-    scale = torch.ldexp(torch.ones_like(largest), (power - torch.where(part <= 0.875, 9, 8)).clamp(min=-100))
+    # (its bits: a power that torch forms need not be exact)
+    power = torch.where(largest > 0, power - torch.where(part <= 0.875, 9, 8), -100).clamp(min=-100)
+    scale = (power + 127 << 23).to(torch.int32).view(torch.float32)
     return (x / scale[..., None, None]).clamp(-448, 448).to(torch.float8_e4m3fn), scale
 
 
@@ -404,14 +406,18 @@ def _exact_append(case, state):
                 part = rows[:, BLOCK * j:BLOCK * (j + 1)]
                 top = part.abs().amax((1, 2))
                 if case["kind"] == "int8":
-                    scale = torch.clamp(top.float() / 127.0, min=2.0 ** -100)
+                    scale = torch.clamp((top / 127.0).float(), min=2.0 ** -100)
                     code = torch.round(part / scale.double()[:, None, None])
                 else:
-                    scale = 2.0 ** torch.clamp(torch.ceil(torch.log2(top / 448.0)), min=-100)
+                    scale = torch.tensor([2.0 ** max(-100, math.ceil(math.log2(x / 448.0))) if x else 2.0 ** -100 for x in top.tolist()],
+                                         dtype=torch.float64, device="cuda")
                     # a step of 2^-3 of the power of two below the value, 2^-9 where that is smaller
                     y = part / scale[:, None, None]
-                    step = 2.0 ** (torch.floor(torch.log2(y.abs().clamp(min=2.0 ** -6))) - 3)
-                    code = torch.round(y / step) * step
+                    code = torch.zeros_like(y)
+                    for power in range(-6, 9):
+                        step = 2.0 ** (power - 3)
+                        here = (y.abs() >= 2.0 ** power) if power > -6 else torch.ones_like(y, dtype=torch.bool)
+                        code = torch.where(here, torch.round(y / step) * step, code)
                 hold[name + "_scale"][i, :, begin // BLOCK + j] = scale.double()
                 if name == "k":
                     hold[name][i, :, begin // BLOCK + j, :, :d] = code
