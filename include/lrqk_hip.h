@@ -326,6 +326,56 @@ int lrqk_evict(float* weights, int32_t* ids, void* k, void* v, const int32_t* le
                int32_t* ids_out, void* k_out, void* v_out, int cap_out, int32_t* new_lengths, int b, int heads, int d, int budget,
                int recent, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
 
+/* No counterpart in the reference.  A cache of keys and values in 8 bits: per sequence and head `blocks` blocks of 64 tokens, the
+ * keys of a block as k [b][heads][blocks][64][w], the values transposed as v [b][heads][blocks][w][64] (w: d rounded up to 64, 128 or
+ * 256; elements d .. of both are 0 and stay so), a scale of each, k_scale, v_scale [b][heads][blocks]: an element is code * scale.
+ * Codes are whole numbers (LRQK_CODE_INT8) or e4m3 numbers (LRQK_CODE_FP8).  k_tail, v_tail [b][heads][128][d], in `dtype`, hold the
+ * last 128 tokens of a sequence as they came, token p in row p % 128; tokens of a block that is not complete are read there.
+ *
+ * lrqk_byte_append puts tokens behind the lengths[sequence] that a sequence has (int32 [b], device, not changed):
+ * counts[sequence] of them (all `most` where NULL; at most that, and what there is room for), the rows path[sequence][0], path[sequence][1] ..
+ * of k_new, v_new [b][heads][t][d] (rows 0, 1 .. where NULL: then most <= t; ids outside 0 .. t - 1 count as the nearest), and the new lengths into
+ * new_lengths.  strides (host): elements between sequences, heads and rows of k_new and v_new, three each, multiples of 16
+ * bytes; rows are contiguous.  A block is coded when its last token arrives, from its 64 rows: scale = amax / 127 (int8), or the
+ * smallest power of two with amax / scale <= 448 (fp8), at least 2^-100, amax over its finite elements; code = element / scale
+ * rounded once to the nearest code, half to even; an infinity becomes the largest code, a NaN 0.  Blocks that are not complete
+ * behind the call, and rows of the tail that no token of it belongs to, are left as they were.
+ *
+ * lrqk_byte_attention: q [b][hq][t][d]; query head h attends to the cached tokens, all lengths[sequence] of them, of cache head
+ * h / (hq / hc), and to the drafted tokens j, k_new, v_new [b][hn][t][d] of head h / (hq / hn), with mask[i][j] != 0 (u8 [t][t],
+ * sequences mask_batch_stride apart, 0: one for all); k_new, v_new and mask NULL: to the cached ones alone.  out [b][hq][t][d], lse
+ * (or NULL) as lrqk_tree_attention leaves them, also for masked drafted tokens that are not finite and for queries that see
+ * nothing.  Scores of bf16 queries come from their elements as they are (those below 2^-28 of a query's largest lose bits); what
+ * probabilities are multiplied with codes in has 11 bits (bf16 tensors) or 22 (fp32), and 16 or 24 for the tail and the drafted.  Limits: as
+ * lrqk_tree_attention, blocks up to 2^24.  Workspace as above. */
+enum { LRQK_CODE_INT8 = 0, LRQK_CODE_FP8 = 1 };
+int lrqk_byte_append(const void* k_new, const void* v_new, const int64_t* strides, int t, int most, const int32_t* lengths,
+                     const int32_t* counts, const int32_t* path, int64_t path_stride, int32_t* new_lengths, void* k, void* v, float* k_scale, float* v_scale,
+                     void* k_tail, void* v_tail, int64_t blocks, int b, int heads, int d, int kind, int dtype, void* stream);
+int64_t lrqk_byte_attention_workspace(int b, int hq, int hc, int t, int64_t blocks, int d, int dtype);
+int lrqk_byte_attention(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale, const void* k_tail,
+                        const void* v_tail, int64_t blocks, const int32_t* lengths, const void* k_new, const void* v_new,
+                        const uint8_t* mask, int64_t mask_batch_stride, void* out, float* lse, int b, int hq, int hc, int hn, int t,
+                        int d, float scale, int kind, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
+/* No counterpart in the reference.  Drafted tokens verified against the target's probabilities, from given random numbers.
+ * tokens [b][s]: node 0 of a sequence's tree is certain, node i > 0 was drawn from row parents[i] of `draft`, the drafting model's
+ * probabilities (parents [b][s], or NULL: i - 1, a chain; a node whose parent is not one in front of it is never reached).  target
+ * [b][s][vocab]: row i is the distribution behind node i; draft [b][s - 1 or more][vocab], or NULL: the drafts have no probabilities
+ * (looked up, say).  Strides in elements between sequences and rows; rows are contiguous, fp32 or bf16 (dtype).  uniforms fp32
+ * [b][s], in [0, 1): [0] for the token that follows, [i] for node i's test.
+ * At a node with distribution r of mass Z (first: its row of target, 1) its children are looked at in order; child i with token x
+ * and p = draft[node][x] (1 without draft) is accepted if uniforms[i] p Z < r[x]; otherwise r becomes max(r - Z draft[node], 0)
+ * (without draft: r without x) and Z its sum.  path [b][s]: the accepted nodes, 0 first, -1 behind them; counts [b]: how many; next
+ * [b]: the lowest token x with r[0] + .. + r[x] > uniforms[0] (sum of r), r what is left at the last accepted node (its row of target
+ * if nothing is; -1 if that has nothing).  In fp64; what is not a positive number counts as 0, and a token outside the vocabulary
+ * as one that target and draft give 0.  Limits: s up to 1024, vocab up to 2^30.  Workspace as above. */
+int64_t lrqk_verify_drafts_workspace(int b, int s, int64_t vocab);
+int lrqk_verify_drafts(const int32_t* tokens, const int32_t* parents, const void* target, int64_t target_batch_stride,
+                       int64_t target_row_stride, const void* draft, int64_t draft_batch_stride, int64_t draft_row_stride,
+                       const float* uniforms, int32_t* path, int32_t* counts, int32_t* next, int b, int s, int64_t vocab,
+                       void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
 /* py:803-839 cast_lrqk_decode -> py:529-628 _lrqk_decode_inv_w1 + py:651-665 -- the per-step
  * factor update.  b_q,b_k: [bh][r][d] storage dtype, updated in place.  The active A_K rows
  * are gathered from a_k (heads of head_stride elements) at active_idx[bh][0..n) (py:1156-1171);

@@ -13,6 +13,7 @@ HEADER_PATH = os.path.join(os.path.dirname(_PKG), "include", "lrqk_hip.h")
 CSRC = os.path.join(_PKG, "csrc")
 
 F32, BF16 = 0, 1
+CODES = {"int8": 0, "fp8": 1}
 ROPE = {"plain": 0, "linear": 1, "ntk": 2, "llama3": 3, "yarn": 4}
 
 _lib = None
@@ -85,6 +86,12 @@ def _sig(lib):
         "lrqk_attention_weights": ([vp, vp, i64, i64, i64, i64, vp, vp, vp, vp, i32, i32, i32, i32, i32, f32, vp, i64, i32, vp], i32),
         "lrqk_evict_workspace": ([i32, i32, i32, i32], i64),
         "lrqk_evict": ([vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, vp, i64, i32, vp], i32),
+        "lrqk_byte_append": ([vp, vp, vp, i32, i32, vp, vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, i32, i32, vp], i32),
+        "lrqk_byte_attention_workspace": ([i32, i32, i32, i32, i64, i32, i32], i64),
+        "lrqk_byte_attention": ([vp, vp, vp, vp, vp, vp, vp, i64, vp, vp, vp, vp, i64, vp, vp, i32, i32, i32, i32, i32, i32, f32, i32,
+                                 vp, i64, i32, vp], i32),
+        "lrqk_verify_drafts_workspace": ([i32, i32, i64], i64),
+        "lrqk_verify_drafts": ([vp, vp, vp, i64, i64, vp, i64, i64, vp, vp, vp, vp, i32, i32, i64, vp, i64, i32, vp], i32),
         "lrqk_als_decode": ([vp, vp, vp, vp, i64, vp, i64, vp, i32, i32, vp, vp, i32, i32, i32, i32, i32, i32, f32,
                              vp, vp, i64, i32, vp], i32),
         "lrqk_als_prefill": ([vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i64, i32, i32, i32, f32, i32, vp], i32),

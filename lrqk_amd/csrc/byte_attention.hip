@@ -1,0 +1,492 @@
+// Attention over a cache held in 8 bits (byte_cache.hpp): the t tokens of a query head attend to the cached ones, all of them,
+// and to each other as a mask says,
+//
+//   out_i = sum_j p_ij v_j,  p_ij = exp(scale q_i.k_j - lse_i),  k_j = s_B c_j,  v_j = s'_B c'_j  for the tokens j of a block B.
+//
+// A block's scale leaves the sums: scores are (q_i.c_j) s_B, and o += s'_B (sum over the block of p_ij c'_j), one product an
+// element of o for 64 keys.  Codes are whole numbers up to 127 or e4m3 numbers, both exact in fp16, so fp16 products take
+// them, and probabilities of 11 bits where bf16 would have 8.  A query is scaled by a power of two to where fp16 holds it
+// (bf16 ones exactly but for elements 2^-28 of the largest; fp32 ones as the sum of two fp16 numbers, as their probabilities).
+// Probabilities are formed 2^8 too large, so that those of 2^-22 of the largest keep all bits and those of 2^-33 are not lost.
+//
+// As in tree_attention.hip a query is a lane's column of S^T = C Q^T, and the probabilities are the operand of O^T = C'^T P^T
+// as they lie: row m of the i-th 16 keys of a block is key 16 (m / 4) + 4 i + m % 4, so that a quad's scores are those of 16
+// successive keys, whose codes of an element of V are the 16 bytes that the same quad loads.  Nothing passes through LDS.
+// The tokens that are not in a complete block, and the drafted ones, make a split of their own in their own type.
+#include "byte_cache.hpp"
+#include "tree_parts.hpp"
+
+namespace lrqk {
+
+typedef _Float16 by_h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 by_h8 __attribute__((ext_vector_type(8)));
+typedef float by_f8 __attribute__((ext_vector_type(8)));
+
+constexpr float kByUp = 8.0f;          // binary orders that probabilities are formed too large
+constexpr float kByMuch = 32768.0f;    // a lane's probabilities of a tile may add up to this before the maximum is looked for
+constexpr int kByLong = 256;           // blocks of a split, at most
+
+struct ByteArgs {
+  TreeArgs tree;             // queries, drafted tokens, outputs, scratch; n: tokens that the cache has room for
+  const void *k, *v;         // codes
+  const float *ks, *vs;      // scales
+  const void *k_tail, *v_tail;
+  int blocks, drafts;        // of a head; drafted tokens: t or none
+};
+
+// Eight codes as fp16 numbers, exactly.
+template <bool FP8>
+__device__ __forceinline__ by_h8 by_unpack(uint32_t a, uint32_t b) {
+  union {
+    by_h8 all;
+    by_h2 two[4];
+  } x;
+  if constexpr (FP8) {
+    x.two[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false);
+    x.two[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true);
+    x.two[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false);
+    x.two[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true);
+  } else {
+    // 1024 + u is an fp16 number whose low byte is u, of u = code + 128
+    const by_h2 away = {(_Float16)1152.0f, (_Float16)1152.0f};
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    x.two[0] = __builtin_bit_cast(by_h2, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) - away;
+    x.two[1] = __builtin_bit_cast(by_h2, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) - away;
+    x.two[2] = __builtin_bit_cast(by_h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - away;
+    x.two[3] = __builtin_bit_cast(by_h2, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - away;
+  }
+  return x.all;
+}
+
+__device__ __forceinline__ ar_f4 by_step(by_h8 a, by_h8 b, ar_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// Eight numbers as fp16, and what that leaves of them.
+template <bool TWO>
+__device__ __forceinline__ void by_halves(const float (&x)[8], by_h8& hi, by_h8& lo) {
+  by_f8 v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = x[e];
+  hi = __builtin_convertvector(v, by_h8);
+  if constexpr (TWO) lo = __builtin_convertvector(v - __builtin_convertvector(hi, by_f8), by_h8);
+}
+
+// A tile's scores x become probabilities p = 2^(x f - top), and the running sums, as tree_softmax does; f: of each query.
+template <int MT, int NE, int VW>
+__device__ __forceinline__ void by_softmax(float (&x)[MT][NE], const float (&f)[MT], float (&top)[MT], float (&sum)[MT], ar_f4 (&o)[MT][VW]) {
+  float part[MT], p[MT][NE];
+  bool more = false;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+      p[m][e] = ar_exp2(fmaf(x[m][e], f[m], -top[m]));
+      part[m] = e == 0 ? p[m][0] : part[m] + p[m][e];
+    }
+    more = more | !(part[m] <= kByMuch);
+  }
+  if (__ballot(more)) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float high = x[m][0];
+#pragma unroll
+      for (int e = 1; e < NE; ++e) high = fmaxf(high, x[m][e]);
+      const float now = fmaxf(top[m], ar_quad_max(high) * f[m] - kByUp);
+      const float g = ar_exp2(top[m] - now);
+      top[m] = now;
+      sum[m] *= g;
+#pragma unroll
+      for (int j = 0; j < VW; ++j) o[m][j] *= g;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        p[m][e] = ar_exp2(fmaf(x[m][e], f[m], -now));
+        part[m] = e == 0 ? p[m][0] : part[m] + p[m][e];
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    sum[m] += part[m];
+#pragma unroll
+    for (int e = 0; e < NE; ++e) x[m][e] = p[m][e];
+  }
+}
+
+// How the sequences are cut into splits: the first one of a sequence has what is not in a complete block, the others so many
+// complete blocks each.  From the lengths alone, by every wave for itself.
+struct ByteCut {
+  int b, len, split, splits, slot0, per;
+  static __device__ __forceinline__ int length(const TreeArgs& a, int b) { return min(max(a.lengths[b], 0), a.n); }
+  static __device__ __forceinline__ int share(const TreeArgs& a, int all) {
+    return max(a.least, min((int)(((uint32_t)all + (uint32_t)a.splits - 1u) / (uint32_t)a.splits), a.most));
+  }
+  __device__ __forceinline__ bool find(const TreeArgs& a, int slot) {
+    if (a.b == 1) {
+      b = slot0 = 0;
+      len = length(a, 0);
+      per = share(a, len / kByBlock);
+      splits = 1 + (len / kByBlock + per - 1) / per;
+      split = slot;
+      return slot < splits;
+    }
+    const int lane = lane_id();
+    int all = 0;   // (blocks of all sequences: by_check holds them below 2^31)
+    for (int i = lane; i < a.b; i += kWave) all += length(a, i) / kByBlock;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) all += __shfl_xor(all, off, kWave);
+    per = __builtin_amdgcn_readfirstlane(share(a, all));
+    int before = 0;
+    for (int base = 0; base < a.b; base += kWave) {
+      const int i = base + lane;
+      const int mine = i < a.b ? 1 + (length(a, min(i, a.b - 1)) / kByBlock + per - 1) / per : 0;
+      const int end = before + wave_inclusive_sum(mine);
+      const unsigned long long hit = __ballot(slot < end);
+      if (hit) {
+        const int at = __ffsll(hit) - 1;
+        b = base + at;
+        splits = __builtin_amdgcn_readlane(mine, at);
+        slot0 = __builtin_amdgcn_readlane(end, at) - splits;
+        split = slot - slot0;
+        len = length(a, b);
+        return true;
+      }
+      before = __builtin_amdgcn_readlane(end, kWave - 1);
+    }
+    return false;
+  }
+};
+
+// The tokens that are not in a complete block (of the tail) and the drafted ones, tiles of them in turn over the four waves.
+template <typename T, int DP, int MT>
+__device__ __forceinline__ void by_dense(const ByteArgs& ba, const ByteCut& cut, int hc, int row0, int M, const T* q, const int (&ti)[MT],
+                                         float (&top)[MT], float (&sum)[MT], ar_f4 (&o)[MT][DP / 16], bool& odd) {
+  const TreeArgs& a = ba.tree;
+  using Tile = TreeTile<T, DP, MT>;
+  constexpr int NU = Tile::NU, KT = Tile::KT, NE = Tile::NE, STEPS = Tile::STEPS, VW = Tile::VW, E = (int)sizeof(T);
+  constexpr int VP = TreeV<T, VW>::DW >= 4 ? TreeV<T, VW>::DW / 4 : 1;
+  const int lane = lane_id(), col = lane & 15, quad = lane >> 4, pieces = a.d * E / 16;
+  const int late = cut.len % kByBlock, cached = (late + KT - 1) / KT, tiles = cached + (ba.drafts + KT - 1) / KT;
+  const int64_t tail0 = (((int64_t)cut.b * a.hc + hc) * kByTail + (cut.len - late) % kByTail) * a.d;
+  const int64_t new0 = ((int64_t)cut.b * a.hn + hc / (a.hc / a.hn)) * a.t * a.d;
+  const float f1 = a.scale_log2e;
+  float f[MT];
+  ar_u4 qf[MT][STEPS];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    f[m] = f1;
+    ar_row(q + (int64_t)min(row0 + 16 * m + col, M - 1) * a.d, quad, pieces, qf[m]);
+  }
+  uint32_t vplace[VP];
+#pragma unroll
+  for (int i = 0; i < VP; ++i) vplace[i] = TreeV<T, VW>::place(col, a.d, i);
+  const uint32_t rs = (uint32_t)a.d * E;
+  for (int tile = __builtin_amdgcn_readfirstlane(wave_id()); tile < tiles; tile += kTrWaves) {
+    const bool draft = tile >= cached;
+    const int first = (draft ? tile - cached : tile) * KT, valid = min(KT, (draft ? ba.drafts : late) - first);
+    const T* ks = (draft ? (const T*)a.k_new + new0 : (const T*)ba.k_tail + tail0) + (int64_t)first * a.d;
+    const T* vs = (draft ? (const T*)a.v_new + new0 : (const T*)ba.v_tail + tail0) + (int64_t)first * a.d;
+    TreeV<T, VW> v[NE];
+#pragma unroll
+    for (int e = 0; e < NE; ++e) v[e].load(vs, (uint32_t)min(quad * NE + e, valid - 1) * rs, vplace);
+    float x[MT][NE];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      ar_u4 kf[STEPS];
+      ar_row((const char*)ks + (uint32_t)min(col / 4 * NE + 4 * u + col % 4, valid - 1) * rs, quad, pieces, kf);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        ar_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < STEPS; ++c) s = ar_step<T>(kf[c], qf[m][c], s);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[m][4 * u + r] = s[r];
+      }
+    }
+    if (draft) {
+      tree_mask<MT, NE>(x, a, cut.b, ti, quad, valid, true, first);
+    } else {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < NE; ++e) x[m][e] = quad * NE + e < valid ? x[m][e] : -INFINITY;
+    }
+    by_softmax<MT, NE, VW>(x, f, top, sum, o);
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+#pragma unroll
+      for (int w = 0; w < TreeV<T, VW>::DW; ++w) {
+        v[e].w[w] = quad * NE + e < valid ? v[e].w[w] : 0u;   // (a row that stands for one beyond the end)
+        // queries that do not see a drafted token must not meet what its V holds: the joining launch adds that
+        if (draft) odd = tree_clean<T>(v[e].w[w]) | odd;
+      }
+    Tile::add(v, x, o);
+  }
+}
+
+template <typename T, bool FP8, int DP, int MT>
+__global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba) {
+  const TreeArgs& a = ba.tree;
+  constexpr int VW = DP / 16, CH = DP / 64, JC = 2, JB = kTrWaves * MT * JC * kWave;
+  constexpr bool TWO = sizeof(T) == 4;
+  constexpr int QN = TWO ? 2 : 1;
+  __shared__ ar_u4 smem[JB];
+  __shared__ float ml[kTrWaves][MT][16][2];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), col = lane & 15, quad = lane >> 4;
+  // the row blocks of a unit (a split of a head) follow each other 8 workgroups apart: on one XCD, whose L2 then has the
+  // codes that the first of them brought
+  const int rb = (int)blockIdx.x % (8 * a.row_blocks) / 8;
+  const int unit = (int)blockIdx.x / (8 * a.row_blocks) * 8 + (int)blockIdx.x % 8;
+  if (unit >= a.units) return;
+  ByteCut cut;
+  if (!cut.find(a, unit / a.hc)) return;
+  if (cut.split == 0 && unit % a.hc == 0 && rb == 0 && threadIdx.x == 0) {
+    a.cut[2 * cut.b] = cut.slot0;
+    a.cut[2 * cut.b + 1] = cut.splits;
+  }
+  const int hc = unit % a.hc, gc = a.hq / a.hc, M = gc * a.t, row0 = rb * 16 * MT;
+  const T* q = (const T*)a.q + ((int64_t)cut.b * a.hq + (int64_t)hc * gc) * a.t * a.d;
+  ar_f4 o[MT][VW] = {};
+  float top[MT], sum[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    top[m] = kTrNone;
+    sum[m] = 0.0f;
+  }
+  bool odd = false;
+  if (cut.split == 0) {
+    int ti[MT];   // drafted token of the lane's query
+#pragma unroll
+    for (int m = 0; m < MT; ++m) ti[m] = min(row0 + 16 * m + col, M - 1) % a.t;
+    by_dense<T, DP, MT>(ba, cut, hc, row0, M, q, ti, top, sum, o, odd);
+  } else {
+    const int64_t block0 = ((int64_t)cut.b * a.hc + hc) * ba.blocks;
+    int block = (cut.split - 1) * cut.per + wave;
+    const int end = min(cut.len / kByBlock, cut.split * cut.per);
+    // what a lane reads of a block: CH pieces of 16 keys, and VW pieces of V
+    const uint32_t kat = (uint32_t)((col >> 2) * 16 + (col & 3)) * DP + quad * 16, vat = (uint32_t)(VW * col) * kByBlock + quad * 16;
+    ar_u4 kg[4][CH], vg[VW];
+    float ks = 0.0f, vs = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
+    auto load_k = [&](int i) {
+      const char* src = (const char*)ba.k + (block0 + i) * (kByBlock * DP);
+      ks_next = ba.ks[block0 + i];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int c = 0; c < CH; ++c) kg[u][c] = tree_at<ar_u4>(src + u * 4 * DP + c * 64, kat);
+    };
+    auto load_v = [&](int i) {
+      const char* src = (const char*)ba.v + (block0 + i) * (kByBlock * DP);
+      vs_next = ba.vs[block0 + i];
+#pragma unroll
+      for (int j = 0; j < VW; ++j) vg[j] = tree_at<ar_u4>(src + j * kByBlock, vat);
+    };
+    if (block < end) {
+      load_k(block);
+      load_v(block);
+    }
+    // the queries, of elements 64 c + 16 quad + 8 h ..
+    by_h8 qh[MT][2 * CH], ql[QN == 2 ? MT : 1][2 * CH];
+    float up[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const T* row = q + (int64_t)min(row0 + 16 * m + col, M - 1) * a.d;
+      float x[2 * CH][8], high = 0.0f;
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          constexpr int N = Vec16<T>::N;
+#pragma unroll
+          for (int i = 0; i < 8 / N; ++i) {
+            const int e = 64 * c + 16 * quad + 8 * h + N * i;
+            Vec16<T> p;
+            p.load(row + min(e, a.d - N));
+            float y[N];
+            p.unpack(y);
+#pragma unroll
+            for (int r = 0; r < N; ++r) {
+              x[2 * c + h][N * i + r] = e < a.d ? y[r] : 0.0f;
+              high = fmaxf(high, fabsf(x[2 * c + h][N * i + r]));
+            }
+          }
+        }
+      // a power of two that brings the largest element to 2^14 .. 2^15
+      const uint32_t bits = __float_as_uint(fmaxf(ar_quad_max(high), 0x1p-100f)) & 0x7f800000u;   // 2^E
+      const float to = __uint_as_float(((127u + 14u + 127u) << 23) - bits);
+      up[m] = __uint_as_float(bits) * 0x1p-14f * a.scale_log2e;
+#pragma unroll
+      for (int s = 0; s < 2 * CH; ++s) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[s][e] *= to;
+        by_halves<TWO>(x[s], qh[m][s], ql[QN == 2 ? m : 0][s]);
+      }
+    }
+    for (; block < end; block += kTrWaves) {
+      const int next = block + kTrWaves < end ? block + kTrWaves : block;   // (the next one, or this one again)
+      ks = ks_next;
+      float x[MT][16], f[MT];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        by_h8 kf[2 * CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          kf[2 * c] = by_unpack<FP8>(kg[u][c][0], kg[u][c][1]);
+          kf[2 * c + 1] = by_unpack<FP8>(kg[u][c][2], kg[u][c][3]);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          ar_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int c = 0; c < 2 * CH; ++c) {
+            if constexpr (TWO) s = by_step(kf[c], ql[m][c], s);
+            s = by_step(kf[c], qh[m][c], s);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[m][4 * u + r] = s[r];
+        }
+      }
+      load_k(next);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) f[m] = up[m] * ks;
+      by_softmax<MT, 16, VW>(x, f, top, sum, o);
+      vs = vs_next;
+      by_h8 ph[MT][2], pl[QN == 2 ? MT : 1][2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = x[m][8 * h + e];
+          by_halves<TWO>(y, ph[m][h], pl[QN == 2 ? m : 0][h]);
+        }
+#pragma unroll
+      for (int j = 0; j < VW; ++j) {
+        const by_h8 v0 = by_unpack<FP8>(vg[j][0], vg[j][1]), v1 = by_unpack<FP8>(vg[j][2], vg[j][3]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          ar_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+          if constexpr (TWO) {
+            s = by_step(v0, pl[m][0], s);
+            s = by_step(v1, pl[m][1], s);
+          }
+          s = by_step(v0, ph[m][0], s);
+          s = by_step(v1, ph[m][1], s);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[m][j][r] = fmaf(s[r], vs, o[m][j][r]);
+        }
+      }
+      load_v(next);
+    }
+  }
+  tree_leave<MT, VW>(a, o, top, sum, odd, unit, rb, M, smem, ml);
+}
+
+struct BytePlan {
+  int dp, mt, rows, row_blocks, row_tiles, splits, least, most, units;
+  int64_t part, ml, odd, cut;   // words of 4 bytes
+};
+static BytePlan byte_plan(int b, int hq, int hc, int t, int64_t blocks, int d) {
+  BytePlan p;
+  p.dp = by_width(d);
+  const int64_t M = (int64_t)(hq / hc) * t;
+  p.mt = M <= 16 || p.dp == 256 ? 1 : 2;
+  p.rows = 16 * p.mt;
+  p.row_blocks = (int)((M + p.rows - 1) / p.rows);
+  p.row_tiles = p.row_blocks * p.mt;
+  p.splits = (int)std::max<int64_t>(b, 512 / ((int64_t)hc * p.row_blocks));
+  p.least = (int)std::max<int64_t>(kTrWaves, (blocks + kTrMaxSplits - 2) / (kTrMaxSplits - 1));
+  // (where the heads alone fill the GPU: sums of fp32 numbers over no more than kByLong blocks, in splits of one length)
+  const int64_t longest = std::max<int64_t>(p.least, kByLong), parts = (blocks + longest - 1) / longest;
+  p.most = parts ? (int)((blocks + parts - 1) / parts) : 1;
+  p.most = std::max(p.most, p.least);
+  const int64_t slots = b + std::min<int64_t>(std::max<int64_t>((int64_t)p.splits + b, b * parts), b * ((blocks + p.least - 1) / p.least));
+  p.units = (int)std::min<int64_t>(hc * slots, INT32_MAX);
+  const int64_t groups = (int64_t)p.units * p.row_tiles;
+  p.part = groups * 16 * p.dp;
+  p.ml = groups * 48;
+  p.odd = (int64_t)p.units * p.row_blocks;
+  p.cut = 2 * (int64_t)b;
+  return p;
+}
+
+template <typename T, bool FP8, int DP>
+static int byte_launch(const ByteArgs& a, const BytePlan& p, hipStream_t st) {
+  const dim3 grid((unsigned)(((int64_t)p.units + 7) / 8 * 8 * p.row_blocks));
+  if constexpr (DP < 256)
+    if (p.mt == 2) hipLaunchKernelGGL((byte_stream_kernel<T, FP8, DP, 2>), grid, dim3(kTrThreads), 0, st, a);
+  if (p.mt == 1) hipLaunchKernelGGL((byte_stream_kernel<T, FP8, DP, 1>), grid, dim3(kTrThreads), 0, st, a);
+  LRQK_HIP_CHECK(hipGetLastError());
+  tree_join_launch<T, DP, false>(a.tree, dim3((unsigned)((int64_t)a.tree.b * a.tree.hc * a.tree.row_tiles * 4)), st);
+  LRQK_HIP_CHECK(hipGetLastError());
+  return LRQK_OK;
+}
+template <typename T, bool FP8>
+static int byte_launch_dp(const ByteArgs& a, const BytePlan& p, hipStream_t st) {
+  if (p.dp == 64) return byte_launch<T, FP8, 64>(a, p, st);
+  if (p.dp == 128) return byte_launch<T, FP8, 128>(a, p, st);
+  return byte_launch<T, FP8, 256>(a, p, st);
+}
+
+static int byte_check(int b, int hq, int hc, int t, int64_t blocks, int d, int dtype) {
+  LRQK_REQUIRE(dtype == LRQK_F32 || dtype == LRQK_BF16, LRQK_EINVAL, "dtype=%d", dtype);
+  LRQK_REQUIRE(b > 0 && hq > 0 && hc > 0 && t > 0 && blocks > 0 && d > 0, LRQK_EINVAL, "bad sizes b=%d hq=%d hc=%d t=%d blocks=%lld d=%d", b,
+               hq, hc, t, (long long)blocks, d);
+  LRQK_REQUIRE(hq % hc == 0, LRQK_EINVAL, "%d query heads over %d cache heads", hq, hc);
+  LRQK_REQUIRE(d * (int)elem_size(dtype) % 16 == 0 && d <= 256, LRQK_ELIMIT,
+               "head_dim %d unsupported (rows of whole 16-byte pieces, at most 256 elements)", d);
+  LRQK_REQUIRE(t <= 1024 && blocks <= (1 << 24) && (int64_t)b * hq <= 65535 && b * blocks <= INT32_MAX, LRQK_ELIMIT,
+               "t=%d (at most 1024), blocks=%lld (2^24 a sequence, 2^31 in all), b * hq=%lld (65535)", t, (long long)blocks, (long long)b * hq);
+  return LRQK_OK;
+}
+
+}  // namespace lrqk
+
+using namespace lrqk;
+
+extern "C" int64_t lrqk_byte_attention_workspace(int b, int hq, int hc, int t, int64_t blocks, int d, int dtype) {
+  const int rc = byte_check(b, hq, hc, t, blocks, d, dtype);
+  if (rc) return rc;
+  const BytePlan p = byte_plan(b, hq, hc, t, blocks, d);
+  return (p.part + p.ml + p.odd + p.cut) * (int64_t)sizeof(float);
+}
+
+extern "C" int lrqk_byte_attention(const void* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
+                                   const void* k_tail, const void* v_tail, int64_t blocks, const int32_t* lengths, const void* k_new,
+                                   const void* v_new, const uint8_t* mask, int64_t mask_batch_stride, void* out, float* lse, int b,
+                                   int hq, int hc, int hn, int t, int d, float scale, int kind, void* workspace,
+                                   int64_t workspace_bytes, int dtype, void* stream) {
+  int rc = byte_check(b, hq, hc, t, blocks, d, dtype);
+  if (rc) return rc;
+  LRQK_REQUIRE(kind == LRQK_CODE_INT8 || kind == LRQK_CODE_FP8, LRQK_EINVAL, "kind=%d", kind);
+  LRQK_REQUIRE(q && k && v && k_scale && v_scale && k_tail && v_tail && lengths && out && workspace, LRQK_EINVAL, "null pointer");
+  LRQK_REQUIRE(!k_new == !v_new && !k_new == !mask, LRQK_EINVAL, "drafted keys, values and their mask come together");
+  LRQK_REQUIRE(!k_new || (hn > 0 && hc % hn == 0), LRQK_EINVAL, "%d cache heads over %d heads of drafted tokens", hc, hn);
+  LRQK_REQUIRE(scale > 0.0f && scale < INFINITY, LRQK_EINVAL, "scale=%g has to be positive and finite", (double)scale);
+  LRQK_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0 && (uintptr_t)k_tail % 16 == 0 &&
+                   (uintptr_t)v_tail % 16 == 0 && (uintptr_t)k_new % 16 == 0 && (uintptr_t)v_new % 16 == 0 && (uintptr_t)workspace % 16 == 0,
+               LRQK_EINVAL, "pointers must be 16-byte aligned");
+  const BytePlan p = byte_plan(b, hq, hc, t, blocks, d);
+  const int64_t need = (p.part + p.ml + p.odd + p.cut) * (int64_t)sizeof(float);
+  LRQK_REQUIRE(workspace_bytes >= need, LRQK_EINVAL, "workspace of %lld bytes: %lld are needed", (long long)workspace_bytes,
+               (long long)need);
+  LRQK_REQUIRE(((int64_t)p.units + 7) / 8 * 8 * p.row_blocks <= kMaxThreads / kTrThreads, LRQK_ELIMIT,
+               "%lld blocks of %d heads and %d tokens are more than a launch has places for", (long long)blocks, b * hc, t);
+  float* ws = (float*)workspace;
+  ByteArgs a{};
+  a.tree = TreeArgs{q, nullptr, nullptr, k_new, v_new, mask, lengths, out, lse, ws, ws + p.part, (int32_t*)ws + p.part + p.ml,
+                    (int32_t*)ws + p.part + p.ml + p.odd, 0, 0, 0, mask_batch_stride, b, (int)(blocks * kByBlock), hq, hc, k_new ? hn : hc, t, d,
+                    p.splits, p.least, p.most, p.row_blocks, p.rows, p.row_tiles, p.units, scale * kLog2e};
+  a.k = k;
+  a.v = v;
+  a.ks = k_scale;
+  a.vs = v_scale;
+  a.k_tail = k_tail;
+  a.v_tail = v_tail;
+  a.blocks = (int)blocks;
+  a.drafts = k_new ? t : 0;
+  hipStream_t st = (hipStream_t)stream;
+  const bool fp8 = kind == LRQK_CODE_FP8;
+  if (dtype == LRQK_F32) return fp8 ? byte_launch_dp<float, true>(a, p, st) : byte_launch_dp<float, false>(a, p, st);
+  return fp8 ? byte_launch_dp<bf16_t, true>(a, p, st) : byte_launch_dp<bf16_t, false>(a, p, st);
+}

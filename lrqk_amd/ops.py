@@ -928,6 +928,186 @@ def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Te
     return new
 
 
+class ByteCache:
+    """Keys and values of ``heads`` heads of ``batch`` sequences in 8 bits, room for ``capacity`` tokens (rounded up to whole blocks).
+
+    A block is 64 tokens of a head and has one scale for its keys and one for its values; an element is code * scale.  ``kind``:
+    "int8", whole numbers up to 127, or "fp8", e4m3 numbers up to 448 (elements of very different sizes keep their bits).
+    ``k`` [b,H,blocks,64,w] and ``v`` [b,H,blocks,w,64] hold the codes (w: head_dim rounded up to 64, 128 or 256; the rest is 0),
+    ``k_scale`` and ``v_scale`` fp32 [b,H,blocks]; ``k_tail`` and ``v_tail`` [b,H,128,d], in ``dtype`` (what queries and new tokens
+    come in), the last 128 tokens as they came, token p in row p % 128.  A block is coded once, when its last token arrives; until
+    then its tokens are read from the tail.  Lengths are the caller's (int32 [b] on the device), as of the other caches here."""
+
+    BLOCK, TAIL = 64, 128
+    _CODES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
+
+    def __init__(self, batch: int, heads: int, capacity: int, head_dim: int, dtype=torch.bfloat16, kind: str = "int8", device="cuda:0"):
+        if kind not in self._CODES:
+            raise ValueError(f"unknown kind {kind!r}: one of {sorted(self._CODES)}")
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"unsupported dtype {dtype}: the kernels store float32 or bfloat16")
+        step = 8 if dtype == torch.bfloat16 else 4
+        if min(batch, heads, capacity, head_dim) < 1 or head_dim > 256 or head_dim % step:
+            raise ValueError(f"batch={batch}, heads={heads}, capacity={capacity}, head_dim={head_dim}: at least 1 each, and rows of whole "
+                             "16-byte pieces, at most 256 elements")
+        blocks, w = -(-capacity // self.BLOCK), 64 if head_dim <= 64 else 128 if head_dim <= 128 else 256
+        if blocks > 2 ** 24:
+            raise ValueError(f"capacity={capacity}: at most 2^30 tokens")
+        self.kind, self.dtype, self.head_dim, self.capacity = kind, dtype, head_dim, blocks * self.BLOCK
+        k = torch.zeros((batch, heads, blocks, self.BLOCK, w), dtype=self._CODES[kind], device=device)
+        v = torch.zeros((batch, heads, blocks, w, self.BLOCK), dtype=self._CODES[kind], device=device)
+        scales = (torch.ones((batch, heads, blocks), device=device) for _ in range(2))
+        tails = (torch.zeros((batch, heads, self.TAIL, head_dim), dtype=dtype, device=device) for _ in range(2))
+        self._buffers = (k, v, *scales, *tails)   # (what the calls are given: made here and never others)
+        self._dev = k.get_device()
+        self._sizes = (batch, heads, blocks, head_dim)
+        self._places = tuple(x.data_ptr() for x in self._buffers)
+
+    k, v, k_scale, v_scale, k_tail, v_tail = (property(lambda self, i=i: self._buffers[i]) for i in range(6))
+
+    def _on(self, dev: int):
+        if dev != self._dev:
+            raise ValueError(f"the cache is on {self.k.device}, tensors on device {dev}")
+        return self._sizes
+
+
+def byte_append(cache: ByteCache, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor] = None,
+                path: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Writes tokens behind the ``lengths`` (int32 [b]) that the sequences of ``cache`` have, and returns the new lengths.
+
+    k, v [b,H,t,d]: any strides, rows contiguous.  ``counts`` int32 [b]: how many of them (all t if None; at most what there is room
+    for).  ``path`` int32 [b,m]: which rows, in order (0, 1, .. if None; counts up to m, ids outside the rows count as the nearest):
+    ``verify_drafts`` gives both.  ``lengths`` is not changed: appending again from it writes the same again as long as that is at most
+    64 tokens.  A block's codes: scale = amax / 127 (int8) or the smallest power of two with amax / scale <= 448 (fp8), of its
+    finite elements and at least 2^-100, code = element / scale rounded once, half to even; infinities get the largest code, NaN 0."""
+    dev = _on_one_gpu(k, v, lengths, counts, path)
+    b, h, blocks, d = cache._on(dev)
+    t = k.shape[2] if k.dim() == 4 else 0
+    if t >> 31:
+        _too_large(t)
+    dtype = cache.dtype
+    _expect("k", k, (b, h, t, d), dtype, contiguous=False)
+    _expect("v", v, (b, h, t, d), dtype, contiguous=False)
+    _expect("lengths", lengths, (b,), torch.int32)
+    if path is not None:
+        if path.dim() != 2 or path.shape[0] != b or path.dtype != torch.int32 or (path.shape[1] > 1 and path.stride(1) != 1):
+            raise ValueError(f"path is {tuple(path.shape)} {path.dtype}: int32 [{b},m] with contiguous rows is wanted")
+    most = t if path is None else path.shape[1]
+    if most >> 31:
+        _too_large(most)
+    if counts is not None:
+        _expect("counts", counts, (b,), torch.int32)
+    if t == 0 or most == 0:
+        return lengths.clone()
+    strides = (*_row_strides("k", k, b, h, t, d), *_row_strides("v", v, b, h, t, d))
+    if k.data_ptr() % 16 or v.data_ptr() % 16 or any(x * k.element_size() % 16 for x in strides):
+        k, v = _rows16(k), _rows16(v)
+        strides = (*_row_strides("k", k, b, h, t, d), *_row_strides("v", v, b, h, t, d))
+    new = torch.empty_like(lengths)
+    _launch(dev, _lib.load().lrqk_byte_append, k.data_ptr(), v.data_ptr(), struct.pack("6q", *strides), t, most, lengths.data_ptr(), _ptr(counts),
+            _ptr(path), path.stride(0) if path is not None and b > 1 else 0, new.data_ptr(), *cache._places, blocks, b, h, d, _lib.CODES[cache.kind], _dt(k))
+    return new
+
+
+def byte_attention(q: torch.Tensor, cache: ByteCache, lengths: torch.Tensor, k_new: Optional[torch.Tensor] = None,
+                   v_new: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                   return_lse: bool = False):
+    """``tree_attention`` over a cache held in 8 bits: q [b,Hq,t,d] attends to the first ``lengths`` (int32 [b] on the GPU) tokens of
+    the sequences of ``cache``, and to the drafted tokens k_new, v_new [b,Hn,t,d] as mask (bool or uint8 [t,t] or [b,t,t]: drafted token i
+    sees j) says; without these three to the cached ones alone.  Every number of heads is a multiple of the next: Hq, the
+    cache's, Hn.  ``scale`` (1 / sqrt(d) if None) is positive.  Codes are multiplied as they are, with probabilities of 11 bits (bf16
+    tensors) or 22 (float32); the tail's and the drafted tokens' rows with 16 or 24.  -> [b,Hq,t,d], zeros for a token that sees
+    nothing; with ``return_lse`` also fp32 [b,Hq,t], the logarithm of the sum of the exponentials (-inf for such a token)."""
+    dev = _on_one_gpu(q, lengths, k_new, v_new, mask)
+    cb, hc, blocks, cd = cache._on(dev)
+    b, hq, t, d = q.shape
+    if (b | hq | t | d) >> 31:
+        _too_large(b, hq, t, d)
+    dtype = cache.dtype
+    if (b, d) != (cb, cd) or q.dtype != dtype:
+        raise ValueError(f"q is {tuple(q.shape)} {q.dtype}: [{cb},Hq,t,{cd}] {dtype} is wanted")
+    if hq % hc:
+        raise ValueError(f"{hq} query heads over {hc} heads of the cache")
+    _expect("lengths", lengths, (b,), torch.int32)
+    hn = hc
+    if k_new is None or v_new is None or mask is None:
+        if not (k_new is None and v_new is None and mask is None):
+            raise ValueError("drafted keys, values and their mask come together")
+    else:
+        hn = k_new.shape[1]
+        _expect("k_new", k_new, (b, hn, t, d), dtype, contiguous=False)
+        _expect("v_new", v_new, (b, hn, t, d), dtype, contiguous=False)
+        if hn == 0 or hc % hn:
+            raise ValueError(f"{hc} heads of the cache, {hn} of the drafted tokens: a multiple")
+        if mask.shape not in ((b, t, t), (t, t)) or mask.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"mask is {tuple(mask.shape)} {mask.dtype}: bool or uint8 [t,t] or [b,t,t] is wanted")
+    q = _rows16(q)
+    out = torch.empty_like(q)
+    lse = torch.empty((b, hq, t), dtype=torch.float32, device=q.device) if return_lse else None
+    if b * hq * t:
+        each = 0
+        if k_new is not None:
+            k_new, v_new, mask = _rows16(k_new), _rows16(v_new), mask.contiguous()
+            each = t * t if mask.dim() == 3 else 0
+        dt = _dt(q)
+        need = _scratch_bytes("lrqk_byte_attention_workspace", b, hq, hc, t, blocks, d, dt)
+        ws = _scratch(need, q)
+        _launch(dev, _lib.load().lrqk_byte_attention, q.data_ptr(), *cache._places, blocks, lengths.data_ptr(), _ptr(k_new), _ptr(v_new), _ptr(mask), each,
+                out.data_ptr(), _ptr(lse), b, hq, hc, hn, t, d, d ** -0.5 if scale is None else float(scale), _lib.CODES[cache.kind],
+                ws.data_ptr(), need, dt)
+    return (out, lse) if return_lse else out
+
+
+def verify_drafts(tokens: torch.Tensor, target: torch.Tensor, uniforms: torch.Tensor, draft: Optional[torch.Tensor] = None,
+                  parents: Optional[torch.Tensor] = None):
+    """The accepted path of a tree of drafted tokens, and the token that follows it, from given random numbers: what is accepted and
+    drawn has the target's distribution.
+
+    tokens int32 [b,s]: node 0 of a sequence's tree is certain, node i was drawn from row parents[i] of ``draft``, every child of a
+    node for itself.  ``parents`` int32 [b,s]: a node in front of its children (None: a chain, i - 1; a node whose parent is not in
+    front of it is never reached).  target [b,s,V], row i the probabilities behind node i; draft [b,s,V] or [b,s-1,V], or None for
+    drafts without probabilities (looked up: equal ones among a node's children count once).  Both fp32 or bf16, rows contiguous.
+    ``uniforms`` fp32 [b,s], in [0,1): the first for the token that follows, the others for their nodes' tests.
+
+    At a node the children are looked at in order with what is left of its distribution, r of mass Z (first: its row of target,
+    1): token x is accepted if u draft[x] Z < r[x] (without draft: u Z < r[x]), else r becomes max(r - Z draft, 0) (r without
+    x).  The token that follows is the lowest x with r[0] + .. + r[x] > u sum(r) at the last accepted node (of its row of target
+    if nothing is left, -1 if that has nothing).  In fp64; what is not a positive number counts as 0, a token outside the
+    vocabulary as one of probability 0.
+    -> path int32 [b,s] (accepted nodes, 0 first, -1 behind them), counts int32 [b], the token that follows int32 [b]:
+    ``byte_append`` takes the first two as they are."""
+    dev = _on_one_gpu(target, tokens, uniforms, draft, parents)
+    b, s, vocab = target.shape
+    if (b | s | vocab) >> 31:
+        _too_large(b, s, vocab)
+    dt = _dt(target)
+    _expect("tokens", tokens, (b, s), torch.int32)
+    _expect("uniforms", uniforms, (b, s), torch.float32)
+    if parents is not None:
+        _expect("parents", parents, (b, s), torch.int32)
+    if vocab > 1 and target.stride(2) != 1:
+        raise ValueError("the rows of target must be contiguous")
+    draft_strides = (0, 0)
+    if draft is not None:
+        if draft.shape != (b, s, vocab) and draft.shape != (b, max(s - 1, 0), vocab) or draft.dtype != target.dtype:
+            raise ValueError(f"draft is {tuple(draft.shape)} {draft.dtype}: {(b, s, vocab)} or a row less, {target.dtype} is wanted")
+        if vocab > 1 and draft.stride(2) != 1:
+            raise ValueError("the rows of draft must be contiguous")
+        draft_strides = draft.stride()[:2]
+    path, counts, token = (torch.empty(shape, dtype=torch.int32, device=target.device) for shape in ((b, s), (b,), (b,)))
+    if b == 0:
+        return path, counts, token
+    if s == 0 or vocab == 0:
+        raise ValueError(f"{s} nodes over a vocabulary of {vocab}: at least 1 each")
+    need = _scratch_bytes("lrqk_verify_drafts_workspace", b, s, vocab)
+    ws = _scratch(need, target)
+    st = target.stride()
+    _launch(dev, _lib.load().lrqk_verify_drafts, tokens.data_ptr(), _ptr(parents), target.data_ptr(), st[0], st[1],
+            draft.data_ptr() if draft is not None and s > 1 else None, *draft_strides, uniforms.data_ptr(), path.data_ptr(),
+            counts.data_ptr(), token.data_ptr(), b, s, vocab, ws.data_ptr(), need, dt)
+    return path, counts, token
+
+
 def probe_bandwidth(nbytes: int, reps: int = 10, device="cuda:0"):
     """(read GB/s, copy GB/s of bytes read + bytes written) of plain streaming kernels over ``nbytes``."""
     src = torch.empty(nbytes, dtype=torch.uint8, device=device).fill_(1)
