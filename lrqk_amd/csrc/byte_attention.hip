@@ -71,16 +71,19 @@ __device__ __forceinline__ void by_halves(const float (&x)[8], by_h8& hi, by_h8&
   if constexpr (TWO) lo = __builtin_convertvector(v - __builtin_convertvector(hi, by_f8), by_h8);
 }
 
-// A tile's scores x become probabilities p = 2^(x f - top), and the running sums, as tree_softmax does; f: of each query.
+// A tile's scores x become probabilities p = 2^(x f + shift - top), in place, and the running sums, of 2^(x f - top), as
+// tree_softmax does; f: of each query, less = 2^-shift.
 template <int MT, int NE, int VW>
-__device__ __forceinline__ void by_softmax(float (&x)[MT][NE], const float (&f)[MT], float (&top)[MT], float (&sum)[MT], ar_f4 (&o)[MT][VW]) {
+__device__ __forceinline__ void by_softmax(float (&x)[MT][NE], const float (&f)[MT], float shift, float less, float (&top)[MT], float (&sum)[MT],
+                                           ar_f4 (&o)[MT][VW]) {
   float part[MT], p[MT][NE];
   bool more = false;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
+    const float from = shift - top[m];
 #pragma unroll
     for (int e = 0; e < NE; ++e) {
-      p[m][e] = ar_exp2(fmaf(x[m][e], f[m], -top[m]));
+      p[m][e] = ar_exp2(fmaf(x[m][e], f[m], from));
       part[m] = e == 0 ? p[m][0] : part[m] + p[m][e];
     }
     more = more | !(part[m] <= kByMuch);
@@ -91,26 +94,166 @@ __device__ __forceinline__ void by_softmax(float (&x)[MT][NE], const float (&f)[
       float high = x[m][0];
 #pragma unroll
       for (int e = 1; e < NE; ++e) high = fmaxf(high, x[m][e]);
-      const float now = fmaxf(top[m], ar_quad_max(high) * f[m] - kByUp);
-      const float g = ar_exp2(top[m] - now);
+      const float now = fmaxf(top[m], fmaf(ar_quad_max(high), f[m], shift - kByUp));
+      const float g = ar_exp2(top[m] - now), from = shift - now;
       top[m] = now;
       sum[m] *= g;
 #pragma unroll
       for (int j = 0; j < VW; ++j) o[m][j] *= g;
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
-        p[m][e] = ar_exp2(fmaf(x[m][e], f[m], -now));
+        p[m][e] = ar_exp2(fmaf(x[m][e], f[m], from));
         part[m] = e == 0 ? p[m][0] : part[m] + p[m][e];
       }
     }
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    sum[m] += part[m];
+    sum[m] = fmaf(part[m], less, sum[m]);
 #pragma unroll
     for (int e = 0; e < NE; ++e) x[m][e] = p[m][e];
   }
 }
+
+// What a wave has of its queries: 16 MT of them, scaled by powers of two into fp16 (up: back, and to the exponents' base), and
+// of their outputs.
+template <typename T, int DP, int MT>
+struct ByteWave {
+  static constexpr int VW = DP / 16, CH = DP / 64;
+  static constexpr bool TWO = sizeof(T) == 4;
+  by_h8 qh[MT][2 * CH], ql[TWO ? MT : 1][2 * CH];   // elements 64 c + 16 quad + 8 h .. in [2 c + h]
+  float up[MT], top[MT], sum[MT];
+  ar_f4 o[MT][VW];
+  // Of bf16 tensors outputs are held in units of the first block's scale and the products add to them as they are: the block's
+  // scale over that goes into the probabilities' exponents, as far as fp16 has room for it (2^8 either way; beyond, and of fp32
+  // tensors, whose sums the matrix cores must not cut off, a block's products are multiplied and added).
+  float unit, log_unit;
+
+  __device__ __forceinline__ void begin() {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      top[m] = kTrNone;
+      sum[m] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < VW; ++j) o[m][j] = ar_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    unit = 1.0f;
+  }
+  __device__ __forceinline__ void queries(const T* q, int row0, int M, int d, float scale_log2e) {
+    const int col = lane_id() & 15, quad = lane_id() >> 4;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const T* row = q + (int64_t)min(row0 + 16 * m + col, M - 1) * d;
+      float x[2 * CH][8], high = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 2 * CH; ++s) {
+        constexpr int N = Vec16<T>::N;
+#pragma unroll
+        for (int i = 0; i < 8 / N; ++i) {
+          const int e = 64 * (s / 2) + 16 * quad + 8 * (s % 2) + N * i;
+          Vec16<T> p;
+          p.load(row + min(e, d - N));
+          float y[N];
+          p.unpack(y);
+#pragma unroll
+          for (int r = 0; r < N; ++r) {
+            x[s][N * i + r] = e < d ? y[r] : 0.0f;
+            high = fmaxf(high, fabsf(x[s][N * i + r]));
+          }
+        }
+      }
+      // a power of two that brings the largest element to 2^14 .. 2^15
+      const uint32_t bits = __float_as_uint(fmaxf(ar_quad_max(high), 0x1p-100f)) & 0x7f800000u;   // 2^E
+      const float to = __uint_as_float(((127u + 14u + 127u) << 23) - bits);
+      up[m] = __uint_as_float(bits) * 0x1p-14f * scale_log2e;
+#pragma unroll
+      for (int s = 0; s < 2 * CH; ++s) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[s][e] *= to;
+        by_halves<TWO>(x[s], qh[m][s], ql[TWO ? m : 0][s]);
+      }
+    }
+  }
+  __device__ __forceinline__ void first(float vs) {
+    unit = TWO ? 1.0f : vs;
+    log_unit = TWO ? 0.0f : __builtin_amdgcn_logf(vs);
+  }
+  // A block: k(u, s) and v(j, h) are its operands; between: what is done once the keys are not wanted any more.
+  template <typename K, typename V, typename B>
+  __device__ __forceinline__ void block(float ks, float vs, K k, V v, B between) {
+    float x[MT][16], f[MT];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      by_h8 kf[2 * CH];
+#pragma unroll
+      for (int s = 0; s < 2 * CH; ++s) kf[s] = k(u, s);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        ar_f4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < 2 * CH; ++s) {
+          if constexpr (TWO) c = by_step(kf[s], ql[m][s], c);
+          c = by_step(kf[s], qh[m][s], c);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[m][4 * u + r] = c[r];
+      }
+    }
+    between();
+    const float shift = TWO ? 0.0f : __builtin_amdgcn_logf(vs) - log_unit;
+    const bool apart = TWO || !(fabsf(shift) <= 8.0f);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) f[m] = up[m] * ks;
+    by_softmax<MT, 16, VW>(x, f, apart ? 0.0f : shift, apart ? 1.0f : unit * __builtin_amdgcn_rcpf(vs), top, sum, o);
+    by_h8 ph[MT][2], pl[TWO ? MT : 1][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = x[m][8 * h + e];
+        by_halves<TWO>(y, ph[m][h], pl[TWO ? m : 0][h]);
+      }
+    if (TWO || __builtin_expect(apart, 0)) {
+      const float by = TWO ? vs : vs / unit;
+#pragma unroll
+      for (int j = 0; j < VW; ++j) {
+        const by_h8 v0 = v(j, 0), v1 = v(j, 1);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          ar_f4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+          if constexpr (TWO) {
+            c = by_step(v0, pl[m][0], c);
+            c = by_step(v1, pl[m][1], c);
+          }
+          c = by_step(v0, ph[m][0], c);
+          c = by_step(v1, ph[m][1], c);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[m][j][r] = fmaf(c[r], by, o[m][j][r]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VW; ++j) {
+        const by_h8 v0 = v(j, 0), v1 = v(j, 1);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          o[m][j] = by_step(v0, ph[m][0], o[m][j]);
+          o[m][j] = by_step(v1, ph[m][1], o[m][j]);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void end() {
+    if constexpr (!TWO) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < VW; ++j) o[m][j] *= unit;
+    }
+  }
+};
 
 // How the sequences are cut into splits: the first one of a sequence has what is not in a complete block, the others so many
 // complete blocks each.  From the lengths alone, by every wave for itself.
@@ -156,9 +299,9 @@ struct ByteCut {
   }
 };
 
-// The tokens that are not in a complete block (of the tail) and the drafted ones, tiles of them in turn over the four waves.
+// The tokens that are not in a complete block (of the tail) and the drafted ones: every `step`-th tile of them.
 template <typename T, int DP, int MT>
-__device__ __forceinline__ void by_dense(const ByteArgs& ba, const ByteCut& cut, int hc, int row0, int M, const T* q, const int (&ti)[MT],
+__device__ __forceinline__ void by_dense(const ByteArgs& ba, const ByteCut& cut, int hc, int row0, int M, const T* q, int from, int step,
                                          float (&top)[MT], float (&sum)[MT], ar_f4 (&o)[MT][DP / 16], bool& odd) {
   const TreeArgs& a = ba.tree;
   using Tile = TreeTile<T, DP, MT>;
@@ -170,17 +313,19 @@ __device__ __forceinline__ void by_dense(const ByteArgs& ba, const ByteCut& cut,
   const int64_t new0 = ((int64_t)cut.b * a.hn + hc / (a.hc / a.hn)) * a.t * a.d;
   const float f1 = a.scale_log2e;
   float f[MT];
+  int ti[MT];   // drafted token of the lane's query
   ar_u4 qf[MT][STEPS];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     f[m] = f1;
+    ti[m] = min(row0 + 16 * m + col, M - 1) % a.t;
     ar_row(q + (int64_t)min(row0 + 16 * m + col, M - 1) * a.d, quad, pieces, qf[m]);
   }
   uint32_t vplace[VP];
 #pragma unroll
   for (int i = 0; i < VP; ++i) vplace[i] = TreeV<T, VW>::place(col, a.d, i);
   const uint32_t rs = (uint32_t)a.d * E;
-  for (int tile = __builtin_amdgcn_readfirstlane(wave_id()); tile < tiles; tile += kTrWaves) {
+  for (int tile = from; tile < tiles; tile += step) {
     const bool draft = tile >= cached;
     const int first = (draft ? tile - cached : tile) * KT, valid = min(KT, (draft ? ba.drafts : late) - first);
     const T* ks = (draft ? (const T*)a.k_new + new0 : (const T*)ba.k_tail + tail0) + (int64_t)first * a.d;
@@ -210,7 +355,7 @@ __device__ __forceinline__ void by_dense(const ByteArgs& ba, const ByteCut& cut,
 #pragma unroll
         for (int e = 0; e < NE; ++e) x[m][e] = quad * NE + e < valid ? x[m][e] : -INFINITY;
     }
-    by_softmax<MT, NE, VW>(x, f, top, sum, o);
+    by_softmax<MT, NE, VW>(x, f, 0.0f, 1.0f, top, sum, o);
 #pragma unroll
     for (int e = 0; e < NE; ++e)
 #pragma unroll
@@ -223,52 +368,58 @@ __device__ __forceinline__ void by_dense(const ByteArgs& ba, const ByteCut& cut,
   }
 }
 
+// Where a workgroup is, and whose queries and keys it has.
+struct BytePlace {
+  int rb, unit, hc, M;
+  ByteCut cut;
+  __device__ __forceinline__ bool find(const TreeArgs& a) {   // false: nothing to do
+    // the row blocks of a unit (a split of a head) follow each other 8 workgroups apart: on one XCD, whose L2 then has the
+    // codes that the first of them brought
+    rb = (int)blockIdx.x % (8 * a.row_blocks) / 8;
+    unit = (int)blockIdx.x / (8 * a.row_blocks) * 8 + (int)blockIdx.x % 8;
+    if (unit >= a.units || !cut.find(a, unit / a.hc)) return false;
+    if (cut.split == 0 && unit % a.hc == 0 && rb == 0 && threadIdx.x == 0) {
+      a.cut[2 * cut.b] = cut.slot0;
+      a.cut[2 * cut.b + 1] = cut.splits;
+    }
+    hc = unit % a.hc;
+    M = a.hq / a.hc * a.t;
+    return true;
+  }
+};
+
+// Few queries: the four waves of a workgroup take the blocks of its split in turn, each for itself, its codes as operands from
+// memory.
 template <typename T, bool FP8, int DP, int MT>
 __global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba) {
   const TreeArgs& a = ba.tree;
-  constexpr int VW = DP / 16, CH = DP / 64, JC = 2, JB = kTrWaves * MT * JC * kWave;
-  constexpr bool TWO = sizeof(T) == 4;
-  constexpr int QN = TWO ? 2 : 1;
-  __shared__ ar_u4 smem[JB];
+  using Wave = ByteWave<T, DP, MT>;
+  constexpr int VW = Wave::VW, CH = Wave::CH;
+  __shared__ ar_u4 smem[kTrWaves * MT * 2 * kWave];
   __shared__ float ml[kTrWaves][MT][16][2];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), col = lane & 15, quad = lane >> 4;
-  // the row blocks of a unit (a split of a head) follow each other 8 workgroups apart: on one XCD, whose L2 then has the
-  // codes that the first of them brought
-  const int rb = (int)blockIdx.x % (8 * a.row_blocks) / 8;
-  const int unit = (int)blockIdx.x / (8 * a.row_blocks) * 8 + (int)blockIdx.x % 8;
-  if (unit >= a.units) return;
-  ByteCut cut;
-  if (!cut.find(a, unit / a.hc)) return;
-  if (cut.split == 0 && unit % a.hc == 0 && rb == 0 && threadIdx.x == 0) {
-    a.cut[2 * cut.b] = cut.slot0;
-    a.cut[2 * cut.b + 1] = cut.splits;
-  }
-  const int hc = unit % a.hc, gc = a.hq / a.hc, M = gc * a.t, row0 = rb * 16 * MT;
-  const T* q = (const T*)a.q + ((int64_t)cut.b * a.hq + (int64_t)hc * gc) * a.t * a.d;
-  ar_f4 o[MT][VW] = {};
-  float top[MT], sum[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    top[m] = kTrNone;
-    sum[m] = 0.0f;
-  }
+  BytePlace at;
+  if (!at.find(a)) return;
+  const ByteCut& cut = at.cut;
+  const int row0 = at.rb * 16 * MT;
+  const T* q = (const T*)a.q + ((int64_t)cut.b * a.hc + at.hc) * at.M * a.d;
+  Wave w;
+  w.begin();
   bool odd = false;
   if (cut.split == 0) {
-    int ti[MT];   // drafted token of the lane's query
-#pragma unroll
-    for (int m = 0; m < MT; ++m) ti[m] = min(row0 + 16 * m + col, M - 1) % a.t;
-    by_dense<T, DP, MT>(ba, cut, hc, row0, M, q, ti, top, sum, o, odd);
+    by_dense<T, DP, MT>(ba, cut, at.hc, row0, at.M, q, wave, kTrWaves, w.top, w.sum, w.o, odd);
   } else {
-    const int64_t block0 = ((int64_t)cut.b * a.hc + hc) * ba.blocks;
+    const int64_t block0 = ((int64_t)cut.b * a.hc + at.hc) * ba.blocks;
     int block = (cut.split - 1) * cut.per + wave;
     const int end = min(cut.len / kByBlock, cut.split * cut.per);
-    // what a lane reads of a block: CH pieces of 16 keys, and VW pieces of V
+    // what a lane reads of a block: CH pieces of 4 x 16 keys, and VW pieces of V
     const uint32_t kat = (uint32_t)((col >> 2) * 16 + (col & 3)) * DP + quad * 16, vat = (uint32_t)(VW * col) * kByBlock + quad * 16;
     ar_u4 kg[4][CH], vg[VW];
-    float ks = 0.0f, vs = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
+    float ks, vs, ks_next = 0.0f, vs_next = 0.0f;
     auto load_k = [&](int i) {
       const char* src = (const char*)ba.k + (block0 + i) * (kByBlock * DP);
       ks_next = ba.ks[block0 + i];
+      vs_next = ba.vs[block0 + i];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -276,125 +427,121 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba)
     };
     auto load_v = [&](int i) {
       const char* src = (const char*)ba.v + (block0 + i) * (kByBlock * DP);
-      vs_next = ba.vs[block0 + i];
 #pragma unroll
       for (int j = 0; j < VW; ++j) vg[j] = tree_at<ar_u4>(src + j * kByBlock, vat);
     };
     if (block < end) {
       load_k(block);
       load_v(block);
-    }
-    // the queries, of elements 64 c + 16 quad + 8 h ..
-    by_h8 qh[MT][2 * CH], ql[QN == 2 ? MT : 1][2 * CH];
-    float up[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const T* row = q + (int64_t)min(row0 + 16 * m + col, M - 1) * a.d;
-      float x[2 * CH][8], high = 0.0f;
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          constexpr int N = Vec16<T>::N;
-#pragma unroll
-          for (int i = 0; i < 8 / N; ++i) {
-            const int e = 64 * c + 16 * quad + 8 * h + N * i;
-            Vec16<T> p;
-            p.load(row + min(e, a.d - N));
-            float y[N];
-            p.unpack(y);
-#pragma unroll
-            for (int r = 0; r < N; ++r) {
-              x[2 * c + h][N * i + r] = e < a.d ? y[r] : 0.0f;
-              high = fmaxf(high, fabsf(x[2 * c + h][N * i + r]));
-            }
-          }
-        }
-      // a power of two that brings the largest element to 2^14 .. 2^15
-      const uint32_t bits = __float_as_uint(fmaxf(ar_quad_max(high), 0x1p-100f)) & 0x7f800000u;   // 2^E
-      const float to = __uint_as_float(((127u + 14u + 127u) << 23) - bits);
-      up[m] = __uint_as_float(bits) * 0x1p-14f * a.scale_log2e;
-#pragma unroll
-      for (int s = 0; s < 2 * CH; ++s) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[s][e] *= to;
-        by_halves<TWO>(x[s], qh[m][s], ql[QN == 2 ? m : 0][s]);
-      }
+      w.queries(q, row0, at.M, a.d, a.scale_log2e);
+      w.first(vs_next);
     }
     for (; block < end; block += kTrWaves) {
       const int next = block + kTrWaves < end ? block + kTrWaves : block;   // (the next one, or this one again)
       ks = ks_next;
-      float x[MT][16], f[MT];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        by_h8 kf[2 * CH];
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-          kf[2 * c] = by_unpack<FP8>(kg[u][c][0], kg[u][c][1]);
-          kf[2 * c + 1] = by_unpack<FP8>(kg[u][c][2], kg[u][c][3]);
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          ar_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int c = 0; c < 2 * CH; ++c) {
-            if constexpr (TWO) s = by_step(kf[c], ql[m][c], s);
-            s = by_step(kf[c], qh[m][c], s);
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[m][4 * u + r] = s[r];
-        }
-      }
-      load_k(next);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) f[m] = up[m] * ks;
-      by_softmax<MT, 16, VW>(x, f, top, sum, o);
       vs = vs_next;
-      by_h8 ph[MT][2], pl[QN == 2 ? MT : 1][2];
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float y[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = x[m][8 * h + e];
-          by_halves<TWO>(y, ph[m][h], pl[QN == 2 ? m : 0][h]);
-        }
-#pragma unroll
-      for (int j = 0; j < VW; ++j) {
-        const by_h8 v0 = by_unpack<FP8>(vg[j][0], vg[j][1]), v1 = by_unpack<FP8>(vg[j][2], vg[j][3]);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          ar_f4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-          if constexpr (TWO) {
-            s = by_step(v0, pl[m][0], s);
-            s = by_step(v1, pl[m][1], s);
-          }
-          s = by_step(v0, ph[m][0], s);
-          s = by_step(v1, ph[m][1], s);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[m][j][r] = fmaf(s[r], vs, o[m][j][r]);
-        }
-      }
+      w.block(ks, vs, [&](int u, int s) { return by_unpack<FP8>(kg[u][s / 2][s % 2 * 2], kg[u][s / 2][s % 2 * 2 + 1]); },
+              [&](int j, int h) { return by_unpack<FP8>(vg[j][2 * h], vg[j][2 * h + 1]); }, [&] { load_k(next); });
       load_v(next);
     }
+    w.end();
   }
-  tree_leave<MT, VW>(a, o, top, sum, odd, unit, rb, M, smem, ml);
+  tree_leave<MT, VW>(a, w.o, w.top, w.sum, odd, at.unit, at.rb, at.M, smem, ml);
+}
+
+// Many queries: the four waves have 16 MT of them each and share the blocks.  Each wave makes a quarter of a block's codes
+// fp16 operands and leaves them in LDS, in the order in which lanes read them; two blocks are there, one barrier a block.
+template <typename T, bool FP8, int DP, int MT>
+__global__ __launch_bounds__(kTrThreads, 2) void byte_share_kernel(ByteArgs ba) {
+  const TreeArgs& a = ba.tree;
+  using Wave = ByteWave<T, DP, MT>;
+  constexpr int VW = Wave::VW, CH = Wave::CH, VL = VW / kTrWaves;   // pieces of V of a wave (of K: CH)
+  constexpr int KN = 4 * 2 * CH, VN = VW * 2;                       // operands of a block
+  __shared__ by_h8 held[2][KN + VN][kWave];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), col = lane & 15, quad = lane >> 4;
+  BytePlace at;
+  if (!at.find(a)) return;
+  const ByteCut& cut = at.cut;
+  const int row0 = (at.rb * kTrWaves + wave) * 16 * MT;
+  const T* q = (const T*)a.q + ((int64_t)cut.b * a.hc + at.hc) * at.M * a.d;
+  Wave w;
+  w.begin();
+  bool odd = false;
+  if (cut.split == 0) {
+    if (row0 < at.M) by_dense<T, DP, MT>(ba, cut, at.hc, row0, at.M, q, 0, 1, w.top, w.sum, w.o, odd);
+  } else {
+    const int64_t block0 = ((int64_t)cut.b * a.hc + at.hc) * ba.blocks;
+    const int begin = (cut.split - 1) * cut.per, end = min(cut.len / kByBlock, begin + cut.per);
+    const uint32_t kat = (uint32_t)((col >> 2) * 16 + (col & 3)) * DP + quad * 16, vat = (uint32_t)(VW * col) * kByBlock + quad * 16;
+    ar_u4 kg[CH], vg[VL];
+    auto load = [&](int i) {   // (the wave's part of block i)
+      const char* src = (const char*)ba.k + (block0 + i) * (kByBlock * DP) + wave * 4 * DP;
+      const char* from = (const char*)ba.v + (block0 + i) * (kByBlock * DP) + wave * VL * kByBlock;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) kg[c] = tree_at<ar_u4>(src + c * 64, kat);
+#pragma unroll
+      for (int j = 0; j < VL; ++j) vg[j] = tree_at<ar_u4>(from + j * kByBlock, vat);
+    };
+    auto leave = [&](int side) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) held[side][wave * 2 * CH + 2 * c + h][lane] = by_unpack<FP8>(kg[c][2 * h], kg[c][2 * h + 1]);
+#pragma unroll
+      for (int j = 0; j < VL; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) held[side][KN + (wave * VL + j) * 2 + h][lane] = by_unpack<FP8>(vg[j][2 * h], vg[j][2 * h + 1]);
+    };
+    load(begin);   // (a split has a block at least)
+    w.queries(q, row0, at.M, a.d, a.scale_log2e);
+    w.first(ba.vs[block0 + begin]);
+    leave(0);
+    load(min(begin + 1, end - 1));
+    __syncthreads();
+    for (int block = begin; block < end; ++block) {
+      const int side = (block - begin) & 1;
+      leave(side ^ 1);   // (the next one; behind the last one itself again)
+      load(min(block + 2, end - 1));
+      w.block(ba.ks[block0 + block], ba.vs[block0 + block], [&](int u, int s) { return held[side][u * 2 * CH + s][lane]; },
+              [&](int j, int h) { return held[side][KN + 2 * j + h][lane]; }, [] {});
+      __syncthreads();
+    }
+    w.end();
+  }
+  odd = __syncthreads_or(odd);
+  if (threadIdx.x == 0) a.odd[(int64_t)at.unit * a.row_blocks + at.rb] = odd;
+  const int64_t tile16 = (int64_t)at.unit * a.row_tiles + row0 / 16;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    if (row0 + 16 * m + col >= at.M) continue;
+    const float sum = ar_quad_sum(w.sum[m]);
+    if (quad == 0) {
+      float* dst = a.part_ml + (tile16 + m) * 48 + col;
+      dst[0] = w.top[m];
+      dst[16] = dst[32] = sum;
+    }
+#pragma unroll
+    for (int j = 0; j < VW; ++j) ((ar_f4*)a.part)[((tile16 + m) * VW + j) * kWave + lane] = w.o[m][j];
+  }
 }
 
 struct BytePlan {
-  int dp, mt, rows, row_blocks, row_tiles, splits, least, most, units;
+  int dp, mt;
+  bool share;
+  int rows, row_blocks, row_tiles, splits, least, most, units;
   int64_t part, ml, odd, cut;   // words of 4 bytes
 };
-static BytePlan byte_plan(int b, int hq, int hc, int t, int64_t blocks, int d) {
+static BytePlan byte_plan(int b, int hq, int hc, int t, int64_t blocks, int d, int dtype) {
   BytePlan p;
   p.dp = by_width(d);
   const int64_t M = (int64_t)(hq / hc) * t;
-  p.mt = M <= 16 || p.dp == 256 ? 1 : 2;
-  p.rows = 16 * p.mt;
+  p.share = M > 64;
+  p.mt = M <= 16 || p.dp == 256 || (p.share && dtype == LRQK_F32) ? 1 : 2;
+  p.rows = 16 * p.mt * (p.share ? kTrWaves : 1);
   p.row_blocks = (int)((M + p.rows - 1) / p.rows);
-  p.row_tiles = p.row_blocks * p.mt;
-  p.splits = (int)std::max<int64_t>(b, 512 / ((int64_t)hc * p.row_blocks));
+  p.row_tiles = p.row_blocks * (p.rows / 16);
+  // two workgroups per CU, those of what is not in complete blocks among them
+  p.splits = (int)std::max<int64_t>(b, 512 / ((int64_t)hc * p.row_blocks) - b);
   p.least = (int)std::max<int64_t>(kTrWaves, (blocks + kTrMaxSplits - 2) / (kTrMaxSplits - 1));
   // (where the heads alone fill the GPU: sums of fp32 numbers over no more than kByLong blocks, in splits of one length)
   const int64_t longest = std::max<int64_t>(p.least, kByLong), parts = (blocks + longest - 1) / longest;
@@ -413,9 +560,14 @@ static BytePlan byte_plan(int b, int hq, int hc, int t, int64_t blocks, int d) {
 template <typename T, bool FP8, int DP>
 static int byte_launch(const ByteArgs& a, const BytePlan& p, hipStream_t st) {
   const dim3 grid((unsigned)(((int64_t)p.units + 7) / 8 * 8 * p.row_blocks));
-  if constexpr (DP < 256)
-    if (p.mt == 2) hipLaunchKernelGGL((byte_stream_kernel<T, FP8, DP, 2>), grid, dim3(kTrThreads), 0, st, a);
-  if (p.mt == 1) hipLaunchKernelGGL((byte_stream_kernel<T, FP8, DP, 1>), grid, dim3(kTrThreads), 0, st, a);
+  constexpr int SHARE = DP < 256 && sizeof(T) == 2 ? 2 : 1;
+  if (p.share) {
+    hipLaunchKernelGGL((byte_share_kernel<T, FP8, DP, SHARE>), grid, dim3(kTrThreads), 0, st, a);
+  } else {
+    if constexpr (DP < 256)
+      if (p.mt == 2) hipLaunchKernelGGL((byte_stream_kernel<T, FP8, DP, 2>), grid, dim3(kTrThreads), 0, st, a);
+    if (p.mt == 1) hipLaunchKernelGGL((byte_stream_kernel<T, FP8, DP, 1>), grid, dim3(kTrThreads), 0, st, a);
+  }
   LRQK_HIP_CHECK(hipGetLastError());
   tree_join_launch<T, DP, false>(a.tree, dim3((unsigned)((int64_t)a.tree.b * a.tree.hc * a.tree.row_tiles * 4)), st);
   LRQK_HIP_CHECK(hipGetLastError());
@@ -447,7 +599,7 @@ using namespace lrqk;
 extern "C" int64_t lrqk_byte_attention_workspace(int b, int hq, int hc, int t, int64_t blocks, int d, int dtype) {
   const int rc = byte_check(b, hq, hc, t, blocks, d, dtype);
   if (rc) return rc;
-  const BytePlan p = byte_plan(b, hq, hc, t, blocks, d);
+  const BytePlan p = byte_plan(b, hq, hc, t, blocks, d, dtype);
   return (p.part + p.ml + p.odd + p.cut) * (int64_t)sizeof(float);
 }
 
@@ -466,7 +618,7 @@ extern "C" int lrqk_byte_attention(const void* q, const void* k, const void* v, 
   LRQK_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0 && (uintptr_t)k_tail % 16 == 0 &&
                    (uintptr_t)v_tail % 16 == 0 && (uintptr_t)k_new % 16 == 0 && (uintptr_t)v_new % 16 == 0 && (uintptr_t)workspace % 16 == 0,
                LRQK_EINVAL, "pointers must be 16-byte aligned");
-  const BytePlan p = byte_plan(b, hq, hc, t, blocks, d);
+  const BytePlan p = byte_plan(b, hq, hc, t, blocks, d, dtype);
   const int64_t need = (p.part + p.ml + p.odd + p.cut) * (int64_t)sizeof(float);
   LRQK_REQUIRE(workspace_bytes >= need, LRQK_EINVAL, "workspace of %lld bytes: %lld are needed", (long long)workspace_bytes,
                (long long)need);
