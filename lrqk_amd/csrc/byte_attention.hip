@@ -23,7 +23,7 @@ typedef _Float16 by_h8 __attribute__((ext_vector_type(8)));
 typedef float by_f8 __attribute__((ext_vector_type(8)));
 
 constexpr float kByUp = 8.0f;          // binary orders that probabilities are formed too large
-constexpr float kByMuch = 32768.0f;    // a lane's probabilities of a tile may add up to this before the maximum is looked for
+constexpr float kByMost = 15.0f;       // binary logarithm of the largest one before they are formed anew (fp16 ends at 2^16)
 constexpr int kByLong = 256;           // blocks of a split, at most
 
 struct ByteArgs {
@@ -71,47 +71,42 @@ __device__ __forceinline__ void by_halves(const float (&x)[8], by_h8& hi, by_h8&
   if constexpr (TWO) lo = __builtin_convertvector(v - __builtin_convertvector(hi, by_f8), by_h8);
 }
 
-// A tile's scores x become probabilities p = 2^(x f + shift - top), in place, and the running sums, of 2^(x f - top), as
-// tree_softmax does; f: of each query, less = 2^-shift.
+// A tile's scores x become probabilities p = 2^(x f + shift - top), in place, and sum that of 2^(x f - top); f: of each query,
+// less = 2^-shift.  top is not the maximum so far but what serves as one: as long as no probability is above 2^kByMost it
+// stays, and only where one would be it becomes the maximum less kByUp, o and the sums rescaled to it.
 template <int MT, int NE, int VW>
 __device__ __forceinline__ void by_softmax(float (&x)[MT][NE], const float (&f)[MT], float shift, float less, float (&top)[MT], float (&sum)[MT],
                                            ar_f4 (&o)[MT][VW]) {
-  float part[MT], p[MT][NE];
+  float high[MT];
   bool more = false;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const float from = shift - top[m];
+    high[m] = x[m][0];
 #pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      p[m][e] = ar_exp2(fmaf(x[m][e], f[m], from));
-      part[m] = e == 0 ? p[m][0] : part[m] + p[m][e];
-    }
-    more = more | !(part[m] <= kByMuch);
+    for (int e = 1; e < NE; ++e) high[m] = fmaxf(high[m], x[m][e]);
+    high[m] = fmaf(high[m], f[m], shift);
+    more = more | !(high[m] - top[m] <= kByMost);
   }
   if (__ballot(more)) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      float high = x[m][0];
-#pragma unroll
-      for (int e = 1; e < NE; ++e) high = fmaxf(high, x[m][e]);
-      const float now = fmaxf(top[m], fmaf(ar_quad_max(high), f[m], shift - kByUp));
-      const float g = ar_exp2(top[m] - now), from = shift - now;
+      const float now = fmaxf(top[m], ar_quad_max(high[m]) - kByUp), g = ar_exp2(top[m] - now);
       top[m] = now;
       sum[m] *= g;
 #pragma unroll
       for (int j = 0; j < VW; ++j) o[m][j] *= g;
-#pragma unroll
-      for (int e = 0; e < NE; ++e) {
-        p[m][e] = ar_exp2(fmaf(x[m][e], f[m], from));
-        part[m] = e == 0 ? p[m][0] : part[m] + p[m][e];
-      }
     }
   }
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    sum[m] = fmaf(part[m], less, sum[m]);
+    const float from = shift - top[m];
+    float part = 0.0f;
 #pragma unroll
-    for (int e = 0; e < NE; ++e) x[m][e] = p[m][e];
+    for (int e = 0; e < NE; ++e) {
+      x[m][e] = ar_exp2(fmaf(x[m][e], f[m], from));
+      part = e == 0 ? x[m][0] : part + x[m][e];
+    }
+    sum[m] = fmaf(part, less, sum[m]);
   }
 }
 
@@ -120,13 +115,14 @@ __device__ __forceinline__ void by_softmax(float (&x)[MT][NE], const float (&f)[
 template <typename T, int DP, int MT>
 struct ByteWave {
   static constexpr int VW = DP / 16, CH = DP / 64;
-  static constexpr bool TWO = sizeof(T) == 4;
+  static constexpr bool TWO = sizeof(T) == 4, FOLD = !TWO && MT > 1;
   by_h8 qh[MT][2 * CH], ql[TWO ? MT : 1][2 * CH];   // elements 64 c + 16 quad + 8 h .. in [2 c + h]
   float up[MT], top[MT], sum[MT];
   ar_f4 o[MT][VW];
-  // Of bf16 tensors outputs are held in units of the first block's scale and the products add to them as they are: the block's
-  // scale over that goes into the probabilities' exponents, as far as fp16 has room for it (2^8 either way; beyond, and of fp32
-  // tensors, whose sums the matrix cores must not cut off, a block's products are multiplied and added).
+  // FOLD: outputs are held in units of the first block's scale and the products add to them as they are: the block's scale over
+  // that goes into the probabilities' exponents, as far as fp16 has room for it (2^8 either way).  Beyond, and where the
+  // matrix cores do not bound (one tile of queries), and of fp32 tensors, whose sums they must not cut off, a block's products
+  // are multiplied and added.
   float unit, log_unit;
 
   __device__ __forceinline__ void begin() {
@@ -175,33 +171,52 @@ struct ByteWave {
     }
   }
   __device__ __forceinline__ void first(float vs) {
-    unit = TWO ? 1.0f : vs;
-    log_unit = TWO ? 0.0f : __builtin_amdgcn_logf(vs);
+    unit = FOLD ? vs : 1.0f;
+    log_unit = FOLD ? __builtin_amdgcn_logf(vs) : 0.0f;
   }
-  // A block: k(u, s) and v(j, h) are its operands; between: what is done once the keys are not wanted any more.
-  template <typename K, typename V, typename B>
+  // A block: k(u, s) and v(j, h) are its operands; between: what is done once the keys are not wanted any more.  AHEAD: they
+  // come from LDS, and are asked for in front of what is done before they are wanted.
+  template <bool AHEAD, typename K, typename V, typename B>
   __device__ __forceinline__ void block(float ks, float vs, K k, V v, B between) {
+    constexpr int VA = AHEAD ? VW / 2 : 0;   // (all of them: no registers left)
+    by_h8 va[AHEAD ? VA : 1][2];
     float x[MT][16], f[MT];
+    by_h8 kf[2][2 * CH];
+#pragma unroll
+    for (int s = 0; s < 2 * CH; ++s) kf[0][s] = k(0, s);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      by_h8 kf[2 * CH];
+      if (AHEAD && u < 3) {
 #pragma unroll
-      for (int s = 0; s < 2 * CH; ++s) kf[s] = k(u, s);
+        for (int s = 0; s < 2 * CH; ++s) kf[(u + 1) & 1][s] = k(u + 1, s);
+        __builtin_amdgcn_sched_barrier(0x7f);   // (reads of LDS stay in front)
+      } else if (!AHEAD && u > 0) {
+#pragma unroll
+        for (int s = 0; s < 2 * CH; ++s) kf[u & 1][s] = k(u, s);
+      }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         ar_f4 c = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int s = 0; s < 2 * CH; ++s) {
-          if constexpr (TWO) c = by_step(kf[s], ql[m][s], c);
-          c = by_step(kf[s], qh[m][s], c);
+          if constexpr (TWO) c = by_step(kf[u & 1][s], ql[m][s], c);
+          c = by_step(kf[u & 1][s], qh[m][s], c);
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[m][4 * u + r] = c[r];
       }
     }
     between();
-    const float shift = TWO ? 0.0f : __builtin_amdgcn_logf(vs) - log_unit;
-    const bool apart = TWO || !(fabsf(shift) <= 8.0f);
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int j = 0; j < VA; ++j) {
+        va[j][0] = v(j, 0);
+        va[j][1] = v(j, 1);
+      }
+      __builtin_amdgcn_sched_barrier(0x7f);
+    }
+    const float shift = FOLD ? __builtin_amdgcn_logf(vs) - log_unit : 0.0f;
+    const bool apart = !FOLD || !(fabsf(shift) <= 8.0f);
 #pragma unroll
     for (int m = 0; m < MT; ++m) f[m] = up[m] * ks;
     by_softmax<MT, 16, VW>(x, f, apart ? 0.0f : shift, apart ? 1.0f : unit * __builtin_amdgcn_rcpf(vs), top, sum, o);
@@ -215,11 +230,10 @@ struct ByteWave {
         for (int e = 0; e < 8; ++e) y[e] = x[m][8 * h + e];
         by_halves<TWO>(y, ph[m][h], pl[TWO ? m : 0][h]);
       }
-    if (TWO || __builtin_expect(apart, 0)) {
-      const float by = TWO ? vs : vs / unit;
+    if constexpr (!FOLD) {
 #pragma unroll
       for (int j = 0; j < VW; ++j) {
-        const by_h8 v0 = v(j, 0), v1 = v(j, 1);
+        const by_h8 v0 = j < VA ? va[j < VA ? j : 0][0] : v(j, 0), v1 = j < VA ? va[j < VA ? j : 0][1] : v(j, 1);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           ar_f4 c = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -230,23 +244,38 @@ struct ByteWave {
           c = by_step(v0, ph[m][0], c);
           c = by_step(v1, ph[m][1], c);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[m][j][r] = fmaf(c[r], by, o[m][j][r]);
+          for (int r = 0; r < 4; ++r) o[m][j][r] = fmaf(c[r], vs, o[m][j][r]);
         }
       }
     } else {
+      // (a block whose scale is far from the first's: what there is waits in memory.  As a branch of its own, with products of
+      // its own, it cost every block the copying of all outputs from register to register.)
+      volatile float waiting[MT * VW * 4];
+      if (__builtin_expect(apart, 0)) {
+#pragma unroll
+        for (int i = 0; i < MT * VW * 4; ++i) {
+          waiting[i] = o[i / 4 / VW][i / 4 % VW][i % 4];
+          o[i / 4 / VW][i / 4 % VW][i % 4] = 0.0f;
+        }
+      }
 #pragma unroll
       for (int j = 0; j < VW; ++j) {
-        const by_h8 v0 = v(j, 0), v1 = v(j, 1);
+        const by_h8 v0 = j < VA ? va[j < VA ? j : 0][0] : v(j, 0), v1 = j < VA ? va[j < VA ? j : 0][1] : v(j, 1);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           o[m][j] = by_step(v0, ph[m][0], o[m][j]);
           o[m][j] = by_step(v1, ph[m][1], o[m][j]);
         }
       }
+      if (__builtin_expect(apart, 0)) {
+        const float by = vs / unit;
+#pragma unroll
+        for (int i = 0; i < MT * VW * 4; ++i) o[i / 4 / VW][i / 4 % VW][i % 4] = fmaf(o[i / 4 / VW][i / 4 % VW][i % 4], by, waiting[i]);
+      }
     }
   }
   __device__ __forceinline__ void end() {
-    if constexpr (!TWO) {
+    if constexpr (FOLD) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -395,7 +424,8 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba)
   const TreeArgs& a = ba.tree;
   using Wave = ByteWave<T, DP, MT>;
   constexpr int VW = Wave::VW, CH = Wave::CH;
-  __shared__ ar_u4 smem[kTrWaves * MT * 2 * kWave];
+  constexpr int JC = 8 / MT < VW ? 8 / MT : VW;   // (32 KB; with two blocks at a time a token over 32K took 1.5 us more)
+  __shared__ ar_u4 smem[kTrWaves * MT * JC * kWave];
   __shared__ float ml[kTrWaves][MT][16][2];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), col = lane & 15, quad = lane >> 4;
   BytePlace at;
@@ -440,13 +470,13 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba)
       const int next = block + kTrWaves < end ? block + kTrWaves : block;   // (the next one, or this one again)
       ks = ks_next;
       vs = vs_next;
-      w.block(ks, vs, [&](int u, int s) { return by_unpack<FP8>(kg[u][s / 2][s % 2 * 2], kg[u][s / 2][s % 2 * 2 + 1]); },
+      w.template block<false>(ks, vs, [&](int u, int s) { return by_unpack<FP8>(kg[u][s / 2][s % 2 * 2], kg[u][s / 2][s % 2 * 2 + 1]); },
               [&](int j, int h) { return by_unpack<FP8>(vg[j][2 * h], vg[j][2 * h + 1]); }, [&] { load_k(next); });
       load_v(next);
     }
     w.end();
   }
-  tree_leave<MT, VW>(a, w.o, w.top, w.sum, odd, at.unit, at.rb, at.M, smem, ml);
+  tree_leave<MT, VW, JC>(a, w.o, w.top, w.sum, odd, at.unit, at.rb, at.M, smem, ml);
 }
 
 // Many queries: the four waves have 16 MT of them each and share the blocks.  Each wave makes a quarter of a block's codes
@@ -475,12 +505,12 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_share_kernel(ByteArgs ba) 
     const uint32_t kat = (uint32_t)((col >> 2) * 16 + (col & 3)) * DP + quad * 16, vat = (uint32_t)(VW * col) * kByBlock + quad * 16;
     ar_u4 kg[CH], vg[VL];
     auto load = [&](int i) {   // (the wave's part of block i)
-      const char* src = (const char*)ba.k + (block0 + i) * (kByBlock * DP) + wave * 4 * DP;
-      const char* from = (const char*)ba.v + (block0 + i) * (kByBlock * DP) + wave * VL * kByBlock;
+      const char* ks = (const char*)ba.k + (block0 + i) * (kByBlock * DP) + wave * 4 * DP;
+      const char* vs = (const char*)ba.v + (block0 + i) * (kByBlock * DP) + wave * VL * kByBlock;
 #pragma unroll
-      for (int c = 0; c < CH; ++c) kg[c] = tree_at<ar_u4>(src + c * 64, kat);
+      for (int c = 0; c < CH; ++c) kg[c] = tree_at<ar_u4>(ks + c * 64, kat);
 #pragma unroll
-      for (int j = 0; j < VL; ++j) vg[j] = tree_at<ar_u4>(from + j * kByBlock, vat);
+      for (int j = 0; j < VL; ++j) vg[j] = tree_at<ar_u4>(vs + j * kByBlock, vat);
     };
     auto leave = [&](int side) {
 #pragma unroll
@@ -502,8 +532,8 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_share_kernel(ByteArgs ba) 
       const int side = (block - begin) & 1;
       leave(side ^ 1);   // (the next one; behind the last one itself again)
       load(min(block + 2, end - 1));
-      w.block(ba.ks[block0 + block], ba.vs[block0 + block], [&](int u, int s) { return held[side][u * 2 * CH + s][lane]; },
-              [&](int j, int h) { return held[side][KN + 2 * j + h][lane]; }, [] {});
+      w.template block<true>(ba.ks[block0 + block], ba.vs[block0 + block], [&](int u, int s) { return held[side][u * 2 * CH + s][lane]; },
+                             [&](int j, int h) { return held[side][KN + 2 * j + h][lane]; }, [] {});
       __syncthreads();
     }
     w.end();
@@ -540,8 +570,12 @@ static BytePlan byte_plan(int b, int hq, int hc, int t, int64_t blocks, int d, i
   p.rows = 16 * p.mt * (p.share ? kTrWaves : 1);
   p.row_blocks = (int)((M + p.rows - 1) / p.rows);
   p.row_tiles = p.row_blocks * (p.rows / 16);
-  // two workgroups per CU, those of what is not in complete blocks among them
-  p.splits = (int)std::max<int64_t>(b, 512 / ((int64_t)hc * p.row_blocks) - b);
+  // Workgroups, those of what is not in complete blocks among them: two per CU, which keep each other's time filled.  A single
+  // sequence is cut evenly, and of few queries one per CU then reads as fast and leaves less to be joined (a token over 32K:
+  // 18 us, with two 21, with three 23); of many sequences with one tile of queries three per CU hide that their lengths differ
+  // (16 tokens over 1K .. 8K: 44 us, with two 53).
+  const int wanted = p.share ? 512 : b == 1 ? 256 : p.mt == 1 && b >= 8 ? 768 : 512;
+  p.splits = (int)std::max<int64_t>(b, wanted / ((int64_t)hc * p.row_blocks) - b);
   p.least = (int)std::max<int64_t>(kTrWaves, (blocks + kTrMaxSplits - 2) / (kTrMaxSplits - 1));
   // (where the heads alone fill the GPU: sums of fp32 numbers over no more than kByLong blocks, in splits of one length)
   const int64_t longest = std::max<int64_t>(p.least, kByLong), parts = (blocks + longest - 1) / longest;

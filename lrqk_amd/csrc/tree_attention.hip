@@ -265,7 +265,7 @@ __global__ __launch_bounds__(kTrThreads, MT == 2 && DP == 128 ? 2 : 1) void tree
     for (int e = 0; e < NE; ++e) v[e].load(vs, (uint32_t)min(quad * NE + e, valid - 1) * rs, vplace);
     work(std::false_type{}, valid, draft, first, [] {}, [] {});
   }
-  tree_leave<MT, VW>(a, o, top, sum, odd, at.unit, at.rb, M, smem, ml);   // (the rows of K make room for the sums)
+  tree_leave<MT, VW, JC>(a, o, top, sum, odd, at.unit, at.rb, M, smem, ml);   // (the rows of K make room for the sums)
 }
 
 constexpr int kTlWaves = 4, kTlThreads = kTlWaves * kWave;

@@ -185,12 +185,11 @@ __device__ __forceinline__ void tree_mask(float (&p)[MT][NE], const TreeArgs& a,
 }
 
 // The four waves' sums, each over its own keys, to one maximum and together, and into the scratch as the part of row block
-// `rb` of a unit of the grid.  smem: room for kTrWaves x 2 MT x 64 pieces of 16 bytes, which no wave reads any more behind the
-// first barrier here.
-template <int MT, int VW>
+// `rb` of a unit of the grid.  JC: output blocks that the waves join at a time (two barriers each).  smem: room for kTrWaves x
+// JC MT x 64 pieces of 16 bytes, which no wave reads any more behind the first barrier here.
+template <int MT, int VW, int JC>
 __device__ __forceinline__ void tree_leave(const TreeArgs& a, ar_f4 (&o)[MT][VW], const float (&top)[MT], float (&sum)[MT], bool odd,
                                            int unit, int rb, int M, ar_u4* smem, float (*ml)[MT][16][2]) {
-  constexpr int JC = 2;   // output blocks that the waves join at a time
   const int lane = lane_id(), wave = wave_id(), col = lane & 15, quad = lane >> 4, row0 = rb * 16 * MT;
   __syncthreads();
   ar_f4(*joint)[MT * JC][kWave] = (ar_f4(*)[MT * JC][kWave])smem;
