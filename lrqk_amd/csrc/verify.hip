@@ -31,12 +31,18 @@ struct VerifyArgs {
   int32_t *path, *counts, *next;
   double *cut, *mass;                // [b][s]: C and Z that a node's test is made with (trees with p)
   double* sums;                      // [b][chunks]
-  double* left;                      // [b]: C behind the last accepted node
-  int32_t* end;                      // [b]: the last accepted node
+  struct VerifyEnd* ends;            // [b]
+  int32_t* gone;                     // [b][s]: tokens of the last accepted node's refused children (drafts without p)
   int b, s, vocab, chunks;
 };
 
-__device__ __forceinline__ double vf_positive(double x) { return x > 0.0 ? x : 0.0; }   // (NaN: 0)
+struct VerifyEnd {   // where a sequence's walk ended
+  double cut;        // C there
+  int node, gone;    // the last accepted node; how many tokens are gone
+};
+
+__device__ __forceinline__ double vf_positive(double x) { return fmax(x, 0.0); }         // (NaN: 0)
+__device__ __forceinline__ double vf_probability(float x) { return (double)fmaxf(x, 0.0f); }
 
 // A tree as the threads of a workgroup see it.
 struct VerifyTree {
@@ -68,7 +74,14 @@ __device__ __forceinline__ double vf_sum(double v, double* scratch) {
   return all;
 }
 
-// Z of the children of one node, one after the other: a workgroup has both rows for itself.
+// u p Z < r, with r = max(q - C p, 0).
+__device__ __forceinline__ bool vf_accepts(double u, double px, double mass, double qx, double cut) {
+  return u * px * mass < vf_positive(fma(-cut, px, qx));
+}
+
+// Z of the children of one node, one after the other up to the one that is accepted: a workgroup has both rows for itself.  Bound
+// by one CU, 9.5 us a pass over 128256 tokens: seven instructions an element in 64 bits (6.5) beside 1 MB from the L2 (7.8);
+// more loads ahead changed nothing.  (Several CUs would have to wait for each other, or for a launch a child.)
 template <typename T>
 __global__ __launch_bounds__(kVfWide) void verify_mass_kernel(VerifyArgs a) {
   __shared__ VerifyTree tree;
@@ -84,7 +97,41 @@ __global__ __launch_bounds__(kVfWide) void verify_mass_kernel(VerifyArgs a) {
     if (!first) {
       cut += mass;
       double sum = 0.0;
-      for (int x = threadIdx.x; x < a.vocab; x += kVfWide) sum += vf_positive((double)ld_f32(q, x) - cut * vf_positive((double)ld_f32(p, x)));
+      auto add = [&](float qx, float px) { sum += vf_positive(fma(-cut, vf_probability(px), (double)qx)); };
+      int64_t done = 0;
+      if (((uintptr_t)q | (uintptr_t)p) % 16 == 0) {
+        constexpr int N = Vec16<T>::N, EACH = 4;
+        const int64_t step = (int64_t)EACH * kVfWide * N;
+        for (; done + step <= a.vocab; done += step) {
+          Vec16<T> qv[EACH], pv[EACH];
+#pragma unroll
+          for (int e = 0; e < EACH; ++e) {
+            const int64_t x = done + ((int64_t)e * kVfWide + threadIdx.x) * N;
+            qv[e].load(q + x);
+            pv[e].load(p + x);
+          }
+#pragma unroll
+          for (int e = 0; e < EACH; ++e) {
+            float qs[N], ps[N];
+            qv[e].unpack(qs);
+            pv[e].unpack(ps);
+#pragma unroll
+            for (int i = 0; i < N; ++i) add(qs[i], ps[i]);
+          }
+        }
+      }
+      constexpr int EACH = 8;
+      for (; done + EACH * kVfWide <= a.vocab; done += EACH * kVfWide) {
+        float qs[EACH], ps[EACH];
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+          qs[e] = ld_f32(q, done + e * kVfWide + threadIdx.x);
+          ps[e] = ld_f32(p, done + e * kVfWide + threadIdx.x);
+        }
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) add(qs[e], ps[e]);
+      }
+      for (int64_t x = done + threadIdx.x; x < a.vocab; x += kVfWide) add(ld_f32(q, x), ld_f32(p, x));
       mass = vf_sum<kVfWide>(sum, scratch);
     }
     first = false;
@@ -92,6 +139,9 @@ __global__ __launch_bounds__(kVfWide) void verify_mass_kernel(VerifyArgs a) {
       a.cut[(int64_t)b * a.s + i] = cut;
       a.mass[(int64_t)b * a.s + i] = mass;
     }
+    // (behind an accepted child nobody asks: of a node's accepted children the first counts)
+    const int x = tree.token[i];
+    if (x >= 0 && vf_accepts((double)a.u[(int64_t)b * a.s + i], vf_probability(ld_f32(p, x)), mass, vf_probability(ld_f32(q, x)), cut)) return;
   }
 }
 
@@ -104,7 +154,7 @@ __device__ __forceinline__ void vf_walk(const VerifyArgs& a, int b, VerifyTree& 
   for (int i = threadIdx.x; i < a.s; i += kVfThreads) {
     chosen[i] = INT32_MAX;
     const int up = tree.parent[i], x = tree.token[i];
-    double mine = up >= 0 && x >= 0 ? vf_positive((double)ld_f32(q + up * a.qr, x)) : 0.0;
+    double mine = up >= 0 && x >= 0 ? vf_probability(ld_f32(q + up * a.qr, x)) : 0.0;
     // (without p: a token that an earlier sibling has is gone)
     if (!a.p && a.parents && up >= 0)
       for (int j = up + 1; j < i; ++j)
@@ -118,9 +168,9 @@ __device__ __forceinline__ void vf_walk(const VerifyArgs& a, int b, VerifyTree& 
     const double u = (double)a.u[(int64_t)b * a.s + i];
     bool taken;
     if (a.p) {
-      const double px = vf_positive((double)ld_f32(p + up * a.pr, x));
+      const double px = vf_probability(ld_f32(p + up * a.pr, x));
       const double c = a.parents ? a.cut[(int64_t)b * a.s + i] : 0.0, mass = a.parents ? a.mass[(int64_t)b * a.s + i] : 1.0;
-      taken = u * px * mass < vf_positive(own[i] - c * px);
+      taken = vf_accepts(u, px, mass, own[i], c);
     } else {
       double mass = 1.0;
       if (a.parents)
@@ -150,34 +200,35 @@ __device__ __forceinline__ void vf_walk(const VerifyArgs& a, int b, VerifyTree& 
   }
 }
 
-// The tokens that refused children of node `end` took with them (drafts without p): in any order, they are only looked for.
-// Holds a barrier.
-__device__ __forceinline__ void vf_refused(const VerifyArgs& a, const VerifyTree& tree, int end, int* gone, int& gone_n) {
-  if (a.p) return;
-  for (int i = threadIdx.x; i < a.s; i += kVfThreads)
-    if (tree.parent[i] == end && tree.token[i] >= 0) gone[atomicAdd(&gone_n, 1)] = tree.token[i];
-  __syncthreads();
-}
-
 // What is left of a row, element x.
 template <typename T>
 struct VerifyRow {
-  const T *q, *p;
+  const T *q, *p;     // p: or null
   double cut;
-  const int* gone;
+  const int* gone;    // tokens that are gone
   int gone_n;
-  __device__ __forceinline__ double at(int x) const {
-    double y = (double)ld_f32(q, x);
-    if (p) y -= cut * vf_positive((double)ld_f32(p, x));
-    for (int i = 0; i < gone_n; ++i) y = gone[i] == x ? 0.0 : y;
-    return vf_positive(y);
+  // (the drafting model's row is not looked at where no child was refused: there may be none for the last node)
+  __device__ __forceinline__ VerifyRow(const VerifyArgs& a, int b, int node, double cut, const int* gone, int gone_n)
+      : q((const T*)a.q + b * a.qb + node * a.qr), p(a.p && cut != 0.0 ? (const T*)a.p + b * a.pb + node * a.pr : nullptr), cut(cut), gone(gone),
+        gone_n(gone_n) {}
+  // N elements from x on, `step` apart; 0 behind the end
+  template <int N>
+  __device__ __forceinline__ void load(int64_t x, int step, int64_t end, double (&r)[N]) const {
+    float qs[N], ps[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int64_t at = x + e * step < end ? x + e * step : end - 1;
+      qs[e] = ld_f32(q, at);
+      ps[e] = p ? ld_f32(p, at) : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      r[e] = vf_positive(fma(-cut, vf_probability(ps[e]), (double)qs[e]));
+      for (int i = 0; i < gone_n; ++i) r[e] = gone[i] == (int)(x + e * step) ? 0.0 : r[e];
+      r[e] = x + e * step < end ? r[e] : 0.0;
+    }
   }
 };
-// (the drafting model's row is not looked at where no child was refused: there may be none for the last node)
-template <typename T>
-__device__ __forceinline__ VerifyRow<T> vf_row(const VerifyArgs& a, int b, int end, double cut, const int* gone, int gone_n) {
-  return {(const T*)a.q + b * a.qb + end * a.qr, a.p && cut != 0.0 ? (const T*)a.p + b * a.pb + end * a.pr : nullptr, cut, gone, gone_n};
-}
 
 template <typename T>
 __global__ __launch_bounds__(kVfThreads) void verify_sums_kernel(VerifyArgs a) {
@@ -189,23 +240,25 @@ __global__ __launch_bounds__(kVfThreads) void verify_sums_kernel(VerifyArgs a) {
   int end, count;
   double cut;
   vf_walk<T>(a, b, tree, own, chosen, end, cut, count);
+  if (!a.p) {   // (in any order: they are only looked for)
+    for (int i = end + 1 + tid; i < a.s; i += kVfThreads)
+      if (tree.parent[i] == end && tree.token[i] >= 0) gone[atomicAdd(&gone_n, 1)] = tree.token[i];
+    __syncthreads();
+  }
   if (chunk == 0) {
     for (int i = count + tid; i < a.s; i += kVfThreads) a.path[(int64_t)b * a.s + i] = -1;
+    for (int i = tid; i < gone_n; i += kVfThreads) a.gone[(int64_t)b * a.s + i] = gone[i];
     if (tid == 0) {
       a.counts[b] = count;
-      a.end[b] = end;
-      a.left[b] = cut;
+      a.ends[b] = {cut, end, gone_n};
       for (int i = 0, at = 0; i < count; ++i, at = chosen[at]) a.path[(int64_t)b * a.s + i] = at;
     }
   }
-  vf_refused(a, tree, end, gone, gone_n);
-  const VerifyRow<T> row = vf_row<T>(a, b, end, cut, gone, gone_n);
-  double sum = 0.0;
+  const VerifyRow<T> row(a, b, end, cut, gone, gone_n);
+  double r[kVfEach], sum = 0.0;
+  row.load((int64_t)chunk * kVfChunk + tid, kVfThreads, a.vocab, r);
 #pragma unroll
-  for (int e = 0; e < kVfEach; ++e) {
-    const int64_t x = (int64_t)chunk * kVfChunk + e * kVfThreads + tid;
-    if (x < a.vocab) sum += row.at((int)x);
-  }
+  for (int e = 0; e < kVfEach; ++e) sum += r[e];
   sum = vf_sum<kVfThreads>(sum, scratch);
   if (tid == 0) a.sums[(int64_t)b * a.chunks + chunk] = sum;
 }
@@ -233,66 +286,117 @@ __device__ __forceinline__ double vf_scan(double v, double* scratch, double& bef
   return base + x;
 }
 
-// The first of n numbers whose sum with those in front of it is above a border (the last that is not 0, where rounding hides it;
-// -1 if all are), and the border less what stands in front of it.  SHARE: the border is `share` of the sum of all.
+// The first of the workgroup's numbers, kVfEach successive ones a thread, whose sum with those in front of it is above a border
+// (the last that is not 0, where rounding hides it; -1 if all are), and the border less what stands in front of it.  SHARE: the
+// border is `share` of the sum of all.
 struct VerifyPlace {
   int64_t i;
   double rest;
 };
-template <bool SHARE, typename F>
-__device__ __forceinline__ VerifyPlace vf_first(int64_t n, F number, double share, double* scratch, VerifyPlace& found, int* who) {
-  const int64_t each = (n + kVfThreads - 1) / kVfThreads, lo = min(threadIdx.x * each, n), hi = min(lo + each, n);
+struct VerifyFind {
+  double scratch[kVfThreads / kWave];
+  int first, last;
+  VerifyPlace found;
+};
+template <bool SHARE>
+__device__ __forceinline__ VerifyPlace vf_first(const double (&r)[kVfEach], double share, VerifyFind& f) {
   double mine = 0.0, before, all;
-  for (int64_t i = lo; i < hi; ++i) mine += number(i);
+#pragma unroll
+  for (int e = 0; e < kVfEach; ++e) mine += r[e];
   if (threadIdx.x == 0) {
-    who[0] = INT32_MAX;
-    who[1] = found.i = -1;
+    f.first = INT32_MAX;
+    f.last = -1;
+    f.found.i = -1;
   }
-  const double upto = vf_scan(mine, scratch, before, all), border = SHARE ? share * all : share;   // (holds barriers)
-  if (mine > 0.0) {
-    if (upto > border) atomicMin(&who[0], (int)threadIdx.x);
-    atomicMax(&who[1], (int)threadIdx.x);
+  const double upto = vf_scan(mine, f.scratch, before, all), border = SHARE ? share * all : share;   // (holds barriers)
+  // the first such thread of each wave and the last one with anything, then of all
+  const unsigned long long over = __ballot(mine > 0.0 && upto > border), some = __ballot(mine > 0.0);
+  if (lane_id() == 0) {
+    if (over) atomicMin(&f.first, (int)threadIdx.x + __ffsll(over) - 1);
+    if (some) atomicMax(&f.last, (int)threadIdx.x + 63 - __clzll(some));
   }
   __syncthreads();
-  if ((int)threadIdx.x == (who[0] != INT32_MAX ? who[0] : who[1])) {
+  if ((int)threadIdx.x == (f.first != INT32_MAX ? f.first : f.last)) {
     double sum = before;
-    for (int64_t i = lo; i < hi; ++i) {
-      const double x = number(i);
-      if (!(x > 0.0)) continue;
-      found = {i, border - sum};
-      sum += x;
-      if (sum > border) break;
+    bool done = false;
+#pragma unroll
+    for (int e = 0; e < kVfEach; ++e) {
+      if (!done && r[e] > 0.0) f.found = {(int64_t)threadIdx.x * kVfEach + e, border - sum};
+      sum += r[e];
+      done = done || (r[e] > 0.0 && sum > border);
     }
   }
   __syncthreads();
-  return found;
+  return f.found;
+}
+
+// The sums of runs of equal length, as many as vf_first looks through at once, that n numbers are made of.
+template <typename F>
+__device__ __forceinline__ void vf_runs(int64_t n, int64_t run, F number, double (&r)[kVfEach]) {
+#pragma unroll
+  for (int e = 0; e < kVfEach; ++e) {
+    const int64_t lo = min(((int64_t)threadIdx.x * kVfEach + e) * run, n), hi = min(lo + run, n);
+    double sum = 0.0;
+    for (int64_t i = lo; i < hi; ++i) sum += number(i);
+    r[e] = sum;
+  }
 }
 
 template <typename T>
 __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) {
-  __shared__ VerifyTree tree;
-  __shared__ double scratch[kVfThreads / kWave];
-  __shared__ int gone[kVfMost], gone_n, who[2];
-  __shared__ VerifyPlace found;
-  const int b = blockIdx.x;
-  if (threadIdx.x == 0) gone_n = 0;
-  vf_read<kVfThreads>(a, b, tree);
-  const int end = a.end[b];
-  vf_refused(a, tree, end, gone, gone_n);
+  __shared__ VerifyFind find;
+  __shared__ int gone[kVfMost];
+  const int b = blockIdx.x, tid = threadIdx.x;
+  const VerifyEnd end = a.ends[b];
   const double* sums = a.sums + (int64_t)b * a.chunks;
   const double u = (double)a.u[(int64_t)b * a.s];
-  const VerifyPlace chunk = vf_first<true>(a.chunks, [&](int64_t i) { return sums[i]; }, u, scratch, found, who);
-  __syncthreads();
-  int64_t token;
-  if (chunk.i >= 0) {
-    const VerifyRow<T> row = vf_row<T>(a, b, end, a.left[b], gone, gone_n);
-    const int64_t x0 = chunk.i * kVfChunk;
-    token = x0 + vf_first<false>(min((int64_t)kVfChunk, a.vocab - x0), [&](int64_t i) { return row.at((int)(x0 + i)); }, chunk.rest, scratch, found, who).i;
-  } else {   // nothing is left: of the target's distribution as it is
-    const VerifyRow<T> row = vf_row<T>(a, b, end, 0.0, gone, 0);
-    token = vf_first<true>(a.vocab, [&](int64_t i) { return row.at((int)i); }, u, scratch, found, who).i;
+  double r[kVfEach];
+  const int64_t run = (a.chunks + kVfChunk - 1) / kVfChunk;   // (1 up to 4 million tokens)
+  if (run == 1) {
+#pragma unroll
+    for (int e = 0; e < kVfEach; ++e) r[e] = tid * kVfEach + e < a.chunks ? sums[min(tid * kVfEach + e, a.chunks - 1)] : 0.0;
+  } else {
+    vf_runs(a.chunks, run, [&](int64_t i) { return sums[i]; }, r);
   }
-  if (threadIdx.x == 0) a.next[b] = (int)token;
+  for (int i = tid; i < end.gone; i += kVfThreads) gone[i] = a.gone[(int64_t)b * a.s + i];
+  VerifyPlace at = vf_first<true>(r, u, find);   // (its barriers are those of `gone` too)
+  const bool nothing = at.i < 0;                 // of the target's distribution as it is, then
+  const VerifyRow<T> row(a, b, end.node, nothing ? 0.0 : end.cut, gone, nothing ? 0 : end.gone);
+  int64_t token = -1;
+  if (!nothing) {
+    if (run > 1) {
+      double border = at.rest;
+      int64_t i = at.i * run;
+      while (i + 1 < min((at.i + 1) * run, (int64_t)a.chunks) && !(sums[i] > border)) border -= sums[i++];
+      at = {i, border};
+    }
+    const int64_t x0 = at.i * kVfChunk;
+    row.load(x0 + (int64_t)tid * kVfEach, 1, a.vocab, r);
+    __syncthreads();
+    const VerifyPlace place = vf_first<false>(r, at.rest, find);
+    token = place.i < 0 ? -1 : x0 + place.i;
+  } else {
+    const int64_t part = (a.vocab + kVfChunk - 1) / kVfChunk;
+    auto number = [&](int64_t i) {
+      double one[1];
+      row.load(i, 1, a.vocab, one);
+      return one[0];
+    };
+    vf_runs(a.vocab, part, number, r);
+    __syncthreads();
+    const VerifyPlace place = vf_first<true>(r, u, find);
+    if (place.i >= 0) {
+      double border = place.rest;
+      const int64_t stop = min((place.i + 1) * part, (int64_t)a.vocab);
+      for (int64_t i = place.i * part; i < stop; ++i) {
+        const double x = number(i);
+        if (x > 0.0) token = i;
+        if (x > 0.0 && x > border) break;
+        border -= x;
+      }
+    }
+  }
+  if (tid == 0) a.next[b] = (int)token;
 }
 
 static int verify_check(int b, int s, int64_t vocab) {
@@ -303,7 +407,7 @@ static int verify_check(int b, int s, int64_t vocab) {
 }
 static int64_t verify_chunks(int64_t vocab) { return (vocab + kVfChunk - 1) / kVfChunk; }
 // 64-bit words of the scratch
-static int64_t verify_words(int b, int s, int64_t vocab) { return b * (2 * (int64_t)s + verify_chunks(vocab) + 2); }
+static int64_t verify_words(int b, int s, int64_t vocab) { return b * (2 * (int64_t)s + verify_chunks(vocab) + 2) + ((int64_t)b * s + 1) / 2; }
 
 template <typename T>
 static int verify_launch(const VerifyArgs& a, hipStream_t st) {
@@ -341,9 +445,10 @@ extern "C" int lrqk_verify_drafts(const int32_t* tokens, const int32_t* parents,
                (long long)workspace_bytes, (long long)(8 * verify_words(b, s, vocab)));
   double* ws = (double*)workspace;
   const int64_t nodes = (int64_t)b * s, chunks = verify_chunks(vocab);
+  double* ends = ws + 2 * nodes + b * chunks;
   VerifyArgs a{tokens, parents, target, draft, target_batch_stride, target_row_stride, draft_batch_stride, draft_row_stride, uniforms, path,
-               counts, next, ws, ws + nodes, ws + 2 * nodes, ws + 2 * nodes + b * chunks,
-               (int32_t*)(ws + 2 * nodes + b * chunks + b), b, s, (int)vocab, (int)chunks};
+               counts, next, ws, ws + nodes, ws + 2 * nodes, (VerifyEnd*)ends, (int32_t*)(ends + 2 * (int64_t)b), b, s, (int)vocab,
+               (int)chunks};
   hipStream_t st = (hipStream_t)stream;
   return dtype == LRQK_F32 ? verify_launch<float>(a, st) : verify_launch<bf16_t>(a, st);
 }

@@ -1094,13 +1094,13 @@ def verify_drafts(tokens: torch.Tensor, target: torch.Tensor, uniforms: torch.Te
         if vocab > 1 and draft.stride(2) != 1:
             raise ValueError("the rows of draft must be contiguous")
         draft_strides = draft.stride()[:2]
-    path, counts, token = (torch.empty(shape, dtype=torch.int32, device=target.device) for shape in ((b, s), (b,), (b,)))
+    path, counts, token = torch.empty_like(tokens), tokens.new_empty(b), tokens.new_empty(b)
     if b == 0:
         return path, counts, token
     if s == 0 or vocab == 0:
         raise ValueError(f"{s} nodes over a vocabulary of {vocab}: at least 1 each")
     need = _scratch_bytes("lrqk_verify_drafts_workspace", b, s, vocab)
-    ws = _scratch(need, target)
+    ws = tokens.new_empty(need // 4)   # (of whole 8-byte words)
     st = target.stride()
     _launch(dev, _lib.load().lrqk_verify_drafts, tokens.data_ptr(), _ptr(parents), target.data_ptr(), st[0], st[1],
             draft.data_ptr() if draft is not None and s > 1 else None, *draft_strides, uniforms.data_ptr(), path.data_ptr(),

@@ -709,6 +709,24 @@ def test_verify_places_and_the_largest_trees(ops):
     assert [x.shape for x in empty] == [(0, 3), (0,), (0,)]
 
 
+def test_verify_vocabularies_of_many_chunks(ops):
+    """More tokens than one look finds a place among, and rows of them that nothing is left of."""
+    print("verify large", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(24)
+    for vocab in (2048 * 2048 + 7, 3 * 2048 * 2048 - 1):
+        target = torch.rand((2, 3, vocab), generator=g, device=DEV)
+        target /= target.sum(-1, keepdim=True)
+        draft = torch.rand((2, 3, vocab), generator=g, device=DEV)
+        draft /= draft.sum(-1, keepdim=True)
+        tokens = torch.randint(0, vocab, (2, 3), generator=g, device=DEV, dtype=torch.int32)
+        parents = _i32(-1, 0, 0).repeat(2, 1)
+        for u in (0.0, 0.3, 0.99999):
+            uniforms = torch.full((2, 3), 1 - 2.0 ** -24, device=DEV)
+            uniforms[:, 0] = u
+            _check_verify(ops, tokens, target, uniforms, draft, parents, what=(vocab, u))
+            _check_verify(ops, tokens, target, uniforms, 3 * target, parents, what=(vocab, u, "nothing left"))
+
+
 @pytest.mark.parametrize("children", [1, 3])
 @pytest.mark.parametrize("drafted", [True, False])
 def test_what_is_accepted_or_drawn_has_the_targets_distribution(ops, drafted, children):
