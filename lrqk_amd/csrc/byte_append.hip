@@ -26,43 +26,72 @@ struct AppendArgs {
   int blocks, h, t, most, d;
 };
 
-// Sixteen bytes of four successive rows of a block.
+// The largest magnitude among sixteen bytes of elements, as bits of an fp32 number: of all, and of the finite ones.
+typedef uint16_t ap_u16x2 __attribute__((ext_vector_type(2)));
 template <typename T>
-struct AppendPart {
-  static constexpr int N = Vec16<T>::N;
-  float x[4][N];
-};
-
-__device__ __forceinline__ uint32_t ap_finite(float x) {   // magnitude's bits, 0 if it is not finite
-  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
-  return u < 0x7f800000u ? u : 0u;
+__device__ __forceinline__ uint32_t ap_top(const Vec16<T>& v) {
+  const uint32_t* w = (const uint32_t*)&v.raw;
+  if constexpr (sizeof(T) == 4) {
+    return max(max(w[0] & 0x7fffffffu, w[1] & 0x7fffffffu), max(w[2] & 0x7fffffffu, w[3] & 0x7fffffffu));
+  } else {   // (of bf16 numbers two at a time)
+    ap_u16x2 top = __builtin_bit_cast(ap_u16x2, w[0] & 0x7fff7fffu);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(ap_u16x2, w[i] & 0x7fff7fffu));
+    return (uint32_t)max(top[0], top[1]) << 16;
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t ap_finite_top(const Vec16<T>& v) {
+  float x[Vec16<T>::N];
+  v.unpack(x);
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < Vec16<T>::N; ++i) {
+    const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
+    top = max(top, u < 0x7f800000u ? u : 0u);
+  }
+  return top;
 }
 
-// Four codes in a word.
+// Four codes in a word.  odd: there may be infinities and NaN among them.
 template <bool FP8>
-__device__ __forceinline__ uint32_t ap_codes(float a, float b, float c, float d, float s, float inv) {
+__device__ __forceinline__ uint32_t ap_codes(float a, float b, float c, float d, float s, float inv, bool odd) {
   float x[4] = {a, b, c, d};
+  constexpr float MOST = FP8 ? 448.0f : 127.0f;
   if constexpr (FP8) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] *= inv;   // exact (or far below the smallest code)
-      x[i] = x[i] == x[i] ? fminf(fmaxf(x[i], -448.0f), 448.0f) : 0.0f;
+    for (int i = 0; i < 4; ++i) x[i] *= inv;   // exact (or far below the smallest code)
+    if (odd) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = x[i] == x[i] ? fminf(fmaxf(x[i], -MOST), MOST) : 0.0f;
     }
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
   } else {
-    uint32_t w = 0;
+    // added to 1.5 2^23 a number is rounded to a whole one, which is then in the lowest bits
+    constexpr float ROUND = 12582912.0f;
+    float r[4], near = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float y = x[i] == x[i] ? x[i] : 0.0f;
-      float q = rintf(y * inv);
-      // what is left is exact where it is near half of s (a multiple of half a unit of s, and at most s): so is the decision
-      const float left = fmaf(-q, s, y), half = 0.5f * s;
-      const bool odd = (q - 2.0f * floorf(0.5f * q)) != 0.0f;
-      if (fabsf(left) > half || (fabsf(left) == half && odd)) q += copysignf(1.0f, left);
-      w |= ((uint32_t)(int)fminf(fmaxf(q, -127.0f), 127.0f) & 0xffu) << (8 * i);
+      r[i] = fmaf(x[i], inv, ROUND);
+      near = fmaxf(near, fabsf(fmaf(x[i], inv, ROUND - r[i])));
     }
-    return w;
+    // x / s and x * inv differ by less than 2^-15, so that a code may be another one next to a half alone
+    if (__builtin_expect(near > 0.4999f || odd, 0)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y = x[i] == x[i] ? x[i] : 0.0f;
+        float q = rintf(y * inv);
+        // what is left is exact where it is near half of s (a multiple of half a unit of s, and at most s): so is the decision
+        const float left = fmaf(-q, s, y), half = 0.5f * s;
+        const bool uneven = (q - 2.0f * floorf(0.5f * q)) != 0.0f;
+        if (fabsf(left) > half || (fabsf(left) == half && uneven)) q += copysignf(1.0f, left);
+        r[i] = fminf(fmaxf(q, -MOST), MOST) + ROUND;
+      }
+    }
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(r[3]), __float_as_uint(r[2]), 0x04000c0cu);
+    return lo | hi;
   }
 }
 
@@ -104,7 +133,7 @@ __global__ __launch_bounds__(kBaThreads) void byte_append_kernel(AppendArgs a, i
   __shared__ uint32_t turned[256 * 17];   // codes of V: [element][row / 4], a word of four rows
   __shared__ uint32_t tops[2][kBaThreads / kWave];
   if (whole) {
-    AppendPart<T> kx[U], vx[U];
+    Vec16<T> kx[U][4], vx[U][4];   // sixteen bytes of four successive rows
     uint32_t k_top = 0, v_top = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -115,29 +144,44 @@ __global__ __launch_bounds__(kBaThreads) void byte_append_kernel(AppendArgs a, i
         const int token = block * kByBlock + 4 * rows + r;
         const bool old = token < len;
         const int64_t at = old ? 0 : fresh(token);
-        Vec16<T> y;
-        y.load((old ? kt + (int64_t)(token % kByTail) * a.d : kn + at * a.kr) + N * piece);
-        y.unpack(kx[u].x[r]);
-        y.load((old ? vt + (int64_t)(token % kByTail) * a.d : vn + at * a.vr) + N * piece);
-        y.unpack(vx[u].x[r]);
+        kx[u][r].load((old ? kt + (int64_t)(token % kByTail) * a.d : kn + at * a.kr) + N * piece);
+        vx[u][r].load((old ? vt + (int64_t)(token % kByTail) * a.d : vn + at * a.vr) + N * piece);
+      }
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          k_top = max(k_top, ap_finite(kx[u].x[r][e]));
-          v_top = max(v_top, ap_finite(vx[u].x[r][e]));
-        }
+      for (int r = 0; r < 4; ++r) {
+        k_top = max(k_top, ap_top(kx[u][r]));
+        v_top = max(v_top, ap_top(vx[u][r]));
       }
     }
-    k_top = wave_reduce_u32(k_top, [](uint32_t x, uint32_t y) { return max(x, y); });
-    v_top = wave_reduce_u32(v_top, [](uint32_t x, uint32_t y) { return max(x, y); });
-    if (lane_id() == 0) {
-      tops[0][wave_id()] = k_top;
-      tops[1][wave_id()] = v_top;
-    }
-    __syncthreads();
+    auto all = [&](uint32_t& k, uint32_t& v) {   // over the workgroup; holds barriers
+      k = wave_reduce_u32(k, [](uint32_t x, uint32_t y) { return max(x, y); });
+      v = wave_reduce_u32(v, [](uint32_t x, uint32_t y) { return max(x, y); });
+      __syncthreads();
+      if (lane_id() == 0) {
+        tops[0][wave_id()] = k;
+        tops[1][wave_id()] = v;
+      }
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kBaThreads / kWave; ++w) {
-      k_top = max(k_top, tops[0][w]);
-      v_top = max(v_top, tops[1][w]);
+      for (int w = 0; w < kBaThreads / kWave; ++w) {
+        k = max(k, tops[0][w]);
+        v = max(v, tops[1][w]);
+      }
+    };
+    all(k_top, v_top);
+    const bool odd = max(k_top, v_top) >= 0x7f800000u;
+    if (odd) {
+      k_top = v_top = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if ((tid + u * kBaThreads) / pieces >= kByBlock / 4) continue;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          k_top = max(k_top, ap_finite_top(kx[u][r]));
+          v_top = max(v_top, ap_finite_top(vx[u][r]));
+        }
+      }
+      all(k_top, v_top);
     }
     const float ks = ap_scale<FP8>(k_top), vs = ap_scale<FP8>(v_top), k_inv = 1.0f / ks, v_inv = 1.0f / vs;
     const int64_t at = head * a.blocks + block;
@@ -153,17 +197,22 @@ __global__ __launch_bounds__(kBaThreads) void byte_append_kernel(AppendArgs a, i
       if (rows >= kByBlock / 4) continue;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
+        float x[N];
+        kx[u][r].unpack(x);
         uint32_t w[N / 4];
 #pragma unroll
-        for (int e = 0; e < N / 4; ++e)
-          w[e] = ap_codes<FP8>(kx[u].x[r][4 * e], kx[u].x[r][4 * e + 1], kx[u].x[r][4 * e + 2], kx[u].x[r][4 * e + 3], ks, k_inv);
-        uint32_t* to = (uint32_t*)(kc + (4 * rows + r) * dp + N * piece);
-#pragma unroll
-        for (int e = 0; e < N / 4; ++e) to[e] = w[e];
+        for (int e = 0; e < N / 4; ++e) w[e] = ap_codes<FP8>(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3], ks, k_inv, odd);
+        char* to = kc + (4 * rows + r) * dp + N * piece;
+        if constexpr (N == 8)
+          *(uint2*)to = make_uint2(w[0], w[1]);
+        else
+          *(uint32_t*)to = w[0];
       }
+      float x[4][N];
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        turned[(N * piece + e) * 17 + rows] = ap_codes<FP8>(vx[u].x[0][e], vx[u].x[1][e], vx[u].x[2][e], vx[u].x[3][e], vs, v_inv);
+      for (int r = 0; r < 4; ++r) vx[u][r].unpack(x[r]);
+#pragma unroll
+      for (int e = 0; e < N; ++e) turned[(N * piece + e) * 17 + rows] = ap_codes<FP8>(x[0][e], x[1][e], x[2][e], x[3][e], vs, v_inv, odd);
     }
     __syncthreads();
     for (int i = tid; i < a.d * 4; i += kBaThreads) {
