@@ -107,23 +107,24 @@ __device__ __forceinline__ float ap_scale(uint32_t top_bits) {
   }
 }
 
-// A workgroup: a block of a head that the call reaches, and in the first of them what goes into the tail.  (That one reads the
-// rows that the tail has of the block before it writes there.)
+// A workgroup: the keys or the values (blockIdx.z) of a block of a head that the call reaches, and in the first of them what
+// goes into the tail.  (That one reads the rows that the tail has of the block before it writes there.)  Bound by memory: a
+// prompt of 32K tokens, 8 heads of 128 bf16 elements, 210 MB in 43 us, what a copy takes; few tokens by the chain of lengths,
+// rows, scale and codes, 5 us.
 template <typename T, bool FP8, int U>
 __global__ __launch_bounds__(kBaThreads) void byte_append_kernel(AppendArgs a, int dp) {
   constexpr int N = Vec16<T>::N;
   const int b = (int)blockIdx.y / a.h, h = (int)blockIdx.y % a.h, tid = threadIdx.x;
+  const bool values = blockIdx.z != 0;
   const int len = min(max(a.lengths[b], 0), a.blocks * kByBlock);
   const int count = min(a.counts ? min(max(a.counts[b], 0), a.most) : a.most, a.blocks * kByBlock - len), end = len + count;
-  if (blockIdx.x == 0 && h == 0 && tid == 0) a.new_lengths[b] = end;
+  if (blockIdx.x == 0 && h == 0 && !values && tid == 0) a.new_lengths[b] = end;
   const int block = len / kByBlock + (int)blockIdx.x;
   const bool whole = (block + 1) * kByBlock <= end;   // (blocks * 64 <= 2^30)
   if (!whole && blockIdx.x != 0) return;
-  const T* kn = (const T*)a.k_new + b * a.kb + h * a.kh;
-  const T* vn = (const T*)a.v_new + b * a.vb + h * a.vh;
-  const int64_t head = (int64_t)b * a.h + h;
-  T* kt = (T*)a.k_tail + head * kByTail * a.d;
-  T* vt = (T*)a.v_tail + head * kByTail * a.d;
+  const int64_t head = (int64_t)b * a.h + h, row_stride = values ? a.vr : a.kr;
+  const T* rows_new = values ? (const T*)a.v_new + b * a.vb + h * a.vh : (const T*)a.k_new + b * a.kb + h * a.kh;
+  T* tail = (T*)(values ? a.v_tail : a.k_tail) + head * kByTail * a.d;
   const int32_t* path = a.path ? a.path + b * a.path_b : nullptr;
   auto fresh = [&](int token) {   // the new row that a token is
     const int i = token - len;
@@ -131,114 +132,102 @@ __global__ __launch_bounds__(kBaThreads) void byte_append_kernel(AppendArgs a, i
   };
   const int pieces = a.d / N;
   __shared__ uint32_t turned[256 * 17];   // codes of V: [element][row / 4], a word of four rows
-  __shared__ uint32_t tops[2][kBaThreads / kWave];
+  __shared__ uint32_t tops[kBaThreads / kWave];
   if (whole) {
-    Vec16<T> kx[U][4], vx[U][4];   // sixteen bytes of four successive rows
-    uint32_t k_top = 0, v_top = 0;
+    Vec16<T> x[U][4];   // sixteen bytes of four successive rows
+    int rows[U], piece[U];
+    uint32_t top = 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int unit = tid + u * kBaThreads, rows = unit / pieces, piece = unit % pieces;
-      if (rows >= kByBlock / 4) continue;
+      const int unit = tid + u * kBaThreads;
+      rows[u] = unit / pieces;
+      piece[u] = unit % pieces;
+      if (rows[u] >= kByBlock / 4) continue;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int token = block * kByBlock + 4 * rows + r;
-        const bool old = token < len;
-        const int64_t at = old ? 0 : fresh(token);
-        kx[u][r].load((old ? kt + (int64_t)(token % kByTail) * a.d : kn + at * a.kr) + N * piece);
-        vx[u][r].load((old ? vt + (int64_t)(token % kByTail) * a.d : vn + at * a.vr) + N * piece);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        k_top = max(k_top, ap_top(kx[u][r]));
-        v_top = max(v_top, ap_top(vx[u][r]));
+        const int token = block * kByBlock + 4 * rows[u] + r;
+        x[u][r].load((token < len ? tail + (int64_t)(token % kByTail) * a.d : rows_new + fresh(token) * row_stride) + N * piece[u]);
       }
     }
-    auto all = [&](uint32_t& k, uint32_t& v) {   // over the workgroup; holds barriers
-      k = wave_reduce_u32(k, [](uint32_t x, uint32_t y) { return max(x, y); });
-      v = wave_reduce_u32(v, [](uint32_t x, uint32_t y) { return max(x, y); });
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (rows[u] < kByBlock / 4)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = max(top, ap_top(x[u][r]));
+    auto all = [&](uint32_t v) {   // over the workgroup; holds barriers
+      v = wave_reduce_u32(v, [](uint32_t a, uint32_t b) { return max(a, b); });
       __syncthreads();
-      if (lane_id() == 0) {
-        tops[0][wave_id()] = k;
-        tops[1][wave_id()] = v;
-      }
+      if (lane_id() == 0) tops[wave_id()] = v;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < kBaThreads / kWave; ++w) {
-        k = max(k, tops[0][w]);
-        v = max(v, tops[1][w]);
-      }
+      for (int w = 0; w < kBaThreads / kWave; ++w) v = max(v, tops[w]);
+      return v;
     };
-    all(k_top, v_top);
-    const bool odd = max(k_top, v_top) >= 0x7f800000u;
+    top = all(top);
+    const bool odd = top >= 0x7f800000u;
     if (odd) {
-      k_top = v_top = 0;
+      top = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (rows[u] < kByBlock / 4)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) top = max(top, ap_finite_top(x[u][r]));
+      top = all(top);
+    }
+    const float s = ap_scale<FP8>(top), inv = 1.0f / s;
+    const int64_t at = head * a.blocks + block;
+    if (tid == 0) (values ? a.vs : a.ks)[at] = s;
+    char* codes = (char*)(values ? a.v : a.k) + at * kByBlock * dp;
+    if (!values) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if ((tid + u * kBaThreads) / pieces >= kByBlock / 4) continue;
+        if (rows[u] >= kByBlock / 4) continue;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          k_top = max(k_top, ap_finite_top(kx[u][r]));
-          v_top = max(v_top, ap_finite_top(vx[u][r]));
+          float y[N];
+          x[u][r].unpack(y);
+          uint32_t w[N / 4];
+#pragma unroll
+          for (int e = 0; e < N / 4; ++e) w[e] = ap_codes<FP8>(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3], s, inv, odd);
+          char* to = codes + (4 * rows[u] + r) * dp + N * piece[u];
+          if constexpr (N == 8)
+            *(uint2*)to = make_uint2(w[0], w[1]);
+          else
+            *(uint32_t*)to = w[0];
         }
       }
-      all(k_top, v_top);
-    }
-    const float ks = ap_scale<FP8>(k_top), vs = ap_scale<FP8>(v_top), k_inv = 1.0f / ks, v_inv = 1.0f / vs;
-    const int64_t at = head * a.blocks + block;
-    if (tid == 0) {
-      a.ks[at] = ks;
-      a.vs[at] = vs;
-    }
-    char* kc = (char*)a.k + at * kByBlock * dp;
-    char* vc = (char*)a.v + at * kByBlock * dp;
+    } else {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int unit = tid + u * kBaThreads, rows = unit / pieces, piece = unit % pieces;
-      if (rows >= kByBlock / 4) continue;
+      for (int u = 0; u < U; ++u) {
+        if (rows[u] >= kByBlock / 4) continue;
+        float y[4][N];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float x[N];
-        kx[u][r].unpack(x);
-        uint32_t w[N / 4];
+        for (int r = 0; r < 4; ++r) x[u][r].unpack(y[r]);
 #pragma unroll
-        for (int e = 0; e < N / 4; ++e) w[e] = ap_codes<FP8>(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3], ks, k_inv, odd);
-        char* to = kc + (4 * rows + r) * dp + N * piece;
-        if constexpr (N == 8)
-          *(uint2*)to = make_uint2(w[0], w[1]);
-        else
-          *(uint32_t*)to = w[0];
+        for (int e = 0; e < N; ++e) turned[(N * piece[u] + e) * 17 + rows[u]] = ap_codes<FP8>(y[0][e], y[1][e], y[2][e], y[3][e], s, inv, odd);
       }
-      float x[4][N];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) vx[u][r].unpack(x[r]);
-#pragma unroll
-      for (int e = 0; e < N; ++e) turned[(N * piece + e) * 17 + rows] = ap_codes<FP8>(x[0][e], x[1][e], x[2][e], x[3][e], vs, v_inv, odd);
-    }
-    __syncthreads();
-    for (int i = tid; i < a.d * 4; i += kBaThreads) {
-      const uint32_t* from = turned + (i / 4) * 17 + 4 * (i % 4);
-      *(uint4*)(vc + 16 * i) = make_uint4(from[0], from[1], from[2], from[3]);
+      __syncthreads();
+      for (int i = tid; i < a.d * 4; i += kBaThreads) {
+        const uint32_t* from = turned + (i / 4) * 17 + 4 * (i % 4);
+        *(uint4*)(codes + 16 * i) = make_uint4(from[0], from[1], from[2], from[3]);
+      }
     }
   }
   if (blockIdx.x == 0) {
     // (every row of the tail that the block wanted has been read: the barriers above)
     const int first = max(len, end - kByTail);
     for (int i = tid; i < (end - first) * pieces; i += kBaThreads) {
-      const int token = first + i / pieces, piece = i % pieces;
-      const int64_t from = fresh(token);
-      Vec16<T> x, y;
-      x.load(kn + from * a.kr + N * piece);
-      y.load(vn + from * a.vr + N * piece);
-      const int64_t to = (int64_t)(token % kByTail) * a.d + N * piece;
-      x.store(kt + to);
-      y.store(vt + to);
+      const int token = first + i / pieces;
+      Vec16<T> y;
+      y.load(rows_new + fresh(token) * row_stride + N * (i % pieces));
+      y.store(tail + (int64_t)(token % kByTail) * a.d + N * (i % pieces));
     }
   }
 }
 
 template <typename T, bool FP8>
 static int append_launch(const AppendArgs& a, int b, hipStream_t st) {
-  const dim3 grid((unsigned)std::min<int64_t>(((int64_t)a.most + kByBlock - 1) / kByBlock + 1, a.blocks), (unsigned)(b * a.h));
+  const dim3 grid((unsigned)std::min<int64_t>(((int64_t)a.most + kByBlock - 1) / kByBlock + 1, a.blocks), (unsigned)(b * a.h), 2);
   LRQK_REQUIRE((int64_t)grid.x * kBaThreads <= kMaxThreads, LRQK_ELIMIT, "%d tokens are more than a launch has places for", a.most);
   const int units = a.d / Vec16<T>::N * (kByBlock / 4), dp = by_width(a.d);
   if (units <= kBaThreads) hipLaunchKernelGGL((byte_append_kernel<T, FP8, 1>), grid, dim3(kBaThreads), 0, st, a, dp);
