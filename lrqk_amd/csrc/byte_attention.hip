@@ -20,7 +20,9 @@ namespace lrqk {
 
 typedef _Float16 by_h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 by_h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 by_h4 __attribute__((ext_vector_type(4)));
 typedef float by_f8 __attribute__((ext_vector_type(8)));
+typedef float by_f4 __attribute__((ext_vector_type(4)));
 
 constexpr float kByUp = 8.0f;          // binary orders that probabilities are formed too large
 constexpr float kByMost = 15.0f;       // binary logarithm of the largest one before they are formed anew (fp16 ends at 2^16)
@@ -71,12 +73,12 @@ __device__ __forceinline__ void by_halves(const float (&x)[8], by_h8& hi, by_h8&
   if constexpr (TWO) lo = __builtin_convertvector(v - __builtin_convertvector(hi, by_f8), by_h8);
 }
 
-// A tile's scores x become probabilities p = 2^(x f + shift - top), in place, and sum that of 2^(x f - top); f: of each query,
-// less = 2^-shift.  top is not the maximum so far but what serves as one: as long as no probability is above 2^kByMost it
-// stays, and only where one would be it becomes the maximum less kByUp, o and the sums rescaled to it.
+// Before scores x become probabilities 2^(x f + shift - top); f: of each query.  top is not the maximum so far but what serves
+// as one: as long as no probability is above 2^kByMost it stays, and only where one would be it becomes the maximum less
+// kByUp, o and the sums rescaled to it.
 template <int MT, int NE, int VW>
-__device__ __forceinline__ void by_softmax(float (&x)[MT][NE], const float (&f)[MT], float shift, float less, float (&top)[MT], float (&sum)[MT],
-                                           ar_f4 (&o)[MT][VW]) {
+__device__ __forceinline__ void by_top(const float (&x)[MT][NE], const float (&f)[MT], float shift, float (&top)[MT], float (&sum)[MT],
+                                       ar_f4 (&o)[MT][VW]) {
   float high[MT];
   bool more = false;
 #pragma unroll
@@ -96,17 +98,6 @@ __device__ __forceinline__ void by_softmax(float (&x)[MT][NE], const float (&f)[
 #pragma unroll
       for (int j = 0; j < VW; ++j) o[m][j] *= g;
     }
-  }
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const float from = shift - top[m];
-    float part = 0.0f;
-#pragma unroll
-    for (int e = 0; e < NE; ++e) {
-      x[m][e] = ar_exp2(fmaf(x[m][e], f[m], from));
-      part = e == 0 ? x[m][0] : part + x[m][e];
-    }
-    sum[m] = fmaf(part, less, sum[m]);
   }
 }
 
@@ -174,105 +165,95 @@ struct ByteWave {
     unit = FOLD ? vs : 1.0f;
     log_unit = FOLD ? __builtin_amdgcn_logf(vs) : 0.0f;
   }
-  // A block: k(u, s) and v(j, h) are its operands; between: what is done once the keys are not wanted any more.  AHEAD: they
-  // come from LDS, and are asked for in front of what is done before they are wanted.
-  template <bool AHEAD, typename K, typename V, typename B>
-  __device__ __forceinline__ void block(float ks, float vs, K k, V v, B between) {
-    constexpr int VA = AHEAD ? VW / 2 : 0;   // (all of them: no registers left)
-    by_h8 va[AHEAD ? VA : 1][2];
-    float x[MT][16], f[MT];
-    by_h8 kf[2][2 * CH];
+  float x[MT][16];   // scores of a block's keys, key 16 quad + 4 u + r in [4 u + r]
+  // Scores of its u-th 16 keys, whose operands are kf.
+  __device__ __forceinline__ void scores(int u, const by_h8 (&kf)[2 * CH]) {
 #pragma unroll
-    for (int s = 0; s < 2 * CH; ++s) kf[0][s] = k(0, s);
+    for (int m = 0; m < MT; ++m) {
+      ar_f4 c = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (AHEAD && u < 3) {
-#pragma unroll
-        for (int s = 0; s < 2 * CH; ++s) kf[(u + 1) & 1][s] = k(u + 1, s);
-        __builtin_amdgcn_sched_barrier(0x7f);   // (reads of LDS stay in front)
-      } else if (!AHEAD && u > 0) {
-#pragma unroll
-        for (int s = 0; s < 2 * CH; ++s) kf[u & 1][s] = k(u, s);
+      for (int s = 0; s < 2 * CH; ++s) {
+        if constexpr (TWO) c = by_step(kf[s], ql[m][s], c);
+        c = by_step(kf[s], qh[m][s], c);
       }
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        ar_f4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int r = 0; r < 4; ++r) x[m][4 * u + r] = c[r];
+    }
+  }
+  // What a block's scales make of its scores and products.
+  struct Scales {
+    float f[MT], from[MT], less, by;
+    bool apart;
+  };
+  __device__ __forceinline__ Scales scales(float ks, float vs) {
+    Scales g;
+    float shift = FOLD ? __builtin_amdgcn_logf(vs) - log_unit : 0.0f;
+    g.apart = !FOLD || !(fabsf(shift) <= 8.0f);
+    g.less = g.apart ? 1.0f : unit * __builtin_amdgcn_rcpf(vs);
+    g.by = vs / unit;
+    shift = g.apart ? 0.0f : shift;
 #pragma unroll
-        for (int s = 0; s < 2 * CH; ++s) {
-          if constexpr (TWO) c = by_step(kf[u & 1][s], ql[m][s], c);
-          c = by_step(kf[u & 1][s], qh[m][s], c);
-        }
+    for (int m = 0; m < MT; ++m) g.f[m] = up[m] * ks;
+    by_top<MT, 16, VW>(x, g.f, shift, top, sum, o);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[m][4 * u + r] = c[r];
+    for (int m = 0; m < MT; ++m) g.from[m] = shift - top[m];
+    return g;
+  }
+  // Probabilities of keys 4 u .. 4 u + 3 of every quad, in p: 16-bit halves of [m][u / 2].
+  __device__ __forceinline__ void probabilities(int u, const Scales& g, float (&part)[MT], by_h4 (&ph)[MT][4], by_h4 (&pl)[TWO ? MT : 1][4]) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      by_f4 p;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        p[r] = ar_exp2(fmaf(x[m][4 * u + r], g.f[m], g.from[m]));
+        part[m] = u + r == 0 ? p[0] : part[m] + p[r];
+      }
+      ph[m][u] = __builtin_convertvector(p, by_h4);
+      if constexpr (TWO) pl[m][u] = __builtin_convertvector(p - __builtin_convertvector(ph[m][u], by_f4), by_h4);
+    }
+  }
+  // o += of the j-th 16 elements; v0, v1: V's operands of the first and the last 8 keys of every quad
+  __device__ __forceinline__ void products(int j, by_h8 v0, by_h8 v1, const Scales& g, const by_h4 (&ph)[MT][4], const by_h4 (&pl)[TWO ? MT : 1][4]) {
+    auto both = [](by_h4 a, by_h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); };
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      ar_f4 c = FOLD ? o[m][j] : ar_f4{0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (TWO) {
+        c = by_step(v0, both(pl[m][0], pl[m][1]), c);
+        c = by_step(v1, both(pl[m][2], pl[m][3]), c);
+      }
+      c = by_step(v0, both(ph[m][0], ph[m][1]), c);
+      c = by_step(v1, both(ph[m][2], ph[m][3]), c);
+      if constexpr (FOLD) {
+        o[m][j] = c;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[m][j][r] = fmaf(c[r], g.by, o[m][j][r]);
       }
     }
-    between();
-    if constexpr (AHEAD) {
-#pragma unroll
-      for (int j = 0; j < VA; ++j) {
-        va[j][0] = v(j, 0);
-        va[j][1] = v(j, 1);
-      }
-      __builtin_amdgcn_sched_barrier(0x7f);
-    }
-    const float shift = FOLD ? __builtin_amdgcn_logf(vs) - log_unit : 0.0f;
-    const bool apart = !FOLD || !(fabsf(shift) <= 8.0f);
-#pragma unroll
-    for (int m = 0; m < MT; ++m) f[m] = up[m] * ks;
-    by_softmax<MT, 16, VW>(x, f, apart ? 0.0f : shift, apart ? 1.0f : unit * __builtin_amdgcn_rcpf(vs), top, sum, o);
-    by_h8 ph[MT][2], pl[TWO ? MT : 1][2];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = x[m][8 * h + e];
-        by_halves<TWO>(y, ph[m][h], pl[TWO ? m : 0][h]);
-      }
-    if constexpr (!FOLD) {
-#pragma unroll
-      for (int j = 0; j < VW; ++j) {
-        const by_h8 v0 = j < VA ? va[j < VA ? j : 0][0] : v(j, 0), v1 = j < VA ? va[j < VA ? j : 0][1] : v(j, 1);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          ar_f4 c = {0.0f, 0.0f, 0.0f, 0.0f};
-          if constexpr (TWO) {
-            c = by_step(v0, pl[m][0], c);
-            c = by_step(v1, pl[m][1], c);
-          }
-          c = by_step(v0, ph[m][0], c);
-          c = by_step(v1, ph[m][1], c);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[m][j][r] = fmaf(c[r], vs, o[m][j][r]);
-        }
-      }
-    } else {
-      // (a block whose scale is far from the first's: what there is waits in memory.  As a branch of its own, with products of
-      // its own, it cost every block the copying of all outputs from register to register.)
-      volatile float waiting[MT * VW * 4];
-      if (__builtin_expect(apart, 0)) {
+  }
+  // Around the products of a block whose scale is far from the first's (FOLD): what there is waits in memory meanwhile.  (As a
+  // branch with products of its own it cost every block the copying of all outputs from register to register.)
+  struct Waiting {
+    volatile float o[FOLD ? MT * VW * 4 : 1];
+  };
+  __device__ __forceinline__ void put_by(const Scales& g, Waiting& w) {
+    if constexpr (FOLD)
+      if (__builtin_expect(g.apart, 0)) {
 #pragma unroll
         for (int i = 0; i < MT * VW * 4; ++i) {
-          waiting[i] = o[i / 4 / VW][i / 4 % VW][i % 4];
+          w.o[i] = o[i / 4 / VW][i / 4 % VW][i % 4];
           o[i / 4 / VW][i / 4 % VW][i % 4] = 0.0f;
         }
       }
+  }
+  __device__ __forceinline__ void take_up(const Scales& g, Waiting& w) {
+    if constexpr (FOLD)
+      if (__builtin_expect(g.apart, 0)) {
 #pragma unroll
-      for (int j = 0; j < VW; ++j) {
-        const by_h8 v0 = j < VA ? va[j < VA ? j : 0][0] : v(j, 0), v1 = j < VA ? va[j < VA ? j : 0][1] : v(j, 1);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          o[m][j] = by_step(v0, ph[m][0], o[m][j]);
-          o[m][j] = by_step(v1, ph[m][1], o[m][j]);
-        }
+        for (int i = 0; i < MT * VW * 4; ++i) o[i / 4 / VW][i / 4 % VW][i % 4] = fmaf(o[i / 4 / VW][i / 4 % VW][i % 4], g.by, w.o[i]);
       }
-      if (__builtin_expect(apart, 0)) {
-        const float by = vs / unit;
-#pragma unroll
-        for (int i = 0; i < MT * VW * 4; ++i) o[i / 4 / VW][i / 4 % VW][i % 4] = fmaf(o[i / 4 / VW][i / 4 % VW][i % 4], by, waiting[i]);
-      }
-    }
   }
   __device__ __forceinline__ void end() {
     if constexpr (FOLD) {
@@ -384,7 +365,17 @@ __device__ __forceinline__ void by_dense(const ByteArgs& ba, const ByteCut& cut,
 #pragma unroll
         for (int e = 0; e < NE; ++e) x[m][e] = quad * NE + e < valid ? x[m][e] : -INFINITY;
     }
-    by_softmax<MT, NE, VW>(x, f, 0.0f, 1.0f, top, sum, o);
+    by_top<MT, NE, VW>(x, f, 0.0f, top, sum, o);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      float part = 0.0f;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        x[m][e] = ar_exp2(fmaf(x[m][e], f[m], -top[m]));
+        part += x[m][e];
+      }
+      sum[m] += part;
+    }
 #pragma unroll
     for (int e = 0; e < NE; ++e)
 #pragma unroll
@@ -445,7 +436,7 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba)
     // what a lane reads of a block: CH pieces of 4 x 16 keys, and VW pieces of V
     const uint32_t kat = (uint32_t)((col >> 2) * 16 + (col & 3)) * DP + quad * 16, vat = (uint32_t)(VW * col) * kByBlock + quad * 16;
     ar_u4 kg[4][CH], vg[VW];
-    float ks, vs, ks_next = 0.0f, vs_next = 0.0f;
+    float ks_next = 0.0f, vs_next = 0.0f;
     auto load_k = [&](int i) {
       const char* src = (const char*)ba.k + (block0 + i) * (kByBlock * DP);
       ks_next = ba.ks[block0 + i];
@@ -468,10 +459,27 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba)
     }
     for (; block < end; block += kTrWaves) {
       const int next = block + kTrWaves < end ? block + kTrWaves : block;   // (the next one, or this one again)
-      ks = ks_next;
-      vs = vs_next;
-      w.template block<false>(ks, vs, [&](int u, int s) { return by_unpack<FP8>(kg[u][s / 2][s % 2 * 2], kg[u][s / 2][s % 2 * 2 + 1]); },
-              [&](int j, int h) { return by_unpack<FP8>(vg[j][2 * h], vg[j][2 * h + 1]); }, [&] { load_k(next); });
+      const float ks = ks_next, vs = vs_next;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        by_h8 kf[2 * CH];
+#pragma unroll
+        for (int s = 0; s < 2 * CH; ++s) kf[s] = by_unpack<FP8>(kg[u][s / 2][s % 2 * 2], kg[u][s / 2][s % 2 * 2 + 1]);
+        w.scores(u, kf);
+      }
+      load_k(next);
+      const typename Wave::Scales g = w.scales(ks, vs);
+      float part[MT];
+      by_h4 ph[MT][4], pl[Wave::TWO ? MT : 1][4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) w.probabilities(u, g, part, ph, pl);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) w.sum[m] = fmaf(part[m], g.less, w.sum[m]);
+      typename Wave::Waiting put;
+      w.put_by(g, put);
+#pragma unroll
+      for (int j = 0; j < VW; ++j) w.products(j, by_unpack<FP8>(vg[j][0], vg[j][1]), by_unpack<FP8>(vg[j][2], vg[j][3]), g, ph, pl);
+      w.take_up(g, put);
       load_v(next);
     }
     w.end();
@@ -480,14 +488,16 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba)
 }
 
 // Many queries: the four waves have 16 MT of them each and share the blocks.  Each wave makes a quarter of a block's codes
-// fp16 operands and leaves them in LDS, in the order in which lanes read them; two blocks are there, one barrier a block.
+// fp16 operands and leaves them in LDS, in the order in which lanes read them.  While a block's probabilities are formed the
+// next one's scores are multiplied, 16 keys at a time into the registers that those 16 leave, since a wave's exponentials and
+// products run side by side only if they are next to each other: so LDS has a block's values and the next one's keys, and
+// those that follow are written meanwhile; one barrier a block.
 template <typename T, bool FP8, int DP, int MT>
 __global__ __launch_bounds__(kTrThreads, 2) void byte_share_kernel(ByteArgs ba) {
   const TreeArgs& a = ba.tree;
   using Wave = ByteWave<T, DP, MT>;
   constexpr int VW = Wave::VW, CH = Wave::CH, VL = VW / kTrWaves;   // pieces of V of a wave (of K: CH)
-  constexpr int KN = 4 * 2 * CH, VN = VW * 2;                       // operands of a block
-  __shared__ by_h8 held[2][KN + VN][kWave];
+  __shared__ by_h8 keys[2][4 * 2 * CH][kWave], values[2][VW * 2][kWave];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), col = lane & 15, quad = lane >> 4;
   BytePlace at;
   if (!at.find(a)) return;
@@ -501,39 +511,80 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_share_kernel(ByteArgs ba) 
     if (row0 < at.M) by_dense<T, DP, MT>(ba, cut, at.hc, row0, at.M, q, 0, 1, w.top, w.sum, w.o, odd);
   } else {
     const int64_t block0 = ((int64_t)cut.b * a.hc + at.hc) * ba.blocks;
-    const int begin = (cut.split - 1) * cut.per, end = min(cut.len / kByBlock, begin + cut.per);
+    const int begin = (cut.split - 1) * cut.per, last = min(cut.len / kByBlock, begin + cut.per) - 1;   // (a split has a block at least)
     const uint32_t kat = (uint32_t)((col >> 2) * 16 + (col & 3)) * DP + quad * 16, vat = (uint32_t)(VW * col) * kByBlock + quad * 16;
-    ar_u4 kg[CH], vg[VL];
-    auto load = [&](int i) {   // (the wave's part of block i)
-      const char* ks = (const char*)ba.k + (block0 + i) * (kByBlock * DP) + wave * 4 * DP;
-      const char* vs = (const char*)ba.v + (block0 + i) * (kByBlock * DP) + wave * VL * kByBlock;
+    ar_u4 kg[CH], vg[VL];   // the wave's part of the next keys and values to be written
+    auto load_k = [&](int i) {   // (behind the last block it comes again)
+      const char* src = (const char*)ba.k + (block0 + min(i, last)) * (kByBlock * DP) + wave * 4 * DP;
 #pragma unroll
-      for (int c = 0; c < CH; ++c) kg[c] = tree_at<ar_u4>(ks + c * 64, kat);
-#pragma unroll
-      for (int j = 0; j < VL; ++j) vg[j] = tree_at<ar_u4>(vs + j * kByBlock, vat);
+      for (int c = 0; c < CH; ++c) kg[c] = tree_at<ar_u4>(src + c * 64, kat);
     };
-    auto leave = [&](int side) {
+    auto load_v = [&](int i) {
+      const char* src = (const char*)ba.v + (block0 + min(i, last)) * (kByBlock * DP) + wave * VL * kByBlock;
+#pragma unroll
+      for (int j = 0; j < VL; ++j) vg[j] = tree_at<ar_u4>(src + j * kByBlock, vat);
+    };
+    auto leave_k = [&](int side) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) held[side][wave * 2 * CH + 2 * c + h][lane] = by_unpack<FP8>(kg[c][2 * h], kg[c][2 * h + 1]);
+        for (int h = 0; h < 2; ++h) keys[side][wave * 2 * CH + 2 * c + h][lane] = by_unpack<FP8>(kg[c][2 * h], kg[c][2 * h + 1]);
+    };
+    auto leave_v = [&](int side) {
 #pragma unroll
       for (int j = 0; j < VL; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) held[side][KN + (wave * VL + j) * 2 + h][lane] = by_unpack<FP8>(vg[j][2 * h], vg[j][2 * h + 1]);
+        for (int h = 0; h < 2; ++h) values[side][(wave * VL + j) * 2 + h][lane] = by_unpack<FP8>(vg[j][2 * h], vg[j][2 * h + 1]);
     };
-    load(begin);   // (a split has a block at least)
+    auto operands = [&](int side, int u, by_h8 (&kf)[2 * CH]) {
+#pragma unroll
+      for (int s = 0; s < 2 * CH; ++s) kf[s] = keys[side][u * 2 * CH + s][lane];
+    };
+    load_k(begin);
+    load_v(begin);
     w.queries(q, row0, at.M, a.d, a.scale_log2e);
     w.first(ba.vs[block0 + begin]);
-    leave(0);
-    load(min(begin + 1, end - 1));
+    leave_k(0);
+    load_k(begin + 1);
+    leave_v(0);
+    load_v(begin + 1);
+    leave_k(1);
+    load_k(begin + 2);
     __syncthreads();
-    for (int block = begin; block < end; ++block) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      by_h8 kf[2 * CH];
+      operands(0, u, kf);
+      w.scores(u, kf);
+    }
+    __syncthreads();
+    // (a block's scales are asked for a block ahead: a wait for them is one for all of LDS's reads too)
+    float ks = ba.ks[block0 + begin], vs = ba.vs[block0 + begin];
+    for (int block = begin; block <= last; ++block) {
       const int side = (block - begin) & 1;
-      leave(side ^ 1);   // (the next one; behind the last one itself again)
-      load(min(block + 2, end - 1));
-      w.template block<true>(ba.ks[block0 + block], ba.vs[block0 + block], [&](int u, int s) { return held[side][u * 2 * CH + s][lane]; },
-                             [&](int j, int h) { return held[side][KN + 2 * j + h][lane]; }, [] {});
+      const typename Wave::Scales g = w.scales(ks, vs);
+      ks = ba.ks[block0 + min(block + 1, last)];
+      vs = ba.vs[block0 + min(block + 1, last)];
+      typename Wave::Waiting put;
+      w.put_by(g, put);
+      float part[MT];
+      by_h4 ph[MT][4], pl[Wave::TWO ? MT : 1][4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        by_h8 kf[2 * CH];
+        operands(side ^ 1, u, kf);
+        w.probabilities(u, g, part, ph, pl);
+        w.scores(u, kf);
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) w.sum[m] = fmaf(part[m], g.less, w.sum[m]);
+      leave_v(side ^ 1);
+      load_v(block + 2);
+      leave_k(side);
+      load_k(block + 3);
+#pragma unroll
+      for (int j = 0; j < VW; ++j) w.products(j, values[side][2 * j][lane], values[side][2 * j + 1][lane], g, ph, pl);
+      w.take_up(g, put);
       __syncthreads();
     }
     w.end();
@@ -565,7 +616,7 @@ static BytePlan byte_plan(int b, int hq, int hc, int t, int64_t blocks, int d, i
   BytePlan p;
   p.dp = by_width(d);
   const int64_t M = (int64_t)(hq / hc) * t;
-  p.share = M > 64;
+  p.share = M > (p.dp == 256 || dtype == LRQK_F32 ? 32 : 64);
   p.mt = M <= 16 || p.dp == 256 || (p.share && dtype == LRQK_F32) ? 1 : 2;
   p.rows = 16 * p.mt * (p.share ? kTrWaves : 1);
   p.row_blocks = (int)((M + p.rows - 1) / p.rows);
