@@ -616,8 +616,10 @@ static BytePlan byte_plan(int b, int hq, int hc, int t, int64_t blocks, int d, i
   BytePlan p;
   p.dp = by_width(d);
   const int64_t M = (int64_t)(hq / hc) * t;
-  p.share = M > (p.dp == 256 || dtype == LRQK_F32 ? 32 : 64);
-  p.mt = M <= 16 || p.dp == 256 || (p.share && dtype == LRQK_F32) ? 1 : 2;
+  p.share = M > (p.dp == 256 || (dtype == LRQK_F32 && blocks > 512) ? 32 : 64);
+  // 16 queries a wave: all there are, or all that registers have room for; or few blocks, which one workgroup per 16 queries is
+  // through sooner (32 queries over 8K: 14.5 us, with 32 a wave 17.1; over 64K 41.5 and 36.5, 64 over 64K 74 and 52)
+  p.mt = M <= 16 || p.dp == 256 || dtype == LRQK_F32 || (!p.share && b * hc * blocks <= 2048) ? 1 : 2;
   p.rows = 16 * p.mt * (p.share ? kTrWaves : 1);
   p.row_blocks = (int)((M + p.rows - 1) / p.rows);
   p.row_tiles = p.row_blocks * (p.rows / 16);
@@ -649,7 +651,7 @@ static int byte_launch(const ByteArgs& a, const BytePlan& p, hipStream_t st) {
   if (p.share) {
     hipLaunchKernelGGL((byte_share_kernel<T, FP8, DP, SHARE>), grid, dim3(kTrThreads), 0, st, a);
   } else {
-    if constexpr (DP < 256)
+    if constexpr (SHARE == 2)
       if (p.mt == 2) hipLaunchKernelGGL((byte_stream_kernel<T, FP8, DP, 2>), grid, dim3(kTrThreads), 0, st, a);
     if (p.mt == 1) hipLaunchKernelGGL((byte_stream_kernel<T, FP8, DP, 1>), grid, dim3(kTrThreads), 0, st, a);
   }
