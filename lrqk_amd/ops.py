@@ -928,6 +928,9 @@ def evict(weights: torch.Tensor, ids: torch.Tensor, k: torch.Tensor, v: torch.Te
     return new
 
 
+_SIX = struct.Struct("6q")
+
+
 class ByteCache:
     """Keys and values of ``heads`` heads of ``batch`` sequences in 8 bits, room for ``capacity`` tokens (rounded up to whole blocks).
 
@@ -962,6 +965,7 @@ class ByteCache:
         self._dev = k.get_device()
         self._sizes = (batch, heads, blocks, head_dim)
         self._places = tuple(x.data_ptr() for x in self._buffers)
+        self._code = _lib.CODES[kind]
 
     k, v, k_scale, v_scale, k_tail, v_tail = (property(lambda self, i=i: self._buffers[i]) for i in range(6))
 
@@ -982,30 +986,35 @@ def byte_append(cache: ByteCache, k: torch.Tensor, v: torch.Tensor, lengths: tor
     finite elements and at least 2^-100, code = element / scale rounded once, half to even; infinities get the largest code, NaN 0."""
     dev = _on_one_gpu(k, v, lengths, counts, path)
     b, h, blocks, d = cache._on(dev)
-    t = k.shape[2] if k.dim() == 4 else 0
+    t, dtype = k.shape[2] if k.dim() == 4 else 0, cache.dtype
     if t >> 31:
         _too_large(t)
-    dtype = cache.dtype
     _expect("k", k, (b, h, t, d), dtype, contiguous=False)
     _expect("v", v, (b, h, t, d), dtype, contiguous=False)
     _expect("lengths", lengths, (b,), torch.int32)
+    most, path_at, path_stride = t, None, 0
     if path is not None:
         if path.dim() != 2 or path.shape[0] != b or path.dtype != torch.int32 or (path.shape[1] > 1 and path.stride(1) != 1):
             raise ValueError(f"path is {tuple(path.shape)} {path.dtype}: int32 [{b},m] with contiguous rows is wanted")
-    most = t if path is None else path.shape[1]
-    if most >> 31:
-        _too_large(most)
+        most, path_at = path.shape[1], path.data_ptr()
+        if most >> 31:
+            _too_large(most)
+        if b > 1:
+            path_stride = path.stride(0)
     if counts is not None:
         _expect("counts", counts, (b,), torch.int32)
     if t == 0 or most == 0:
         return lengths.clone()
-    strides = (*_row_strides("k", k, b, h, t, d), *_row_strides("v", v, b, h, t, d))
-    if k.data_ptr() % 16 or v.data_ptr() % 16 or any(x * k.element_size() % 16 for x in strides):
+    k_at, v_at = k.data_ptr(), v.data_ptr()
+    ks, vs = _row_strides("k", k, b, h, t, d), _row_strides("v", v, b, h, t, d)
+    step = 7 if dtype == torch.bfloat16 else 3   # (elements of 16 bytes, less one)
+    if (k_at | v_at) & 15 or (ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) & step:
         k, v = _rows16(k), _rows16(v)
-        strides = (*_row_strides("k", k, b, h, t, d), *_row_strides("v", v, b, h, t, d))
+        k_at, v_at, ks, vs = k.data_ptr(), v.data_ptr(), _row_strides("k", k, b, h, t, d), _row_strides("v", v, b, h, t, d)
     new = torch.empty_like(lengths)
-    _launch(dev, _lib.load().lrqk_byte_append, k.data_ptr(), v.data_ptr(), struct.pack("6q", *strides), t, most, lengths.data_ptr(), _ptr(counts),
-            _ptr(path), path.stride(0) if path is not None and b > 1 else 0, new.data_ptr(), *cache._places, blocks, b, h, d, _lib.CODES[cache.kind], _dt(k))
+    _launch(dev, _lib.load().lrqk_byte_append, k_at, v_at, _SIX.pack(*ks, *vs), t, most, lengths.data_ptr(),
+            None if counts is None else counts.data_ptr(), path_at, path_stride, new.data_ptr(), *cache._places, blocks, b, h, d, cache._code,
+            _lib.F32 if step == 3 else _lib.BF16)
     return new
 
 
@@ -1024,7 +1033,7 @@ def byte_attention(q: torch.Tensor, cache: ByteCache, lengths: torch.Tensor, k_n
     if (b | hq | t | d) >> 31:
         _too_large(b, hq, t, d)
     dtype = cache.dtype
-    if (b, d) != (cb, cd) or q.dtype != dtype:
+    if b != cb or d != cd or q.dtype != dtype:
         raise ValueError(f"q is {tuple(q.shape)} {q.dtype}: [{cb},Hq,t,{cd}] {dtype} is wanted")
     if hq % hc:
         raise ValueError(f"{hq} query heads over {hc} heads of the cache")
@@ -1043,18 +1052,19 @@ def byte_attention(q: torch.Tensor, cache: ByteCache, lengths: torch.Tensor, k_n
             raise ValueError(f"mask is {tuple(mask.shape)} {mask.dtype}: bool or uint8 [t,t] or [b,t,t] is wanted")
     q = _rows16(q)
     out = torch.empty_like(q)
-    lse = torch.empty((b, hq, t), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = q.new_empty((b, hq, t), dtype=torch.float32) if return_lse else None
     if b * hq * t:
-        each = 0
+        each, kn_at, vn_at, mask_at = 0, None, None, None
         if k_new is not None:
             k_new, v_new, mask = _rows16(k_new), _rows16(v_new), mask.contiguous()
+            kn_at, vn_at, mask_at = k_new.data_ptr(), v_new.data_ptr(), mask.data_ptr()
             each = t * t if mask.dim() == 3 else 0
-        dt = _dt(q)
+        dt = _lib.F32 if dtype == torch.float32 else _lib.BF16
         need = _scratch_bytes("lrqk_byte_attention_workspace", b, hq, hc, t, blocks, d, dt)
-        ws = _scratch(need, q)
-        _launch(dev, _lib.load().lrqk_byte_attention, q.data_ptr(), *cache._places, blocks, lengths.data_ptr(), _ptr(k_new), _ptr(v_new), _ptr(mask), each,
-                out.data_ptr(), _ptr(lse), b, hq, hc, hn, t, d, d ** -0.5 if scale is None else float(scale), _lib.CODES[cache.kind],
-                ws.data_ptr(), need, dt)
+        ws = lengths.new_empty(need // 4)   # (of whole 4-byte words)
+        _launch(dev, _lib.load().lrqk_byte_attention, q.data_ptr(), *cache._places, blocks, lengths.data_ptr(), kn_at, vn_at, mask_at, each,
+                out.data_ptr(), None if lse is None else lse.data_ptr(), b, hq, hc, hn, t, d, d ** -0.5 if scale is None else float(scale),
+                cache._code, ws.data_ptr(), need, dt)
     return (out, lse) if return_lse else out
 
 
