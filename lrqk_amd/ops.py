@@ -939,7 +939,8 @@ class ByteCache:
     ``k`` [b,H,blocks,64,w] and ``v`` [b,H,blocks,w,64] hold the codes (w: head_dim rounded up to 64, 128 or 256; the rest is 0),
     ``k_scale`` and ``v_scale`` fp32 [b,H,blocks]; ``k_tail`` and ``v_tail`` [b,H,128,d], in ``dtype`` (what queries and new tokens
     come in), the last 128 tokens as they came, token p in row p % 128.  A block is coded once, when its last token arrives; until
-    then its tokens are read from the tail.  Lengths are the caller's (int32 [b] on the device), as of the other caches here."""
+    then its tokens are read from the tail.  Lengths are the caller's (int32 [b] on the device), as of the other caches here, and
+    so is the order of calls on one cache: those that write it and those that read it come one after the other."""
 
     BLOCK, TAIL = 64, 128
     _CODES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
@@ -965,6 +966,7 @@ class ByteCache:
         self._dev = k.get_device()
         self._sizes = (batch, heads, blocks, head_dim)
         self._places = tuple(x.data_ptr() for x in self._buffers)
+        self._ranges = tuple((x.data_ptr(), x.data_ptr() + x.nbytes) for x in self._buffers)
         self._code = _lib.CODES[kind]
 
     k, v, k_scale, v_scale, k_tail, v_tail = (property(lambda self, i=i: self._buffers[i]) for i in range(6))
@@ -982,7 +984,8 @@ def byte_append(cache: ByteCache, k: torch.Tensor, v: torch.Tensor, lengths: tor
     k, v [b,H,t,d]: any strides, rows contiguous.  ``counts`` int32 [b]: how many of them (all t if None; at most what there is room
     for).  ``path`` int32 [b,m]: which rows, in order (0, 1, .. if None; counts up to m, ids outside the rows count as the nearest):
     ``verify_drafts`` gives both.  ``lengths`` is not changed: appending again from it writes the same again as long as that is at most
-    64 tokens.  A block's codes: scale = amax / 127 (int8) or the smallest power of two with amax / scale <= 448 (fp8), of its
+    64 tokens.  (A sequence may also be made shorter: to whole blocks, or to where the block that it then ends in lies in the
+    tail as a whole.)  k and v are apart from the cache.  A block's codes: scale = amax / 127 (int8) or the smallest power of two with amax / scale <= 448 (fp8), of its
     finite elements and at least 2^-100, code = element / scale rounded once, half to even; infinities get the largest code, NaN 0."""
     dev = _on_one_gpu(k, v, lengths, counts, path)
     b, h, blocks, d = cache._on(dev)
@@ -1011,6 +1014,12 @@ def byte_append(cache: ByteCache, k: torch.Tensor, v: torch.Tensor, lengths: tor
     if (k_at | v_at) & 15 or (ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) & step:
         k, v = _rows16(k), _rows16(v)
         k_at, v_at, ks, vs = k.data_ptr(), v.data_ptr(), _row_strides("k", k, b, h, t, d), _row_strides("v", v, b, h, t, d)
+    e = 16 // (step + 1)
+    k_end = k_at + e * ((b - 1) * ks[0] + (h - 1) * ks[1] + (t - 1) * ks[2] + d)
+    v_end = v_at + e * ((b - 1) * vs[0] + (h - 1) * vs[1] + (t - 1) * vs[2] + d)
+    for lo, hi in cache._ranges:
+        if k_at < hi and lo < k_end or v_at < hi and lo < v_end:
+            raise ValueError("k or v overlaps the cache")
     new = torch.empty_like(lengths)
     _launch(dev, _lib.load().lrqk_byte_append, k_at, v_at, _SIX.pack(*ks, *vs), t, most, lengths.data_ptr(),
             None if counts is None else counts.data_ptr(), path_at, path_stride, new.data_ptr(), *cache._places, blocks, b, h, d, cache._code,
@@ -1073,7 +1082,7 @@ def verify_drafts(tokens: torch.Tensor, target: torch.Tensor, uniforms: torch.Te
     """The accepted path of a tree of drafted tokens, and the token that follows it, from given random numbers: what is accepted and
     drawn has the target's distribution.
 
-    tokens int32 [b,s]: node 0 of a sequence's tree is certain, node i was drawn from row parents[i] of ``draft``, every child of a
+    tokens int32 [b,s] (as all whole numbers here): node 0 of a sequence's tree is certain, node i was drawn from row parents[i] of ``draft``, every child of a
     node for itself.  ``parents`` int32 [b,s]: a node in front of its children (None: a chain, i - 1; a node whose parent is not in
     front of it is never reached).  target [b,s,V], row i the probabilities behind node i; draft [b,s,V] or [b,s-1,V], or None for
     drafts without probabilities (looked up: equal ones among a node's children count once).  Both fp32 or bf16, rows contiguous.

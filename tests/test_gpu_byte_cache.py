@@ -270,6 +270,15 @@ def test_append_places_and_strides(ops):
         _check_append(ops, cache, k[:, :, ::3], v[:, :, ::3], _i32(0, 1))
 
 
+def test_append_refuses_rows_of_the_cache(ops):
+    cache = ops.ByteCache(2, 2, 128, 64, BF, "int8", DEV)
+    n, k = _i32(0, 0), torch.zeros((2, 2, 3, 64), dtype=BF, device=DEV)
+    for x in (cache.k_tail[:, :, 3:6], cache.v_tail[:, :, ::50], cache.k.view(BF).view(-1)[:2 * 2 * 3 * 64].view(2, 2, 3, 64)):
+        for bad in ((x, k), (k, x)):
+            with pytest.raises(ValueError, match="overlaps"):
+                ops.byte_append(cache, *bad, n)
+
+
 def test_append_refusals(ops):
     cache = ops.ByteCache(2, 2, 128, 64, BF, "int8", DEV)
     k = torch.zeros((2, 2, 3, 64), dtype=BF, device=DEV)
@@ -301,14 +310,15 @@ def _rows64(cache, i, h, n):
     return (torch.cat((x.reshape(-1, d), tail[i, h][late].double())) for x, tail in ((k, cache.k_tail), (v, cache.v_tail)))
 
 
-def _attention64(q, cache, lengths, kn, vn, mask, scale):
-    """(out, lse, tolerance of out, of lse) in fp64.  Where a masked token holds something that is not finite, it is not met."""
+def _attention64(q, cache, lengths, kn, vn, mask, scale, only=None):
+    """(out, lse, tolerance of out, of lse) in fp64 (of the sequences `only`, if that is given).  Where a masked token holds
+    something that is not finite, it is not met."""
     b, hq, t, d = q.shape
     hc = cache.k.shape[1]
     out = torch.zeros((b, hq, t, d), dtype=torch.float64, device=DEV)
     lse = torch.full((b, hq, t), -INF, dtype=torch.float64, device=DEV)
     tol, tol_l = torch.zeros_like(out), torch.zeros_like(lse)
-    for i in range(b):
+    for i in range(b) if only is None else only:
         m = min(max(int(lengths[i]), 0), cache.capacity)
         sees = torch.ones((t, m), dtype=torch.bool, device=DEV)
         if mask is not None:
@@ -467,6 +477,45 @@ def test_scores_that_rise_and_fall(ops, dtype, kind, t, hq):
     wide[..., 0] *= 1e4   # elements of one query far apart
     wide[..., 1] *= 1e-4
     _check_attention(ops, wide, cache, lengths, kn, vn, mask, scale=1e-4, what="wide")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype,b,hq,hc,t,n,d", [
+    (BF, 1, 32, 16, 10, 9000, 128), (BF, 2, 16, 8, 32, 9000, 64), (BF, 1, 16, 16, 64, 9000, 128),   # 32 queries a wave, each its blocks
+    (BF, 1, 8, 2, 17, 1000, 128), (BF, 1, 8, 2, 24, 1000, 64),                                      # shared blocks
+    (BF, 1, 4, 2, 16, 1000, 256), (BF, 1, 4, 2, 17, 1000, 256), (BF, 1, 4, 1, 33, 1000, 136),       # wide heads, alone and sharing
+    (FP, 1, 4, 1, 8, 3000, 128), (FP, 1, 4, 1, 10, 33000, 128), (FP, 1, 4, 1, 17, 1000, 64), (FP, 1, 4, 1, 9, 1000, 256)])
+def test_attention_of_every_kernel(ops, dtype, kind, b, hq, hc, t, n, d):
+    """Each way that a call may take, over blocks whose values differ by orders of magnitude."""
+    print("byte kernels", dtype, kind, b, hq, hc, t, n, d, flush=True)
+    g = _gen(t + n)
+    cache = ops.ByteCache(b, hc, n, d, dtype, kind, DEV)
+    size = torch.exp2(torch.randint(-14, 15, ((n + 63) // 64,), generator=g).float()).to(DEV).repeat_interleave(64)[:n, None]
+    for spread in (torch.ones_like(size), size):
+        k, v = _randn(g, b, hc, n, d, dtype=dtype), (_randn(g, b, hc, n, d) * spread).to(dtype)
+        lengths = ops.byte_append(cache, k, v, torch.zeros(b, dtype=torch.int32, device=DEV))
+        q, kn, vn, mask = _drafts(g, b, hq, hc, t, d, dtype)
+        _check_attention(ops, q, cache, lengths, kn, vn, mask)
+
+
+@pytest.mark.parametrize("b,t", [(700, 1), (400, 33), (400, 70)])
+def test_attention_of_heads_that_fill_the_gpu(ops, b, t):
+    """Sequences of several long splits each: sums over no more than 256 blocks."""
+    print("byte many heads", b, t, flush=True)
+    n, d = 17000, 64
+    g = torch.Generator(device=DEV).manual_seed(b)
+    cache = ops.ByteCache(b, 1, n, d, BF, "int8", DEV)
+    k, v = (torch.randn((b, 1, n, d), generator=g, device=DEV).to(BF) for _ in range(2))
+    lengths = ops.byte_append(cache, k, v, torch.zeros(b, dtype=torch.int32, device=DEV))
+    lengths[1::3] -= 64 * 40 + 5
+    lengths[1::3] = lengths[1::3] // 64 * 64
+    q, kn, vn = (torch.randn((b, 1, t, d), generator=g, device=DEV).to(BF) for _ in range(3))
+    mask = torch.ones((t, t), dtype=torch.bool, device=DEV).tril()
+    out, lse = ops.byte_attention(q, cache, lengths, kn, vn, mask, return_lse=True)
+    only = [0, 1, b // 2, b - 1]
+    e, el, tol, tol_l = _attention64(q, cache, lengths, kn, vn, mask, d ** -0.5, only)
+    _within(out[only], e[only], tol[only])
+    _within(lse[only], el[only], tol_l[only])
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])
