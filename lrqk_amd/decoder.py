@@ -7,6 +7,10 @@ single-query attention per decoded token.  Projections, norms, rotary embedding,
 prompt attention are plain PyTorch-ROCm library calls on random-initialised weights (scaled or
 interleaved rotary positions: the HIP library's); the cache path (factorisation, selection, fetch, decode attention) is the HIP library.
 
+``new_byte_caches`` gives a dense K/V cache in 8 bits instead, which ``generate`` takes as any other and
+``generate_drafted`` decodes several looked-up tokens at once over (rotary positions, attention, verification and the
+cache are the HIP library's there).
+
 ``cache=None`` runs the same module with a dense K/V cache; with ``k + lite`` at least as long as
 the whole sequence the LRQK run returns every cached token (the growing-prefix branch,
 lrqk_attention.py:1526-1545) and must produce the same tokens.
@@ -49,6 +53,18 @@ def _rms(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
     return (v * w.float()).to(x.dtype)
 
 
+class ByteCaches:
+    """A dense K/V cache in 8 bits: an ``ops.ByteCache`` a layer, and the lengths that they share (int32 [b])."""
+
+    def __init__(self, cfg: DecoderConfig, batch: int, capacity: int, dtype, kind: str, device):
+        self.layers = [ops.ByteCache(batch, cfg.kv_heads, capacity, cfg.head_dim, dtype, kind, device) for _ in range(cfg.layers)]
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+
+    @property
+    def capacity(self) -> int:
+        return self.layers[0].capacity
+
+
 class LlamaShapeDecoder:
     def __init__(self, cfg: DecoderConfig = LLAMA3_8B, dtype=torch.bfloat16, device="cuda:0", seed: int = 0,
                  mlp_chunk: int = 16384, context_scale: float = 0.0):
@@ -84,6 +100,7 @@ class LlamaShapeDecoder:
         self.rope = None   # (else the library turns q and k, in one launch)
         if c.rope_interleaved or c.rope_scaling is not None:
             self.rope = ops.RotaryPlan(c.head_dim, c.rope_theta, c.rope_interleaved, c.rope_scaling, self.device)
+        self._plan = None  # of generate_drafted, whose sequences have positions of their own
         self.ws = ops.Workspace()
         self.dense: Optional[List[Tuple[torch.Tensor, torch.Tensor]]] = None
         self.progress = None   # optional callable(str), called once per layer while the prompt is processed
@@ -112,6 +129,10 @@ class LlamaShapeDecoder:
                                 tol=tol, max_sequence_length=max_sequence_length,
                                 num_key_value_groups=self.cfg.heads // self.cfg.kv_heads)
 
+    def new_byte_caches(self, batch: int, capacity: int, kind: str = "int8") -> ByteCaches:
+        """``kind`` as ``ops.ByteCache`` takes it; ``capacity``: tokens of a sequence, the generated ones among them."""
+        return ByteCaches(self.cfg, batch, capacity, self.dtype, kind, self.device)
+
     # ------------------------------------------------------------------ one forward over s new positions
     @torch.inference_mode()
     def forward(self, ids: torch.Tensor, pos0: int, cache: Optional[DynamicLRQKCache]) -> torch.Tensor:
@@ -123,6 +144,11 @@ class LlamaShapeDecoder:
             x = x + self.context
         if cache is None and self.dense is None:
             self.dense = [None] * c.layers
+        if isinstance(cache, ByteCaches):
+            if pos0 + s > cache.capacity or (s > 1 and pos0 > 0):
+                raise ValueError(f"tokens {pos0} .. {pos0 + s - 1}: the cache has room for {cache.capacity}, and a prompt comes at once")
+            if pos0 == 0:
+                cache.lengths = torch.zeros_like(cache.lengths)
         for li, L in enumerate(self.layers):
             hcur = _rms(x, L["n1"], c.rms_eps)
             q = (hcur @ L["wq"]).view(b, s, c.heads, c.head_dim).transpose(1, 2)
@@ -139,6 +165,14 @@ class LlamaShapeDecoder:
                     self.dense[li] = (torch.cat([self.dense[li][0], k], 2), torch.cat([self.dense[li][1], v], 2))
                 K, V = self.dense[li]
                 o = F.scaled_dot_product_attention(q, K, V, is_causal=s > 1, enable_gqa=True)
+            elif isinstance(cache, ByteCaches):
+                seen = ops.byte_append(cache.layers[li], k, v, cache.lengths)
+                if s > 1:
+                    o = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
+                else:
+                    o = ops.byte_attention(q, cache.layers[li], seen)
+                if li == c.layers - 1:
+                    cache.lengths = seen
             elif s > 1:
                 cache.update(q, k, v, li)   # factorises the prompt; the prompt itself attends densely
                 o = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
@@ -187,3 +221,81 @@ class LlamaShapeDecoder:
         torch.cuda.synchronize()
         t_decode = time.perf_counter() - t0
         return torch.stack(out, 1), t_prefill, t_decode, steps
+
+    # ------------------------------------------------------------------ several drafted tokens at once
+    @torch.inference_mode()
+    def _draft_logits(self, ids: torch.Tensor, mask: torch.Tensor, positions: torch.Tensor, caches: ByteCaches):
+        """ids [b,s] of which token i sees the cached ones and those of mask [s,s] -> logits of every position [b,s,vocab], and k, v
+        of every layer, which go into the cache once it is known which tokens stay."""
+        c = self.cfg
+        b, s = ids.shape
+        if self._plan is None:
+            self._plan = self.rope or ops.RotaryPlan(c.head_dim, c.rope_theta, device=self.device)
+        x = self.embed[ids]
+        if self.context_scale:
+            x = x + self.context
+        rows = []
+        for L, layer in zip(self.layers, caches.layers):
+            hcur = _rms(x, L["n1"], c.rms_eps)
+            q = (hcur @ L["wq"]).view(b, s, c.heads, c.head_dim).transpose(1, 2)
+            k = (hcur @ L["wk"]).view(b, s, c.kv_heads, c.head_dim).transpose(1, 2)
+            v = (hcur @ L["wv"]).view(b, s, c.kv_heads, c.head_dim).transpose(1, 2)
+            q, k = ops.rotary(self._plan, q, k, positions)
+            o = ops.byte_attention(q, layer, caches.lengths, k, v, mask)
+            rows.append((k, v))
+            x = x + o.transpose(1, 2).reshape(b, s, c.heads * c.head_dim) @ L["wo"]
+            x = x + self._mlp(L, _rms(x, L["n2"], c.rms_eps))
+        return (_rms(x, self.final_norm, c.rms_eps) @ self.lm_head).float(), rows
+
+    @staticmethod
+    def _look_up(tokens: List[int], drafts: int, ngram: int) -> List[int]:
+        """What followed the last ``ngram`` tokens where they stood before, the last time that they did; -1: nothing."""
+        for at in range(len(tokens) - ngram - 1, -1, -1):
+            if tokens[at:at + ngram] == tokens[-ngram:]:
+                found = tokens[at + ngram:at + ngram + drafts]
+                return found + [-1] * (drafts - len(found))
+        return [-1] * drafts
+
+    @torch.inference_mode()
+    def generate_drafted(self, ids: torch.Tensor, new_tokens: int, caches: ByteCaches, drafts: int = 7, ngram: int = 2,
+                         temperature: float = 0.0, generator: Optional[torch.Generator] = None):
+        """Decoding with drafts that are looked up in the sequence itself: a round attends with a sequence's last token and up to
+        ``drafts`` that followed its last ``ngram`` tokens before, verifies them against the model's probabilities (of
+        ``temperature``; 0: its most probable token) and keeps those that stand.  The tokens have the distribution that ``generate``
+        at that temperature has.  ids [b,l] -> (tokens [b,new_tokens], rounds)."""
+        b, l = ids.shape
+        if drafts < 1 or ngram < 1 or new_tokens < 1 or temperature < 0:
+            raise ValueError(f"drafts={drafts}, ngram={ngram}, new_tokens={new_tokens}, temperature={temperature}")
+        if l + new_tokens + drafts > caches.capacity:
+            raise ValueError(f"{l} + {new_tokens} tokens and {drafts} drafts beyond the cache's {caches.capacity}")
+
+        def chances(logits):
+            if temperature == 0.0:
+                return torch.zeros_like(logits).scatter_(-1, logits.argmax(-1, keepdim=True), 1.0)
+            return torch.softmax(logits / temperature, -1)
+
+        def drawn(s):
+            return torch.rand((b, s), generator=generator, device=self.device)
+        first = chances(self.forward(ids, 0, caches))[:, None]
+        _, _, token = ops.verify_drafts(torch.zeros((b, 1), dtype=torch.int32, device=self.device), first, drawn(1))
+        told = [row + [t] for row, t in zip(ids.tolist(), token.tolist())]
+        s = drafts + 1
+        mask = torch.ones((s, s), dtype=torch.bool, device=self.device).tril()
+        steps = torch.arange(s, dtype=torch.int32, device=self.device)
+        rounds = 0
+        while min(len(row) for row in told) < l + new_tokens:
+            # (a sequence that has all its tokens goes along and keeps none)
+            full = [len(row) >= l + new_tokens for row in told]
+            nodes = torch.tensor([[row[-1]] + ([-1] * drafts if done else self._look_up(row, drafts, ngram)) for row, done in zip(told, full)],
+                                 dtype=torch.int32, device=self.device)
+            logits, rows = self._draft_logits(nodes.clamp(min=0).long(), mask, caches.lengths[:, None] + steps, caches)
+            path, counts, token = ops.verify_drafts(nodes, chances(logits), drawn(s))
+            counts = torch.where(torch.tensor(full, device=self.device), torch.zeros_like(counts), counts)
+            for layer, (k, v) in zip(caches.layers, rows):
+                seen = ops.byte_append(layer, k, v, caches.lengths, counts, path)
+            caches.lengths = seen
+            for row, kept, n, t in zip(told, nodes.tolist(), counts.tolist(), token.tolist()):
+                if n:
+                    row += kept[1:n] + [t]
+            rounds += 1
+        return torch.tensor([row[l:l + new_tokens] for row in told], device=self.device), rounds

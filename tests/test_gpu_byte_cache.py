@@ -942,3 +942,50 @@ def test_two_streams_at_once(ops):
     for i in range(2):
         assert all(torch.equal(a, z) for r, w in zip(got[i], want[i]) for a, z in zip(r, w))
         assert all(torch.equal(getattr(sides[i][0], n).float(), getattr(alone[i][0], n).float()) for n in NAMES)
+
+
+# ---------------------------------------------------------------------------------------------------------- a decoder
+
+def _model(dtype, d=16, **kw):
+    from lrqk_amd import decoder
+    cfg = decoder.DecoderConfig(layers=2, hidden=64, heads=4, kv_heads=2, head_dim=d, intermediate=128, vocab=97, rope_theta=1e4, **kw)
+    return decoder.LlamaShapeDecoder(cfg, dtype, DEV, seed=3)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_decoder_over_byte_caches(ops, kind):
+    """While no block is complete every token is read as it came: the tokens of the dense cache.  Beyond that it runs."""
+    print("decoder", kind, flush=True)
+    m = _model(FP)
+    ids = torch.randint(0, 97, (2, 24), generator=_gen(0)).to(DEV)
+    dense, *_ = m.generate(ids, 20, None)
+    caches = m.new_byte_caches(2, 200, kind)
+    got, *_ = m.generate(ids, 20, caches)
+    assert torch.equal(got, dense) and caches.lengths.tolist() == [43, 43]
+    caches = m.new_byte_caches(2, 200, kind)
+    m.generate(ids, 5, caches)   # (a prompt begins anew)
+    long, *_ = m.generate(torch.cat((ids, dense, ids, ids), 1), 90, caches)
+    assert long.shape == (2, 90) and caches.lengths.tolist() == [24 * 3 + 20 + 89] * 2 and int(long.min()) >= 0 and int(long.max()) < 97
+    with pytest.raises(ValueError, match="room"):
+        m.generate(ids, 300, caches)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_drafted_generation_is_greedy_generation(ops, kind):
+    """Neighbouring pairs are turned by the library in both: the same tokens in fewer rounds."""
+    print("drafted", kind, flush=True)
+    m = _model(FP, rope_interleaved=True)
+    ids = torch.randint(0, 97, (3, 20), generator=_gen(1)).to(DEV)
+    ids = torch.cat((ids, ids, ids), 1)
+    want, *_ = m.generate(ids, 80, m.new_byte_caches(3, 200, kind))
+    caches = m.new_byte_caches(3, 200, kind)
+    got, rounds = m.generate_drafted(ids, 80, caches, drafts=5)
+    assert torch.equal(got, want) and rounds < 79, rounds
+    # what is cached are the tokens but the last, and those behind the wanted ones that came with them
+    assert all(60 + 79 <= n <= 60 + 79 + 6 for n in caches.lengths.tolist())
+    drawn, _ = m.generate_drafted(ids, 30, m.new_byte_caches(3, 200, kind), drafts=5, temperature=1.0,
+                                  generator=torch.Generator(device=DEV).manual_seed(0))
+    assert drawn.shape == (3, 30) and int(drawn.min()) >= 0 and int(drawn.max()) < 97
+    for bad in (dict(drafts=0), dict(new_tokens=0), dict(ngram=0), dict(temperature=-1.0), dict(new_tokens=190)):
+        with pytest.raises(ValueError):
+            m.generate_drafted(**{**dict(ids=ids, new_tokens=5, caches=caches), **bad})
