@@ -812,6 +812,40 @@ def test_verify_refusals(ops):
         ops.verify_drafts(torch.zeros((1, 1025), dtype=torch.int32, device=DEV), torch.zeros((1, 1025, 4), device=DEV), torch.zeros((1, 1025), device=DEV))
 
 
+def test_offsets_beyond_32_bits(ops):
+    """Codes behind the first 4 GB, rows of new tokens and of probabilities that far apart."""
+    print("far", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(40)
+    heads, n, d = 68, 2 ** 20, 64
+    k, v = (torch.randn((1, 1, n, d), generator=g, device=DEV).to(BF) for _ in range(2))
+    cache = ops.ByteCache(1, heads, n, d, BF, "fp8", DEV)
+    assert cache.k.numel() > 2 ** 32
+    lengths = ops.byte_append(cache, k.expand(1, heads, n, d), v.expand(1, heads, n, d), _i32(0), counts=_i32(n - 30))
+    for t in (2, 70):
+        q = torch.randn((1, 1, t, d), generator=g, device=DEV).to(BF)
+        out, lse = ops.byte_attention(q.expand(1, heads, t, d).contiguous(), cache, lengths, return_lse=True)
+        assert all(torch.equal(out[0, 0], out[0, h]) and torch.equal(lse[0, 0], lse[0, h]) for h in (1, 62, 63, 64, 66, 67))
+        one = ops.ByteCache(1, 1, n, d, BF, "fp8", DEV)
+        for name in NAMES:
+            getattr(one, name).copy_(getattr(cache, name)[:, heads - 1:])
+        e, el, tol, tol_l = _attention64(q, one, lengths, None, None, None, d ** -0.5)
+        _within(out[:, -1:], e, tol, t)
+        _within(lse[:, -1:], el, tol_l, t)
+    del cache, one, k, v
+    flat = torch.empty(2 * 2 ** 30 + 1000, device=DEV)
+    target = flat.as_strided((1, 3, 900), (1, 2 ** 30, 1))
+    target.copy_(torch.softmax(torch.randn((1, 3, 900), generator=g, device=DEV), -1))
+    draft = target.flip(-1).contiguous()
+    tokens = torch.tensor([[0, 5, 600]], dtype=torch.int32, device=DEV)
+    for u in (0.0, 0.5, 0.999):
+        uniforms = torch.full((1, 3), u, device=DEV)
+        _check_verify(ops, tokens, target, uniforms, draft)
+        _check_verify(ops, tokens, target, uniforms)
+    rows = flat.view(BF).as_strided((1, 1, 3, 64), (8, 8, 2 ** 31, 1))
+    rows.copy_(torch.randn((1, 1, 3, 64), generator=g, device=DEV))
+    _check_append(ops, ops.ByteCache(1, 1, 128, 64, BF, "int8", DEV), rows, rows.contiguous(), _i32(62))
+
+
 # ---------------------------------------------------------------------------------------------------------- together
 
 def _seen(parents):
