@@ -102,18 +102,19 @@ __device__ __forceinline__ void by_top(const float (&x)[MT][NE], const float (&f
 }
 
 // What a wave has of its queries: 16 MT of them, scaled by powers of two into fp16 (up: back, and to the exponents' base), and
-// of their outputs.
-template <typename T, int DP, int MT>
+// of their outputs.  FOLD: these are held in units of the first block's scale and the products add to them as they are: the
+// block's scale over that goes into the probabilities' exponents, as far as fp16 has room for it (2^8 either way); of a block
+// beyond, as of all without FOLD, the products are multiplied and added.  It pays where the matrix cores bound (80 queries over
+// 64K of four sequences: 223 us, without 233; 128 over 128K 98 and 101) and costs where loads do, of which it holds registers
+// (64 over 32K, a split's blocks dealt to waves: 29.4 us, without 27.2; a token over 32K 19.0 and 18.2).  Sums of fp32 tensors
+// do not take it: the matrix cores cut off what they add to them.
+template <typename T, int DP, int MT, bool FOLD>
 struct ByteWave {
   static constexpr int VW = DP / 16, CH = DP / 64;
-  static constexpr bool TWO = sizeof(T) == 4, FOLD = !TWO && MT > 1;
+  static constexpr bool TWO = sizeof(T) == 4, FOLDS = FOLD;
   by_h8 qh[MT][2 * CH], ql[TWO ? MT : 1][2 * CH];   // elements 64 c + 16 quad + 8 h .. in [2 c + h]
   float up[MT], top[MT], sum[MT];
   ar_f4 o[MT][VW];
-  // FOLD: outputs are held in units of the first block's scale and the products add to them as they are: the block's scale over
-  // that goes into the probabilities' exponents, as far as fp16 has room for it (2^8 either way).  Beyond, and where the
-  // matrix cores do not bound (one tile of queries), and of fp32 tensors, whose sums they must not cut off, a block's products
-  // are multiplied and added.
   float unit, log_unit;
 
   __device__ __forceinline__ void begin() {
@@ -125,6 +126,7 @@ struct ByteWave {
       for (int j = 0; j < VW; ++j) o[m][j] = ar_f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     unit = 1.0f;
+    log_unit = 0.0f;
   }
   __device__ __forceinline__ void queries(const T* q, int row0, int M, int d, float scale_log2e) {
     const int col = lane_id() & 15, quad = lane_id() >> 4;
@@ -161,9 +163,9 @@ struct ByteWave {
       }
     }
   }
-  __device__ __forceinline__ void first(float vs) {
-    unit = FOLD ? vs : 1.0f;
-    log_unit = FOLD ? __builtin_amdgcn_logf(vs) : 0.0f;
+  __device__ __forceinline__ void first(float vs) {   // (FOLD)
+    unit = vs;
+    log_unit = __builtin_amdgcn_logf(vs);
   }
   float x[MT][16];   // scores of a block's keys, key 16 quad + 4 u + r in [4 u + r]
   // Scores of its u-th 16 keys, whose operands are kf.
@@ -190,7 +192,7 @@ struct ByteWave {
     float shift = FOLD ? __builtin_amdgcn_logf(vs) - log_unit : 0.0f;
     g.apart = !FOLD || !(fabsf(shift) <= 8.0f);
     g.less = g.apart ? 1.0f : unit * __builtin_amdgcn_rcpf(vs);
-    g.by = vs / unit;
+    g.by = FOLD ? vs / unit : vs;
     shift = g.apart ? 0.0f : shift;
 #pragma unroll
     for (int m = 0; m < MT; ++m) g.f[m] = up[m] * ks;
@@ -233,8 +235,8 @@ struct ByteWave {
       }
     }
   }
-  // Around the products of a block whose scale is far from the first's (FOLD): what there is waits in memory meanwhile.  (As a
-  // branch with products of its own it cost every block the copying of all outputs from register to register.)
+  // Around the products of a block whose scale is far from the first's (FOLD): what there is waits in memory meanwhile.  (A
+  // branch with products of its own costs every block the copying of all outputs from register to register.)
   struct Waiting {
     volatile float o[FOLD ? MT * VW * 4 : 1];
   };
@@ -413,7 +415,7 @@ struct BytePlace {
 template <typename T, bool FP8, int DP, int MT>
 __global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba) {
   const TreeArgs& a = ba.tree;
-  using Wave = ByteWave<T, DP, MT>;
+  using Wave = ByteWave<T, DP, MT, false>;
   constexpr int VW = Wave::VW, CH = Wave::CH;
   constexpr int JC = 8 / MT < VW ? 8 / MT : VW;   // (32 KB; with two blocks at a time a token over 32K took 1.5 us more)
   __shared__ ar_u4 smem[kTrWaves * MT * JC * kWave];
@@ -455,7 +457,6 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba)
       load_k(block);
       load_v(block);
       w.queries(q, row0, at.M, a.d, a.scale_log2e);
-      w.first(vs_next);
     }
     for (; block < end; block += kTrWaves) {
       const int next = block + kTrWaves < end ? block + kTrWaves : block;   // (the next one, or this one again)
@@ -475,14 +476,10 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba)
       for (int u = 0; u < 4; ++u) w.probabilities(u, g, part, ph, pl);
 #pragma unroll
       for (int m = 0; m < MT; ++m) w.sum[m] = fmaf(part[m], g.less, w.sum[m]);
-      typename Wave::Waiting put;
-      w.put_by(g, put);
 #pragma unroll
       for (int j = 0; j < VW; ++j) w.products(j, by_unpack<FP8>(vg[j][0], vg[j][1]), by_unpack<FP8>(vg[j][2], vg[j][3]), g, ph, pl);
-      w.take_up(g, put);
       load_v(next);
     }
-    w.end();
   }
   tree_leave<MT, VW, JC>(a, w.o, w.top, w.sum, odd, at.unit, at.rb, at.M, smem, ml);
 }
@@ -495,7 +492,7 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba)
 template <typename T, bool FP8, int DP, int MT>
 __global__ __launch_bounds__(kTrThreads, 2) void byte_share_kernel(ByteArgs ba) {
   const TreeArgs& a = ba.tree;
-  using Wave = ByteWave<T, DP, MT>;
+  using Wave = ByteWave<T, DP, MT, sizeof(T) == 2 && MT == 2>;
   constexpr int VW = Wave::VW, CH = Wave::CH, VL = VW / kTrWaves;   // pieces of V of a wave (of K: CH)
   __shared__ by_h8 keys[2][4 * 2 * CH][kWave], values[2][VW * 2][kWave];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), col = lane & 15, quad = lane >> 4;
@@ -543,7 +540,7 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_share_kernel(ByteArgs ba) 
     load_k(begin);
     load_v(begin);
     w.queries(q, row0, at.M, a.d, a.scale_log2e);
-    w.first(ba.vs[block0 + begin]);
+    if constexpr (Wave::FOLDS) w.first(ba.vs[block0 + begin]);
     leave_k(0);
     load_k(begin + 1);
     leave_v(0);
