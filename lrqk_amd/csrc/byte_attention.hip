@@ -104,10 +104,10 @@ __device__ __forceinline__ void by_top(const float (&x)[MT][NE], const float (&f
 // What a wave has of its queries: 16 MT of them, scaled by powers of two into fp16 (up: back, and to the exponents' base), and
 // of their outputs.  FOLD: these are held in units of the first block's scale and the products add to them as they are: the
 // block's scale over that goes into the probabilities' exponents, as far as fp16 has room for it (2^8 either way); of a block
-// beyond, as of all without FOLD, the products are multiplied and added.  It pays where the matrix cores bound (80 queries over
-// 64K of four sequences: 223 us, without 233; 128 over 128K 98 and 101) and costs where loads do, of which it holds registers
-// (64 over 32K, a split's blocks dealt to waves: 29.4 us, without 27.2; a token over 32K 19.0 and 18.2).  Sums of fp32 tensors
-// do not take it: the matrix cores cut off what they add to them.
+// beyond, as of all without FOLD, the products are multiplied and added.  It pays where the matrix cores bound (256 queries
+// over up to 64K of four sequences: 223 us, without 233; 100 over 128K 98 and 101) and costs where loads do, of whose registers
+// it needs some (64 over 32K in byte_stream_kernel: 29.4 us, without 27.2; a token over 32K 19.0 and 18.2).  Sums of fp32
+// tensors do not take it: the matrix cores cut off what they add to them.
 template <typename T, int DP, int MT, bool FOLD>
 struct ByteWave {
   static constexpr int VW = DP / 16, CH = DP / 64;
@@ -411,9 +411,13 @@ struct BytePlace {
 };
 
 // Few queries: the four waves of a workgroup take the blocks of its split in turn, each for itself, its codes as operands from
-// memory.
+// memory; a block's keys are asked for when the one's before have become scores, its values when those have become products.
+// Reading bounds it: a token over 32K (int8, 8 heads of 128, bf16) is 67 MB in 15.2 us, 4.4 TB/s where the largest reads reach
+// 5.5, and 16 over 1K .. 8K 151 MB in 31.6 (4.8 TB/s); the joining launch makes them 18 and 44.  Small ones are bound by their
+// chain of waits: 7 fp32 queries of 7 heads over 4K, 6 MB, take 10.3.  Heads of 256 need more than the 256 registers that two
+// waves a SIMD have each (a token over 32K: 37.6 us in all, with two waves 45; fp32 39 and 67).
 template <typename T, bool FP8, int DP, int MT>
-__global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba) {
+__global__ __launch_bounds__(kTrThreads, DP == 256 ? 1 : 2) void byte_stream_kernel(ByteArgs ba) {
   const TreeArgs& a = ba.tree;
   using Wave = ByteWave<T, DP, MT, false>;
   constexpr int VW = Wave::VW, CH = Wave::CH;
@@ -489,6 +493,15 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_stream_kernel(ByteArgs ba)
 // next one's scores are multiplied, 16 keys at a time into the registers that those 16 leave, since a wave's exponentials and
 // products run side by side only if they are next to each other: so LDS has a block's values and the next one's keys, and
 // those that follow are written meanwhile; one barrier a block.
+//
+// What bounds it is what a SIMD has to issue for a block, products, exponentials and reads of LDS, which overlap in part: 256
+// queries of each of four sequences over up to 64K (int8, 8 heads of 128) are 184 GFLOP in 218 us, 840 TFLOP/s (a large product
+// of the library reaches 1075), 100 over 128K 54 in 92.6, 580, or 740 with the rows up to 128 that are multiplied too.  The
+// matrix cores are busy a third of all cycles in both.  Two waves a SIMD are what registers allow.  64 queries a wave moved
+// operands between register files (150 us for the 100), eight waves of a workgroup on the same blocks 210 us for the first and
+// 157 for the second, two blocks asked for ahead spilled.
+// From 65 queries on: up to 64 the other kernel's waves, which each read the codes, are faster (64 over 32K 27.2 us, here 36.2);
+// fp32 queries of long caches and heads of 256 come here from 33 on.
 template <typename T, bool FP8, int DP, int MT>
 __global__ __launch_bounds__(kTrThreads, 2) void byte_share_kernel(ByteArgs ba) {
   const TreeArgs& a = ba.tree;

@@ -13,6 +13,9 @@
 //
 // Three launches: Z of the nodes with several children (trees with p only); the walk, by every workgroup for itself, and the
 // sums of what is left by chunks of the vocabulary; the chunk and the token.
+// Bound by launches and their chains of reads: over one fp32 row of 128256 tokens the sums take 3.9 us and the token 5.0 (8.4
+// together, as replayed), over 16 trees of 16 nodes without p 7.8 and 5.9; an eager call costs the host 14 .. 17.  (One launch
+// for both would have its workgroups wait for each other.)
 #include <algorithm>
 
 #include "common.hpp"
