@@ -12,7 +12,7 @@
 // As in tree_attention.hip a query is a lane's column of S^T = C Q^T, and the probabilities are the operand of O^T = C'^T P^T
 // as they lie: row m of the i-th 16 keys of a block is key 16 (m / 4) + 4 i + m % 4, so that a quad's scores are those of 16
 // successive keys, whose codes of an element of V are the 16 bytes that the same quad loads.  Nothing passes through LDS.
-// The tokens that are not in a complete block, and the drafted ones, make a split of their own in their own type.
+// The tokens that are not in a complete block, and the drafted ones, are multiplied in their own type.
 #include "byte_cache.hpp"
 #include "tree_parts.hpp"
 
@@ -34,6 +34,7 @@ struct ByteArgs {
   const float *ks, *vs;      // scales
   const void *k_tail, *v_tail;
   int blocks, drafts;        // of a head; drafted tokens: t or none
+  bool apart;                // the tokens of no complete block and the drafted ones have a split of their own
 };
 
 // Eight codes as fp16 numbers, exactly.
@@ -267,20 +268,25 @@ struct ByteWave {
   }
 };
 
-// How the sequences are cut into splits: the first one of a sequence has what is not in a complete block, the others so many
-// complete blocks each.  From the lengths alone, by every wave for itself.
+// How the sequences are cut into splits of so many complete blocks each.  What is not in a complete block is a split of its
+// own, a sequence's first (apart), or what the last one does when it is through with its blocks.  From the lengths alone, by
+// every wave for itself.
 struct ByteCut {
   int b, len, split, splits, slot0, per;
   static __device__ __forceinline__ int length(const TreeArgs& a, int b) { return min(max(a.lengths[b], 0), a.n); }
   static __device__ __forceinline__ int share(const TreeArgs& a, int all) {
     return max(a.least, min((int)(((uint32_t)all + (uint32_t)a.splits - 1u) / (uint32_t)a.splits), a.most));
   }
-  __device__ __forceinline__ bool find(const TreeArgs& a, int slot) {
+  static __device__ __forceinline__ int parts(int blocks, int per, bool apart) {
+    const int n = (blocks + per - 1) / per;
+    return apart ? 1 + n : max(n, 1);
+  }
+  __device__ __forceinline__ bool find(const TreeArgs& a, int slot, bool apart) {
     if (a.b == 1) {
       b = slot0 = 0;
       len = length(a, 0);
       per = share(a, len / kByBlock);
-      splits = 1 + (len / kByBlock + per - 1) / per;
+      splits = parts(len / kByBlock, per, apart);
       split = slot;
       return slot < splits;
     }
@@ -293,7 +299,7 @@ struct ByteCut {
     int before = 0;
     for (int base = 0; base < a.b; base += kWave) {
       const int i = base + lane;
-      const int mine = i < a.b ? 1 + (length(a, min(i, a.b - 1)) / kByBlock + per - 1) / per : 0;
+      const int mine = i < a.b ? parts(length(a, min(i, a.b - 1)) / kByBlock, per, apart) : 0;
       const int end = before + wave_inclusive_sum(mine);
       const unsigned long long hit = __ballot(slot < end);
       if (hit) {
@@ -394,12 +400,12 @@ __device__ __forceinline__ void by_dense(const ByteArgs& ba, const ByteCut& cut,
 struct BytePlace {
   int rb, unit, hc, M;
   ByteCut cut;
-  __device__ __forceinline__ bool find(const TreeArgs& a) {   // false: nothing to do
+  __device__ __forceinline__ bool find(const TreeArgs& a, bool apart) {   // false: nothing to do
     // the row blocks of a unit (a split of a head) follow each other 8 workgroups apart: on one XCD, whose L2 then has the
     // codes that the first of them brought
     rb = (int)blockIdx.x % (8 * a.row_blocks) / 8;
     unit = (int)blockIdx.x / (8 * a.row_blocks) * 8 + (int)blockIdx.x % 8;
-    if (unit >= a.units || !cut.find(a, unit / a.hc)) return false;
+    if (unit >= a.units || !cut.find(a, unit / a.hc, apart)) return false;
     if (cut.split == 0 && unit % a.hc == 0 && rb == 0 && threadIdx.x == 0) {
       a.cut[2 * cut.b] = cut.slot0;
       a.cut[2 * cut.b + 1] = cut.splits;
@@ -426,19 +432,18 @@ __global__ __launch_bounds__(kTrThreads, DP == 256 ? 1 : 2) void byte_stream_ker
   __shared__ float ml[kTrWaves][MT][16][2];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), col = lane & 15, quad = lane >> 4;
   BytePlace at;
-  if (!at.find(a)) return;
+  if (!at.find(a, ba.apart)) return;
   const ByteCut& cut = at.cut;
   const int row0 = at.rb * 16 * MT;
   const T* q = (const T*)a.q + ((int64_t)cut.b * a.hc + at.hc) * at.M * a.d;
   Wave w;
   w.begin();
   bool odd = false;
-  if (cut.split == 0) {
-    by_dense<T, DP, MT>(ba, cut, at.hc, row0, at.M, q, wave, kTrWaves, w.top, w.sum, w.o, odd);
-  } else {
+  const int before = cut.split - ba.apart;   // splits of blocks in front of this one
+  if (before >= 0) {
     const int64_t block0 = ((int64_t)cut.b * a.hc + at.hc) * ba.blocks;
-    int block = (cut.split - 1) * cut.per + wave;
-    const int end = min(cut.len / kByBlock, cut.split * cut.per);
+    int block = before * cut.per + wave;
+    const int end = min(cut.len / kByBlock, (before + 1) * cut.per);
     // what a lane reads of a block: CH pieces of 4 x 16 keys, and VW pieces of V
     const uint32_t kat = (uint32_t)((col >> 2) * 16 + (col & 3)) * DP + quad * 16, vat = (uint32_t)(VW * col) * kByBlock + quad * 16;
     ar_u4 kg[4][CH], vg[VW];
@@ -485,6 +490,8 @@ __global__ __launch_bounds__(kTrThreads, DP == 256 ? 1 : 2) void byte_stream_ker
       load_v(next);
     }
   }
+  if (cut.split == (ba.apart ? 0 : cut.splits - 1))
+    by_dense<T, DP, MT>(ba, cut, at.hc, row0, at.M, q, wave, kTrWaves, w.top, w.sum, w.o, odd);
   tree_leave<MT, VW, JC>(a, w.o, w.top, w.sum, odd, at.unit, at.rb, at.M, smem, ml);
 }
 
@@ -510,7 +517,7 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_share_kernel(ByteArgs ba) 
   __shared__ by_h8 keys[2][4 * 2 * CH][kWave], values[2][VW * 2][kWave];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(wave_id()), col = lane & 15, quad = lane >> 4;
   BytePlace at;
-  if (!at.find(a)) return;
+  if (!at.find(a, true)) return;
   const ByteCut& cut = at.cut;
   const int row0 = (at.rb * kTrWaves + wave) * 16 * MT;
   const T* q = (const T*)a.q + ((int64_t)cut.b * a.hc + at.hc) * at.M * a.d;
@@ -618,7 +625,7 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_share_kernel(ByteArgs ba) 
 
 struct BytePlan {
   int dp, mt;
-  bool share;
+  bool share, apart;
   int rows, row_blocks, row_tiles, splits, least, most, units;
   int64_t part, ml, odd, cut;   // words of 4 bytes
 };
@@ -630,13 +637,17 @@ static BytePlan byte_plan(int b, int hq, int hc, int t, int64_t blocks, int d, i
   // 16 queries a wave: all there are, or all that registers have room for; or few blocks, which one workgroup per 16 queries is
   // through sooner (32 queries over 8K: 14.5 us, with 32 a wave 17.1; over 64K 41.5 and 36.5, 64 over 64K 74 and 52)
   p.mt = M <= 16 || p.dp == 256 || dtype == LRQK_F32 || (!p.share && b * hc * blocks <= 2048) ? 1 : 2;
+  // Many sequences are enough workgroups without those (64 tokens over 1 .. 1K 35 us, without 30; 48 of 16 over 1K .. 8K 51 and
+  // 47, a token of each 44 and 43); of fewer they are done beside the others (8 tokens over 1K .. 8K 25 us, otherwise 26).
+  p.apart = p.share || b < 16;
   p.rows = 16 * p.mt * (p.share ? kTrWaves : 1);
   p.row_blocks = (int)((M + p.rows - 1) / p.rows);
   p.row_tiles = p.row_blocks * (p.rows / 16);
   // Workgroups, those of what is not in complete blocks among them: two per CU, which keep each other's time filled.  A single
   // sequence is cut evenly, and of few queries one per CU then reads as fast and leaves less to be joined (a token over 32K:
   // 18 us, with two 21, with three 23); of many sequences with one tile of queries three per CU hide that their lengths differ
-  // (16 tokens over 1K .. 8K: 44 us, with two 53).
+  // (16 tokens over 1K .. 8K: 42.7 us, with two
+  // 44.3, with four 42.4; 32 over 0 .. 2K 26.6, 28.7, 27.9).
   const int wanted = p.share ? 512 : b == 1 ? 256 : p.mt == 1 && b >= 8 ? 768 : 512;
   p.splits = (int)std::max<int64_t>(b, wanted / ((int64_t)hc * p.row_blocks) - b);
   p.least = (int)std::max<int64_t>(kTrWaves, (blocks + kTrMaxSplits - 2) / (kTrMaxSplits - 1));
@@ -726,6 +737,7 @@ extern "C" int lrqk_byte_attention(const void* q, const void* k, const void* v, 
   a.tree = TreeArgs{q, nullptr, nullptr, k_new, v_new, mask, lengths, out, lse, ws, ws + p.part, (int32_t*)ws + p.part + p.ml,
                     (int32_t*)ws + p.part + p.ml + p.odd, 0, 0, 0, mask_batch_stride, b, (int)(blocks * kByBlock), hq, hc, k_new ? hn : hc, t, d,
                     p.splits, p.least, p.most, p.row_blocks, p.rows, p.row_tiles, p.units, scale * kLog2e};
+  a.apart = p.apart;
   a.k = k;
   a.v = v;
   a.ks = k_scale;

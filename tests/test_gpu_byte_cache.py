@@ -498,6 +498,27 @@ def test_attention_of_every_kernel(ops, dtype, kind, b, hq, hc, t, n, d):
         _check_attention(ops, q, cache, lengths, kn, vn, mask)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("b,t,hq,d", [(16, 1, 2, 128), (17, 6, 8, 64), (70, 3, 2, 64), (16, 20, 4, 128), (16, 5, 2, 256)])
+def test_attention_of_many_sequences(ops, dtype, kind, b, t, hq, d):
+    """Sequences of none to many blocks, one split each and several, with drafted tokens that nobody sees and that hold infinities."""
+    print("byte many sequences", dtype, kind, b, t, hq, d, flush=True)
+    g = _gen(b + t)
+    n = 64 * 30 + 8
+    cache, full = _cache(ops, g, b, 2, n, d, dtype, kind)
+    q, kn, vn, mask = _drafts(g, b, hq, 2, t, d, dtype)
+    mask[1::3] = False
+    some = torch.tensor([0, 1, 63, 64, 65, 127, 64 * 8, 64 * 8 + 1, 64 * 30, n], dtype=torch.int32, device=DEV)
+    mixed = some[torch.randint(0, 10, (b,), generator=g).to(DEV)]
+    # (a tail has a sequence's last 128 tokens: those of shorter lengths are other ones, finite all the same)
+    for lengths in (full, mixed, mixed.flip(0), some[torch.arange(b, device=DEV) % 3], torch.zeros_like(full)):
+        _check_attention(ops, q, cache, lengths, kn, vn, mask, what=lengths.tolist())
+        _check_attention(ops, q, cache, lengths, what=lengths.tolist())
+    vn[:, :, 0, ::3], vn[:, :, 0, 1::3] = INF, NAN
+    _check_attention(ops, q, cache, mixed, kn, vn, mask, what="odd")
+
+
 @pytest.mark.parametrize("b,t", [(700, 1), (400, 33), (400, 70)])
 def test_attention_of_heads_that_fill_the_gpu(ops, b, t):
     """Sequences of several long splits each: sums over no more than 256 blocks."""
