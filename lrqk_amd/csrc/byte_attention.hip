@@ -419,8 +419,8 @@ struct BytePlace {
 // Few queries: the four waves of a workgroup take the blocks of its split in turn, each for itself, its codes as operands from
 // memory; a block's keys are asked for when the one's before have become scores, its values when those have become products.
 // Reading bounds it: a token over 32K (int8, 8 heads of 128, bf16) is 67 MB in 15.2 us, 4.4 TB/s where the largest reads reach
-// 5.5, and 16 over 1K .. 8K 151 MB in 31.6 (4.8 TB/s); the joining launch makes them 18 and 44.  Small ones are bound by their
-// chain of waits: 7 fp32 queries of 7 heads over 4K, 6 MB, take 10.3.  Heads of 256 need more than the 256 registers that two
+// 5.5, and 16 over 1K .. 8K 158 MB in 31.3 (5.1 TB/s); the joining launch makes them 18 and 43.  Small ones are bound by their
+// chain of waits: 7 fp32 queries of 28 heads over 4K, 4 MB, take 9.8.  Heads of 256 need more than the 256 registers that two
 // waves a SIMD have each (a token over 32K: 37.6 us in all, with two waves 45; fp32 39 and 67).
 template <typename T, bool FP8, int DP, int MT>
 __global__ __launch_bounds__(kTrThreads, DP == 256 ? 1 : 2) void byte_stream_kernel(ByteArgs ba) {
@@ -646,9 +646,12 @@ static BytePlan byte_plan(int b, int hq, int hc, int t, int64_t blocks, int d, i
   // Workgroups, those of what is not in complete blocks among them: two per CU, which keep each other's time filled.  A single
   // sequence is cut evenly, and of few queries one per CU then reads as fast and leaves less to be joined (a token over 32K:
   // 18 us, with two 21, with three 23); of many sequences with one tile of queries three per CU hide that their lengths differ
-  // (16 tokens over 1K .. 8K: 42.7 us, with two
-  // 44.3, with four 42.4; 32 over 0 .. 2K 26.6, 28.7, 27.9).
-  const int wanted = p.share ? 512 : b == 1 ? 256 : p.mt == 1 && b >= 8 ? 768 : 512;
+  // (16 tokens over 1K .. 8K 42.7 us, with two 44.3, with four 42.4; 32 over up to 2K 26.6, 28.7 and 27.9).
+  // Where blocks are shared and a workgroup would have no more than 12 of them, what it leaves costs more than a second one per
+  // CU gains (100 queries over 16K, 32K, 64K: 29.8, 38.7, 60.8 us, with one 26.7, 36.6, 63.0); of heads of 256 registers have
+  // room for one alone (64 over 64K: 92 us, 82.5).
+  const bool one = p.share ? p.dp == 256 || (int64_t)b * hc * blocks * p.row_blocks <= 12 * 512 : b == 1;
+  const int wanted = one ? 256 : !p.share && p.mt == 1 && b >= 8 ? 768 : 512;
   p.splits = (int)std::max<int64_t>(b, wanted / ((int64_t)hc * p.row_blocks) - b);
   p.least = (int)std::max<int64_t>(kTrWaves, (blocks + kTrMaxSplits - 2) / (kTrMaxSplits - 1));
   // (where the heads alone fill the GPU: sums of fp32 numbers over no more than kByLong blocks, in splits of one length)

@@ -65,6 +65,22 @@ class ByteCaches:
         return self.layers[0].capacity
 
 
+class LookedUp:
+    """A sequence's tokens, and where every ``ngram`` of them ended the last time."""
+
+    def __init__(self, tokens: List[int], ngram: int):
+        self.tokens, self.ngram, self._ends, self._done = list(tokens), ngram, {}, ngram
+
+    def drafts(self, n: int) -> List[int]:
+        """n tokens: those that followed the last ``ngram`` where they stood before, the last time that they did; -1: nothing."""
+        for end in range(self._done, len(self.tokens)):
+            self._ends[tuple(self.tokens[end - self.ngram:end])] = end
+        self._done = max(self._done, len(self.tokens))
+        end = self._ends.get(tuple(self.tokens[-self.ngram:]), len(self.tokens))
+        found = self.tokens[end:end + n]
+        return found + [-1] * (n - len(found))
+
+
 class LlamaShapeDecoder:
     def __init__(self, cfg: DecoderConfig = LLAMA3_8B, dtype=torch.bfloat16, device="cuda:0", seed: int = 0,
                  mlp_chunk: int = 16384, context_scale: float = 0.0):
@@ -247,15 +263,6 @@ class LlamaShapeDecoder:
             x = x + self._mlp(L, _rms(x, L["n2"], c.rms_eps))
         return (_rms(x, self.final_norm, c.rms_eps) @ self.lm_head).float(), rows
 
-    @staticmethod
-    def _look_up(tokens: List[int], drafts: int, ngram: int) -> List[int]:
-        """What followed the last ``ngram`` tokens where they stood before, the last time that they did; -1: nothing."""
-        for at in range(len(tokens) - ngram - 1, -1, -1):
-            if tokens[at:at + ngram] == tokens[-ngram:]:
-                found = tokens[at + ngram:at + ngram + drafts]
-                return found + [-1] * (drafts - len(found))
-        return [-1] * drafts
-
     @torch.inference_mode()
     def generate_drafted(self, ids: torch.Tensor, new_tokens: int, caches: ByteCaches, drafts: int = 7, ngram: int = 2,
                          temperature: float = 0.0, generator: Optional[torch.Generator] = None):
@@ -278,24 +285,24 @@ class LlamaShapeDecoder:
             return torch.rand((b, s), generator=generator, device=self.device)
         first = chances(self.forward(ids, 0, caches))[:, None]
         _, _, token = ops.verify_drafts(torch.zeros((b, 1), dtype=torch.int32, device=self.device), first, drawn(1))
-        told = [row + [t] for row, t in zip(ids.tolist(), token.tolist())]
+        told = [LookedUp(row + [t], ngram) for row, t in zip(ids.tolist(), token.tolist())]
         s = drafts + 1
         mask = torch.ones((s, s), dtype=torch.bool, device=self.device).tril()
         steps = torch.arange(s, dtype=torch.int32, device=self.device)
         rounds = 0
-        while min(len(row) for row in told) < l + new_tokens:
+        while min(len(row.tokens) for row in told) < l + new_tokens:
             # (a sequence that has all its tokens goes along and keeps none)
-            full = [len(row) >= l + new_tokens for row in told]
-            nodes = torch.tensor([[row[-1]] + ([-1] * drafts if done else self._look_up(row, drafts, ngram)) for row, done in zip(told, full)],
-                                 dtype=torch.int32, device=self.device)
+            full = [len(row.tokens) >= l + new_tokens for row in told]
+            asked = [row.tokens[-1:] + row.drafts(drafts) for row in told]
+            nodes = torch.tensor(asked, dtype=torch.int32, device=self.device)
             logits, rows = self._draft_logits(nodes.clamp(min=0).long(), mask, caches.lengths[:, None] + steps, caches)
             path, counts, token = ops.verify_drafts(nodes, chances(logits), drawn(s))
             counts = torch.where(torch.tensor(full, device=self.device), torch.zeros_like(counts), counts)
             for layer, (k, v) in zip(caches.layers, rows):
                 seen = ops.byte_append(layer, k, v, caches.lengths, counts, path)
             caches.lengths = seen
-            for row, kept, n, t in zip(told, nodes.tolist(), counts.tolist(), token.tolist()):
+            for row, kept, n, t in zip(told, asked, counts.tolist(), token.tolist()):
                 if n:
-                    row += kept[1:n] + [t]
+                    row.tokens += kept[1:n] + [t]
             rounds += 1
-        return torch.tensor([row[l:l + new_tokens] for row in told], device=self.device), rounds
+        return torch.tensor([row.tokens[l:l + new_tokens] for row in told], device=self.device), rounds

@@ -103,3 +103,18 @@ def test_sizes_beyond_32_bits_do_not_reach_the_library_as_others(monkeypatch, ca
     cache = ops.ByteCache(1, 1, 64, 64, device="cpu")
     with pytest.raises(ValueError, match="beyond 32 bits"):
         call(lambda *shape: torch.empty(shape, device="meta"), cache)
+
+
+@pytest.mark.parametrize("ngram", [1, 2, 3])
+def test_drafts_are_what_followed_the_last_time(ngram):
+    from lrqk_amd.decoder import LookedUp
+    g = torch.Generator().manual_seed(ngram)
+    row = LookedUp(torch.randint(0, 4, (5,), generator=g).tolist(), ngram)
+    for _ in range(60):
+        t, want = row.tokens, [-1] * 4
+        for at in range(len(t) - ngram):
+            if t[at:at + ngram] == t[-ngram:]:
+                want = (t[at + ngram:] + [-1] * 4)[:4]
+        assert row.drafts(4) == want
+        row.tokens += torch.randint(0, 4, (int(torch.randint(1, 4, (), generator=g)),), generator=g).tolist()
+    assert LookedUp([1], 2).drafts(2) == [-1, -1]
