@@ -210,6 +210,28 @@ def test_token_by_token_is_as_at_once(ops, dtype, kind):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dtype", [BF, FP])
+def test_sequences_made_shorter(ops, dtype, kind):
+    """To whole blocks, to where the tail has the block that they end in, and again from the same lengths: what is appended then and
+    what is read is that of the shorter ones."""
+    print("byte shorter", dtype, kind, flush=True)
+    g = _gen(21)
+    b, d = 4, 64
+    for n in (300, 320, 383):
+        cache = ops.ByteCache(b, 2, 500, d, dtype, kind, DEV)
+        k, v = (_randn(g, b, 2, n, d, dtype=dtype) for _ in range(2))
+        ops.byte_append(cache, k, v, torch.zeros(b, dtype=torch.int32, device=DEV))
+        lengths = _i32(n // 64 * 64 - 64, 64, (n - 128 + 63) // 64 * 64 + 5, 0)
+        for t in (1, 64, 40):
+            q, kn, vn, mask = _drafts(g, b, 4, 2, t, d, dtype)
+            _check_attention(ops, q, cache, lengths, kn, vn, mask, what=(n, t))
+            for _ in range(2):
+                _check_append(ops, cache, kn, vn, lengths, what=(n, t))
+        lengths = ops.byte_append(cache, kn, vn, lengths)
+        _check_attention(ops, q, cache, lengths, what=n)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [BF, FP])
 def test_append_odd_values(ops, dtype, kind):
     """Elements next to and on the border between two codes, of all sizes, blocks of zeros, infinities and NaN."""
     print("append values", dtype, kind, flush=True)
@@ -419,6 +441,19 @@ def test_attention_long_caches_and_splits(ops, dtype, kind):
         q, kn, vn, mask = _drafts(g, b, hq, hc, t, 64, dtype)
         lengths = _i32(*([n] + [n // 3] * (b - 1)))
         _check_attention(ops, q, cache, lengths, kn, vn, mask, what=(b, n))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_attention_of_the_most_drafts(ops, dtype):
+    """1024 drafted tokens, over nothing and over a few blocks; one more is refused."""
+    print("byte most drafts", dtype, flush=True)
+    g = _gen(1024)
+    cache, lengths = _cache(ops, g, 2, 1, 200, 64, dtype, "int8")
+    q, kn, vn, mask = _drafts(g, 2, 2, 1, 1025, 64, dtype, 0.02)
+    first = [x[:, :, :1024] for x in (q, kn, vn)] + [mask[:, :1024, :1024]]
+    _check_attention(ops, first[0], cache, _i32(0, 200), *first[1:])
+    with pytest.raises(Exception, match="1024"):
+        ops.byte_attention(q, cache, lengths, kn, vn, mask)
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])
@@ -1044,3 +1079,14 @@ def test_drafted_generation_is_greedy_generation(ops, kind):
     for bad in (dict(drafts=0), dict(new_tokens=0), dict(ngram=0), dict(temperature=-1.0), dict(new_tokens=190)):
         with pytest.raises(ValueError):
             m.generate_drafted(**{**dict(ids=ids, new_tokens=5, caches=caches), **bad})
+
+
+def test_drafted_generation_of_short_prompts(ops):
+    """Prompts of one token, fewer than are looked up with, and a cache that is full at the end."""
+    print("drafted short", flush=True)
+    m = _model(FP, rope_interleaved=True)
+    for b, l, new in ((1, 1, 1), (2, 1, 40), (1, 3, 57)):
+        ids = torch.randint(0, 97, (b, l), generator=_gen(l)).to(DEV)
+        want, *_ = m.generate(ids, new, m.new_byte_caches(b, 64))
+        got, _ = m.generate_drafted(ids, new, m.new_byte_caches(b, 64), drafts=4, ngram=3)
+        assert torch.equal(got, want), (b, l, new)
