@@ -962,12 +962,20 @@ class ByteCache:
         v = torch.zeros((batch, heads, blocks, w, self.BLOCK), dtype=self._CODES[kind], device=device)
         scales = (torch.ones((batch, heads, blocks), device=device) for _ in range(2))
         tails = (torch.zeros((batch, heads, self.TAIL, head_dim), dtype=dtype, device=device) for _ in range(2))
-        self._buffers = (k, v, *scales, *tails)   # (what the calls are given: made here and never others)
-        self._dev = k.get_device()
         self._sizes = (batch, heads, blocks, head_dim)
-        self._places = tuple(x.data_ptr() for x in self._buffers)
-        self._ranges = tuple((x.data_ptr(), x.data_ptr() + x.nbytes) for x in self._buffers)
         self._code = _lib.CODES[kind]
+        self._hold((k, v, *scales, *tails))
+
+    def _hold(self, buffers):
+        """What the calls are given: the places of these buffers, which never become others."""
+        self._buffers = buffers
+        self._dev = buffers[0].get_device()
+        self._places = tuple(x.data_ptr() for x in buffers)
+        self._ranges = tuple((x.data_ptr(), x.data_ptr() + x.nbytes) for x in buffers)
+
+    def __setstate__(self, state):   # (a copy has buffers of its own)
+        self.__dict__.update(state)
+        self._hold(self._buffers)
 
     k, v, k_scale, v_scale, k_tail, v_tail = (property(lambda self, i=i: self._buffers[i]) for i in range(6))
 

@@ -1,7 +1,9 @@
 """The 8-bit cache, its attention and the verification of drafts as far as they go without a GPU: what the entry points refuse
 before they launch anything (the pointers that these calls are given lead nowhere), and the sizes of their scratch."""
+import copy
 import ctypes
 import math
+import pickle
 
 import pytest
 import torch
@@ -118,3 +120,11 @@ def test_drafts_are_what_followed_the_last_time(ngram):
         assert row.drafts(4) == want
         row.tokens += torch.randint(0, 4, (int(torch.randint(1, 4, (), generator=g)),), generator=g).tolist()
     assert LookedUp([1], 2).drafts(2) == [-1, -1]
+
+
+def test_copies_of_a_cache_are_given_their_own_buffers():
+    one = ops.ByteCache(1, 2, 100, 16, torch.float32, "int8", "cpu")
+    for other in (copy.deepcopy(one), pickle.loads(pickle.dumps(one))):
+        assert other._places == tuple(x.data_ptr() for x in other._buffers) and not set(other._places) & set(one._places)
+        assert [lo for lo, _ in other._ranges] == list(other._places)
+    assert copy.copy(one)._places == one._places

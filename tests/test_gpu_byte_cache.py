@@ -292,6 +292,17 @@ def test_append_places_and_strides(ops):
         _check_append(ops, cache, k[:, :, ::3], v[:, :, ::3], _i32(0, 1))
 
 
+def test_a_copy_of_a_cache_is_written_for_itself(ops):
+    import copy
+    g = _gen(3)
+    cache, lengths = _cache(ops, g, 2, 2, 70, 64, BF, "int8")
+    before = _held(cache)
+    twin = copy.deepcopy(cache)
+    k, v = (_randn(g, 2, 2, 60, 64, dtype=BF) for _ in range(2))
+    _check_append(ops, twin, k, v, lengths)
+    _same(cache, before)
+
+
 def test_append_refuses_rows_of_the_cache(ops):
     cache = ops.ByteCache(2, 2, 128, 64, BF, "int8", DEV)
     n, k = _i32(0, 0), torch.zeros((2, 2, 3, 64), dtype=BF, device=DEV)
