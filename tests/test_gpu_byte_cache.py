@@ -1018,6 +1018,36 @@ def test_rounds_replayed_from_graphs(ops, dtype, s, hq):
             assert all(torch.equal(getattr(cache, n).float(), getattr(mine[0], n).float()) for n in NAMES)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("b,t,hq", [(1, 1, 4), (20, 1, 4), (20, 7, 8), (3, 40, 4)])
+def test_graphs_of_one_pool_over_changing_lengths(ops, dtype, b, t, hq):
+    """Two captured attentions that share the memory that they allocate, replayed in turn over lengths that change, eager calls
+    between: the same bits as eager calls."""
+    print("pool", dtype, b, t, hq, flush=True)
+    g = _gen(b + t)
+    cache, full = _cache(ops, g, b, 2, 900, 64, dtype, "int8")
+    inputs = [_drafts(g, b, hq, 2, t, 64, dtype) for _ in range(2)]
+    lengths = full.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.byte_attention(inputs[0][0], cache, lengths, *inputs[0][1:], return_lse=True)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs, pool = [], [], torch.cuda.graph_pool_handle()
+    for q, kn, vn, mask in inputs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append([x.clone() for x in ops.byte_attention(q, cache, lengths, kn, vn, mask, return_lse=True)])
+        graphs.append(graph)
+    for _ in range(6):
+        lengths.copy_(torch.randint(0, 901, (b,), generator=g).to(torch.int32))
+        for graph, out, (q, kn, vn, mask) in zip(graphs, outs, inputs):
+            want = ops.byte_attention(q, cache, lengths, kn, vn, mask, return_lse=True)
+            graph.replay()
+            assert all(torch.equal(x, y) for x, y in zip(out, want))
+            torch.cuda.synchronize()
+
+
 def test_two_streams_at_once(ops):
     """The same calls on two streams at once and on one after the other have the same bits."""
     print("streams", flush=True)
