@@ -13,8 +13,8 @@
 //
 // Three launches: Z of the nodes with several children (trees with p only); the walk, by every workgroup for itself, and the
 // sums of what is left by chunks of the vocabulary; the chunk and the token.
-// Bound by launches and their chains of reads: over one fp32 row of 128256 tokens the sums take 3.9 us and the token 5.0 (8.4
-// together, as replayed), over 16 trees of 16 nodes without p 7.8 and 5.9; an eager call costs the host 14 .. 17.  (One launch
+// Bound by launches and their chains of reads: over one fp32 row of 128256 tokens the sums take 3.4 us and the token 4.8 (7.9
+// together, as replayed), over 16 trees of 16 nodes without p 7.6 and 6.2; an eager call costs the host 14 .. 17.  (One launch
 // for both would have its workgroups wait for each other.)
 #include <algorithm>
 
@@ -45,7 +45,7 @@ struct VerifyEnd {   // where a sequence's walk ended
 };
 
 __device__ __forceinline__ double vf_positive(double x) { return fmax(x, 0.0); }         // (NaN: 0)
-__device__ __forceinline__ double vf_probability(float x) { return (double)fmaxf(x, 0.0f); }
+__device__ __forceinline__ double vf_probability(float x) { return fmax((double)x, 0.0); }   // (a maximum in fp32 is two instructions)
 
 // A tree as the threads of a workgroup see it.
 struct VerifyTree {
@@ -82,9 +82,47 @@ __device__ __forceinline__ bool vf_accepts(double u, double px, double mass, dou
   return u * px * mass < vf_positive(fma(-cut, px, qx));
 }
 
+// add(q, p) of two rows of n pieces of N elements, by a workgroup, EACH pieces of a thread at a time.  (The end is one such step
+// too, with those behind it left out: one after the other they wait for memory as often.)
+template <typename T, int N, int EACH, bool END, typename F>
+__device__ __forceinline__ void vf_step(const T* q, const T* p, int64_t at, int64_t n, F add) {
+  float qs[EACH][N], ps[EACH][N];
+  [[maybe_unused]] Vec16<T> qv[EACH], pv[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    if (END && at - (int)threadIdx.x + e * kVfWide >= n) break;
+    const int64_t x = (END ? min(at + e * kVfWide, n - 1) : at + e * kVfWide) * N;
+    if constexpr (N == 1) {
+      qs[e][0] = ld_f32(q, x);
+      ps[e][0] = ld_f32(p, x);
+    } else {
+      qv[e].load(q + x);
+      pv[e].load(p + x);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    if (END && at - (int)threadIdx.x + e * kVfWide >= n) break;
+    if constexpr (N > 1) {
+      qv[e].unpack(qs[e]);
+      pv[e].unpack(ps[e]);
+    }
+    if (END && at + e * kVfWide >= n) continue;
+#pragma unroll
+    for (int i = 0; i < N; ++i) add(qs[e][i], ps[e][i]);
+  }
+}
+template <typename T, int N, int EACH, typename F>
+__device__ __forceinline__ void vf_pass(const T* q, const T* p, int64_t n, F add) {
+  int64_t done = 0;
+  for (; done + EACH * kVfWide <= n; done += EACH * kVfWide) vf_step<T, N, EACH, false>(q, p, done + threadIdx.x, n, add);
+  if (done < n) vf_step<T, N, EACH, true>(q, p, done + threadIdx.x, n, add);
+}
+
 // Z of the children of one node, one after the other up to the one that is accepted: a workgroup has both rows for itself.  Bound
-// by one CU, 9.5 us a pass over 128256 tokens: seven instructions an element in 64 bits (6.5) beside 1 MB from the L2 (7.8);
-// more loads ahead changed nothing.  (Several CUs would have to wait for each other, or for a launch a child.)
+// by one CU's arithmetic, 9 us a pass over 128256 tokens, six instructions an element in 64 bits: rows of half the bytes take as
+// long, and rows kept in registers and LDS from pass to pass.  (Several CUs would have to wait for each other, or for a launch a
+// child.)
 template <typename T>
 __global__ __launch_bounds__(kVfWide) void verify_mass_kernel(VerifyArgs a) {
   __shared__ VerifyTree tree;
@@ -95,109 +133,92 @@ __global__ __launch_bounds__(kVfWide) void verify_mass_kernel(VerifyArgs a) {
   const T* p = (const T*)a.p + b * a.pb + n * a.pr;
   double cut = 0.0, mass = 1.0;
   bool first = true;
-  for (int i = n + 1; i < a.s; ++i) {
-    if (tree.parent[i] != n) continue;
-    if (!first) {
-      cut += mass;
-      double sum = 0.0;
-      auto add = [&](float qx, float px) { sum += vf_positive(fma(-cut, vf_probability(px), (double)qx)); };
-      int64_t done = 0;
-      if (((uintptr_t)q | (uintptr_t)p) % 16 == 0) {
-        constexpr int N = Vec16<T>::N, EACH = 4;
-        const int64_t step = (int64_t)EACH * kVfWide * N;
-        for (; done + step <= a.vocab; done += step) {
-          Vec16<T> qv[EACH], pv[EACH];
-#pragma unroll
-          for (int e = 0; e < EACH; ++e) {
-            const int64_t x = done + ((int64_t)e * kVfWide + threadIdx.x) * N;
-            qv[e].load(q + x);
-            pv[e].load(p + x);
-          }
-#pragma unroll
-          for (int e = 0; e < EACH; ++e) {
-            float qs[N], ps[N];
-            qv[e].unpack(qs);
-            pv[e].unpack(ps);
-#pragma unroll
-            for (int i = 0; i < N; ++i) add(qs[i], ps[i]);
-          }
-        }
+  for (int base = n + 1; base < a.s; base += kWave) {
+    const int mine = base + lane_id();
+    unsigned long long children = __ballot(mine < a.s && tree.parent[min(mine, a.s - 1)] == n);
+    for (; children; children &= children - 1) {
+      const int i = base + __ffsll(children) - 1, x = tree.token[i];
+      const int64_t at = (int64_t)b * a.s + i;
+      // (asked for before the pass, which they do not wait for)
+      const float u = a.u[at], qx = ld_f32(q, max(x, 0)), px = ld_f32(p, max(x, 0));
+      if (!first) {
+        cut += mass;
+        double sum = 0.0;
+        auto add = [&](float qy, float py) { sum += vf_positive(fma(-cut, vf_probability(py), (double)qy)); };
+        constexpr int N = Vec16<T>::N;
+        const int64_t whole = ((uintptr_t)q | (uintptr_t)p) % 16 == 0 ? a.vocab / N : 0;
+        vf_pass<T, N, 4>(q, p, whole, add);
+        vf_pass<T, 1, 8>(q + whole * N, p + whole * N, a.vocab - whole * N, add);
+        mass = vf_sum<kVfWide>(sum, scratch);
       }
-      constexpr int EACH = 8;
-      for (; done + EACH * kVfWide <= a.vocab; done += EACH * kVfWide) {
-        float qs[EACH], ps[EACH];
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-          qs[e] = ld_f32(q, done + e * kVfWide + threadIdx.x);
-          ps[e] = ld_f32(p, done + e * kVfWide + threadIdx.x);
-        }
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) add(qs[e], ps[e]);
+      first = false;
+      if (threadIdx.x == 0) {
+        a.cut[at] = cut;
+        a.mass[at] = mass;
       }
-      for (int64_t x = done + threadIdx.x; x < a.vocab; x += kVfWide) add(ld_f32(q, x), ld_f32(p, x));
-      mass = vf_sum<kVfWide>(sum, scratch);
+      // (behind an accepted child nobody asks: of a node's accepted children the first counts)
+      if (x >= 0 && vf_accepts((double)u, vf_probability(px), mass, vf_probability(qx), cut)) return;
     }
-    first = false;
-    if (threadIdx.x == 0) {
-      a.cut[(int64_t)b * a.s + i] = cut;
-      a.mass[(int64_t)b * a.s + i] = mass;
-    }
-    // (behind an accepted child nobody asks: of a node's accepted children the first counts)
-    const int x = tree.token[i];
-    if (x >= 0 && vf_accepts((double)a.u[(int64_t)b * a.s + i], vf_probability(ld_f32(p, x)), mass, vf_probability(ld_f32(q, x)), cut)) return;
   }
 }
 
 // The walk from the root.  Every node is tested, as if its earlier siblings were refused; then the path is followed.
 template <typename T>
 __device__ __forceinline__ void vf_walk(const VerifyArgs& a, int b, VerifyTree& tree, double* own, int* chosen, int& end, double& cut, int& count) {
-  vf_read<kVfThreads>(a, b, tree);
+  end = 0;
+  count = 1;
+  cut = 0.0;
+  if (a.s == 1) return;
+  for (int i = threadIdx.x; i < a.s; i += kVfThreads) chosen[i] = INT32_MAX;
+  vf_read<kVfThreads>(a, b, tree);   // (holds a barrier)
   const T* q = (const T*)a.q + b * a.qb;
   const T* p = (const T*)a.p + b * a.pb;
-  for (int i = threadIdx.x; i < a.s; i += kVfThreads) {
-    chosen[i] = INT32_MAX;
-    const int up = tree.parent[i], x = tree.token[i];
-    double mine = up >= 0 && x >= 0 ? vf_probability(ld_f32(q + up * a.qr, x)) : 0.0;
-    // (without p: a token that an earlier sibling has is gone)
-    if (!a.p && a.parents && up >= 0)
-      for (int j = up + 1; j < i; ++j)
-        if (tree.parent[j] == up && tree.token[j] == x) mine = 0.0;
-    own[i] = mine;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.s; i += kVfThreads) {
-    const int up = tree.parent[i], x = tree.token[i];
-    if (up < 0 || x < 0) continue;
-    const double u = (double)a.u[(int64_t)b * a.s + i];
-    bool taken;
-    if (a.p) {
-      const double px = vf_probability(ld_f32(p + up * a.pr, x));
-      const double c = a.parents ? a.cut[(int64_t)b * a.s + i] : 0.0, mass = a.parents ? a.mass[(int64_t)b * a.s + i] : 1.0;
-      taken = vf_accepts(u, px, mass, own[i], c);
-    } else {
+  if (a.p) {
+    for (int i = threadIdx.x; i < a.s; i += kVfThreads) {
+      const int up = tree.parent[i], x = tree.token[i];
+      if (up < 0 || x < 0) continue;
+      const int64_t at = (int64_t)b * a.s + i;
+      const double c = a.parents ? a.cut[at] : 0.0, mass = a.parents ? a.mass[at] : 1.0;
+      if (vf_accepts((double)a.u[at], vf_probability(ld_f32(p + up * a.pr, x)), mass, vf_probability(ld_f32(q + up * a.qr, x)), c))
+        atomicMin(&chosen[up], i);
+    }
+  } else {
+    for (int i = threadIdx.x; i < a.s; i += kVfThreads) {
+      const int up = tree.parent[i], x = tree.token[i];
+      double mine = up >= 0 && x >= 0 ? vf_probability(ld_f32(q + up * a.qr, x)) : 0.0;
+      // (a token that an earlier sibling has is gone)
+      if (a.parents && up >= 0)
+        for (int j = up + 1; j < i; ++j)
+          if (tree.parent[j] == up && tree.token[j] == x) mine = 0.0;
+      own[i] = mine;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.s; i += kVfThreads) {
+      const int up = tree.parent[i];
+      if (up < 0 || tree.token[i] < 0) continue;
       double mass = 1.0;
       if (a.parents)
         for (int j = up + 1; j < i; ++j)
           if (tree.parent[j] == up) mass -= own[j];
-      taken = u * mass < own[i];
+      if ((double)a.u[(int64_t)b * a.s + i] * mass < own[i]) atomicMin(&chosen[up], i);
     }
-    if (taken) atomicMin(&chosen[up], i);
   }
   __syncthreads();
-  end = 0;
-  count = 1;
   while (chosen[end] != INT32_MAX) {   // (a child stands behind its parent: at most s steps)
     end = chosen[end];
     ++count;
   }
   // what the last node's distribution has lost to its children, all of them refused
-  cut = 0.0;
   if (a.p) {
-    if (!a.parents)
+    if (!a.parents) {
       cut = end + 1 < a.s ? 1.0 : 0.0;
-    else {
+    } else {
       int last = -1;
-      for (int i = end + 1; i < a.s; ++i) last = tree.parent[i] == end ? i : last;
+      for (int base = end + 1; base < a.s; base += kWave) {
+        const int i = base + lane_id();
+        const unsigned long long children = __ballot(i < a.s && tree.parent[min(i, a.s - 1)] == end);
+        if (children) last = base + 63 - __clzll(children);
+      }
       if (last >= 0) cut = a.cut[(int64_t)b * a.s + last] + a.mass[(int64_t)b * a.s + last];
     }
   }
@@ -248,16 +269,18 @@ __global__ __launch_bounds__(kVfThreads) void verify_sums_kernel(VerifyArgs a) {
       if (tree.parent[i] == end && tree.token[i] >= 0) gone[atomicAdd(&gone_n, 1)] = tree.token[i];
     __syncthreads();
   }
+  const int lost = a.p ? 0 : gone_n;
   if (chunk == 0) {
     for (int i = count + tid; i < a.s; i += kVfThreads) a.path[(int64_t)b * a.s + i] = -1;
-    for (int i = tid; i < gone_n; i += kVfThreads) a.gone[(int64_t)b * a.s + i] = gone[i];
+    for (int i = tid; i < lost; i += kVfThreads) a.gone[(int64_t)b * a.s + i] = gone[i];
     if (tid == 0) {
       a.counts[b] = count;
-      a.ends[b] = {cut, end, gone_n};
-      for (int i = 0, at = 0; i < count; ++i, at = chosen[at]) a.path[(int64_t)b * a.s + i] = at;
+      a.ends[b] = {cut, end, lost};
+      a.path[(int64_t)b * a.s] = 0;
+      for (int i = 1, at = 0; i < count; ++i) a.path[(int64_t)b * a.s + i] = at = chosen[at];
     }
   }
-  const VerifyRow<T> row(a, b, end, cut, gone, gone_n);
+  const VerifyRow<T> row(a, b, end, cut, gone, lost);
   double r[kVfEach], sum = 0.0;
   row.load((int64_t)chunk * kVfChunk + tid, kVfThreads, a.vocab, r);
 #pragma unroll

@@ -751,6 +751,25 @@ def test_verify_chains_and_trees(ops, dtype, vocab):
             _check_verify(ops, tokens, target, uniforms, None, up, what=(b, s, children, "no draft"))
 
 
+def test_verify_of_a_single_node_with_a_row_of_the_drafting_model(ops):
+    """The library's entry may be given one (the Python call leaves it out): it is not looked at."""
+    from lrqk_amd import _lib
+    lib, b, vocab = _lib.load(), 5, 5000
+    g = _gen(6)
+    target, draft = (_probabilities(g, b, 1, vocab, FP)[i].to(DEV) for i in range(2))
+    tokens, u = torch.zeros((b, 1), dtype=torch.int32, device=DEV), torch.rand((b, 1), generator=g).to(DEV)
+    want = ops.verify_drafts(tokens, target, u)
+    need = lib.lrqk_verify_drafts_workspace(b, 1, vocab)
+    for parents in (None, tokens):
+        ws = torch.full((need // 4,), -1, dtype=torch.int32, device=DEV)
+        path, counts, token = torch.empty_like(tokens), tokens.new_empty(b), tokens.new_empty(b)
+        assert lib.lrqk_verify_drafts(tokens.data_ptr(), None if parents is None else parents.data_ptr(), target.data_ptr(), vocab, vocab,
+                                      draft.data_ptr(), vocab, vocab, u.data_ptr(), path.data_ptr(), counts.data_ptr(), token.data_ptr(), b, 1,
+                                      vocab, ws.data_ptr(), need, _lib.F32, torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip((path, counts, token), want))
+
+
 def test_verify_accepts_all_or_nothing(ops):
     """uniforms of 0 accept what has any probability; drafts equal to the target are always accepted; tokens of probability 0 never."""
     print("verify ends", flush=True)
