@@ -14,7 +14,7 @@
 // Three launches: Z of the nodes with several children (trees with p only); the walk, by every workgroup for itself, and the
 // sums of what is left by chunks of the vocabulary; the chunk and the token.
 // Bound by launches and their chains of reads: over one fp32 row of 128256 tokens the sums take 3.4 us and the token 4.8 (7.9
-// together, as replayed), over 16 trees of 16 nodes without p 7.6 and 6.2; an eager call costs the host 14 .. 17.  (One launch
+// together, as replayed), over 16 trees of 16 nodes without p 7 and 6; an eager call costs the host 14 .. 17.  (One launch
 // for both would have its workgroups wait for each other.)
 #include <algorithm>
 
@@ -185,12 +185,14 @@ __device__ __forceinline__ void vf_walk(const VerifyArgs& a, int b, VerifyTree& 
   } else {
     for (int i = threadIdx.x; i < a.s; i += kVfThreads) {
       const int up = tree.parent[i], x = tree.token[i];
-      double mine = up >= 0 && x >= 0 ? vf_probability(ld_f32(q + up * a.qr, x)) : 0.0;
+      const double mine = up >= 0 && x >= 0 ? vf_probability(ld_f32(q + up * a.qr, x)) : 0.0;
       // (a token that an earlier sibling has is gone)
+      // (without branches, as below: then the reads of many j are under way at once)
+      bool gone = false;
       if (a.parents && up >= 0)
-        for (int j = up + 1; j < i; ++j)
-          if (tree.parent[j] == up && tree.token[j] == x) mine = 0.0;
-      own[i] = mine;
+#pragma unroll 8
+        for (int j = up + 1; j < i; ++j) gone = gone | ((tree.parent[j] == up) & (tree.token[j] == x));
+      own[i] = gone ? 0.0 : mine;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < a.s; i += kVfThreads) {
@@ -198,8 +200,11 @@ __device__ __forceinline__ void vf_walk(const VerifyArgs& a, int b, VerifyTree& 
       if (up < 0 || tree.token[i] < 0) continue;
       double mass = 1.0;
       if (a.parents)
-        for (int j = up + 1; j < i; ++j)
-          if (tree.parent[j] == up) mass -= own[j];
+#pragma unroll 8
+        for (int j = up + 1; j < i; ++j) {
+          const double theirs = own[j];
+          mass -= tree.parent[j] == up ? theirs : 0.0;
+        }
       if ((double)a.u[(int64_t)b * a.s + i] * mass < own[i]) atomicMin(&chosen[up], i);
     }
   }
@@ -224,20 +229,33 @@ __device__ __forceinline__ void vf_walk(const VerifyArgs& a, int b, VerifyTree& 
   }
 }
 
+// Which elements of a chunk are gone, a bit each.  (Every element held against every token that is gone: 4 sequences of 64
+// looked-up siblings took 31 us instead of 16.)
+struct VerifyGone {
+  uint32_t bits[kVfChunk / 32];
+  __device__ __forceinline__ void fill(const int* gone, int n, int64_t first) {   // by the workgroup; holds barriers
+    for (int i = threadIdx.x; i < kVfChunk / 32; i += kVfThreads) bits[i] = 0u;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kVfThreads) {
+      const int64_t x = gone[i] - first;
+      if (x >= 0 && x < kVfChunk) atomicOr(&bits[x / 32], 1u << (x % 32));
+    }
+    __syncthreads();
+  }
+  __device__ __forceinline__ bool has(int64_t x) const { return bits[x % kVfChunk / 32] >> (x % 32) & 1u; }
+};
+
 // What is left of a row, element x.
 template <typename T>
 struct VerifyRow {
   const T *q, *p;     // p: or null
   double cut;
-  const int* gone;    // tokens that are gone
-  int gone_n;
   // (the drafting model's row is not looked at where no child was refused: there may be none for the last node)
-  __device__ __forceinline__ VerifyRow(const VerifyArgs& a, int b, int node, double cut, const int* gone, int gone_n)
-      : q((const T*)a.q + b * a.qb + node * a.qr), p(a.p && cut != 0.0 ? (const T*)a.p + b * a.pb + node * a.pr : nullptr), cut(cut), gone(gone),
-        gone_n(gone_n) {}
-  // N elements from x on, `step` apart; 0 behind the end
+  __device__ __forceinline__ VerifyRow(const VerifyArgs& a, int b, int node, double cut)
+      : q((const T*)a.q + b * a.qb + node * a.qr), p(a.p && cut != 0.0 ? (const T*)a.p + b * a.pb + node * a.pr : nullptr), cut(cut) {}
+  // N elements from x on, `step` apart, without those that are gone (or null); 0 behind the end
   template <int N>
-  __device__ __forceinline__ void load(int64_t x, int step, int64_t end, double (&r)[N]) const {
+  __device__ __forceinline__ void load(int64_t x, int step, int64_t end, const VerifyGone* gone, double (&r)[N]) const {
     float qs[N], ps[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -248,7 +266,7 @@ struct VerifyRow {
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       r[e] = vf_positive(fma(-cut, vf_probability(ps[e]), (double)qs[e]));
-      for (int i = 0; i < gone_n; ++i) r[e] = gone[i] == (int)(x + e * step) ? 0.0 : r[e];
+      if (gone) r[e] = gone->has(x + e * step) ? 0.0 : r[e];
       r[e] = x + e * step < end ? r[e] : 0.0;
     }
   }
@@ -257,6 +275,7 @@ struct VerifyRow {
 template <typename T>
 __global__ __launch_bounds__(kVfThreads) void verify_sums_kernel(VerifyArgs a) {
   __shared__ VerifyTree tree;
+  __shared__ VerifyGone out;
   __shared__ double own[kVfMost], scratch[kVfThreads / kWave];
   __shared__ int chosen[kVfMost], gone[kVfMost], gone_n;
   const int chunk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
@@ -280,9 +299,10 @@ __global__ __launch_bounds__(kVfThreads) void verify_sums_kernel(VerifyArgs a) {
       for (int i = 1, at = 0; i < count; ++i) a.path[(int64_t)b * a.s + i] = at = chosen[at];
     }
   }
-  const VerifyRow<T> row(a, b, end, cut, gone, lost);
+  if (lost) out.fill(gone, lost, (int64_t)chunk * kVfChunk);
+  const VerifyRow<T> row(a, b, end, cut);
   double r[kVfEach], sum = 0.0;
-  row.load((int64_t)chunk * kVfChunk + tid, kVfThreads, a.vocab, r);
+  row.load((int64_t)chunk * kVfChunk + tid, kVfThreads, a.vocab, lost ? &out : nullptr, r);
 #pragma unroll
   for (int e = 0; e < kVfEach; ++e) sum += r[e];
   sum = vf_sum<kVfThreads>(sum, scratch);
@@ -371,7 +391,7 @@ __device__ __forceinline__ void vf_runs(int64_t n, int64_t run, F number, double
 template <typename T>
 __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) {
   __shared__ VerifyFind find;
-  __shared__ int gone[kVfMost];
+  __shared__ VerifyGone out;
   const int b = blockIdx.x, tid = threadIdx.x;
   const VerifyEnd end = a.ends[b];
   const double* sums = a.sums + (int64_t)b * a.chunks;
@@ -384,10 +404,9 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
   } else {
     vf_runs(a.chunks, run, [&](int64_t i) { return sums[i]; }, r);
   }
-  for (int i = tid; i < end.gone; i += kVfThreads) gone[i] = a.gone[(int64_t)b * a.s + i];
-  VerifyPlace at = vf_first<true>(r, u, find);   // (its barriers are those of `gone` too)
-  const bool nothing = at.i < 0;                 // of the target's distribution as it is, then
-  const VerifyRow<T> row(a, b, end.node, nothing ? 0.0 : end.cut, gone, nothing ? 0 : end.gone);
+  VerifyPlace at = vf_first<true>(r, u, find);
+  const bool nothing = at.i < 0;   // of the target's distribution as it is, then
+  const VerifyRow<T> row(a, b, end.node, nothing ? 0.0 : end.cut);
   int64_t token = -1;
   if (!nothing) {
     if (run > 1) {
@@ -397,7 +416,8 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
       at = {i, border};
     }
     const int64_t x0 = at.i * kVfChunk;
-    row.load(x0 + (int64_t)tid * kVfEach, 1, a.vocab, r);
+    if (end.gone) out.fill(a.gone + (int64_t)b * a.s, end.gone, x0);
+    row.load(x0 + (int64_t)tid * kVfEach, 1, a.vocab, end.gone ? &out : nullptr, r);
     __syncthreads();
     const VerifyPlace place = vf_first<false>(r, at.rest, find);
     token = place.i < 0 ? -1 : x0 + place.i;
@@ -405,7 +425,7 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
     const int64_t part = (a.vocab + kVfChunk - 1) / kVfChunk;
     auto number = [&](int64_t i) {
       double one[1];
-      row.load(i, 1, a.vocab, one);
+      row.load(i, 1, a.vocab, nullptr, one);
       return one[0];
     };
     vf_runs(a.vocab, part, number, r);
