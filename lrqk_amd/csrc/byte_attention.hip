@@ -27,6 +27,7 @@ typedef float by_f4 __attribute__((ext_vector_type(4)));
 constexpr float kByUp = 8.0f;          // binary orders that probabilities are formed too large
 constexpr float kByMost = 15.0f;       // binary logarithm of the largest one before they are formed anew (fp16 ends at 2^16)
 constexpr int kByLong = 256;           // blocks of a split, at most
+constexpr float kByLargest = 0x1p24f;  // unit that outputs are held in, at most (ByteWave)
 
 struct ByteArgs {
   TreeArgs tree;             // queries, drafted tokens, outputs, scratch; n: tokens that the cache has room for
@@ -103,16 +104,18 @@ __device__ __forceinline__ void by_top(const float (&x)[MT][NE], const float (&f
 }
 
 // What a wave has of its queries: 16 MT of them, scaled by powers of two into fp16 (up: back, and to the exponents' base), and
-// of their outputs.  FOLD: these are held in units of the first block's scale and the products add to them as they are: the
-// block's scale over that goes into the probabilities' exponents, as far as fp16 has room for it (2^8 either way); of a block
-// beyond, as of all without FOLD, the products are multiplied and added.  It pays where the matrix cores bound (256 queries
+// of their outputs.  FOLD: these are held in units of the largest scale of V so far, or half of it, and the products add to them
+// as they are: the block's scale over that goes into the probabilities' exponents, as far as fp16 has room for it (down to 2^-8);
+// of a block below, as of all without FOLD, the products are multiplied and added.  A unit that is kept while larger scales
+// come ends in infinities: blocks of zeros have 2^-100.  At most it is kByLargest, so that no ratio of a scale to it leaves
+// fp32's range.  It pays where the matrix cores bound (256 queries
 // over up to 64K of four sequences: 223 us, without 233; 100 over 128K 98 and 101) and costs where loads do, of whose registers
 // it needs some (64 over 32K in byte_stream_kernel: 29.4 us, without 27.2; a token over 32K 19.0 and 18.2).  Sums of fp32
 // tensors do not take it: the matrix cores cut off what they add to them.
 template <typename T, int DP, int MT, bool FOLD>
 struct ByteWave {
   static constexpr int VW = DP / 16, CH = DP / 64;
-  static constexpr bool TWO = sizeof(T) == 4, FOLDS = FOLD;
+  static constexpr bool TWO = sizeof(T) == 4;
   by_h8 qh[MT][2 * CH], ql[TWO ? MT : 1][2 * CH];   // elements 64 c + 16 quad + 8 h .. in [2 c + h]
   float up[MT], top[MT], sum[MT];
   ar_f4 o[MT][VW];
@@ -126,8 +129,8 @@ struct ByteWave {
 #pragma unroll
       for (int j = 0; j < VW; ++j) o[m][j] = ar_f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    unit = 1.0f;
-    log_unit = 0.0f;
+    unit = 0x1p-100f;   // (the least scale)
+    log_unit = -100.0f;
   }
   __device__ __forceinline__ void queries(const T* q, int row0, int M, int d, float scale_log2e) {
     const int col = lane_id() & 15, quad = lane_id() >> 4;
@@ -164,10 +167,6 @@ struct ByteWave {
       }
     }
   }
-  __device__ __forceinline__ void first(float vs) {   // (FOLD)
-    unit = vs;
-    log_unit = __builtin_amdgcn_logf(vs);
-  }
   float x[MT][16];   // scores of a block's keys, key 16 quad + 4 u + r in [4 u + r]
   // Scores of its u-th 16 keys, whose operands are kf.
   __device__ __forceinline__ void scores(int u, const by_h8 (&kf)[2 * CH]) {
@@ -190,8 +189,22 @@ struct ByteWave {
   };
   __device__ __forceinline__ Scales scales(float ks, float vs) {
     Scales g;
-    float shift = FOLD ? __builtin_amdgcn_logf(vs) - log_unit : 0.0f;
-    g.apart = !FOLD || !(fabsf(shift) <= 8.0f);
+    float shift = 0.0f;
+    if constexpr (FOLD) {
+      const float log_vs = __builtin_amdgcn_logf(vs);
+      shift = log_vs - log_unit;
+      if (shift > 1.0f) {   // (for every block in which they grow: a few of a split)
+        const float now = fminf(vs, kByLargest), less = unit / now;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int j = 0; j < VW; ++j) o[m][j] *= less;
+        unit = now;
+        log_unit = __builtin_amdgcn_logf(now);
+        shift = log_vs - log_unit;
+      }
+    }
+    g.apart = !FOLD || !(shift >= -8.0f && shift <= 1.0f);
     g.less = g.apart ? 1.0f : unit * __builtin_amdgcn_rcpf(vs);
     g.by = FOLD ? vs / unit : vs;
     shift = g.apart ? 0.0f : shift;
@@ -236,7 +249,7 @@ struct ByteWave {
       }
     }
   }
-  // Around the products of a block whose scale is far from the first's (FOLD): what there is waits in memory meanwhile.  (A
+  // Around the products of a block whose scale is far below the unit (FOLD): what there is waits in memory meanwhile.  (A
   // branch with products of its own costs every block the copying of all outputs from register to register.)
   struct Waiting {
     volatile float o[FOLD ? MT * VW * 4 : 1];
@@ -560,7 +573,6 @@ __global__ __launch_bounds__(kTrThreads, 2) void byte_share_kernel(ByteArgs ba) 
     load_k(begin);
     load_v(begin);
     w.queries(q, row0, at.M, a.d, a.scale_log2e);
-    if constexpr (Wave::FOLDS) w.first(ba.vs[block0 + begin]);
     leave_k(0);
     load_k(begin + 1);
     leave_v(0);

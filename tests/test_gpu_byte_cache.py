@@ -600,6 +600,35 @@ def test_scales_from_end_to_end(ops, dtype):
         _check_attention(ops, q, cache, lengths, kn, vn, mask, what=kind)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("t,hq", [(65, 1), (50, 2)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_blocks_of_small_values_in_front_of_larger_ones(ops, kind, d, t, hq):
+    """Every fourth block, the first of a split where blocks are shared, has values of (almost) nothing beside the others'; scores
+    are equal, rise behind such a block, or leave the larger blocks without weight."""
+    print("byte small and large", kind, d, t, hq, flush=True)
+    n = 64 * 9 + 17
+    small = (torch.arange(n, device=DEV) // 64 % 4 == 0)[:, None] & (torch.arange(n, device=DEV) < 64 * 9)[:, None]
+    for seed, (little, size) in enumerate((x, y) for x in (0.0, 1e-30) for y in (1.0, 100.0, 1e10, 1e25)):
+        g = _gen(seed)
+        v = ((0.5 + torch.rand((1, 1, n, d), generator=g).to(DEV)) * torch.where(small, little, size)).to(BF)
+        q, kn, vn, mask = _drafts(g, 1, hq, 1, t, d, BF, 0.1)
+        q[..., 0], vn = 2.0, (vn.float().abs() * size).to(BF)
+        for nats in (0.0, 5.0, -200.0):
+            k = _randn(g, 1, 1, n, d, dtype=BF, scale=0.0 if nats == 0.0 else 0.02)
+            k[..., 0] = torch.where(small[:, 0], 0.0, nats / 2).to(BF)
+            drafts = (kn, vn, mask) if nats >= 0.0 else (None, None, None)
+            cache = ops.ByteCache(1, 1, n, d, BF, kind, DEV)
+            lengths = ops.byte_append(cache, k, v, _i32(0))
+            _check_attention(ops, q, cache, lengths, *drafts, scale=1.0, what=(little, size, nats))
+            out, _ = _check_attention(ops, q, cache, lengths // 64 * 64, scale=1.0, what=(little, size, nats, "blocks alone"))
+            if nats < 0.0 and little:
+                # the small values alone: an output's and a probability's rounding, 2^-12 of the scores' arithmetic (products of 128
+                # elements that add up to 5, and 4 more units), V of one sign (the larger blocks' weight is e^-195 / 200)
+                want = _attention64(q, cache, lengths // 64 * 64, None, None, None, 1.0)[0]
+                _within(out, want, (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -12) * want.abs(), (little, size, "small alone"))
+
+
 def test_queries_that_are_not_finite(ops):
     """They spoil their own outputs alone."""
     print("byte odd queries", flush=True)
