@@ -4,8 +4,8 @@ Only the call pattern matters here: every layer calls ``cache.update(q, k, v, la
 as the reference's patched attention does (lrqk_attention.py:2254-2290, 2326-2344) -- raw K/V
 and ordinary causal attention over the prompt, the active set ``[b,Hq,k+L,d]`` and exact
 single-query attention per decoded token.  Projections, norms, rotary embedding, SwiGLU and the
-prompt attention are plain PyTorch-ROCm library calls on random-initialised weights (scaled or
-interleaved rotary positions: the HIP library's); the cache path (factorisation, selection, fetch, decode attention) is the HIP library.
+prompt attention are plain PyTorch-ROCm library calls on random-initialised weights (rotary positions
+that are scaled, interleaved or over caches in 8 bits: the HIP library's); the cache path (factorisation, selection, fetch, decode attention) is the HIP library.
 
 ``new_byte_caches`` gives a dense K/V cache in 8 bits instead, which ``generate`` takes as any other and
 ``generate_drafted`` decodes several looked-up tokens at once over (rotary positions, attention, verification and the
@@ -116,7 +116,7 @@ class LlamaShapeDecoder:
         self.rope = None   # (else the library turns q and k, in one launch)
         if c.rope_interleaved or c.rope_scaling is not None:
             self.rope = ops.RotaryPlan(c.head_dim, c.rope_theta, c.rope_interleaved, c.rope_scaling, self.device)
-        self._plan = None  # of generate_drafted, whose sequences have positions of their own
+        self._byte_plan = self.rope   # over caches in 8 bits, whose sequences have positions of their own
         self.ws = ops.Workspace()
         self.dense: Optional[List[Tuple[torch.Tensor, torch.Tensor]]] = None
         self.progress = None   # optional callable(str), called once per layer while the prompt is processed
@@ -130,6 +130,12 @@ class LlamaShapeDecoder:
         cos, sin = torch.cos(ang), torch.sin(ang)
         x1, x2 = x[..., :d // 2].float(), x[..., d // 2:].float()
         return torch.cat([x1 * cos - x2 * sin, x2 * cos + x1 * sin], dim=-1).to(x.dtype)
+
+    def _rotary_plan(self) -> ops.RotaryPlan:
+        """Of prompts, tokens and drafts over caches in 8 bits alike (at 100K ``_rope``'s angles in fp32 are off by up to 4e-3)."""
+        if self._byte_plan is None:
+            self._byte_plan = ops.RotaryPlan(self.cfg.head_dim, self.cfg.rope_theta, device=self.device)
+        return self._byte_plan
 
     def _mlp(self, L, x: torch.Tensor) -> torch.Tensor:
         out = torch.empty_like(x)
@@ -152,9 +158,11 @@ class LlamaShapeDecoder:
     # ------------------------------------------------------------------ one forward over s new positions
     @torch.inference_mode()
     def forward(self, ids: torch.Tensor, pos0: int, cache: Optional[DynamicLRQKCache]) -> torch.Tensor:
-        """ids [b,s] -> logits of the last position [b,vocab]."""
+        """ids [b,s] -> logits of the last position [b,vocab].  pos0: the first one's position (0 begins anew; over caches in 8 bits
+        a token stands behind what its sequence has, which ``generate_drafted`` may leave different)."""
         c = self.cfg
         b, s = ids.shape
+        rope, where = self.rope, pos0
         x = self.embed[ids]
         if self.context_scale:
             x = x + self.context
@@ -163,17 +171,20 @@ class LlamaShapeDecoder:
         if isinstance(cache, ByteCaches):
             if pos0 + s > cache.capacity or (s > 1 and pos0 > 0):
                 raise ValueError(f"tokens {pos0} .. {pos0 + s - 1}: the cache has room for {cache.capacity}, and a prompt comes at once")
+            rope = self._rotary_plan()
             if pos0 == 0:
                 cache.lengths = torch.zeros_like(cache.lengths)
+            else:
+                where = cache.lengths[:, None]
         for li, L in enumerate(self.layers):
             hcur = _rms(x, L["n1"], c.rms_eps)
             q = (hcur @ L["wq"]).view(b, s, c.heads, c.head_dim).transpose(1, 2)
             k = (hcur @ L["wk"]).view(b, s, c.kv_heads, c.head_dim).transpose(1, 2)
             v = (hcur @ L["wv"]).view(b, s, c.kv_heads, c.head_dim).transpose(1, 2).contiguous()
-            if self.rope is None:
+            if rope is None:
                 q, k = self._rope(q, pos0).contiguous(), self._rope(k, pos0).contiguous()
             else:
-                q, k = ops.rotary(self.rope, q, k, pos0)
+                q, k = ops.rotary(rope, q, k, where)
             if cache is None:
                 if self.dense[li] is None:
                     self.dense[li] = (k, v)
@@ -245,8 +256,7 @@ class LlamaShapeDecoder:
         of every layer, which go into the cache once it is known which tokens stay."""
         c = self.cfg
         b, s = ids.shape
-        if self._plan is None:
-            self._plan = self.rope or ops.RotaryPlan(c.head_dim, c.rope_theta, device=self.device)
+        plan = self._rotary_plan()
         x = self.embed[ids]
         if self.context_scale:
             x = x + self.context
@@ -256,7 +266,7 @@ class LlamaShapeDecoder:
             q = (hcur @ L["wq"]).view(b, s, c.heads, c.head_dim).transpose(1, 2)
             k = (hcur @ L["wk"]).view(b, s, c.kv_heads, c.head_dim).transpose(1, 2)
             v = (hcur @ L["wv"]).view(b, s, c.kv_heads, c.head_dim).transpose(1, 2)
-            q, k = ops.rotary(self._plan, q, k, positions)
+            q, k = ops.rotary(plan, q, k, positions)
             o = ops.byte_attention(q, layer, caches.lengths, k, v, mask)
             rows.append((k, v))
             x = x + o.transpose(1, 2).reshape(b, s, c.heads * c.head_dim) @ L["wo"]

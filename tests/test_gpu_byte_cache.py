@@ -1179,3 +1179,61 @@ def test_drafted_generation_of_short_prompts(ops):
         want, *_ = m.generate(ids, new, m.new_byte_caches(b, 64))
         got, _ = m.generate_drafted(ids, new, m.new_byte_caches(b, 64), drafts=4, ngram=3)
         assert torch.equal(got, want), (b, l, new)
+
+
+def _turned64(x, positions, theta):
+    """x [b,H,s,d] turned to positions [b,s] by halves, in fp64."""
+    half = x.shape[-1] // 2
+    freq = theta ** (-torch.arange(half, dtype=torch.float64, device=DEV) / half)
+    angle = positions.double()[:, None, :, None] * freq
+    a, z = x[..., :half].double(), x[..., half:].double()
+    return torch.cat((a * torch.cos(angle) - z * torch.sin(angle), z * torch.cos(angle) + a * torch.sin(angle)), -1)
+
+
+def test_positions_of_prompts_tokens_and_drafts(ops):
+    """Keys of a prompt, of single tokens and of drafts are turned to the same far positions alike, also where sequences have
+    different lengths."""
+    print("decoder positions", flush=True)
+    from lrqk_amd.decoder import _rms
+    m, far = _model(FP), 100000
+
+    def keys(ids):   # of the first layer, as they are before they are turned
+        return (_rms(m.embed[ids], m.layers[0]["n1"], m.cfg.rms_eps) @ m.layers[0]["wk"]).view(*ids.shape, 2, 16).transpose(1, 2)
+
+    def check(got, ids, positions, what):
+        # two products, and a sine and a cosine of 2 units each; the sums of 64 products come in another order for another count
+        x = keys(ids)
+        pair = torch.cat([torch.hypot(x[..., :8], x[..., 8:])] * 2, -1).double()
+        sums = _rms(m.embed[ids], m.layers[0]["n1"], m.cfg.rms_eps).abs() @ m.layers[0]["wk"].abs()
+        tol = 6 * U * pair + 64 * U * sums.view(*ids.shape, 2, 16).transpose(1, 2).double().amax(-1, keepdim=True)
+        _within(got, _turned64(x, positions, m.cfg.rope_theta), tol, what)
+
+    ids = torch.randint(0, 97, (2, 3000), generator=_gen(0)).to(DEV)
+    caches = m.new_byte_caches(2, far + 100)
+    m.forward(ids, 0, caches)
+    last = torch.arange(3000 - 128, 3000, device=DEV)
+    check(caches.layers[0].k_tail[:, :, last % 128], ids[:, last], last.expand(2, -1), "prompt")
+    for lengths in (_i32(far, far), _i32(far, far - 70)):
+        caches.lengths = lengths
+        m.forward(ids[:, :1], far, caches)
+        got = torch.stack([caches.layers[0].k_tail[i, :, n % 128] for i, n in enumerate(lengths.tolist())])[:, :, None]
+        check(got, ids[:, :1], lengths[:, None], ("token", lengths.tolist()))
+        steps = torch.arange(4, dtype=torch.int32, device=DEV)
+        _, rows = m._draft_logits(ids[:, :4], torch.ones((4, 4), dtype=torch.bool, device=DEV).tril(), lengths[:, None] + steps, caches)
+        check(rows[0][0], ids[:, :4], lengths[:, None] + steps, ("drafts", lengths.tolist()))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_drafted_generation_of_the_default_layout(ops, dtype):
+    """Halves, turned by the library in both.  While no block is complete every token is read as it came, and fp32 tokens are the
+    same (beyond, a token that completes a block sees it in 8 bits, a round as it came)."""
+    print("drafted halves", dtype, flush=True)
+    m = _model(dtype)
+    ids = torch.randint(0, 97, (2, 20), generator=_gen(5)).to(DEV).repeat(1, 3)
+    got, _ = m.generate_drafted(ids, 60, m.new_byte_caches(2, 200), drafts=5)
+    assert got.shape == (2, 60) and int(got.min()) >= 0 and int(got.max()) < 97
+    got, _ = m.generate_drafted(ids[:, :20], 38, m.new_byte_caches(2, 64), drafts=5)
+    assert got.shape == (2, 38)
+    if dtype == FP:
+        want, *_ = m.generate(ids[:, :20], 38, m.new_byte_caches(2, 64))
+        assert torch.equal(got, want)
