@@ -278,8 +278,10 @@ class LlamaShapeDecoder:
                          temperature: float = 0.0, generator: Optional[torch.Generator] = None):
         """Decoding with drafts that are looked up in the sequence itself: a round attends with a sequence's last token and up to
         ``drafts`` that followed its last ``ngram`` tokens before, verifies them against the model's probabilities (of
-        ``temperature``; 0: its most probable token) and keeps those that stand.  The tokens have the distribution that ``generate``
-        at that temperature has.  ids [b,l] -> (tokens [b,new_tokens], rounds)."""
+        ``temperature``; 0: its most probable token) and keeps those that stand.  A round's tokens have the distribution that its own
+        logits give, token after token as without drafts.  Those of ``generate``, which is greedy, are not the same to the last
+        bit: products are rounded otherwise, and a block that a round completes is read as it came until the round is over, where
+        ``generate`` reads it in 8 bits from its last token on.  ids [b,l] -> (tokens [b,new_tokens], rounds)."""
         b, l = ids.shape
         if drafts < 1 or ngram < 1 or new_tokens < 1 or temperature < 0:
             raise ValueError(f"drafts={drafts}, ngram={ngram}, new_tokens={new_tokens}, temperature={temperature}")

@@ -1237,3 +1237,82 @@ def test_drafted_generation_of_the_default_layout(ops, dtype):
     if dtype == FP:
         want, *_ = m.generate(ids[:, :20], 38, m.new_byte_caches(2, 64))
         assert torch.equal(got, want)
+
+
+def _model64(m, ids, positions, keys, dtype=torch.float64):
+    """The decoder's logits [b,s,vocab] by torch in `dtype`.  keys(layer, sequence, head, k, v) -> what the s tokens attend to,
+    whose own rows [s,d] are k and v, in `dtype`: (keys [n,d], values [n,d], bool [s,n])."""
+    c = m.cfg
+    (b, s), d = ids.shape, c.head_dim
+
+    def rms(x):
+        return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + c.rms_eps)
+
+    def heads(x, w):
+        return (x @ w.to(dtype)).view(b, s, -1, d).transpose(1, 2)
+    x = m.embed[ids].to(dtype)
+    for li, L in enumerate(m.layers):
+        y = rms(x)
+        q, k = (_turned64(heads(y, L[w]), positions, c.rope_theta).to(dtype) for w in ("wq", "wk"))
+        v, o = heads(y, L["wv"]), torch.zeros_like(q)
+        for i in range(b):
+            for h in range(c.heads):
+                g = h * c.kv_heads // c.heads
+                K, V, sees = keys(li, i, g, k[i, g], v[i, g])
+                o[i, h] = torch.softmax((q[i, h] @ K.T * d ** -0.5).masked_fill(~sees, -INF), -1) @ V
+        x = x + o.transpose(1, 2).reshape(b, s, -1) @ L["wo"].to(dtype)
+        y = rms(x)
+        x = x + (torch.nn.functional.silu(y @ L["wg"].to(dtype)) * (y @ L["wu"].to(dtype))) @ L["wd"].to(dtype)
+    return rms(x) @ m.lm_head.to(dtype)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_logits_over_a_cache_in_8_bits(ops, kind):
+    """Tokens and rounds of drafts beyond the first block: the logits are those of the rows that the cache holds by then, in 64 bits.
+    Off by 16 times what the same sums in fp32 by torch are off by (queries and probabilities have 22 bits where those have 24,
+    codes are scaled behind the sums)."""
+    print("decoder logits", kind, flush=True)
+    m = _model(FP)
+    g = _gen(9)
+    ids = torch.randint(0, 97, (2, 400), generator=g).to(DEV)
+    caches = m.new_byte_caches(2, 400, kind)
+    m.forward(ids[:, :100], 0, caches)
+
+    def near(got, new, positions, keys):
+        want, rough = (_model64(m, new, positions, lambda *a: keys(dt, *a), dt) for dt in (torch.float64, FP))
+        _within(got, want, torch.full_like(want, 16 * float((rough - want).abs().max())))
+
+    for n in range(100, 134):   # (the token at 127 is the last one of a block, and sees itself in 8 bits)
+        got = m.forward(ids[:, n:n + 1], n, caches)
+
+        def held(dt, li, i, h, k, v):
+            K, V = (x.to(dt) for x in _rows64(caches.layers[li], i, h, n + 1))
+            return K, V, torch.ones((1, n + 1), dtype=torch.bool, device=DEV)
+        near(got[:, None], ids[:, n:n + 1], torch.full((2, 1), n, device=DEV), held)
+    s, at = 6, torch.arange(2, device=DEV)[:, None]
+    steps, mask = torch.arange(s, dtype=torch.int32, device=DEV), torch.ones((s, s), dtype=torch.bool, device=DEV).tril()
+    for _ in range(12):   # rounds of which the sequences keep different numbers
+        lengths = caches.lengths
+        new = ids[at, lengths[:, None] + steps]
+        got, rows = m._draft_logits(new, mask, lengths[:, None] + steps, caches)
+
+        def both(dt, li, i, h, k, v):
+            n = int(lengths[i])
+            K, V = (torch.cat((x.to(dt), y)) for x, y in zip(_rows64(caches.layers[li], i, h, n), (k, v)))
+            return K, V, torch.cat((torch.ones((s, n), dtype=torch.bool, device=DEV), mask), 1)
+        near(got, new, lengths[:, None] + steps, both)
+        counts = torch.randint(1, s + 1, (2,), generator=g, dtype=torch.int32).to(DEV)
+        for layer, (k, v) in zip(caches.layers, rows):
+            seen = ops.byte_append(layer, k, v, lengths, counts)
+        caches.lengths = seen
+    # and a token where the sequences have different lengths
+    lengths = caches.lengths
+    assert lengths[0] != lengths[1]
+    new = ids[at, lengths[:, None]]
+    got = m.forward(new, int(lengths.max()), caches)
+
+    def ragged(dt, li, i, h, k, v):
+        n = int(lengths[i]) + 1
+        K, V = (x.to(dt) for x in _rows64(caches.layers[li], i, h, n))
+        return K, V, torch.ones((1, n), dtype=torch.bool, device=DEV)
+    near(got[:, None], new, lengths[:, None], ragged)
