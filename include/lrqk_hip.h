@@ -366,7 +366,7 @@ int lrqk_byte_attention(const void* q, const void* k, const void* v, const float
  * [b][s], in [0, 1): [0] for the token that follows, [i] for node i's test.
  * At a node with distribution r of mass Z (first: its row of target, 1) its children are looked at in order; child i with token x
  * and p = draft[node][x] (1 without draft) is accepted if uniforms[i] p Z < r[x]; otherwise r becomes max(r - Z draft[node], 0)
- * (without draft: r without x) and Z its sum.  path [b][s]: the accepted nodes, 0 first, -1 behind them; counts [b]: how many; next
+ * and Z its sum (without draft: r without x, and Z less r[x]: 1 less what the refused tokens had, whatever the row adds up to).  path [b][s]: the accepted nodes, 0 first, -1 behind them; counts [b]: how many; next
  * [b]: the lowest token x with r[0] + .. + r[x] > uniforms[0] (sum of r), r what is left at the last accepted node (its row of target
  * if nothing is; -1 if that has nothing).  In fp64; what is not a positive number counts as 0, and a token outside the vocabulary
  * as one that target and draft give 0.  Limits: s up to 1024, vocab up to 2^30.  Workspace as above. */

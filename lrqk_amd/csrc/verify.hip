@@ -7,7 +7,8 @@
 //   r_j = max(r_(j-1) - Z_(j-1) p, 0) = max(q - C_j p, 0),  C_j = C_(j-1) + Z_(j-1), C_0 = 0,  Z_j = sum of r_j,
 //
 // so that one pass over two rows gives Z_j, and only nodes with several children need one.  Drafts without probabilities have
-// p = 1 at their token: r_j is r_(j-1) without it.  Behind the last accepted node the next token is drawn from what is left:
+// p = 1 at their token: r_j is r_(j-1) without it, and Z_j = Z_(j-1) - r_(j-1)(x_j), 1 less what the refused ones had, whatever
+// the row adds up to (its sum would be a pass; a row of bf16 probabilities is off by up to 2^-8).  Behind the last accepted node the next token is drawn from what is left:
 // the lowest x with r(0) + .. + r(x) > u_0 sum(r).  Everything is formed in 64 bits, since a vocabulary's sums in 32 would
 // put the border between two tokens elsewhere; what is not a positive number counts as 0.
 //

@@ -1097,8 +1097,9 @@ def verify_drafts(tokens: torch.Tensor, target: torch.Tensor, uniforms: torch.Te
     ``uniforms`` fp32 [b,s], in [0,1): the first for the token that follows, the others for their nodes' tests.
 
     At a node the children are looked at in order with what is left of its distribution, r of mass Z (first: its row of target,
-    1): token x is accepted if u draft[x] Z < r[x] (without draft: u Z < r[x]), else r becomes max(r - Z draft, 0) (r without
-    x).  The token that follows is the lowest x with r[0] + .. + r[x] > u sum(r) at the last accepted node (of its row of target
+    1): token x is accepted if u draft[x] Z < r[x] (without draft: u Z < r[x]), else r becomes max(r - Z draft, 0) and Z
+    its sum (without draft: r without x and Z less r[x], that is 1 less what the refused tokens had, whatever the row adds up
+    to).  The token that follows is the lowest x with r[0] + .. + r[x] > u sum(r) at the last accepted node (of its row of target
     if nothing is left, -1 if that has nothing).  In fp64; what is not a positive number counts as 0, a token outside the
     vocabulary as one of probability 0.
     -> path int32 [b,s] (accepted nodes, 0 first, -1 behind them), counts int32 [b], the token that follows int32 [b]:

@@ -855,6 +855,25 @@ def test_verify_odd_inputs(ops):
                 _check_verify(ops, tokens, target, uniforms, d, parents, what=kind)
 
 
+def test_verify_looked_up_drafts_of_rows_that_do_not_add_up_to_one(ops):
+    """Without probabilities of the drafts, Z is 1 less those of the refused tokens, whatever a row adds up to; with them it is the
+    sum of what is left."""
+    print("verify unequal sums", flush=True)
+    target = torch.zeros((1, 3, 8), device=DEV)
+    target[..., 0], target[..., 1] = 0.3, 0.2
+    tokens, parents = _i32(5, 0, 1)[None], _i32(-1, 0, 0)[None]
+    draft = torch.full_like(target, 0.125)
+    for u, looked_up, drawn in ((0.28, True, True), (0.29, False, True), (0.999, False, True)):
+        uniforms = torch.tensor([[0.5, 0.9, u]], device=DEV)   # 0.9 > 0.3: refused; then u 0.7 < 0.2, if the sum counted u 0.2 < 0.2
+        _, counts, _ = _check_verify(ops, tokens, target, uniforms, None, parents, what=u)
+        assert counts.tolist() == [1 + looked_up]
+        # (0.9 / 8 < 0.3 would be accepted: 0.9 of a target of 0.1.  Left are then 0.075 of token 1, and Z is that)
+        less = target.clone()
+        less[..., 0] = 0.1
+        _, counts, _ = _check_verify(ops, tokens, less, uniforms, draft, parents, what=u)
+        assert counts.tolist() == [1 + drawn]
+
+
 def test_verify_places_and_the_largest_trees(ops):
     print("verify places", flush=True)
     g = _gen(22)
