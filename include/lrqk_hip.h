@@ -346,7 +346,9 @@ int lrqk_evict(float* weights, int32_t* ids, void* k, void* v, const int32_t* le
  * sequences mask_batch_stride apart, 0: one for all); k_new, v_new and mask NULL: to the cached ones alone.  out [b][hq][t][d], lse
  * (or NULL) as lrqk_tree_attention leaves them, also for masked drafted tokens that are not finite and for queries that see
  * nothing.  Scores of bf16 queries come from their elements as they are (those below 2^-28 of a query's largest lose bits); what
- * probabilities are multiplied with codes in has 11 bits (bf16 tensors) or 22 (fp32), and 16 or 24 for the tail and the drafted.  Limits: as
+ * probabilities are multiplied with codes in has 11 bits (bf16 tensors) or 22 (fp32), and 16 or 24 for the tail and the drafted; they
+ * are full down to 2^-22 of a query's largest (2^-13 in blocks of smaller values among more than 64 bf16 queries a cache head).
+ * 2^15 times the sum of all tokens' largest |v| has to be a finite fp32 number.  Limits: as
  * lrqk_tree_attention, blocks up to 2^24.  Workspace as above. */
 enum { LRQK_CODE_INT8 = 0, LRQK_CODE_FP8 = 1 };
 int lrqk_byte_append(const void* k_new, const void* v_new, const int64_t* strides, int t, int most, const int32_t* lengths,

@@ -8,6 +8,8 @@
 // them, and probabilities of 11 bits where bf16 would have 8.  A query is scaled by a power of two to where fp16 holds it
 // (bf16 ones exactly but for elements 2^-28 of the largest; fp32 ones as the sum of two fp16 numbers, as their probabilities).
 // Probabilities are formed 2^8 too large, so that those of 2^-22 of the largest keep all bits and those of 2^-33 are not lost.
+// (Of more than 64 bf16 queries a cache head less: where a block's scale of V is 2^-n of the largest before it, n up to 9, its
+// probabilities are 2^n smaller, full to 2^(n-22) and lost beyond 2^(n-33); they are sums' parts in fp32 all the same.)
 //
 // As in tree_attention.hip a query is a lane's column of S^T = C Q^T, and the probabilities are the operand of O^T = C'^T P^T
 // as they lie: row m of the i-th 16 keys of a block is key 16 (m / 4) + 4 i + m % 4, so that a quad's scores are those of 16

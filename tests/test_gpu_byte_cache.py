@@ -629,6 +629,33 @@ def test_blocks_of_small_values_in_front_of_larger_ones(ops, kind, d, t, hq):
                 _within(out, want, (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -12) * want.abs(), (little, size, "small alone"))
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_blocks_of_smaller_values_keep_small_probabilities(ops, kind):
+    """One element is large, in every fourth block alone; the others are there in the other blocks alone, 2^-order as large, with
+    probabilities that end near what fp16 holds."""
+    print("byte smaller values", kind, flush=True)
+    n, d, t = 64 * 12, 64, 70
+    g = _gen(31)
+    large = (torch.arange(n, device=DEV) // 64 % 4 == 0)[:, None]
+    q = torch.zeros((1, 1, t, d), dtype=BF, device=DEV)
+    q[..., 0] = 1.0
+    for order in (2, 5, 7, 9.5):
+        for nats in (4.0, 8.0, 12.0, 18.0):
+            v = torch.where(large, 0.0, _randn(g, 1, 1, n, d) * 2.0 ** -order)
+            v[..., :1] = torch.where(large, 3.0, 0.0)
+            k = torch.zeros((1, 1, n, d), device=DEV)
+            k[..., 0] = torch.where(large[:, 0], 0.0, -nats) + 0.01 * _randn(g, 1, 1, n)
+            cache = ops.ByteCache(1, 1, n, d, BF, kind, DEV)
+            lengths = ops.byte_append(cache, k.to(BF), v.to(BF), _i32(0))
+            out, lse = ops.byte_attention(q, cache, lengths, scale=1.0, return_lse=True)
+            e, el, tol, tol_l = _attention64(q, cache, lengths, None, None, None, 1.0)
+            if order < 8:   # (what is multiplied in units of the larger scale: 2^-9 of the room that probabilities have)
+                V = list(_rows64(cache, 0, 0, n))[1]
+                tol += (2.0 ** -24 - 2.0 ** -33) * torch.where(large, 0.0, V.abs()).sum(0)
+            _within(out, e, tol, (order, nats))
+            _within(lse, el, tol_l, (order, nats))
+
+
 def test_queries_that_are_not_finite(ops):
     """They spoil their own outputs alone."""
     print("byte odd queries", flush=True)
