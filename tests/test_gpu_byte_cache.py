@@ -656,6 +656,26 @@ def test_blocks_of_smaller_values_keep_small_probabilities(ops, kind):
             _within(lse, el, tol_l, (order, nats))
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("t", [3, 70])
+def test_values_near_the_largest(ops, dtype, t):
+    """As large as 2^15 times a long cache's values may be, cached, in the tail and drafted; also where scores rise behind the first
+    block by almost what probabilities have room for."""
+    print("byte large values", dtype, t, flush=True)
+    n, d = 64 * 300 + 20, 64
+    g = _gen(41)
+    q, kn, _, mask = _drafts(g, 1, 1, 1, t, d, dtype)
+    q[..., 0] = 1.0
+    most = 2.0 ** (127 - 15 - math.log2(n + t))
+    v = most * (0.5 + 0.5 * torch.rand((1, 1, n + t, d), generator=g).to(DEV))
+    for nats in (0.0, 4.8):
+        k = torch.zeros((1, 1, n, d), device=DEV)
+        k[:, :, 64:, 0] = nats
+        cache = ops.ByteCache(1, 1, n, d, dtype, "int8", DEV)
+        lengths = ops.byte_append(cache, k.to(dtype), v[:, :, :n].to(dtype), _i32(0))
+        _check_attention(ops, q, cache, lengths, kn, v[:, :, n:].to(dtype), mask, scale=1.0, what=nats)
+
+
 def test_queries_that_are_not_finite(ops):
     """They spoil their own outputs alone."""
     print("byte odd queries", flush=True)
