@@ -411,10 +411,15 @@ __global__ __launch_bounds__(kVfThreads) void verify_token_kernel(VerifyArgs a) 
   int64_t token = -1;
   if (!nothing) {
     if (run > 1) {
+      // (the last chunk with anything, where rounding hides the border: there may be zeros behind it)
       double border = at.rest;
-      int64_t i = at.i * run;
-      while (i + 1 < min((at.i + 1) * run, (int64_t)a.chunks) && !(sums[i] > border)) border -= sums[i++];
-      at = {i, border};
+      const int64_t stop = min((at.i + 1) * run, (int64_t)a.chunks);
+      for (int64_t i = at.i * run; i < stop; ++i) {
+        const double x = sums[i];
+        if (x > 0.0) at = {i, border};
+        if (x > 0.0 && x > border) break;
+        border -= x;
+      }
     }
     const int64_t x0 = at.i * kVfChunk;
     if (end.gone) out.fill(a.gone + (int64_t)b * a.s, end.gone, x0);

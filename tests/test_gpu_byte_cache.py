@@ -957,6 +957,22 @@ def test_verify_vocabularies_of_many_chunks(ops):
             _check_verify(ops, tokens, target, uniforms, 3 * target, parents, what=(vocab, u, "nothing left"))
 
 
+def test_verify_of_the_last_token_in_front_of_zeros(ops):
+    """More chunks than are looked through at once, the border at the sum itself: the last token that has anything, whatever zeros
+    follow it in its run of chunks, in its chunk and behind both."""
+    print("verify zeros behind", flush=True)
+    vocab = 2048 * 2048 * 2 + 4096 + 5
+    target = torch.zeros((4, 1, vocab), device=DEV)
+    for i, last in enumerate((5, 2048 * 2 * 9 + 3, 2048 * 2 * 9 + 2048 + 2047, vocab - 1)):
+        target[i, 0, 1], target[i, 0, last] = 0.5, 0.25
+    uniforms = torch.ones((4, 1), device=DEV)
+    tokens = torch.zeros((4, 1), dtype=torch.int32, device=DEV)
+    for dtype in (FP, BF):
+        _check_verify(ops, tokens, target.to(dtype), uniforms)
+        _check_verify(ops, tokens, target.to(dtype), uniforms * 0.6)
+        _check_verify(ops, tokens, target.to(dtype), uniforms * 0.7)
+
+
 @pytest.mark.parametrize("children", [1, 3])
 @pytest.mark.parametrize("drafted", [True, False])
 def test_what_is_accepted_or_drawn_has_the_targets_distribution(ops, drafted, children):
