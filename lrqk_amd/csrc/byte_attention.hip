@@ -8,7 +8,7 @@
 // them, and probabilities of 11 bits where bf16 would have 8.  A query is scaled by a power of two to where fp16 holds it
 // (bf16 ones exactly but for elements 2^-28 of the largest; fp32 ones as the sum of two fp16 numbers, as their probabilities).
 // Probabilities are formed 2^8 too large, so that those of 2^-22 of the largest keep all bits and those of 2^-33 are not lost.
-// (Of more than 64 bf16 queries a cache head less: where a block's scale of V is 2^-n of the largest before it, n up to 9, its
+// (Of more than 64 bf16 queries a cache head less: where a block's scale of V is 2^-n of another one's near it, n up to 9, its
 // probabilities are 2^n smaller, full to 2^(n-22) and lost beyond 2^(n-33); they are sums' parts in fp32 all the same.)
 //
 // As in tree_attention.hip a query is a lane's column of S^T = C Q^T, and the probabilities are the operand of O^T = C'^T P^T
@@ -29,7 +29,7 @@ typedef float by_f4 __attribute__((ext_vector_type(4)));
 constexpr float kByUp = 8.0f;          // binary orders that probabilities are formed too large
 constexpr float kByMost = 15.0f;       // binary logarithm of the largest one before they are formed anew (fp16 ends at 2^16)
 constexpr int kByLong = 256;           // blocks of a split, at most
-constexpr float kByLargest = 0x1p24f;  // unit that outputs are held in, at most (ByteWave)
+constexpr float kByLargest = 0x1p24f, kByBelow = 0x1p-60f;   // unit that outputs are held in, at most, and over the largest scale, at least
 
 struct ByteArgs {
   TreeArgs tree;             // queries, drafted tokens, outputs, scratch; n: tokens that the cache has room for
@@ -106,11 +106,12 @@ __device__ __forceinline__ void by_top(const float (&x)[MT][NE], const float (&f
 }
 
 // What a wave has of its queries: 16 MT of them, scaled by powers of two into fp16 (up: back, and to the exponents' base), and
-// of their outputs.  FOLD: these are held in units of the largest scale of V so far, or half of it, and the products add to them
-// as they are: the block's scale over that goes into the probabilities' exponents, as far as fp16 has room for it (down to 2^-8);
-// of a block below, as of all without FOLD, the products are multiplied and added.  A unit that is kept while larger scales
-// come ends in infinities: blocks of zeros have 2^-100.  At most it is kByLargest, so that no ratio of a scale to it leaves
-// fp32's range.  It pays where the matrix cores bound (256 queries
+// of their outputs.  FOLD: these are held in units of a block's scale of V, and the products add to them as they are: the next
+// block's scale over that goes into the probabilities' exponents, as far as it costs fp16 no more than 8 of its bits (2^-8 .. 2);
+// one beyond becomes the unit itself.  (A unit that is kept while larger scales come ends in infinities: blocks of zeros have
+// 2^-100.)  Far below the largest scale so far, kByBelow, outputs have no room for it in fp32: the products of such a block, as of all
+// without FOLD, are multiplied and added.  At most the unit is kByLargest, so that no ratio of a scale to it leaves fp32's
+// range.  It pays where the matrix cores bound (256 queries
 // over up to 64K of four sequences: 223 us, without 233; 100 over 128K 98 and 101) and costs where loads do, of whose registers
 // it needs some (64 over 32K in byte_stream_kernel: 29.4 us, without 27.2; a token over 32K 19.0 and 18.2).  Sums of fp32
 // tensors do not take it: the matrix cores cut off what they add to them.
@@ -121,7 +122,7 @@ struct ByteWave {
   by_h8 qh[MT][2 * CH], ql[TWO ? MT : 1][2 * CH];   // elements 64 c + 16 quad + 8 h .. in [2 c + h]
   float up[MT], top[MT], sum[MT];
   ar_f4 o[MT][VW];
-  float unit, log_unit;
+  float unit, log_unit, most;   // (most: the largest scale so far)
 
   __device__ __forceinline__ void begin() {
 #pragma unroll
@@ -131,7 +132,7 @@ struct ByteWave {
 #pragma unroll
       for (int j = 0; j < VW; ++j) o[m][j] = ar_f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    unit = 0x1p-100f;   // (the least scale)
+    unit = most = 0x1p-100f;   // (the least scale)
     log_unit = -100.0f;
   }
   __device__ __forceinline__ void queries(const T* q, int row0, int M, int d, float scale_log2e) {
@@ -195,7 +196,8 @@ struct ByteWave {
     if constexpr (FOLD) {
       const float log_vs = __builtin_amdgcn_logf(vs);
       shift = log_vs - log_unit;
-      if (shift > 1.0f) {   // (for every block in which they grow: a few of a split)
+      most = fmaxf(most, vs);
+      if (shift > 1.0f || (shift < -8.0f && vs >= most * kByBelow)) {
         const float now = fminf(vs, kByLargest), less = unit / now;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
