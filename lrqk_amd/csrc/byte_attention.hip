@@ -437,7 +437,7 @@ struct BytePlace {
 // memory; a block's keys are asked for when the one's before have become scores, its values when those have become products.
 // Reading bounds it: a token over 32K (int8, 8 heads of 128, bf16) is 67 MB in 15.2 us, 4.4 TB/s where the largest reads reach
 // 5.5, and 16 over 1K .. 8K 158 MB in 31.3 (5.1 TB/s); the joining launch makes them 18 and 43.  Small ones are bound by their
-// chain of waits: 7 fp32 queries of 28 heads over 4K, 4 MB, take 9.8.  Heads of 256 need more than the 256 registers that two
+// chain of waits: 7 fp32 queries of 28 heads over 4K, 4.2 MB of codes, take 9.8.  Heads of 256 need more than the 256 registers that two
 // waves a SIMD have each (a token over 32K: 37.6 us in all, with two waves 45; fp32 39 and 67).
 template <typename T, bool FP8, int DP, int MT>
 __global__ __launch_bounds__(kTrThreads, DP == 256 ? 1 : 2) void byte_stream_kernel(ByteArgs ba) {
@@ -519,9 +519,10 @@ __global__ __launch_bounds__(kTrThreads, DP == 256 ? 1 : 2) void byte_stream_ker
 // those that follow are written meanwhile; one barrier a block.
 //
 // What bounds it is what a SIMD has to issue for a block, products, exponentials and reads of LDS, which overlap in part: 256
-// queries of each of four sequences over up to 64K (int8, 8 heads of 128) are 184 GFLOP in 218 us, 840 TFLOP/s (a large product
-// of the library reaches 1075), 100 over 128K 54 in 92.6, 580, or 740 with the rows up to 128 that are multiplied too.  The
-// matrix cores are busy a third of all cycles in both.  Two waves a SIMD are what registers allow.  64 queries a wave moved
+// queries of each of four sequences over up to 64K, 148K .. 214K tokens in all (int8, 8 heads of 128), are 155 .. 224 GFLOP in
+// 207 .. 284 us with the join's 11, 720 .. 800 TFLOP/s (a large product of the library reaches 1075), 100 over 128K 54 in 92.6,
+// 580, or 740 with the rows up to 128 that are multiplied too.  The matrix cores are busy a third of all cycles in both.  Two
+// waves a SIMD are what registers allow.  64 queries a wave moved
 // operands between register files (150 us for the 100), eight waves of a workgroup on the same blocks 210 us for the first and
 // 157 for the second, two blocks asked for ahead spilled.
 // From 65 queries on: up to 64 the other kernel's waves, which each read the codes, are faster (64 over 32K 27.2 us, here 36.2);

@@ -8,9 +8,9 @@
 //
 // so that one pass over two rows gives Z_j, and only nodes with several children need one.  Drafts without probabilities have
 // p = 1 at their token: r_j is r_(j-1) without it, and Z_j = Z_(j-1) - r_(j-1)(x_j), 1 less what the refused ones had, whatever
-// the row adds up to (its sum would be a pass; a row of bf16 probabilities is off by up to 2^-8).  Behind the last accepted node the next token is drawn from what is left:
-// the lowest x with r(0) + .. + r(x) > u_0 sum(r).  Everything is formed in 64 bits, since a vocabulary's sums in 32 would
-// put the border between two tokens elsewhere; what is not a positive number counts as 0.
+// the row adds up to (its sum would be a pass; a row of bf16 probabilities is off by up to 2^-8).  Behind the last accepted node
+// the next token is drawn from what is left: the lowest x with r(0) + .. + r(x) > u_0 sum(r).  Everything is formed in 64 bits,
+// since a vocabulary's sums in 32 would put the border between two tokens elsewhere; what is not a positive number counts as 0.
 //
 // Three launches: Z of the nodes with several children (trees with p only); the walk, by every workgroup for itself, and the
 // sums of what is left by chunks of the vocabulary; the chunk and the token.
@@ -123,7 +123,7 @@ __device__ __forceinline__ void vf_pass(const T* q, const T* p, int64_t n, F add
 // Z of the children of one node, one after the other up to the one that is accepted: a workgroup has both rows for itself.  Bound
 // by one CU's arithmetic, 9 us a pass over 128256 tokens, six instructions an element in 64 bits: rows of half the bytes take as
 // long, and rows kept in registers and LDS from pass to pass.  (Several CUs would have to wait for each other, or for a launch a
-// child.)
+// child; that of the second child alone, at C = 1, is known beforehand.)
 template <typename T>
 __global__ __launch_bounds__(kVfWide) void verify_mass_kernel(VerifyArgs a) {
   __shared__ VerifyTree tree;

@@ -159,7 +159,7 @@ class LlamaShapeDecoder:
     @torch.inference_mode()
     def forward(self, ids: torch.Tensor, pos0: int, cache: Optional[DynamicLRQKCache]) -> torch.Tensor:
         """ids [b,s] -> logits of the last position [b,vocab].  pos0: the first one's position (0 begins anew; over caches in 8 bits
-        a token stands behind what its sequence has, which ``generate_drafted`` may leave different)."""
+        a token stands behind what its sequence has, which ``generate_drafted`` may leave different: then that of the longest)."""
         c = self.cfg
         b, s = ids.shape
         rope, where = self.rope, pos0
