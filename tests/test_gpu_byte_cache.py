@@ -630,6 +630,31 @@ def test_blocks_of_small_values_in_front_of_larger_ones(ops, kind, d, t, hq):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_blocks_of_all_sizes_in_turn(ops, kind, d):
+    """Shared blocks whose values lie up to 2^90 apart, as they come, in order and in turn; a second call gives the same bits."""
+    print("byte all sizes", kind, d, flush=True)
+    blocks, t = 70, 80
+    n = 64 * blocks
+    g = _gen(51)
+    falling = torch.linspace(45, -45, blocks)
+    sizes = (torch.randint(-45, 46, (blocks,), generator=g).float(), falling, falling.flip(0), torch.where(torch.arange(blocks) % 2 == 0, 0.0, -55.0),
+             torch.where(torch.arange(blocks) % 5 == 2, 12.0, 0.0))
+    for i, size in enumerate(sizes):
+        v = _randn(g, 1, 1, n, d) * torch.exp2(size).to(DEV).repeat_interleave(64)[:, None]
+        for back in (0.0, 1.0):   # (scores that make up for the sizes: all blocks count)
+            k = _randn(g, 1, 1, n, d, scale=0.3)
+            k[..., 0] = back * -math.log(2) * size.to(DEV).repeat_interleave(64)
+            q, kn, vn, mask = _drafts(g, 1, 1, 1, t, d, BF)
+            q[..., 0] = 1.0
+            cache = ops.ByteCache(1, 1, n, d, BF, kind, DEV)
+            lengths = ops.byte_append(cache, k.to(BF), v.to(BF), _i32(0))
+            out, lse = _check_attention(ops, q, cache, lengths, kn, vn, mask, scale=1.0, what=(i, back))
+            again = ops.byte_attention(q, cache, lengths, kn, vn, mask, 1.0, return_lse=True)
+            assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_blocks_of_smaller_values_keep_small_probabilities(ops, kind):
     """One element is large, in every fourth block alone; the others are there in the other blocks alone, 2^-order as large, with
     probabilities that end near what fp16 holds."""
