@@ -253,7 +253,7 @@ struct ByteWave {
       }
     }
   }
-  // Around the products of a block whose scale is far below the unit (FOLD): what there is waits in memory meanwhile.  (A
+  // Around the products of a block whose scale is far from any unit (FOLD): what there is waits in memory meanwhile.  (A
   // branch with products of its own costs every block the copying of all outputs from register to register.)
   struct Waiting {
     volatile float o[FOLD ? MT * VW * 4 : 1];
